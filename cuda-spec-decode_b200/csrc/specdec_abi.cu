@@ -960,4 +960,146 @@ int specdec_dflash_attention_backward(const uint16_t* q, const uint16_t* k, cons
   return e == cudaSuccess ? ok() : cuda_fail(e, "attention backward launch");
 }
 
+
+}  // extern "C"
+
+namespace {
+
+RotaryTensor rotary_tensor(const void* p, const int64_t* strides, int32_t T, int32_t heads, int32_t D) {
+  RotaryTensor t;
+  t.p = p;
+  t.s[0] = strides ? strides[0] : (int64_t)T * heads * D;
+  t.s[1] = strides ? strides[1] : (int64_t)heads * D;
+  t.s[2] = strides ? strides[2] : D;
+  return t;
+}
+
+// Checks shared by the three rotary entry points, and the fields they share.
+int rotary_args(RotaryArgs& A, const int64_t* positions, int64_t pos_stride, const double* inv_freq, int32_t batch,
+                int32_t T, int32_t q_heads, int32_t k_heads, int32_t D, int32_t R, int32_t interleaved, float scale,
+                float eps, int32_t dtype, int* sms) {
+  if (batch < 0 || T < 0 || q_heads < 1 || k_heads < 0) return fail(SPECDEC_ERR_ARGUMENT, "bad shape");
+  if ((int64_t)batch * T > INT32_MAX) return fail(SPECDEC_ERR_ARGUMENT, "batch * T must fit in int32");
+  if ((int64_t)q_heads + k_heads > 65536) return fail(SPECDEC_ERR_ARGUMENT, "at most 65536 heads");
+  if (D < 2 || D > 512 || D % 2) return fail(SPECDEC_ERR_ARGUMENT, "head_dim must be even and in [2, 512], got %d", D);
+  if (R < 2 || R > D || R % 2)
+    return fail(SPECDEC_ERR_ARGUMENT, "rotary_dim must be even and in [2, head_dim], got %d", R);
+  if (dtype != kDtypeF32 && dtype != kDtypeBF16) return fail(SPECDEC_ERR_ARGUMENT, "unknown dtype %d", dtype);
+  if (!std::isfinite(scale)) return fail(SPECDEC_ERR_VALUE, "scale must be finite");
+  if (!(eps >= 0.f)) return fail(SPECDEC_ERR_VALUE, "eps must be >= 0, got %g", (double)eps);
+  A.positions = positions;
+  A.pos_stride = pos_stride;
+  A.inv_freq = inv_freq;
+  A.N = (int64_t)batch * T;
+  A.T = T;
+  A.D = D;
+  A.R = R;
+  A.interleaved = interleaved ? 1 : 0;
+  A.dtype = dtype;
+  A.heads[0] = q_heads;
+  A.heads[1] = k_heads;
+  A.H = q_heads + k_heads;
+  A.scale = A.sin_scale = scale;
+  A.eps = eps;
+  if (A.N == 0) return ok();
+  if (!positions || !inv_freq) return fail(SPECDEC_ERR_ARGUMENT, "null positions or inv_freq");
+  const int dev = current_device();
+  if (dev < 0) return fail(SPECDEC_ERR_CUDA, "cudaGetDevice failed");
+  if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return fail(SPECDEC_ERR_CUDA, "device query failed");
+  return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+int specdec_rotary(const void* x, const int64_t* x_strides, void* y, const int64_t* positions,
+                   int64_t position_stride, const double* inv_freq, int32_t batch, int32_t T, int32_t heads,
+                   int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float scale, int32_t inverse,
+                   int32_t dtype, void* stream) {
+  RotaryArgs A;
+  int sms = 0;
+  const int rc = rotary_args(A, positions, position_stride, inv_freq, batch, T, heads, 0, head_dim, rotary_dim,
+                             interleaved, scale, 0.f, dtype, &sms);
+  if (rc != SPECDEC_OK || A.N == 0) return rc;
+  if (!x || !y) return fail(SPECDEC_ERR_ARGUMENT, "null input or output pointer");
+  if (inverse) A.sin_scale = -scale;
+  A.x[0] = rotary_tensor(x, x_strides, T, heads, head_dim);
+  A.y[0] = rotary_tensor(y, nullptr, T, heads, head_dim);
+  const cudaError_t e = rotary_fwd_launch(A, false, sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ok() : cuda_fail(e, "rotary launch");
+}
+
+int specdec_qk_norm_rotary_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                   const float* q_weight, const float* k_weight, void* q_out, void* k_out,
+                                   const int64_t* positions, int64_t position_stride, const double* inv_freq,
+                                   int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                   int32_t rotary_dim, int32_t interleaved, float scale, float eps, int32_t dtype,
+                                   void* stream) {
+  RotaryArgs A;
+  int sms = 0;
+  if (k_heads < 1) return fail(SPECDEC_ERR_ARGUMENT, "bad shape");
+  const int rc = rotary_args(A, positions, position_stride, inv_freq, batch, T, q_heads, k_heads, head_dim, rotary_dim,
+                             interleaved, scale, eps, dtype, &sms);
+  if (rc != SPECDEC_OK || A.N == 0) return rc;
+  if (!q || !k || !q_weight || !k_weight || !q_out || !k_out)
+    return fail(SPECDEC_ERR_ARGUMENT, "null input or output pointer");
+  A.x[0] = rotary_tensor(q, q_strides, T, q_heads, head_dim);
+  A.x[1] = rotary_tensor(k, k_strides, T, k_heads, head_dim);
+  A.y[0] = rotary_tensor(q_out, nullptr, T, q_heads, head_dim);
+  A.y[1] = rotary_tensor(k_out, nullptr, T, k_heads, head_dim);
+  A.w[0] = q_weight;
+  A.w[1] = k_weight;
+  const cudaError_t e = rotary_fwd_launch(A, true, sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ok() : cuda_fail(e, "norm and rotary launch");
+}
+
+size_t specdec_qk_norm_rotary_workspace_bytes(int32_t batch, int32_t T, int32_t head_dim, int device) {
+  int sms = 0;
+  if (batch <= 0 || T <= 0 || head_dim <= 0 ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return 256;
+  return align256((size_t)qk_norm_bwd_ctas((int64_t)batch * T, sms) * 2 * (size_t)head_dim * sizeof(float));
+}
+
+int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                    const float* q_weight, const float* k_weight, const void* dq_out,
+                                    const int64_t* dq_out_strides, const void* dk_out, const int64_t* dk_out_strides,
+                                    void* dq, void* dk, float* dq_weight, float* dk_weight, const int64_t* positions,
+                                    int64_t position_stride, const double* inv_freq, int32_t batch, int32_t T,
+                                    int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                                    int32_t interleaved, float scale, float eps, int32_t dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  RotaryArgs A;
+  int sms = 0;
+  if (k_heads < 1) return fail(SPECDEC_ERR_ARGUMENT, "bad shape");
+  const int rc = rotary_args(A, positions, position_stride, inv_freq, batch, T, q_heads, k_heads, head_dim, rotary_dim,
+                             interleaved, scale, eps, dtype, &sms);
+  if (rc != SPECDEC_OK) return rc;
+  if (!dq_weight || !dk_weight) return fail(SPECDEC_ERR_ARGUMENT, "null weight gradient");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (A.N == 0) {
+    cudaError_t e = cudaMemsetAsync(dq_weight, 0, (size_t)head_dim * sizeof(float), st);
+    if (e == cudaSuccess) e = cudaMemsetAsync(dk_weight, 0, (size_t)head_dim * sizeof(float), st);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "cudaMemsetAsync");
+  }
+  if (!q || !k || !q_weight || !k_weight || !dq_out || !dk_out || !dq || !dk || !workspace)
+    return fail(SPECDEC_ERR_ARGUMENT, "null input, output or workspace pointer");
+  const size_t need = (size_t)qk_norm_bwd_ctas(A.N, sms) * 2 * (size_t)head_dim * sizeof(float);
+  if (workspace_bytes < need)
+    return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  A.sin_scale = -scale;
+  A.x[0] = rotary_tensor(q, q_strides, T, q_heads, head_dim);
+  A.x[1] = rotary_tensor(k, k_strides, T, k_heads, head_dim);
+  A.dy[0] = rotary_tensor(dq_out, dq_out_strides, T, q_heads, head_dim);
+  A.dy[1] = rotary_tensor(dk_out, dk_out_strides, T, k_heads, head_dim);
+  A.y[0] = rotary_tensor(dq, nullptr, T, q_heads, head_dim);
+  A.y[1] = rotary_tensor(dk, nullptr, T, k_heads, head_dim);
+  A.w[0] = q_weight;
+  A.w[1] = k_weight;
+  const cudaError_t e = qk_norm_bwd_launch(A, static_cast<float*>(workspace), dq_weight, dk_weight, sms, st);
+  return e == cudaSuccess ? ok() : cuda_fail(e, "norm and rotary backward launch");
+}
+
 }  // extern "C"

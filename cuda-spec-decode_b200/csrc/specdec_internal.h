@@ -183,6 +183,31 @@ cudaError_t rmsnorm_fwd_launch(int dtype, const void* x, const float* w, void* y
 cudaError_t rmsnorm_bwd_launch(int dtype, const void* x, const float* w, const float* rstd, const void* dy,
                                void* dx, float* dw, float* part, int64_t rows, int D, int ctas, cudaStream_t st);
 
+// Rotary positions, alone or fused with the RMSNorm of queries and keys
+// (drafter_rotary.cu). Two tensors per launch: queries and keys; a plain
+// rotation leaves the second one without heads.
+struct RotaryTensor {
+  const void* p = nullptr;         // [batch, T, heads, D], elements of a head contiguous
+  int64_t s[3] = {0, 0, 0};        // batch, token, head stride in elements
+};
+
+struct RotaryArgs {
+  RotaryTensor x[2], dy[2], y[2];  // inputs, output gradients (backward), outputs (y or dx)
+  const float* w[2] = {nullptr, nullptr};  // [D] norm weights
+  const int64_t* positions;
+  int64_t pos_stride;              // between sequences (0: shared); tokens are contiguous
+  const double* inv_freq;          // [R / 2]
+  int64_t N;                       // batch * T
+  int T, D, R, interleaved, dtype;
+  int heads[2], H;                 // H = heads[0] + heads[1]
+  float scale, sin_scale, eps;     // sin_scale = -scale turns the other way
+  // set by the launch
+  int TT, lg, nchunk, hchunk;      // tokens per CTA, log2 lanes per head, units per token, heads per unit
+};
+cudaError_t rotary_fwd_launch(RotaryArgs A, bool norm, int sms, cudaStream_t st);
+int qk_norm_bwd_ctas(int64_t tokens, int sms);
+cudaError_t qk_norm_bwd_launch(RotaryArgs A, float* part, float* dwq, float* dwk, int sms, cudaStream_t st);
+
 // Attention of the drafter on the tensor cores (drafter_attention.cu):
 // bf16 q/k/v/o [B, T, H, 64], lse fp32 [B, H, T].
 cudaError_t dflash_attn_fwd_launch(const void* q, const void* k, const void* v, void* o, float* lse, int batch, int T,

@@ -9,6 +9,11 @@
   Forward and backward run on the tensor cores (tcgen05: products in tensor
   memory); the backward recomputes the probabilities from the forward's
   log-sum-exp and accumulates dq, dk, dv in a fixed order.
+- ``rotary(x, positions, inv_freq)``: rotary positions (half or interleaved
+  pairs, all or part of the head); ``rotary_frequencies`` gives the
+  frequencies, also scaled for long contexts.
+- ``qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq)``: RMSNorm
+  of every query and key head and the rotation in one pass.
 
 Reference: models/dflash/model.py:25-53 (DFlashAttention), :56-73 (the
 pre-norm layer, torch.nn.RMSNorm), :123-131 (the mask).
@@ -18,7 +23,11 @@ dtypes above.
 """
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -134,3 +143,199 @@ def dflash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_ctx: i
     """Attention under the DFlash mask; q, k, v bf16 [B, T, H, 64] -> o [B, T, H, 64]."""
     s = q.shape[-1] ** -0.5 if scale is None else float(scale)
     return _DFlashAttention.apply(q, k, v, n_ctx, s)
+
+
+# ---- rotary positions, norms of queries and keys --------------------------------
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str | None = None, *, factor: float = 1.0,
+                       original_length: int | None = None, low: float | None = None, high: float | None = None,
+                       device=None) -> tuple[torch.Tensor, float]:
+    """(inv_freq, scale) for ``rotary`` over ``dim`` elements of a head:
+    inv_freq[i] = base^(-2i / dim), fp64 [dim / 2] on ``device``, and the factor
+    on the rotated elements. ``scaling`` stretches them to contexts ``factor``
+    times as long as the ``original_length`` they were trained for:
+
+    - "linear": every frequency divided by factor (positions interpolated);
+    - "ntk": base * factor^(dim / (dim - 2)): the slowest pair is divided by
+      factor, the fastest stays;
+    - "ramp": pairs that turn more than ``high`` times within original_length
+      stay, those that turn less than ``low`` times are divided by factor, a
+      linear ramp in the number of turns between them (defaults 1 and 4);
+    - "yarn": the ramp from 1 to 32 turns, and scale 0.1 ln(factor) + 1
+      (Peng et al., 2023, arXiv:2309.00071, equations 17, 18 and 22).
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError(f"dim must be even and >= 2, got {dim}")
+    if not base > 0 or not factor > 0:
+        raise ValueError("base and factor must be > 0")
+    exponent = -torch.arange(0, dim, 2, dtype=torch.float64) / dim
+    freq = float(base) ** exponent
+    scale = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "ntk":
+        if dim < 4:
+            raise ValueError("ntk scaling needs dim >= 4")
+        freq = (float(base) * factor ** (dim / (dim - 2))) ** exponent
+    elif scaling in ("ramp", "yarn"):
+        if original_length is None or original_length < 1:
+            raise ValueError(f"{scaling} scaling needs original_length >= 1")
+        lo, hi = (1.0, 4.0) if scaling == "ramp" else (1.0, 32.0)
+        lo, hi = lo if low is None else float(low), hi if high is None else float(high)
+        if not hi > lo:
+            raise ValueError("high must be > low")
+        keep = ((original_length * freq / (2.0 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
+        freq = keep * freq + (1.0 - keep) * freq / factor
+        if scaling == "yarn":
+            scale = 0.1 * math.log(max(factor, 1.0)) + 1.0
+    elif scaling is not None:
+        raise ValueError(f"unknown scaling {scaling!r}, expected linear, ntk, ramp or yarn")
+    return freq.to(device=device), scale
+
+
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    """A head's elements contiguous; the other dimensions as they are."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides(t: torch.Tensor):
+    """The C ABI's three element strides (None: contiguous)."""
+    return None if t.is_contiguous() else (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _check_heads(name: str, x: torch.Tensor, like: torch.Tensor | None = None) -> None:
+    assert x.is_cuda and x.dim() == 4 and x.dtype in _DTYPES, f"{name} must be cuda float32 or bfloat16 [B, T, heads, D]"
+    if like is not None:
+        assert x.device == like.device and x.dtype == like.dtype and x.shape[:2] == like.shape[:2] \
+            and x.shape[3] == like.shape[3], f"{name} must match q's device, dtype, batch, length and head size"
+
+
+def _check_rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    assert positions.device == x.device and positions.dtype in (torch.int64, torch.int32) \
+        and (positions.shape == x.shape[:2] or positions.shape == x.shape[1:2]), \
+        "positions must be int64 (or int32) [T] or [B, T] on the heads' device"
+    assert inv_freq.device == x.device and inv_freq.dtype == torch.float64 and inv_freq.dim() == 1, \
+        "inv_freq must be float64 [rotary_dim / 2] on the heads' device"
+    assert 0 < 2 * inv_freq.numel() <= x.shape[3], "inv_freq must turn at least one pair and at most the head"
+    positions = positions.long()
+    if positions.stride(-1) != 1 and positions.shape[-1] > 1:
+        positions = positions.contiguous()
+    return positions, inv_freq.contiguous()
+
+
+def _position_stride(positions: torch.Tensor) -> int:
+    return positions.stride(0) if positions.dim() == 2 else 0
+
+
+def _rotary(x, positions, inv_freq, interleaved, scale, inverse):
+    lib = _lib.load()
+    B, T, H, D = x.shape
+    x = _strided(x)
+    y = torch.empty((B, T, H, D), dtype=x.dtype, device=x.device)
+    with _lib.on_device(x.device):
+        _lib.check(lib.specdec_rotary(
+            x.data_ptr(), _strides(x), y.data_ptr(), positions.data_ptr(), _position_stride(positions),
+            inv_freq.data_ptr(), B, T, H, D, 2 * inv_freq.numel(), interleaved, scale, inverse, _DTYPES[x.dtype],
+            _stream(x)), "specdec_rotary")
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, interleaved, scale):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = interleaved, scale
+        return _rotary(x, positions, inv_freq, interleaved, scale, 0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        positions, inv_freq = ctx.saved_tensors
+        return _rotary(dy, positions, inv_freq, *ctx.how, 1), None, None, None, None
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
+           scale: float = 1.0) -> torch.Tensor:
+    """Rotary positions of every head of x [B, T, heads, D] (fp32 or bf16, any
+    strides; D even, <= 512): of the first R = 2 len(inv_freq) elements, pair i
+    -- (i, i + R/2), or (2i, 2i + 1) with ``interleaved`` -- turns by the angle
+    position * inv_freq[i] and is multiplied by ``scale``; the rest is copied.
+    positions: int64 [T] or [B, T]; inv_freq: fp64 (``rotary_frequencies``).
+    Angles are formed in fp64. Differentiable in x."""
+    _check_heads("x", x)
+    positions, inv_freq = _check_rotary(x, positions, inv_freq)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Rotary.apply(x, positions, inv_freq, int(bool(interleaved)), float(scale))
+    return _rotary(x.detach(), positions, inv_freq, int(bool(interleaved)), float(scale), 0)
+
+
+def _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale):
+    lib = _lib.load()
+    B, T, Hq, D = q.shape
+    yq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    yk = torch.empty((B, T, k.shape[2], D), dtype=q.dtype, device=q.device)
+    with _lib.on_device(q.device):
+        _lib.check(lib.specdec_qk_norm_rotary_forward(
+            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), yq.data_ptr(),
+            yk.data_ptr(), positions.data_ptr(), _position_stride(positions), inv_freq.data_ptr(), B, T, Hq, k.shape[2],
+            D, 2 * inv_freq.numel(), interleaved, scale, eps, _DTYPES[q.dtype], _stream(q)),
+            "specdec_qk_norm_rotary_forward")
+    return yq, yk
+
+
+class _QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, scale):
+        q, k = _strided(q), _strided(k)
+        wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
+        ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
+        ctx.how = eps, interleaved, scale
+        ctx.wdtypes = q_weight.dtype, k_weight.dtype
+        return _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dyq, dyk):
+        lib = _lib.load()
+        q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
+        eps, interleaved, scale = ctx.how
+        B, T, Hq, D = q.shape
+        Hk = k.shape[2]
+        dyq, dyk = _strided(dyq), _strided(dyk)
+        dq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+        dk = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
+        dw = torch.empty((2, D), dtype=torch.float32, device=q.device)
+        with _lib.on_device(q.device):
+            ws_bytes = lib.specdec_qk_norm_rotary_workspace_bytes(B, T, D, q.device.index)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            _lib.check(lib.specdec_qk_norm_rotary_backward(
+                q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), dyq.data_ptr(),
+                _strides(dyq), dyk.data_ptr(), _strides(dyk), dq.data_ptr(), dk.data_ptr(), dw[0].data_ptr(),
+                dw[1].data_ptr(), positions.data_ptr(), _position_stride(positions), inv_freq.data_ptr(), B, T, Hq, Hk,
+                D, 2 * inv_freq.numel(), interleaved, scale, eps, _DTYPES[q.dtype], ws.data_ptr(), ws_bytes,
+                _stream(q)), "specdec_qk_norm_rotary_backward")
+        return dq, dk, dw[0].to(ctx.wdtypes[0]), dw[1].to(ctx.wdtypes[1]), None, None, None, None, None
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                   positions: torch.Tensor, inv_freq: torch.Tensor, *, eps: float | None = None,
+                   interleaved: bool = False, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm over the elements of every head of q [B, T, Hq, D] and k
+    [B, T, Hk, D] (weights [D]; eps None = finfo(dtype).eps), then ``rotary`` of
+    both, in one pass: x / sqrt(mean(x^2) + eps) * weight, rotated. fp32 or bf16,
+    any strides (views of one fused projection); fp32 arithmetic, one rounding.
+    Differentiable in q, k and the weights (their gradients are summed in a
+    fixed order)."""
+    _check_heads("q", q)
+    _check_heads("k", k, q)
+    D = q.shape[3]
+    assert q_weight.shape == (D,) and k_weight.shape == (D,) and q_weight.device == q.device \
+        and k_weight.device == q.device, "weights must be [D] on q's device"
+    positions, inv_freq = _check_rotary(q, positions, inv_freq)
+    e = torch.finfo(q.dtype).eps if eps is None else float(eps)
+    how = e, int(bool(interleaved)), float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
+                                    or k_weight.requires_grad):
+        return _QKNormRotary.apply(q, k, q_weight, k_weight, positions, inv_freq, *how)
+    return _qk_norm_rotary(_strided(q.detach()), _strided(k.detach()), q_weight.detach().float().contiguous(),
+                           k_weight.detach().float().contiguous(), positions, inv_freq, *how)

@@ -336,6 +336,69 @@ int specdec_dflash_attention_backward(const uint16_t* q, const uint16_t* k, cons
                                       size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* Long-context attention layer of the drafter                                */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Rotary positions, norms of queries and keys, sliding-window attention. No
+ * counterpart in the reference, whose drafter attention
+ * (models/dflash/model.py:25-53) has no positions, norms or window.
+ *
+ * Tensors [batch, T, heads, head_dim] of these entry points may be strided:
+ * `*_strides` is a host array of three element strides (batch, token, head),
+ * NULL for a contiguous tensor; the elements of a head are contiguous.
+ * Outputs are contiguous. Element strides that are multiples of 16 bytes (and
+ * 16-byte-aligned pointers) take the vectorised kernels, others run with
+ * one-element accesses.
+ */
+
+/*
+ * Rotary positions: the first rotary_dim elements of every head form pairs,
+ * (i, i + rotary_dim / 2), or neighbours with `interleaved`; pair i of the
+ * token at position m turns by the angle m * inv_freq[i] (by its opposite
+ * with `inverse`: the gradient) and is multiplied by `scale`; the other
+ * elements are copied.
+ *   positions  int64, token t of sequence b at positions[b * position_stride + t]
+ *              (position_stride 0: shared by the sequences)
+ *   inv_freq   [rotary_dim / 2] fp64; angles are formed and reduced in fp64
+ * head_dim even, <= 512; rotary_dim even, in [2, head_dim]; batch * T must
+ * fit in int32. x, y: `dtype` (SPECDEC_DTYPE_*). y may equal x if x is contiguous.
+ */
+int specdec_rotary(const void* x, const int64_t* x_strides, void* y, const int64_t* positions,
+                   int64_t position_stride, const double* inv_freq, int32_t batch, int32_t T, int32_t heads,
+                   int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float scale, int32_t inverse,
+                   int32_t dtype, void* stream);
+
+/*
+ * RMSNorm of every query and key head (over head_dim, fp32 weights
+ * [head_dim]) followed by the rotation above, in one pass:
+ * q_out = rotary(q / sqrt(mean(q^2) + eps) * q_weight), k_out likewise.
+ */
+int specdec_qk_norm_rotary_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                   const float* q_weight, const float* k_weight, void* q_out, void* k_out,
+                                   const int64_t* positions, int64_t position_stride, const double* inv_freq,
+                                   int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                   int32_t rotary_dim, int32_t interleaved, float scale, float eps, int32_t dtype,
+                                   void* stream);
+
+/* Workspace bytes of specdec_qk_norm_rotary_backward (partial weight gradients). */
+size_t specdec_qk_norm_rotary_workspace_bytes(int32_t batch, int32_t T, int32_t head_dim, int device);
+
+/*
+ * Its backward: dq, dk (the inputs' dtype, contiguous) and the fp32 weight
+ * gradients [head_dim] (fixed summation order: bitwise repeatable) from the
+ * inputs and the output gradients dq_out, dk_out. Saves nothing of the forward.
+ */
+int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                    const float* q_weight, const float* k_weight, const void* dq_out,
+                                    const int64_t* dq_out_strides, const void* dk_out, const int64_t* dk_out_strides,
+                                    void* dq, void* dk, float* dq_weight, float* dk_weight, const int64_t* positions,
+                                    int64_t position_stride, const double* inv_freq, int32_t batch, int32_t T,
+                                    int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                                    int32_t interleaved, float scale, float eps, int32_t dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Launch tuning                                                              */
 /* ------------------------------------------------------------------------- */
 

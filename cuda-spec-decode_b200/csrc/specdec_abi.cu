@@ -1103,3 +1103,201 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
 }
 
 }  // extern "C"
+
+namespace {
+
+// Checks shared by the window attention entry points, and the fields they share.
+int window_args(WindowArgs& A, int32_t batch, int32_t Tq, int32_t Tk, int32_t q_heads, int32_t k_heads, int32_t D,
+                int32_t n_block, int32_t window, int32_t sinks, float scale) {
+  if (D != 64 && D != 128) return fail(SPECDEC_ERR_ARGUMENT, "head_dim must be 64 or 128, got %d", D);
+  if (batch < 0 || Tq < 0 || Tk < 0 || q_heads < 1 || k_heads < 1) return fail(SPECDEC_ERR_ARGUMENT, "bad shape");
+  if (q_heads % k_heads)
+    return fail(SPECDEC_ERR_ARGUMENT, "q_heads must be a multiple of k_heads (%d, %d)", q_heads, k_heads);
+  if (window < 1) return fail(SPECDEC_ERR_ARGUMENT, "window must be >= 1, got %d", window);
+  if (sinks < 0) return fail(SPECDEC_ERR_ARGUMENT, "sinks must be >= 0, got %d", sinks);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(SPECDEC_ERR_VALUE, "scale must be > 0 and finite");
+  const int64_t G = q_heads / k_heads, M = (int64_t)Tq * G;
+  if (Tk > (1 << 30) || M > INT32_MAX - 256) return fail(SPECDEC_ERR_ARGUMENT, "too many tokens");
+  if ((M + 127) / 128 > 65535) return fail(SPECDEC_ERR_ARGUMENT, "at most 65535 * 128 query rows per key head");
+  if ((int64_t)batch * k_heads * ((M + 127) / 128 + (Tq + 127) / 128) > INT32_MAX ||
+      (int64_t)batch * Tq * q_heads / 4 >= INT32_MAX)
+    return fail(SPECDEC_ERR_ARGUMENT, "too many rows");
+  A = WindowArgs{};
+  A.B = batch;
+  A.Tq = Tq;
+  A.Tk = Tk;
+  A.Hq = q_heads;
+  A.Hk = k_heads;
+  A.G = (int)G;
+  A.M = (int)M;
+  int l = 0;
+  while ((int64_t(1) << l) < G) ++l;
+  A.gshift = 31 + l;
+  A.gmul = (uint32_t)(((uint64_t(1) << (31 + l)) + G - 1) / G);
+  A.n_block = n_block;
+  A.W = std::min(window, 1 << 30);
+  A.S = sinks;
+  A.scale = scale;
+  A.scale_log2 = scale * kLog2e;
+  A.splits = 1;
+  return ok();
+}
+
+// A strided input: 16-byte-aligned rows.
+int window_input(const char* name, const void* p, const int64_t* strides, int32_t batch, int32_t T, int32_t heads,
+                 int32_t D, int64_t (&s)[3]) {
+  s[0] = strides ? strides[0] : (int64_t)T * heads * D;
+  s[1] = strides ? strides[1] : (int64_t)heads * D;
+  s[2] = strides ? strides[2] : D;
+  if (!p) return fail(SPECDEC_ERR_ARGUMENT, "null %s", name);
+  if (!aligned(p, 16) || (batch > 1 && s[0] % 8) || (T > 1 && s[1] % 8) || (heads > 1 && s[2] % 8))
+    return fail(SPECDEC_ERR_ARGUMENT, "%s: rows must be 16-byte aligned", name);
+  return SPECDEC_OK;
+}
+
+int64_t window_most_keys(int64_t Tq, int64_t Tk, int64_t n_block, int64_t window, int64_t sinks) {
+  return std::min<int64_t>(Tk, window + sinks + Tq + n_block);
+}
+
+}  // namespace
+
+extern "C" {
+
+int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
+                                     const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
+                                     uint16_t* o, float* lse, const int32_t* ctx_lens, int32_t batch, int32_t T,
+                                     int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx, int32_t window,
+                                     int32_t sinks, float scale, int32_t* status, void* stream) {
+  WindowArgs A;
+  if (n_ctx < 0 || n_ctx > T)
+    return fail(SPECDEC_ERR_ARGUMENT, "n_ctx must be in [0, T] (n_ctx=%d, T=%d)", n_ctx, T);
+  int rc = window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, scale);
+  if (rc != SPECDEC_OK || batch == 0 || T == 0) return rc;
+  if ((rc = window_input("q", q, q_strides, batch, T, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
+  if ((rc = window_input("k", k, k_strides, batch, T, k_heads, head_dim, A.ks)) != SPECDEC_OK) return rc;
+  if ((rc = window_input("v", v, v_strides, batch, T, k_heads, head_dim, A.vs)) != SPECDEC_OK) return rc;
+  if (!o || !aligned(o, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o must be 16-byte aligned");
+  A.q = q;
+  A.k = k;
+  A.v = v;
+  A.o = o;
+  A.lse = lse;
+  A.ctx_lens = ctx_lens;
+  A.n_ctx = n_ctx;
+  A.status = status;
+  A.withhold = take_withhold_stage();
+  const cudaError_t e = window_fwd_launch(A, head_dim, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ok() : cuda_fail(e, "window attention forward launch");
+}
+
+size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads) {
+  if (batch <= 0 || T <= 0 || q_heads <= 0) return 256;
+  return align256((size_t)batch * (size_t)q_heads * (size_t)T * sizeof(float));
+}
+
+int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
+                                      const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
+                                      const uint16_t* o, const float* lse, const uint16_t* dout, uint16_t* dq,
+                                      uint16_t* dk, uint16_t* dv, const int32_t* ctx_lens, int32_t batch, int32_t T,
+                                      int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx,
+                                      int32_t window, int32_t sinks, float scale, int32_t* status, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  WindowArgs A;
+  if (n_ctx < 0 || n_ctx > T)
+    return fail(SPECDEC_ERR_ARGUMENT, "n_ctx must be in [0, T] (n_ctx=%d, T=%d)", n_ctx, T);
+  int rc = window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, scale);
+  if (rc != SPECDEC_OK || batch == 0 || T == 0) return rc;
+  if ((rc = window_input("q", q, q_strides, batch, T, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
+  if ((rc = window_input("k", k, k_strides, batch, T, k_heads, head_dim, A.ks)) != SPECDEC_OK) return rc;
+  if ((rc = window_input("v", v, v_strides, batch, T, k_heads, head_dim, A.vs)) != SPECDEC_OK) return rc;
+  if (!lse || !workspace) return fail(SPECDEC_ERR_ARGUMENT, "null lse or workspace");
+  const void* ptrs[] = {o, dout, dq, dk, dv};
+  for (const void* p : ptrs)
+    if (!p || !aligned(p, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o, dout, dq, dk and dv must be 16-byte aligned");
+  const size_t need = (size_t)batch * (size_t)q_heads * (size_t)T * sizeof(float);
+  if (workspace_bytes < need)
+    return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  A.q = q;
+  A.k = k;
+  A.v = v;
+  A.o = const_cast<uint16_t*>(o);
+  A.lse = const_cast<float*>(lse);
+  A.dO = dout;
+  A.dq = dq;
+  A.dk = dk;
+  A.dv = dv;
+  A.delta = static_cast<float*>(workspace);
+  A.ctx_lens = ctx_lens;
+  A.n_ctx = n_ctx;
+  A.status = status;
+  A.withhold = take_withhold_stage();
+  const cudaError_t e = window_bwd_launch(A, head_dim, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ok() : cuda_fail(e, "window attention backward launch");
+}
+
+size_t specdec_window_attention_cached_workspace_bytes(int32_t batch, int32_t q_len, int32_t cache_len,
+                                                       int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                                       int32_t n_block, int32_t window, int32_t sinks, int device) {
+  int sms = 0;
+  if (batch <= 0 || q_len <= 0 || cache_len <= 0 || q_heads <= 0 || k_heads <= 0 || q_heads % k_heads ||
+      (head_dim != 64 && head_dim != 128) || window < 1 || sinks < 0 || n_block < 0 ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return 256;
+  const int64_t M = (int64_t)q_len * (q_heads / k_heads), bh = (int64_t)batch * k_heads;
+  const int splits = window_splits(head_dim, bh * ((M + 127) / 128),
+                                   window_most_keys(q_len, cache_len, n_block, window, sinks), sms);
+  if (splits == 1) return 256;
+  return align256((size_t)bh * M * splits * head_dim * sizeof(float)) + align256((size_t)bh * M * splits * sizeof(float2));
+}
+
+int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides, const uint16_t* k_cache,
+                                    const int64_t* k_strides, const uint16_t* v_cache, const int64_t* v_strides,
+                                    uint16_t* o, const int32_t* ctx_lens, int32_t batch, int32_t q_len,
+                                    int32_t cache_len, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                    int32_t n_block, int32_t window, int32_t sinks, float scale, int32_t* status,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  WindowArgs A;
+  if (n_block < 0 || n_block > cache_len)
+    return fail(SPECDEC_ERR_ARGUMENT, "n_block must be in [0, cache_len] (n_block=%d, cache_len=%d)", n_block, cache_len);
+  int rc = window_args(A, batch, q_len, cache_len, q_heads, k_heads, head_dim, n_block, window, sinks, scale);
+  if (rc != SPECDEC_OK || batch == 0 || q_len == 0) return rc;
+  if (!ctx_lens) return fail(SPECDEC_ERR_ARGUMENT, "null ctx_lens");
+  if ((rc = window_input("q", q, q_strides, batch, q_len, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
+  if (!o || !aligned(o, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o must be 16-byte aligned");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (cache_len == 0) {  // no token anywhere: every query is empty
+    const cudaError_t e = cudaMemsetAsync(o, 0, (size_t)batch * q_len * q_heads * head_dim * sizeof(uint16_t), st);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "cudaMemsetAsync");
+  }
+  if ((rc = window_input("k_cache", k_cache, k_strides, batch, cache_len, k_heads, head_dim, A.ks)) != SPECDEC_OK)
+    return rc;
+  if ((rc = window_input("v_cache", v_cache, v_strides, batch, cache_len, k_heads, head_dim, A.vs)) != SPECDEC_OK)
+    return rc;
+  const int dev = current_device();
+  int sms = 0;
+  if (dev < 0 || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return fail(SPECDEC_ERR_CUDA, "device query failed");
+  const int64_t bh = (int64_t)batch * k_heads;
+  A.splits = window_splits(head_dim, bh * ((A.M + 127) / 128),
+                           window_most_keys(q_len, cache_len, n_block, window, sinks), sms);
+  if (A.splits > 1) {
+    const size_t rows = (size_t)bh * A.M * A.splits, at = align256(rows * head_dim * sizeof(float));
+    const size_t need = at + rows * sizeof(float2);
+    if (!workspace || workspace_bytes < need)
+      return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace ? workspace_bytes : 0);
+    A.part_o = static_cast<float*>(workspace);
+    A.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + at);
+  }
+  A.q = q;
+  A.k = k_cache;
+  A.v = v_cache;
+  A.o = o;
+  A.ctx_lens = ctx_lens;
+  A.cached = 1;
+  A.status = status;
+  A.withhold = take_withhold_stage();
+  const cudaError_t e = window_fwd_launch(A, head_dim, st);
+  return e == cudaSuccess ? ok() : cuda_fail(e, "window attention launch");
+}
+
+}  // extern "C"

@@ -217,6 +217,32 @@ cudaError_t dflash_attn_bwd_launch(const void* q, const void* k, const void* v, 
                                    const void* dO, void* dq, void* dk, void* dv, float* delta, int batch, int T, int H,
                                    int n_ctx, float scale, int* status, int withhold, cudaStream_t st);
 
+// Sliding-window attention with sinks (drafter_window.cu).
+struct WindowArgs {
+  const bf16_t *q, *k, *v;         // [B, Tq | Tk, heads, D], strided
+  int64_t qs[3], ks[3], vs[3];     // batch, token, head stride in elements
+  bf16_t* o;                       // [B, Tq, Hq, D]
+  float* lse;                      // [B, Hk, M] of packed rows (token * G + head of the group), or null
+  const int* ctx_lens;             // [B], or null (training: every context is n_ctx long)
+  int B, Tq, Tk, Hq, Hk, G, M;     // M = Tq * G packed rows per key head
+  uint32_t gmul;                   // m / G = (m * gmul) >> gshift
+  int gshift;
+  int cached;                      // 1: keys are a cache of Tk rows, the queries its last tokens
+  int n_ctx, n_block, W, S;        // W <= 2^30
+  float scale, scale_log2;
+  int splits;                      // of the keys (cached form)
+  float* part_o;                   // [B * Hk * M, splits, D]
+  float2* part_ml;                 // [B * Hk * M, splits]: reference maximum, sum
+  const bf16_t* dO;                // backward: [B, Tq, Hq, D]
+  float* delta;                    // [B, Hk, M]
+  bf16_t *dq, *dk, *dv;
+  int* status;
+  int withhold;
+};
+int window_splits(int D, int64_t ctas, int64_t most_keys, int sms);
+cudaError_t window_fwd_launch(const WindowArgs& A, int D, cudaStream_t st);
+cudaError_t window_bwd_launch(const WindowArgs& A, int D, cudaStream_t st);
+
 // Sets the calling thread's specdec_last_error() text.
 void set_last_error(const char* msg);
 

@@ -90,6 +90,18 @@ _SIGNATURES = {
     "specdec_qk_norm_rotary_backward": (ctypes.c_int, [
         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p,
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_f32, _c_i32, _c_p, _c_sz, _c_p]),
+    "specdec_window_attention_forward": (ctypes.c_int, [
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_i32, _c_i32, _c_f32, _c_p, _c_p]),
+    "specdec_window_attention_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32]),
+    "specdec_window_attention_backward": (ctypes.c_int, [
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32,
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32, _c_p, _c_p, _c_sz, _c_p]),
+    "specdec_window_attention_cached_workspace_bytes": (_c_sz, [
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_int]),
+    "specdec_window_attention_cached": (ctypes.c_int, [
+        _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_i32, _c_i32, _c_f32, _c_p, _c_p, _c_sz, _c_p]),
 }
 # bf16 entry points take the same arguments as their fp32 counterparts
 for _name in ("specdec_dpace_forward", "specdec_dpace_backward", "specdec_dflash_forward",

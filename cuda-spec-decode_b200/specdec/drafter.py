@@ -14,6 +14,11 @@
   frequencies, also scaled for long contexts.
 - ``qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq)``: RMSNorm
   of every query and key head and the rotation in one pass.
+- ``window_attention(q, k, v, n_ctx, window=, sinks=)``: attention under the
+  DFlash mask with a sliding window over the context and a few first tokens
+  that stay visible; shared key heads, heads of 64 or 128, padded contexts;
+  forward and backward on the tensor cores. ``window_attention_cached`` is its
+  serving form: the last few tokens' queries against a cache.
 
 Reference: models/dflash/model.py:25-53 (DFlashAttention), :56-73 (the
 pre-norm layer, torch.nn.RMSNorm), :123-131 (the mask).
@@ -339,3 +344,145 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
         return _QKNormRotary.apply(q, k, q_weight, k_weight, positions, inv_freq, *how)
     return _qk_norm_rotary(_strided(q.detach()), _strided(k.detach()), q_weight.detach().float().contiguous(),
                            k_weight.detach().float().contiguous(), positions, inv_freq, *how)
+
+
+# ---- sliding-window attention with sinks ------------------------------------------
+
+_NO_WINDOW = 2 ** 31 - 1
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t itself if every row of a head starts on a 16-byte boundary, else a copy."""
+    if t.data_ptr() % 16 == 0 and t.stride(3) == 1 and all(
+            t.stride(d) % 8 == 0 or t.shape[d] <= 1 for d in range(3)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_window(q, k, v, window, sinks, scale) -> tuple[int, int, float]:
+    assert q.is_cuda and q.dtype == torch.bfloat16 and q.dim() == 4, "q must be cuda bfloat16 [B, T, heads, D]"
+    assert q.shape[3] in (64, 128), f"heads must have 64 or 128 elements, got {q.shape[3]}"
+    assert k.dim() == 4 and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3], \
+        "k and v must be [B, T, k_heads, D] with q's batch and head size"
+    assert k.dtype == q.dtype and v.dtype == q.dtype and k.device == q.device and v.device == q.device, \
+        "k and v must have q's dtype and device"
+    assert k.shape[2] > 0 and q.shape[2] > 0 and q.shape[2] % k.shape[2] == 0, \
+        f"query heads must be a multiple of key heads ({q.shape[2]}, {k.shape[2]})"
+    assert window is None or window >= 1, f"window must be >= 1 or None, got {window}"
+    assert sinks >= 0, f"sinks must be >= 0, got {sinks}"
+    return (_NO_WINDOW if window is None else min(int(window), _NO_WINDOW), min(int(sinks), _NO_WINDOW),
+            q.shape[3] ** -0.5 if scale is None else float(scale))
+
+
+def _check_lens(ctx_lens: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
+    assert ctx_lens.shape == (q.shape[0],) and ctx_lens.dtype in (torch.int32, torch.int64) \
+        and ctx_lens.device == q.device, "ctx_lens must be int32 (or int64) [B] on q's device"
+    return ctx_lens.to(torch.int32).contiguous()
+
+
+def _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, want_lse):
+    lib = _lib.load()
+    B, T, Hq, D = q.shape
+    Hk = k.shape[2]
+    o = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hk, T, Hq // Hk), dtype=torch.float32, device=q.device) if want_lse else None
+    with _lib.on_device(q.device):
+        _lib.check(lib.specdec_window_attention_forward(
+            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
+            _lib.ptr(lse), _lib.ptr(ctx_lens), B, T, Hq, Hk, D, n_ctx, window, sinks, scale, _status(q.device),
+            _stream(q)), "specdec_window_attention_forward")
+    return o, lse
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, ctx_lens, n_ctx, window, sinks, scale):
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        o, lse = _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, ctx_lens)
+        ctx.how = n_ctx, window, sinks, scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        lib = _lib.load()
+        q, k, v, o, lse, ctx_lens = ctx.saved_tensors
+        B, T, Hq, D = q.shape
+        Hk = k.shape[2]
+        do = do.contiguous()
+        if do.data_ptr() % 16:
+            do = do.clone()
+        dq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        with _lib.on_device(q.device):
+            ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            _lib.check(lib.specdec_window_attention_backward(
+                q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
+                lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ctx_lens), B, T,
+                Hq, Hk, D, *ctx.how, _status(q.device), ws.data_ptr(), ws_bytes, _stream(q)),
+                "specdec_window_attention_backward")
+        return dq, dk, dv, None, None, None, None, None
+
+
+def window_attention_supported(q: torch.Tensor) -> bool:
+    return ENABLED and q.is_cuda and q.dtype == torch.bfloat16 and q.dim() == 4 and q.shape[-1] in (64, 128)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_ctx: int, *, window: int | None = None,
+                     sinks: int = 0, scale: float | None = None, ctx_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention under the DFlash mask with a sliding window; q bf16
+    [B, T, Hq, D], k and v [B, T, Hk, D] (Hk divides Hq: head h reads key head
+    h // (Hq // Hk); D 64 or 128; any strides) -> o [B, T, Hq, D].
+
+    The first n_ctx rows are context, the others block slots (n_ctx = T: an
+    ordinary causal attention). A context query sees, of the keys up to itself,
+    the last ``window`` (itself included; None: all) and the first ``sinks``;
+    a block query sees every block token, the last ``window`` context tokens and
+    the sinks. ctx_lens int32 [B] (None: all n_ctx): sequence b has only
+    ctx_lens[b] context tokens, in rows 0 .. ctx_lens[b]-1; the rows behind
+    them up to n_ctx are padding, never read, with zero outputs and gradients.
+    Differentiable in q, k, v; scale None = D^-0.5."""
+    window, sinks, scale = _check_window(q, k, v, window, sinks, scale)
+    assert k.shape[1] == q.shape[1], "k and v must have q's length"
+    assert 0 <= n_ctx <= q.shape[1], f"n_ctx must be in [0, T], got {n_ctx}"
+    if ctx_lens is not None:
+        ctx_lens = _check_lens(ctx_lens, q)
+    how = int(n_ctx), window, sinks, scale
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowAttention.apply(q, k, v, ctx_lens, *how)
+    return _window_forward(_rows16(q.detach()), _rows16(k.detach()), _rows16(v.detach()), ctx_lens, *how, False)[0]
+
+
+def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_lens: torch.Tensor, *,
+                            n_block: int = 0, window: int | None = None, sinks: int = 0,
+                            scale: float | None = None) -> torch.Tensor:
+    """``window_attention`` of the last tokens of each sequence against a cache,
+    forward only. k_cache, v_cache bf16 [B, size, Hk, D] hold sequence b's
+    ctx_lens[b] context tokens (int32 [B], at most size - n_block) in rows
+    0, 1, ... and its n_block block tokens right behind them; later rows are
+    never read. q [B, Tq, Hq, D] are the sequence's last Tq tokens, context and
+    block together (Tq = 1, n_block = 0: the next token); a query in front of
+    the first token gives zeros. The cache is read in place: its rows must start
+    on 16-byte boundaries."""
+    window, sinks, scale = _check_window(q, k_cache, v_cache, window, sinks, scale)
+    assert not (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)), \
+        "window_attention_cached has no backward: call it under torch.no_grad()"
+    ctx_lens = _check_lens(ctx_lens, q)
+    lib = _lib.load()
+    B, Tq, Hq, D = q.shape
+    size, Hk = k_cache.shape[1], k_cache.shape[2]
+    assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the cache's heads must be contiguous"
+    assert 0 <= n_block <= size, f"n_block must be in [0, size of the cache], got {n_block}"
+    q = _rows16(q.detach())
+    o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
+    with _lib.on_device(q.device):
+        ws_bytes = lib.specdec_window_attention_cached_workspace_bytes(B, Tq, size, Hq, Hk, D, n_block, window, sinks,
+                                                                       q.device.index)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        _lib.check(lib.specdec_window_attention_cached(
+            q.data_ptr(), _strides(q), k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
+            o.data_ptr(), ctx_lens.data_ptr(), B, Tq, size, Hq, Hk, D, int(n_block), window, sinks, scale,
+            _status(q.device), ws.data_ptr(), ws_bytes, _stream(q)), "specdec_window_attention_cached")
+    return o

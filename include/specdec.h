@@ -398,6 +398,71 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
                                     int32_t interleaved, float scale, float eps, int32_t dtype, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/*
+ * Sliding-window attention with sinks under the DFlash mask, bf16, on the
+ * tensor cores. Sequence b has c = ctx_lens[b] context tokens (clamped to
+ * [0, n_ctx]; NULL: n_ctx) and T - n_ctx block tokens: rows 0 .. c-1 of its T
+ * rows, and rows n_ctx .. T-1. A context query sees the keys up to itself
+ * that are among the last `window` (itself included) or the first `sinks`
+ * tokens; a block query sees every block token, the last `window` context
+ * tokens and the sinks. Rows c .. n_ctx-1 are padding: never read (they may
+ * hold anything), their outputs and gradients are zero.
+ *   q, o          [batch, T, q_heads, head_dim], k, v [batch, T, k_heads,
+ *                 head_dim] bf16 patterns; head h of q reads head
+ *                 h / (q_heads / k_heads) of k and v; head_dim 64 or 128;
+ *                 q, k, v strided (rows on 16-byte boundaries), o contiguous
+ *   lse           [batch, k_heads, T, q_heads / k_heads] fp32, natural log
+ *                 (-inf for padding), for the backward; or NULL
+ *   window >= 1   (INT32_MAX: no window); sinks >= 0
+ *   status        as in specdec_dflash_attention_forward
+ * A row's probabilities are rounded to bf16 before the second product, all
+ * sums are fp32. A NaN or infinity in v of a token of the sequence may reach
+ * queries whose mask excludes that token (as 0 * inf does in a masked dense
+ * product); masked scores may hold anything.
+ */
+int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
+                                     const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
+                                     uint16_t* o, float* lse, const int32_t* ctx_lens, int32_t batch, int32_t T,
+                                     int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx, int32_t window,
+                                     int32_t sinks, float scale, int32_t* status, void* stream);
+
+/* Workspace bytes of specdec_window_attention_backward. */
+size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads);
+
+/*
+ * Its backward: dq, dk, dv (contiguous, shaped as q, k, v) from q, k, v, the
+ * forward's o and lse, and dout (contiguous). dk and dv are sums over the
+ * query heads that share a key head. Fixed summation order, no atomics.
+ */
+int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
+                                      const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
+                                      const uint16_t* o, const float* lse, const uint16_t* dout, uint16_t* dq,
+                                      uint16_t* dk, uint16_t* dv, const int32_t* ctx_lens, int32_t batch, int32_t T,
+                                      int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx,
+                                      int32_t window, int32_t sinks, float scale, int32_t* status, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of specdec_window_attention_cached on `device`. */
+size_t specdec_window_attention_cached_workspace_bytes(int32_t batch, int32_t q_len, int32_t cache_len,
+                                                       int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                                       int32_t n_block, int32_t window, int32_t sinks, int device);
+
+/*
+ * The same attention from a cache, forward only: k_cache, v_cache [batch,
+ * cache_len, k_heads, head_dim] hold sequence b's ctx_lens[b] context tokens
+ * (clamped to [0, cache_len - n_block]) in rows 0, 1, ... and its n_block block
+ * tokens right behind them; later rows are never read. q [batch, q_len, ...]
+ * are the sequence's last q_len tokens (context and block together); queries
+ * in front of the first token see nothing and give zeros. workspace needs no
+ * initialisation; calls that may run at the same time must not share it.
+ */
+int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides, const uint16_t* k_cache,
+                                    const int64_t* k_strides, const uint16_t* v_cache, const int64_t* v_strides,
+                                    uint16_t* o, const int32_t* ctx_lens, int32_t batch, int32_t q_len,
+                                    int32_t cache_len, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                    int32_t n_block, int32_t window, int32_t sinks, float scale, int32_t* status,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------- */
 /* Launch tuning                                                              */
 /* ------------------------------------------------------------------------- */

@@ -1,0 +1,328 @@
+"""Sliding-window attention with sinks (specdec.drafter.window_attention and
+window_attention_cached) against the definition in float64, from the same bf16
+inputs.
+
+Tolerances, per element (h = 2^-8, half a step of bf16):
+- o: each weight is rounded once (h), the sums are fp32, the result is rounded
+  once (h): |error| <= h sum_j P_j |v_j| + h |o| + 1e-5.
+- dv = P^T do: likewise with sum P |do|.
+- dS = P (dP - delta) scale: P itself is exact to fp32 here, dP to fp32; delta
+  uses the rounded o: at most h sum_d |do_d o_d| off, and the o above is itself
+  h sum P |v| off. dS is rounded once. So each dS element is off by
+  E = h |dS| + scale P h sum_d |do_d| (sum_j P_j |v_jd| + |o_d|), and
+  dq is off by sum_j E |k_j| + h |dq|, dk by sum_i E |q_i| + h |dk|.
+fp32 accumulation of a few thousand terms and exp2's 2^-22 are covered by a
+factor of 1.02 and 1e-5.
+"""
+import math
+
+import pytest
+import torch
+
+from specdec import drafter
+
+H = 2.0 ** -8
+
+
+def _tokens(T, n_ctx, c):
+    """Token of every row of a training batch's sequence, -1 for padding."""
+    r = torch.arange(T)
+    t = torch.where(r < n_ctx, torch.where(r < c, r, -1), c + r - n_ctx)
+    return t
+
+
+def _visible(pq, pk, c, W, S):
+    """[queries, keys] from tokens (-1: padding)."""
+    p, j = pq[:, None], pk[None]
+    ctx = (j <= p) & ((p - j < W) | (j < S))
+    blk = (j >= c) | (c - j <= W) | (j < S)
+    return torch.where(p < c, ctx, blk) & (p >= 0) & (j >= 0)
+
+
+def _oracle(q, k, v, vis, do=None, scale=None):
+    """One sequence, fp64 on the CPU: q [Tq, Hq, D], k, v [Tk, Hk, D], vis
+    [Tq, Tk]. Returns {name: (value, bound)}; rows and keys that are in no
+    visible pair are left out of the arithmetic."""
+    Hq, Hk, D = q.shape[1], k.shape[1], q.shape[2]
+    G = Hq // Hk
+    scale = D ** -0.5 if scale is None else scale
+    used = vis.any(0)
+    rows = vis.any(1)
+    z = lambda t, m: torch.where(m[:, None, None], t.double().cpu(), 0.0)  # noqa: E731
+    q, k, v = z(q, rows), z(k, used), z(v, used)
+    qg = q.view(-1, Hk, G, D)
+    s = torch.einsum("thgd,jhd->hgtj", qg, k) * scale
+    s = s.masked_fill(~vis, -math.inf)
+    p = torch.exp(s - torch.logsumexp(s, -1, keepdim=True)).masked_fill(~vis, 0.0)
+    o = torch.einsum("hgtj,jhd->thgd", p, v)
+    oe = torch.einsum("hgtj,jhd->thgd", p, v.abs())
+    out = {"o": (o.reshape(-1, Hq, D), (H * oe + H * o.abs()).reshape(-1, Hq, D))}
+    if do is None:
+        return out
+    do = z(do, rows).view(-1, Hk, G, D)
+    dv = torch.einsum("hgtj,thgd->jhd", p, do)
+    dve = H * torch.einsum("hgtj,thgd->jhd", p, do.abs()) + H * dv.abs()
+    dp = torch.einsum("thgd,jhd->hgtj", do, v)
+    delta = (do * o).sum(-1).permute(1, 2, 0)[..., None]
+    ds = p * (dp - delta) * scale
+    off = H * (do.abs() * (oe + o.abs())).sum(-1).permute(1, 2, 0)[..., None]
+    e = H * ds.abs() + scale * p * off
+    dq = torch.einsum("hgtj,jhd->thgd", ds, k)
+    dqe = torch.einsum("hgtj,jhd->thgd", e, k.abs()) + H * dq.abs()
+    dk = torch.einsum("hgtj,thgd->jhd", ds, qg)
+    dke = torch.einsum("hgtj,thgd->jhd", e, qg.abs()) + H * dk.abs()
+    return {**out, "dq": (dq.reshape(-1, Hq, D), dqe.reshape(-1, Hq, D)), "dk": (dk, dke), "dv": (dv, dve)}
+
+
+def _near(name, got, want):
+    value, bound = want
+    err = (got.double().cpu() - value).abs()
+    assert bool(torch.isfinite(got.float()).all()), name
+    worst = (err - 1.02 * bound - 1e-5).max() if err.numel() else torch.tensor(0.0)
+    assert float(worst) <= 0.0, (name, float(err.max()), float(worst))
+
+
+def _rand(*shape, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(*shape, device="cuda", generator=g)).to(torch.bfloat16)
+
+
+CASES = [  # B, n_ctx, n_block, Hq, Hk, D, W, S, lens
+    (1, 1, 0, 1, 1, 64, 1, 0, None), (1, 0, 1, 1, 1, 128, 1, 0, None), (2, 0, 16, 4, 2, 64, 5, 3, None),
+    (2, 100, 0, 2, 2, 64, 30, 0, None), (2, 300, 16, 4, 4, 64, 64, 4, None), (1, 513, 7, 2, 1, 128, 100, 1, None),
+    (1, 700, 16, 6, 2, 128, 129, 70, None), (2, 257, 3, 3, 1, 64, 1, 1, None), (1, 640, 16, 5, 1, 64, 1000, 0, None),
+    (4, 200, 9, 4, 2, 64, 40, 2, (0, 1, 200, 130)), (3, 333, 0, 2, 1, 128, 64, 5, (0, 333, 65)),
+    (2, 128, 128, 2, 2, 128, 128, 64, (64, 128)), (1, 1500, 16, 1, 1, 64, 700, 200, None),
+    (1, 400, 16, 130, 1, 64, 50, 4, None), (2, 90, 5, 7, 7, 64, None, 0, (17, 90)), (1, 1100, 33, 8, 2, 128, 256, 4, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n_ctx,nb,Hq,Hk,D,W,S,lens", CASES)
+def test_window_attention_forward_backward(cuda, B, n_ctx, nb, Hq, Hk, D, W, S, lens):
+    T = n_ctx + nb
+    seed = n_ctx + 10 * Hq + D
+    q, do = _rand(B, T, Hq, D, seed=seed), _rand(B, T, Hq, D, seed=seed + 1)
+    k, v = _rand(B, T, Hk, D, seed=seed + 2), _rand(B, T, Hk, D, seed=seed + 3)
+    ctx_lens = None if lens is None else torch.tensor(lens, device="cuda", dtype=torch.int32)
+    cs = [n_ctx] * B if lens is None else lens
+    pads = torch.zeros(B, T, dtype=torch.bool, device="cuda")
+    for b, c in enumerate(cs):
+        pads[b, c:n_ctx] = True
+    for t in (q, k, v, do):  # padding may hold anything
+        t[pads] = float("nan")
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    o = drafter.window_attention(q, k, v, n_ctx, window=W, sinks=S, ctx_lens=ctx_lens)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    got = dict(o=o.detach(), dq=grads[0], dk=grads[1], dv=grads[2])
+    for b, c in enumerate(cs):
+        tok = _tokens(T, n_ctx, c)
+        vis = _visible(tok, tok, c, W or 10 ** 9, S)
+        want = _oracle(q[b].detach(), k[b].detach(), v[b].detach(), vis, do[b])
+        for n, t in got.items():
+            _near(n, t[b], want[n])
+            assert bool((t[b][pads[b]] == 0).all()), n  # padding: zero outputs and gradients
+    with torch.no_grad():
+        assert torch.equal(drafter.window_attention(q, k, v, n_ctx, window=W, sinks=S, ctx_lens=ctx_lens), o)
+    o2 = drafter.window_attention(q, k, v, n_ctx, window=W, sinks=S, ctx_lens=ctx_lens)
+    for a, c in zip(grads, torch.autograd.grad(o2, (q, k, v), do)):  # fixed summation order
+        assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_without_window_it_is_the_dflash_attention(cuda):
+    """window None, no sinks: the mask of dflash_attention; the two kernels
+    round the same quantities, in tiles of their own."""
+    q, k, v = (_rand(2, 528, 4, 64, seed=i) for i in range(3))
+    a = drafter.window_attention(q, k, v, 512)
+    b = drafter.dflash_attention(q, k, v, 512)
+    assert float((a.float() - b.float()).abs().max()) <= 1e-2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_layouts(cuda, D):
+    """Views of one fused projection, heads-first tensors, rows off 16-byte
+    boundaries and an expanded output gradient give the contiguous results."""
+    B, T, Hq, Hk, n_ctx = 2, 150, 4, 2, 140
+    qkv = _rand(B, T, (Hq + 2 * Hk) * D, seed=3)
+    views = [t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hk * D, Hk * D], -1)]
+    first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in views]
+    odd = []
+    for t in views:
+        u = torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)[1:].view(t.shape)
+        odd.append(u.copy_(t))
+    want = None
+    for how in (views, [t.contiguous() for t in views], first, odd, [t.unsqueeze(-1).expand(*t.shape, 2)[..., 0] for t in views]):
+        x = [t.detach().requires_grad_(True) for t in how]
+        o = drafter.window_attention(*x, n_ctx, window=33, sinks=2)
+        got = [o.detach(), *torch.autograd.grad(o.float().sum(), x)]
+        want = got if want is None else want
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_rescale_path(cuda, D):
+    """Scores that grow along the keys: a row's reference maximum is raised
+    many times and O rescaled in tensor memory."""
+    T, n_ctx = 400, 390
+    q, do = _rand(1, T, 2, D, seed=1), _rand(1, T, 2, D, seed=2)
+    k, v = _rand(1, T, 1, D, seed=3), _rand(1, T, 1, D, seed=4)
+    k = (k.float() * (1 + torch.arange(T, device="cuda") / 8.0)[None, :, None, None]).to(torch.bfloat16)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = drafter.window_attention(*x, n_ctx, window=300, sinks=8)
+    grads = torch.autograd.grad(o, x, do)
+    tok = _tokens(T, n_ctx, n_ctx)
+    want = _oracle(q[0].detach(), k[0].detach(), v[0].detach(), _visible(tok, tok, n_ctx, 300, 8), do[0])
+    # scores reach a few hundred: the fp32 exponent s log2 e is off by up to 2^-24 |s| log2 e
+    # ~ 5e-5 relative in p, below the 1e-4 added here to every relative rounding h
+    for n, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        value, bound = want[n]
+        _near(n, t[0].detach(), (value, bound * (1 + 1e-4 / H)))
+
+
+@pytest.mark.gpu
+def test_window_attention_gradient_against_differences(cuda):
+    """Central differences of the fp64 definition along random directions."""
+    T, n_ctx, D = 60, 50, 64
+    q, do = _rand(1, T, 4, D, seed=1), _rand(1, T, 4, D, seed=2)
+    k, v = _rand(1, T, 2, D, seed=3), _rand(1, T, 2, D, seed=4)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(drafter.window_attention(*x, n_ctx, window=20, sinks=3), x, do)
+    tok = _tokens(T, n_ctx, n_ctx)
+    vis = _visible(tok, tok, n_ctx, 20, 3)
+    x64 = [t.detach()[0].double().cpu() for t in x]
+    for i in range(3):
+        d = torch.randn(x64[i].shape, dtype=torch.float64, generator=torch.Generator().manual_seed(i))
+        def loss(e):
+            y = [t + e * d if n == i else t for n, t in enumerate(x64)]
+            return float((_oracle(*y, vis)["o"][0] * do[0].double().cpu()).sum())
+        want = (loss(1e-4) - loss(-1e-4)) / 2e-4
+        got = float((grads[i][0].double().cpu() * d).sum())
+        size = float(grads[i].double().norm()) * float(d.norm())
+        assert abs(got - want) <= 2 * H * size, (i, got, want)
+
+
+CACHED = [  # B, Tq, nb, Hq, Hk, D, size, W, S, lens
+    (1, 1, 0, 1, 1, 64, 1, 1, 0, (1,)), (3, 1, 0, 4, 4, 64, 200, 50, 4, (1, 200, 77)), (2, 1, 0, 8, 2, 128, 900, 300, 4, (900, 0)),
+    (2, 16, 16, 4, 4, 64, 600, 100, 4, (584, 30)), (2, 20, 16, 8, 2, 128, 700, 256, 1, (300, 2)),
+    (1, 5, 4, 32, 1, 64, 3000, 2500, 4, (2996,)), (2, 300, 16, 2, 1, 128, 700, 90, 3, (600, 100)),
+    (4, 3, 0, 3, 1, 64, 130, None, 0, (0, 1, 2, 130)), (1, 1, 1, 16, 1, 128, 5000, 5000, 0, (4999,)),
+    (2, 2, 5, 6, 3, 64, 300, 64, 70, (295, 0)), (40, 1, 0, 8, 8, 128, 300, 200, 4, None), (1, 33, 0, 4, 4, 64, 64, 7, 2, (64,)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Tq,nb,Hq,Hk,D,size,W,S,lens", CACHED)
+def test_window_attention_cached(cuda, B, Tq, nb, Hq, Hk, D, size, W, S, lens):
+    if lens is None:
+        lens = [(37 * b) % (size - nb + 1) for b in range(B)]
+    q = _rand(B, Tq, Hq, D, seed=size + Tq)
+    k, v = _rand(B, size, Hk, D, seed=size + 1), _rand(B, size, Hk, D, seed=size + 2)
+    for b, c in enumerate(lens):  # rows behind the last token may hold anything
+        k[b, c + nb:] = float("nan")
+        v[b, c + nb:] = float("inf")
+    kept = k.clone(), v.clone()
+    ctx = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    o = drafter.window_attention_cached(q, k, v, ctx, n_block=nb, window=W, sinks=S)
+    for b, c in enumerate(lens):
+        pq = c + nb - Tq + torch.arange(Tq)
+        pk = torch.arange(size)
+        pk = torch.where(pk < c + nb, pk, -1)
+        vis = _visible(pq, pk, c, W or 10 ** 9, S)
+        _near("o", o[b], _oracle(q[b], k[b], v[b], vis)["o"])
+    assert torch.equal(o, drafter.window_attention_cached(q, k, v, ctx.long(), n_block=nb, window=W, sinks=S))
+    for a, b in zip(kept, (k, v)):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    # the cache as a slice of a larger one, heads first
+    big = [torch.full((B, Hk, size + 3, D), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    for t, src in zip(big, (k, v)):
+        t[:, :, 2:size + 2] = src.transpose(1, 2)
+    views = [t[:, :, 2:size + 2].transpose(1, 2) for t in big]
+    assert torch.equal(o, drafter.window_attention_cached(q, *views, ctx, n_block=nb, window=W, sinks=S))
+
+
+@pytest.mark.gpu
+def test_cached_lengths_out_of_range_are_clamped(cuda):
+    q, k, v = _rand(3, 2, 2, 64, seed=1), _rand(3, 50, 2, 64, seed=2), _rand(3, 50, 2, 64, seed=3)
+    bad = torch.tensor([-5, 1000, 2 ** 31 - 1], device="cuda", dtype=torch.int32)
+    good = torch.tensor([0, 46, 46], device="cuda", dtype=torch.int32)
+    a = drafter.window_attention_cached(q, k, v, bad, n_block=4, window=16)
+    assert torch.equal(a, drafter.window_attention_cached(q, k, v, good, n_block=4, window=16))
+    x = _rand(3, 20, 2, 64, seed=4)
+    lens = torch.tensor([-1, 99, 7], device="cuda", dtype=torch.int32)
+    a = drafter.window_attention(x, x, x, 16, window=4, ctx_lens=lens)
+    assert torch.equal(a, drafter.window_attention(x, x, x, 16, window=4, ctx_lens=lens.clamp(0, 16)))
+
+
+def test_window_refuses_cpu_tensors():
+    x = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError):
+        drafter.window_attention(x, x, x, 4)
+    with pytest.raises(AssertionError):
+        drafter.window_attention_cached(x, x, x, torch.zeros(1, dtype=torch.int32))
+
+
+def test_window_c_argument_checks():
+    import ctypes
+
+    from specdec import _lib
+
+    lib = _lib.load()
+    p = ctypes.c_void_p(256)  # never dereferenced: the checks fail first
+
+    def fwd(q=p, B=1, T=8, Hq=2, Hk=1, D=64, n_ctx=4, W=4, S=0, scale=0.125):
+        return lib.specdec_window_attention_forward(q, None, p, None, p, None, p, p, None, B, T, Hq, Hk, D, n_ctx, W, S,
+                                                    scale, None, None)
+
+    def bwd(B=1, T=8, Hq=2, Hk=1, D=64, n_ctx=4, W=4, S=0, scale=0.125, ws=1 << 20):
+        return lib.specdec_window_attention_backward(p, None, p, None, p, None, p, p, p, p, p, p, None, B, T, Hq, Hk, D,
+                                                     n_ctx, W, S, scale, None, p, ws, None)
+
+    def cached(B=1, T=1, size=8, Hq=2, Hk=1, D=64, nb=0, W=4, S=0, scale=0.125, lens=p):
+        return lib.specdec_window_attention_cached(p, None, p, None, p, None, p, lens, B, T, size, Hq, Hk, D, nb, W, S,
+                                                   scale, None, p, 1 << 30, None)
+
+    for fn in (fwd, bwd, cached):
+        for bad in (dict(D=32), dict(D=96), dict(Hq=3, Hk=2), dict(Hk=0), dict(Hq=0), dict(B=-1), dict(T=-1), dict(W=0),
+                    dict(W=-3), dict(S=-1)):
+            assert fn(**bad) == _lib.ERR_ARGUMENT, (fn, bad)
+        for bad in (0.0, -1.0, float("nan"), float("inf")):
+            assert fn(scale=bad) == _lib.ERR_VALUE
+        assert fn(B=0) == _lib.OK
+    for fn in (fwd, bwd):
+        assert fn(n_ctx=9) == _lib.ERR_ARGUMENT and fn(n_ctx=-1) == _lib.ERR_ARGUMENT
+        assert fn(T=2 ** 29, Hq=8, Hk=1, n_ctx=0) == _lib.ERR_ARGUMENT
+    assert bwd(ws=16) == _lib.ERR_WORKSPACE
+    assert fwd(q=ctypes.c_void_p(258)) == _lib.ERR_ARGUMENT  # not on a 16-byte boundary
+    assert cached(nb=9) == _lib.ERR_ARGUMENT and cached(nb=-1) == _lib.ERR_ARGUMENT
+    assert cached(lens=None) == _lib.ERR_ARGUMENT
+
+
+@pytest.mark.gpu
+def test_window_refusals(cuda):
+    x = torch.zeros(2, 8, 4, 64, device="cuda", dtype=torch.bfloat16)
+    lens = torch.zeros(2, device="cuda", dtype=torch.int32)
+    for kw in (dict(window=0), dict(sinks=-1), dict(ctx_lens=lens[:1]), dict(ctx_lens=lens.cpu()), dict(ctx_lens=lens.float())):
+        with pytest.raises(AssertionError):
+            drafter.window_attention(x, x, x, 4, **kw)
+    for args in ((x.float(), x.float(), x.float(), 4), (x, x[:, :, :3], x[:, :, :3], 4), (x, x, x, 9), (x, x, x, -1),
+                 (x, x, x[:, :7], 4), (x, x[:, :7], x[:, :7], 4), (x[..., :32], x[..., :32], x[..., :32], 4), (x[0], x[0], x[0], 4)):
+        with pytest.raises(AssertionError):
+            drafter.window_attention(*args)
+    with pytest.raises(ValueError):
+        drafter.window_attention(x, x, x, 4, scale=0.0)
+    with pytest.raises(AssertionError):
+        drafter.window_attention_cached(x, x, x, lens, n_block=9)
+    with pytest.raises(AssertionError):
+        drafter.window_attention_cached(x, x[..., ::1].transpose(2, 3).contiguous().transpose(2, 3), x, lens)
+    odd = torch.zeros(2 * 8 * 4 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(2, 8, 4, 64)
+    with pytest.raises(AssertionError):  # a cache off 16-byte boundaries is refused, never copied
+        drafter.window_attention_cached(x, odd, odd, lens)
+    with pytest.raises(AssertionError):
+        drafter.window_attention_cached(x.clone().requires_grad_(True), x, x, lens)
+    e = drafter.window_attention(x[:, :0], x[:, :0], x[:, :0], 0)
+    assert e.shape == (2, 0, 4, 64)

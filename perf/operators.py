@@ -19,6 +19,9 @@ _DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
 
 
 def _drafter():
+    loaded = sys.modules.get("specdec.drafter")
+    if loaded is not None:
+        return loaded
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cuda-spec-decode_b200")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)

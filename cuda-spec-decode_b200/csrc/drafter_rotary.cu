@@ -23,8 +23,13 @@
 // shuffle; the norm's sums are butterflies over the head's threads. Sizes or
 // strides that 16-byte vectors do not fit take the same code with one-element
 // vectors and a warp per head.
-// dw is summed in registers per thread, per CTA through shared memory in warp
-// order, and over CTAs by a second kernel: fixed orders, bitwise repeatable.
+// Warps work alone, without a block barrier: a unit is one token's heads of
+// one tensor (or, with few heads, as many tokens as fill the warp), its first
+// loads are in flight while the warp builds its table. A CTA serves one of
+// the two tensors, so the weights and their gradients stay in registers.
+// dw is summed per thread over the units in order, per CTA through shared
+// memory in warp order, and over CTAs by a second kernel: fixed orders,
+// bitwise repeatable.
 #include <algorithm>
 
 #include "specdec_common.cuh"
@@ -36,29 +41,38 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
-constexpr int kTableFloats = 4096;  // cos / sin table of a CTA's tokens: at most 16 KB
+constexpr int kTableFloats = 512;  // a warp's table: at most 32 / lanes * 32 pairs' cos, or the R of one token
 
-// V consecutive elements as fp32 (V = 1, or one 16-byte vector).
-template <int V>
-__device__ __forceinline__ void ld(const float* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = *p;
-  } else {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  }
+// V consecutive elements of a row, as loaded: one element, or a 16-byte vector.
+template <class T, int V>
+struct Raw {
+  uint4 q;
+};
+template <class T>
+struct Raw<T, 1> {
+  T q;
+};
+template <class T, int V>
+__device__ __forceinline__ void fetch(const T* p, Raw<T, V>& r) {
+  if constexpr (V == 1)
+    r.q = *p;
+  else
+    r.q = *reinterpret_cast<const uint4*>(p);
 }
-template <int V>
-__device__ __forceinline__ void ld(const bf16_t* p, float (&v)[V]) {
+template <class T, int V>
+__device__ __forceinline__ void widen(const Raw<T, V>& r, float (&v)[V]) {
   if constexpr (V == 1) {
-    v[0] = to_f32(*p);
+    v[0] = to_f32(r.q);
   } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const uint32_t w[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = bf16_lo(w[i]);
-      v[2 * i + 1] = bf16_hi(w[i]);
+      if constexpr (V == 4) {
+        v[i] = __uint_as_float(w[i]);
+      } else {
+        v[2 * i] = bf16_lo(w[i]);
+        v[2 * i + 1] = bf16_hi(w[i]);
+      }
     }
   }
 }
@@ -134,79 +148,135 @@ __device__ __forceinline__ bool slot_place(const RotaryArgs& A, int slot, int& e
   return false;
 }
 
-// The tile's table: cos and sin (times scale) of every token and pair, and
-// the tokens' element offsets in the four tensors.
-__device__ __forceinline__ void build_table(const RotaryArgs& A, int64_t n0, int toks, float* cs, float* sn) {
-  const int half = A.R / 2;
-  for (int i = threadIdx.x; i < toks * half; i += kRotThreads) {
-    const int tok = i / half, f = i - tok * half;
-    const int64_t n = n0 + tok;
-    const int64_t b = n / A.T, t = n - b * A.T;
-    const double turns = (double)A.positions[b * A.pos_stride + t] * A.inv_freq[f] * 0.15915494309189533577;
+// One warp's share of a tensor: the side's units, and this lane's place in one.
+struct Place {
+  int side, H, groups_per_token;
+  int group, sub;      // head group of the lane, lane within it
+  int tw;              // tokens per unit
+  int64_t unit, step, units;
+};
+
+__device__ __forceinline__ Place place_of(const RotaryArgs& A) {
+  Place p;
+  const int lane = threadIdx.x & 31;
+  p.side = (int)blockIdx.x >= A.ctas[0] ? 1 : 0;
+  p.H = A.heads[p.side];
+  const int hpw = 32 >> A.lg;
+  p.group = lane >> A.lg;
+  p.sub = lane & ((1 << A.lg) - 1);
+  p.tw = p.H < hpw ? hpw / p.H : 1;
+  p.step = (int64_t)A.ctas[p.side] * kRotWarps;
+  p.unit = ((int64_t)blockIdx.x - (p.side ? A.ctas[0] : 0)) * kRotWarps + (threadIdx.x >> 5);
+  p.units = (A.N + p.tw - 1) / p.tw * A.nchunk[p.side];
+  return p;
+}
+
+// What this lane touches in a unit: token n (or none) and its heads h, h + hpw, ... < hend.
+struct Unit {
+  int64_t n0, b, t;  // first token; the lane's token as (sequence, row)
+  int h, hend, tok;  // tok: the lane's token within the unit
+};
+
+__device__ __forceinline__ Unit unit_of(const RotaryArgs& A, const Place& p, int64_t u) {
+  Unit r;
+  const int nch = A.nchunk[p.side];
+  const int64_t tile = nch == 1 ? u : u / nch;
+  r.n0 = tile * p.tw;
+  if (p.tw == 1) {
+    const int ch = (int)(u - tile * nch);
+    r.tok = 0;
+    r.h = ch * A.hchunk[p.side] + p.group;
+    r.hend = min(p.H, (ch + 1) * A.hchunk[p.side]);
+  } else {
+    r.tok = p.group / p.H;
+    r.h = p.group - r.tok * p.H;
+    r.hend = r.tok < p.tw && r.n0 + r.tok < A.N ? r.h + 1 : 0;
+  }
+  const uint32_t n = (uint32_t)(r.n0 + r.tok);  // N fits in int32
+  const uint32_t b = n / (uint32_t)A.T;
+  r.b = b;
+  r.t = n - b * (uint32_t)A.T;
+  return r;
+}
+
+// cos and sin (times scale) of the unit's tokens and pairs, by the whole warp.
+__device__ __forceinline__ void build_table(const RotaryArgs& A, const Place& p, int64_t n0, float* cs, float* sn) {
+  const int half = A.R / 2, toks = (int)min((int64_t)p.tw, A.N - n0);
+  __syncwarp();  // the previous unit's table has been read
+  for (int i = threadIdx.x & 31; i < toks * half; i += 32) {
+    const int tok = p.tw == 1 ? 0 : i / half, f = i - tok * half;
+    const uint32_t n = (uint32_t)(n0 + tok), b = n / (uint32_t)A.T, t = n - b * (uint32_t)A.T;
+    const double turns = (double)A.positions[(int64_t)b * A.pos_stride + t] * A.inv_freq[f] * 0.15915494309189533577;
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = c * A.scale;
     sn[i] = s * A.sin_scale;
   }
+  __syncwarp();
 }
 
 template <class T>
-__device__ __forceinline__ const T* head_ptr(const RotaryTensor& t, int64_t b, int64_t tk, int h) {
-  return static_cast<const T*>(t.p) + b * t.s[0] + tk * t.s[1] + (int64_t)h * t.s[2];
+__device__ __forceinline__ T* head_ptr(const RotaryTensor& t, const Unit& u, int h) {
+  return const_cast<T*>(static_cast<const T*>(t.p)) + u.b * t.s[0] + u.t * t.s[1] + (int64_t)h * t.s[2];
 }
 
-// A unit of work is one token and a run of `hchunk` heads, one warp per unit;
-// the warp's 2^lg-lane groups take one head each.
 template <class T, int V, int K, bool NORM, bool INTER>
-__global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const RotaryArgs A) {
-  extern __shared__ __align__(16) float sh[];
-  float* cs = sh;
-  float* sn = cs + A.TT * (A.R / 2);
-  float* wsh = sn + A.TT * (A.R / 2);  // [2][D] weights, 16-byte aligned (R / 2 is a multiple of 4 when V > 1)
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t n0 = (int64_t)blockIdx.x * A.TT;
-  const int toks = (int)min((int64_t)A.TT, A.N - n0);
-  if constexpr (NORM)
-    for (int i = threadIdx.x; i < 2 * A.D; i += kRotThreads) wsh[i] = i < A.D ? A.w[0][i] : A.w[1][i - A.D];
-  build_table(A, n0, toks, cs, sn);
-  __syncthreads();
-  const int lanes = 1 << A.lg, group = lane >> A.lg, sub = lane & (lanes - 1);
+__global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const __grid_constant__ RotaryArgs A) {
+  __shared__ __align__(16) float table[kRotWarps][kTableFloats];
+  float* cs = table[threadIdx.x >> 5];
+  const Place P = place_of(A);
+  float* sn = cs + P.tw * (A.R / 2);
   const int hpw = 32 >> A.lg, slots = A.D / (2 * V);
-  const int units = toks * A.nchunk;
-  for (int u = warp; u < units; u += kRotWarps) {
-    const int tok = u / A.nchunk, ch = u - tok * A.nchunk;
-    const int64_t n = n0 + tok, b = n / A.T, tk = n - b * A.T;
-    float c[K][V], s[K][V];
-    int ea[K], eb[K];
-    bool live[K], rot[K];
+  int ea[K], eb[K];
+  bool live[K], rot[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int slot = sub + k * 32;
-      live[k] = slot < slots;
-      rot[k] = slot_place<V>(A, slot, ea[k], eb[k]) && live[k];
-      if (rot[k]) {
-        ld_sh<V>(cs + tok * (A.R / 2) + slot * V, c[k]);
-        ld_sh<V>(sn + tok * (A.R / 2) + slot * V, s[k]);
+  for (int k = 0; k < K; ++k) {
+    const int slot = P.sub + k * 32;
+    live[k] = slot < slots;
+    rot[k] = slot_place<V>(A, slot, ea[k], eb[k]) && live[k];
+  }
+  float wa[K][V], wb[K][V];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        wa[k][j] = live[k] ? A.w[P.side][ea[k] + j] : 0.f;
+        wb[k][j] = live[k] ? A.w[P.side][eb[k] + j] : 0.f;
       }
-    }
-    const int hend = min(A.H, (ch + 1) * A.hchunk);
-    for (int h0 = ch * A.hchunk; h0 < hend; h0 += hpw) {
-      const int h = h0 + group;
-      const bool on = h < hend;
-      const int side = h >= A.heads[0] ? 1 : 0, hs = h - (side ? A.heads[0] : 0);
+  }
+  for (int64_t u = P.unit; u < P.units; u += P.step) {
+    const Unit U = unit_of(A, P, u);
+    Raw<T, V> ra[K], rb[K];
+    auto load = [&](int h) {
+      if (h < U.hend) {
+        const T* p = head_ptr<T>(A.x[P.side], U, h);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (live[k]) {
+            fetch<T, V>(p + ea[k], ra[k]);
+            fetch<T, V>(p + eb[k], rb[k]);
+          }
+      }
+    };
+    load(U.h);
+    build_table(A, P, U.n0, cs, sn);
+    const int hlast = P.tw == 1 ? U.hend : 1;  // uniform over the warp
+    for (int i = P.tw == 1 ? U.h - P.group : 0, h = U.h; i < hlast; i += hpw, h += hpw) {
       float x[K][V], y[K][V];
+      const bool on = h < U.hend;
       float ss = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (on && live[k]) {
-          const T* p = head_ptr<T>(A.x[side], b, tk, hs);
-          ld<V>(p + ea[k], x[k]);
-          ld<V>(p + eb[k], y[k]);
+          widen<T, V>(ra[k], x[k]);
+          widen<T, V>(rb[k], y[k]);
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) x[k][j] = y[k][j] = 0.f;
         }
       }
+      load(h + hpw);  // in flight while this group is worked on
       if constexpr (NORM) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -214,190 +284,181 @@ __global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const RotaryArg
           for (int j = 0; j < V; ++j) ss = fmaf(x[k][j], x[k][j], fmaf(y[k][j], y[k][j], ss));
         ss = head_sum(ss, A.lg);
       }
-      if (!on) continue;
-      T* q = const_cast<T*>(head_ptr<T>(A.y[side], b, tk, hs));
-      const float r = NORM ? rsqrtf(ss / (float)A.D + A.eps) : 1.f;
+      if (on) {
+        T* q = head_ptr<T>(A.y[P.side], U, h);
+        const float r = NORM ? rsqrtf(ss / (float)A.D + A.eps) : 1.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!live[k]) continue;
-        if constexpr (NORM) {
-          float wa[V], wb[V];
-          ld_sh<V>(wsh + side * A.D + ea[k], wa);
-          ld_sh<V>(wsh + side * A.D + eb[k], wb);
+        for (int k = 0; k < K; ++k) {
+          if (!live[k]) continue;
+          if constexpr (NORM) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            x[k][j] *= r * wa[j];
-            y[k][j] *= r * wb[j];
+            for (int j = 0; j < V; ++j) {
+              x[k][j] *= r * wa[k][j];
+              y[k][j] *= r * wb[k][j];
+            }
           }
+          if (rot[k]) {
+            float c[V], s[V];
+            const int at = U.tok * (A.R / 2) + (P.sub + k * 32) * V;
+            ld_sh<V>(cs + at, c);
+            ld_sh<V>(sn + at, s);
+            turn<V, INTER>(x[k], y[k], c, s);
+          }
+          st<V>(q + ea[k], x[k]);
+          st<V>(q + eb[k], y[k]);
         }
-        if (rot[k]) turn<V, INTER>(x[k], y[k], c[k], s[k]);
-        st<V>(q + ea[k], x[k]);
-        st<V>(q + eb[k], y[k]);
       }
     }
   }
 }
 
-// Backward of norm + rotation. The tiles are walked by a fixed grid; each
-// thread sums the weight gradients of its slots over all it sees.
+// Backward of norm + rotation: dx, and the CTA's partial weight gradient.
 template <class T, int V, int K, bool INTER>
-__global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const RotaryArgs A, float* __restrict__ part) {
-  extern __shared__ __align__(16) float sh[];
-  float* cs = sh;
-  float* sn = cs + A.TT * (A.R / 2);
-  float* wsh = sn + A.TT * (A.R / 2);  // [2][D]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int lanes = 1 << A.lg, group = lane >> A.lg, sub = lane & (lanes - 1);
+__global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_constant__ RotaryArgs A,
+                                                                  float* __restrict__ part) {
+  __shared__ __align__(16) float table[kRotWarps][kTableFloats];
+  float* cs = table[threadIdx.x >> 5];
+  const Place P = place_of(A);
+  float* sn = cs + P.tw * (A.R / 2);
   const int hpw = 32 >> A.lg, slots = A.D / (2 * V);
-  for (int i = threadIdx.x; i < 2 * A.D; i += kRotThreads) wsh[i] = i < A.D ? A.w[0][i] : A.w[1][i - A.D];
-  float acc[2][2][K][V];  // side, vector of the slot
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[i][e][k][j] = 0.f;
   int ea[K], eb[K];
   bool live[K], rot[K];
+  float wa[K][V], wb[K][V], acca[K][V], accb[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int slot = sub + k * 32;
+    const int slot = P.sub + k * 32;
     live[k] = slot < slots;
     rot[k] = slot_place<V>(A, slot, ea[k], eb[k]) && live[k];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      wa[k][j] = live[k] ? A.w[P.side][ea[k] + j] : 0.f;
+      wb[k][j] = live[k] ? A.w[P.side][eb[k] + j] : 0.f;
+      acca[k][j] = accb[k][j] = 0.f;
+    }
   }
-  for (int64_t n0 = (int64_t)blockIdx.x * A.TT; n0 < A.N; n0 += (int64_t)gridDim.x * A.TT) {
-    const int toks = (int)min((int64_t)A.TT, A.N - n0);
-    __syncthreads();  // the previous tile's table has been read
-    build_table(A, n0, toks, cs, sn);
-    __syncthreads();
-    const int units = toks * A.nchunk;
-    for (int u = warp; u < units; u += kRotWarps) {
-      const int tok = u / A.nchunk, ch = u - tok * A.nchunk;
-      const int64_t n = n0 + tok, b = n / A.T, tk = n - b * A.T;
-      const int hend = min(A.H, (ch + 1) * A.hchunk);
-      for (int h0 = ch * A.hchunk; h0 < hend; h0 += hpw) {
-        const int h = h0 + group;
-        const bool on = h < hend;
-        const int side = h >= A.heads[0] ? 1 : 0, hs = h - (side ? A.heads[0] : 0);
-        float xa[K][V], xb[K][V], ga[K][V], gb[K][V];
-        float ss = 0.f, dot = 0.f;
+  for (int64_t u = P.unit; u < P.units; u += P.step) {
+    const Unit U = unit_of(A, P, u);
+    Raw<T, V> ra[K], rb[K], sa[K], sb[K];
+    auto load = [&](int h) {
+      if (h < U.hend) {
+        const T* p = head_ptr<T>(A.x[P.side], U, h);
+        const T* g = head_ptr<T>(A.dy[P.side], U, h);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (on && live[k]) {
-            const T* p = head_ptr<T>(A.x[side], b, tk, hs);
-            const T* g = head_ptr<T>(A.dy[side], b, tk, hs);
-            ld<V>(p + ea[k], xa[k]);
-            ld<V>(p + eb[k], xb[k]);
-            ld<V>(g + ea[k], ga[k]);
-            ld<V>(g + eb[k], gb[k]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) xa[k][j] = xb[k][j] = ga[k][j] = gb[k][j] = 0.f;
+        for (int k = 0; k < K; ++k)
+          if (live[k]) {
+            fetch<T, V>(p + ea[k], ra[k]);
+            fetch<T, V>(p + eb[k], rb[k]);
+            fetch<T, V>(g + ea[k], sa[k]);
+            fetch<T, V>(g + eb[k], sb[k]);
           }
+      }
+    };
+    load(U.h);
+    build_table(A, P, U.n0, cs, sn);
+    const int hlast = P.tw == 1 ? U.hend : 1;
+    for (int i = P.tw == 1 ? U.h - P.group : 0, h = U.h; i < hlast; i += hpw, h += hpw) {
+      float xa[K][V], xb[K][V], ga[K][V], gb[K][V];
+      const bool on = h < U.hend;
+      float ss = 0.f, dot = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (on && live[k]) {
+          widen<T, V>(ra[k], xa[k]);
+          widen<T, V>(rb[k], xb[k]);
+          widen<T, V>(sa[k], ga[k]);
+          widen<T, V>(sb[k], gb[k]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) xa[k][j] = xb[k][j] = ga[k][j] = gb[k][j] = 0.f;
+        }
+      }
+      load(h + hpw);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (rot[k]) {
+          float c[V], s[V];
+          const int at = U.tok * (A.R / 2) + (P.sub + k * 32) * V;
+          ld_sh<V>(cs + at, c);
+          ld_sh<V>(sn + at, s);
+          turn<V, INTER>(ga[k], gb[k], c, s);  // dn = rot^T(dout): sin is negated in the table
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (rot[k]) {
-            const int slot = sub + k * 32;
-            float c[V], s[V];
-            ld_sh<V>(cs + tok * (A.R / 2) + slot * V, c);
-            ld_sh<V>(sn + tok * (A.R / 2) + slot * V, s);
-            turn<V, INTER>(ga[k], gb[k], c, s);  // dn = rot^T(dout): sin is negated in the table
-          }
-          if (!live[k]) continue;
-          float wa[V], wb[V];
-          ld_sh<V>(wsh + side * A.D + ea[k], wa);
-          ld_sh<V>(wsh + side * A.D + eb[k], wb);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            ss = fmaf(xa[k][j], xa[k][j], fmaf(xb[k][j], xb[k][j], ss));
-            dot = fmaf(ga[k][j] * wa[j], xa[k][j], fmaf(gb[k][j] * wb[j], xb[k][j], dot));
-          }
+        for (int j = 0; j < V; ++j) {
+          ss = fmaf(xa[k][j], xa[k][j], fmaf(xb[k][j], xb[k][j], ss));
+          dot = fmaf(ga[k][j] * wa[k][j], xa[k][j], fmaf(gb[k][j] * wb[k][j], xb[k][j], dot));
         }
-        ss = head_sum(ss, A.lg);
-        dot = head_sum(dot, A.lg);
-        if (!on) continue;
+      }
+      ss = head_sum(ss, A.lg);
+      dot = head_sum(dot, A.lg);
+      if (on) {
         const float r = rsqrtf(ss / (float)A.D + A.eps);
         const float m = r * r * r * dot / (float)A.D;
-        T* q = const_cast<T*>(head_ptr<T>(A.y[side], b, tk, hs));
+        T* q = head_ptr<T>(A.y[P.side], U, h);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
-          float wa[V], wb[V], oa[V], ob[V];
-          ld_sh<V>(wsh + side * A.D + ea[k], wa);
-          ld_sh<V>(wsh + side * A.D + eb[k], wb);
-          // the gradient of the other side's weight gains exactly 0
-          const float r0 = side ? 0.f : r, r1 = side ? r : 0.f;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            oa[j] = r * ga[k][j] * wa[j] - xa[k][j] * m;
-            ob[j] = r * gb[k][j] * wb[j] - xb[k][j] * m;
-            const float ta = ga[k][j] * xa[k][j], tb = gb[k][j] * xb[k][j];
-            acc[0][0][k][j] = fmaf(ta, r0, acc[0][0][k][j]);
-            acc[0][1][k][j] = fmaf(tb, r0, acc[0][1][k][j]);
-            acc[1][0][k][j] = fmaf(ta, r1, acc[1][0][k][j]);
-            acc[1][1][k][j] = fmaf(tb, r1, acc[1][1][k][j]);
+            const float ta = r * ga[k][j], tb = r * gb[k][j];
+            acca[k][j] = fmaf(ta, xa[k][j], acca[k][j]);
+            accb[k][j] = fmaf(tb, xb[k][j], accb[k][j]);
+            xa[k][j] = ta * wa[k][j] - xa[k][j] * m;
+            xb[k][j] = tb * wb[k][j] - xb[k][j] * m;
           }
-          st<V>(q + ea[k], oa);
-          st<V>(q + eb[k], ob);
+          st<V>(q + ea[k], xa[k]);
+          st<V>(q + eb[k], xb[k]);
         }
       }
     }
   }
   // over the warp's head groups (butterfly), then over the warps in order
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * A.D; i += kRotThreads) wsh[i] = 0.f;
-  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          for (int o = lanes; o < 32; o <<= 1)
-            acc[i][e][k][j] += __shfl_xor_sync(kFullMask, acc[i][e][k][j], o);
+    for (int j = 0; j < V; ++j)
+      for (int o = 1 << A.lg; o < 32; o <<= 1) {
+        acca[k][j] += __shfl_xor_sync(kFullMask, acca[k][j], o);
+        accb[k][j] += __shfl_xor_sync(kFullMask, accb[k][j], o);
+      }
+  __syncthreads();  // the tables are done with
+  float* sum = &table[0][0];
   for (int w = 0; w < kRotWarps; ++w) {
-    if (warp == w && group == 0) {
+    if ((int)(threadIdx.x >> 5) == w && P.group == 0) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!live[k]) continue;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            wsh[i * A.D + ea[k] + j] += acc[i][0][k][j];
-            wsh[i * A.D + eb[k] + j] += acc[i][1][k][j];
-          }
+        for (int j = 0; j < V; ++j) {
+          sum[ea[k] + j] = (w ? sum[ea[k] + j] : 0.f) + acca[k][j];
+          sum[eb[k] + j] = (w ? sum[eb[k] + j] : 0.f) + accb[k][j];
+        }
       }
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < 2 * A.D; i += kRotThreads) part[(size_t)blockIdx.x * 2 * A.D + i] = wsh[i];
+  for (int i = threadIdx.x; i < A.D; i += kRotThreads) part[(size_t)blockIdx.x * A.D + i] = sum[i];
 }
 
-// dw[k] = sum over partial rows p of part[p, k]: 32 chains per column, then
-// the chains in order. Columns 0..D-1 are dwq, D..2D-1 dwk. blockDim (32, 32).
+// dw[side][k] = sum over the side's partial rows p of part[p, k]: 32 chains per
+// column, then the chains in order. blockDim (32, 32), gridDim.y = 2 sides.
 __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ dwq,
-                                                          float* __restrict__ dwk, int nparts, int D) {
+                                                          float* __restrict__ dwk, int nq, int nk, int D) {
   __shared__ float t[32][33];
   const int k = blockIdx.x * 32 + threadIdx.x;
+  const float* p = part + (blockIdx.y ? (size_t)nq * D : 0);
+  const int n = blockIdx.y ? nk : nq;
   float s = 0.f;
-  if (k < 2 * D)
-    for (int p = threadIdx.y; p < nparts; p += 32) s += part[(size_t)p * 2 * D + k];
+  if (k < D) {
+#pragma unroll 4
+    for (int i = threadIdx.y; i < n; i += 32) s += p[(size_t)i * D + k];
+  }
   t[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && k < 2 * D) {
+  if (threadIdx.y == 0 && k < D) {
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 32; ++q) v += t[q][threadIdx.x];
-    if (k < D)
-      dwq[k] = v;
-    else
-      dwk[k - D] = v;
+    (blockIdx.y ? dwk : dwq)[k] = v;
   }
 }
 
@@ -419,91 +480,101 @@ bool vec_ok(const RotaryArgs& A, bool bwd) {
   return true;
 }
 
-// Tokens per CTA, heads per unit, lanes per head.
-void shape_launch(RotaryArgs& A, bool vec, int sms) {
+// Lanes per head, heads per unit, CTAs per tensor (at most `most` in all).
+void shape_launch(RotaryArgs& A, bool vec, int sms, int most) {
   const int es = A.dtype == kDtypeBF16 ? 2 : 4;
   const int slots = vec ? A.D / (2 * (16 / es)) : 32;
   A.lg = 0;
   while ((1 << A.lg) < slots) ++A.lg;
-  const int hpw = 32 >> A.lg, groups = (A.H + hpw - 1) / hpw;
-  // 16 KB of x per CTA amortises the table; fewer tokens when that leaves SMs idle
-  int64_t tt = 16384 / ((int64_t)A.H * A.D * es);
-  tt = std::min<int64_t>(tt, (A.N + 4 * sms - 1) / (4 * sms));
-  tt = std::min<int64_t>(tt, kTableFloats / A.R);
-  A.TT = (int)std::max<int64_t>(1, tt);
-  A.nchunk = A.TT >= kRotWarps ? 1 : std::min(groups, (kRotWarps + A.TT - 1) / A.TT);
-  A.hchunk = (groups + A.nchunk - 1) / A.nchunk * hpw;
-  A.nchunk = (A.H + A.hchunk - 1) / A.hchunk;
+  const int hpw = 32 >> A.lg;
+  int64_t want[2] = {0, 0};
+  for (int s = 0; s < 2; ++s) {
+    const int H = A.heads[s];
+    A.nchunk[s] = A.hchunk[s] = 1;
+    A.ctas[s] = 0;
+    if (H == 0) continue;
+    const int tw = H < hpw ? hpw / H : 1;
+    const int64_t tiles = (A.N + tw - 1) / tw;
+    if (tw == 1) {  // few tokens: their heads spread over more warps
+      const int groups = (H + hpw - 1) / hpw;
+      const int64_t nch = std::min<int64_t>(groups, std::max<int64_t>(1, (int64_t)sms * 16 / tiles));
+      A.hchunk[s] = (int)((groups + nch - 1) / nch) * hpw;
+      A.nchunk[s] = (H + A.hchunk[s] - 1) / A.hchunk[s];
+    }
+    want[s] = (tiles * A.nchunk[s] + kRotWarps - 1) / kRotWarps;
+  }
+  // over the limit: each tensor by its share of the heads
+  const int64_t k = want[1] ? std::max<int64_t>(1, (int64_t)most * A.heads[1] / A.H) : 0;
+  const bool over = want[0] + want[1] > most;
+  A.ctas[0] = (int)(over ? std::min<int64_t>(want[0], std::max<int64_t>(1, most - k)) : want[0]);
+  A.ctas[1] = (int)(over ? std::min<int64_t>(want[1], k) : want[1]);
 }
 
-size_t smem_bytes(const RotaryArgs& A) { return ((size_t)A.TT * A.R + 2 * (size_t)A.D) * sizeof(float); }
-
 template <class T, int V, int K, bool NORM>
-void launch_fwd(const RotaryArgs& A, unsigned grid, cudaStream_t st) {
+void launch_fwd(const RotaryArgs& A, cudaStream_t st) {
+  const unsigned grid = (unsigned)(A.ctas[0] + A.ctas[1]);
   if (A.interleaved)
-    rotary_fwd_kernel<T, V, K, NORM, true><<<grid, kRotThreads, smem_bytes(A), st>>>(A);
+    rotary_fwd_kernel<T, V, K, NORM, true><<<grid, kRotThreads, 0, st>>>(A);
   else
-    rotary_fwd_kernel<T, V, K, NORM, false><<<grid, kRotThreads, smem_bytes(A), st>>>(A);
+    rotary_fwd_kernel<T, V, K, NORM, false><<<grid, kRotThreads, 0, st>>>(A);
 }
 
 template <class T, bool NORM>
-void dispatch_fwd(const RotaryArgs& A, bool vec, unsigned grid, cudaStream_t st) {
+void dispatch_fwd(const RotaryArgs& A, bool vec, cudaStream_t st) {
   constexpr int NV = 16 / (int)sizeof(T);
   if (vec)
-    launch_fwd<T, NV, 1, NORM>(A, grid, st);
+    launch_fwd<T, NV, 1, NORM>(A, st);
   else if (A.D <= 128)  // pairs per lane: D / 64
-    launch_fwd<T, 1, 2, NORM>(A, grid, st);
+    launch_fwd<T, 1, 2, NORM>(A, st);
   else
-    launch_fwd<T, 1, 8, NORM>(A, grid, st);
+    launch_fwd<T, 1, 8, NORM>(A, st);
 }
 
 template <class T, int V, int K>
-void launch_bwd(const RotaryArgs& A, float* part, unsigned grid, cudaStream_t st) {
+void launch_bwd(const RotaryArgs& A, float* part, cudaStream_t st) {
+  const unsigned grid = (unsigned)(A.ctas[0] + A.ctas[1]);
   if (A.interleaved)
-    qk_norm_bwd_kernel<T, V, K, true><<<grid, kRotThreads, smem_bytes(A), st>>>(A, part);
+    qk_norm_bwd_kernel<T, V, K, true><<<grid, kRotThreads, 0, st>>>(A, part);
   else
-    qk_norm_bwd_kernel<T, V, K, false><<<grid, kRotThreads, smem_bytes(A), st>>>(A, part);
+    qk_norm_bwd_kernel<T, V, K, false><<<grid, kRotThreads, 0, st>>>(A, part);
 }
 
 template <class T>
-void dispatch_bwd(const RotaryArgs& A, bool vec, float* part, unsigned grid, cudaStream_t st) {
+void dispatch_bwd(const RotaryArgs& A, bool vec, float* part, cudaStream_t st) {
   constexpr int NV = 16 / (int)sizeof(T);
   if (vec)
-    launch_bwd<T, NV, 1>(A, part, grid, st);
+    launch_bwd<T, NV, 1>(A, part, st);
   else if (A.D <= 128)
-    launch_bwd<T, 1, 2>(A, part, grid, st);
+    launch_bwd<T, 1, 2>(A, part, st);
   else
-    launch_bwd<T, 1, 8>(A, part, grid, st);
+    launch_bwd<T, 1, 8>(A, part, st);
 }
 
 }  // namespace
 
 cudaError_t rotary_fwd_launch(RotaryArgs A, bool norm, int sms, cudaStream_t st) {
   const bool vec = vec_ok(A, false);
-  shape_launch(A, vec, sms);
-  const unsigned grid = (unsigned)((A.N + A.TT - 1) / A.TT);
+  shape_launch(A, vec, sms, 8 * sms);
   if (A.dtype == kDtypeBF16)
-    norm ? dispatch_fwd<bf16_t, true>(A, vec, grid, st) : dispatch_fwd<bf16_t, false>(A, vec, grid, st);
+    norm ? dispatch_fwd<bf16_t, true>(A, vec, st) : dispatch_fwd<bf16_t, false>(A, vec, st);
   else
-    norm ? dispatch_fwd<float, true>(A, vec, grid, st) : dispatch_fwd<float, false>(A, vec, grid, st);
+    norm ? dispatch_fwd<float, true>(A, vec, st) : dispatch_fwd<float, false>(A, vec, st);
   return cudaGetLastError();
 }
 
 // Partial weight-gradient rows: one per CTA of the backward.
-int qk_norm_bwd_ctas(int64_t tokens, int sms) { return (int)std::max<int64_t>(1, std::min<int64_t>(tokens, 4 * (int64_t)sms)); }
+int qk_norm_bwd_ctas(int sms) { return 4 * sms; }
 
 cudaError_t qk_norm_bwd_launch(RotaryArgs A, float* part, float* dwq, float* dwk, int sms, cudaStream_t st) {
   const bool vec = vec_ok(A, true);
-  shape_launch(A, vec, sms);
-  const int64_t tiles = (A.N + A.TT - 1) / A.TT;
-  const int grid = (int)std::min<int64_t>(tiles, qk_norm_bwd_ctas(A.N, sms));
+  shape_launch(A, vec, sms, qk_norm_bwd_ctas(sms));
   if (A.dtype == kDtypeBF16)
-    dispatch_bwd<bf16_t>(A, vec, part, (unsigned)grid, st);
+    dispatch_bwd<bf16_t>(A, vec, part, st);
   else
-    dispatch_bwd<float>(A, vec, part, (unsigned)grid, st);
+    dispatch_bwd<float>(A, vec, part, st);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  qk_norm_dw_kernel<<<(2 * A.D + 31) / 32, dim3(32, 32), 0, st>>>(part, dwq, dwk, grid, A.D);
+  qk_norm_dw_kernel<<<dim3((A.D + 31) / 32, 2), dim3(32, 32), 0, st>>>(part, dwq, dwk, A.ctas[0], A.ctas[1], A.D);
   return cudaGetLastError();
 }
 

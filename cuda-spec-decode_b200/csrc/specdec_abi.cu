@@ -1060,7 +1060,7 @@ size_t specdec_qk_norm_rotary_workspace_bytes(int32_t batch, int32_t T, int32_t 
   if (batch <= 0 || T <= 0 || head_dim <= 0 ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
     return 256;
-  return align256((size_t)qk_norm_bwd_ctas((int64_t)batch * T, sms) * 2 * (size_t)head_dim * sizeof(float));
+  return align256((size_t)qk_norm_bwd_ctas(sms) * (size_t)head_dim * sizeof(float));
 }
 
 int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1086,7 +1086,7 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
   }
   if (!q || !k || !q_weight || !k_weight || !dq_out || !dk_out || !dq || !dk || !workspace)
     return fail(SPECDEC_ERR_ARGUMENT, "null input, output or workspace pointer");
-  const size_t need = (size_t)qk_norm_bwd_ctas(A.N, sms) * 2 * (size_t)head_dim * sizeof(float);
+  const size_t need = (size_t)qk_norm_bwd_ctas(sms) * (size_t)head_dim * sizeof(float);
   if (workspace_bytes < need)
     return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
   A.sin_scale = -scale;

@@ -202,10 +202,11 @@ struct RotaryArgs {
   int heads[2], H;                 // H = heads[0] + heads[1]
   float scale, sin_scale, eps;     // sin_scale = -scale turns the other way
   // set by the launch
-  int TT, lg, nchunk, hchunk;      // tokens per CTA, log2 lanes per head, units per token, heads per unit
+  int lg;                          // log2 lanes per head
+  int ctas[2], nchunk[2], hchunk[2];  // per tensor: CTAs, units per token, heads per unit
 };
 cudaError_t rotary_fwd_launch(RotaryArgs A, bool norm, int sms, cudaStream_t st);
-int qk_norm_bwd_ctas(int64_t tokens, int sms);
+int qk_norm_bwd_ctas(int sms);
 cudaError_t qk_norm_bwd_launch(RotaryArgs A, float* part, float* dwq, float* dwk, int sms, cudaStream_t st);
 
 // Attention of the drafter on the tensor cores (drafter_attention.cu):

@@ -165,7 +165,10 @@ def on_device(device: torch.device):
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream as an integer (torch's raw-stream query: a
+    tenth of a microsecond, where building a Stream object costs over two)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def set_launch_shape(kernel: int, shape: int, ctas_per_sm: int = 0) -> None:
@@ -225,7 +228,7 @@ _status: dict = {}
 def status_words(device: torch.device) -> torch.Tensor:
     """int32[4] on `device` for the current stream, zero-initialised once; the
     entry points write their status word into it on the device."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index, stream_handle(device))
     t = _status.get(key)
     if t is None:
         t = _status[key] = torch.zeros(4, dtype=torch.int32, device=device)

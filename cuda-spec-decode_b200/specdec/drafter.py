@@ -56,7 +56,18 @@ def _status(dev: torch.device) -> int:
     when a bounded wait expires (their failed rows are then NaN); the next
     synchronising check (specdec.ops.check_backward, a validating D-PACE
     forward, GraphedStep.check) raises RuntimeError and clears it."""
-    return _lib.status_words(dev)[_lib.STATUS_DRAFTER:].data_ptr()
+    return _lib.status_words(dev).data_ptr() + 4 * _lib.STATUS_DRAFTER
+
+
+def _once(fn):
+    """once_differentiable, but only where a graph of the backward is being
+    built: its wrapper costs 20 us per call."""
+    slow = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return slow(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return backward
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -253,7 +264,7 @@ class _Rotary(torch.autograd.Function):
         return _rotary(x, positions, inv_freq, interleaved, scale, 0)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         positions, inv_freq = ctx.saved_tensors
         return _rotary(dy, positions, inv_freq, *ctx.how, 1), None, None, None, None
@@ -271,7 +282,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     positions, inv_freq = _check_rotary(x, positions, inv_freq)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Rotary.apply(x, positions, inv_freq, int(bool(interleaved)), float(scale))
-    return _rotary(x.detach(), positions, inv_freq, int(bool(interleaved)), float(scale), 0)
+    return _rotary(x, positions, inv_freq, int(bool(interleaved)), float(scale), 0)
 
 
 def _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale):
@@ -292,14 +303,14 @@ class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, scale):
         q, k = _strided(q), _strided(k)
-        wq, wk = q_weight.detach().float().contiguous(), k_weight.detach().float().contiguous()
+        wq, wk = q_weight.float().contiguous(), k_weight.float().contiguous()
         ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
         ctx.how = eps, interleaved, scale
         ctx.wdtypes = q_weight.dtype, k_weight.dtype
         return _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dyq, dyk):
         lib = _lib.load()
         q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
@@ -342,8 +353,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
                                     or k_weight.requires_grad):
         return _QKNormRotary.apply(q, k, q_weight, k_weight, positions, inv_freq, *how)
-    return _qk_norm_rotary(_strided(q.detach()), _strided(k.detach()), q_weight.detach().float().contiguous(),
-                           k_weight.detach().float().contiguous(), positions, inv_freq, *how)
+    return _qk_norm_rotary(_strided(q), _strided(k), q_weight.float().contiguous(), k_weight.float().contiguous(),
+                           positions, inv_freq, *how)
 
 
 # ---- sliding-window attention with sinks ------------------------------------------
@@ -404,7 +415,7 @@ class _WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         lib = _lib.load()
         q, k, v, o, lse, ctx_lens = ctx.saved_tensors
@@ -452,7 +463,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_ctx: i
     how = int(n_ctx), window, sinks, scale
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, ctx_lens, *how)
-    return _window_forward(_rows16(q.detach()), _rows16(k.detach()), _rows16(v.detach()), ctx_lens, *how, False)[0]
+    return _window_forward(_rows16(q), _rows16(k), _rows16(v), ctx_lens, *how, False)[0]
 
 
 def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_lens: torch.Tensor, *,
@@ -475,7 +486,7 @@ def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     size, Hk = k_cache.shape[1], k_cache.shape[2]
     assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the cache's heads must be contiguous"
     assert 0 <= n_block <= size, f"n_block must be in [0, size of the cache], got {n_block}"
-    q = _rows16(q.detach())
+    q = _rows16(q)
     o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
     with _lib.on_device(q.device):
         ws_bytes = lib.specdec_window_attention_cached_workspace_bytes(B, Tq, size, Hq, Hk, D, n_block, window, sinks,

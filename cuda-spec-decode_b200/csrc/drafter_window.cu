@@ -99,25 +99,27 @@ __device__ __forceinline__ bool token_range(const WindowArgs& A, const Seq& s, i
   return true;
 }
 
-// The 64-key tiles of a query tile: `ns` over the sinks in front of the
+// The KN-key tiles of a run of queries: `ns` over the sinks in front of the
 // window, then the window from the first query's lo to the last query's hi.
+template <int KN>
 struct KeyTiles {
   int lo, hi, sink, ns, n;
-  int lo_last, hi_first;
   __device__ __forceinline__ KeyTiles(const WindowArgs& A, const Seq& s, int p0, int p1) {
     lo = low_of(A, s, p0);
     hi = high_of(s, p1);
-    lo_last = low_of(A, s, p1);
-    hi_first = high_of(s, p0);
     sink = min(A.S, lo);
-    ns = (sink + kTN - 1) / kTN;
-    n = ns + (hi - lo + kTN - 1) / kTN;
+    ns = (sink + KN - 1) / KN;
+    n = ns + (hi - lo + KN - 1) / KN;
   }
-  __device__ __forceinline__ int start(int i) const { return i < ns ? i * kTN : lo + (i - ns) * kTN; }
-  __device__ __forceinline__ int end(int i) const { return i < ns ? min(sink, i * kTN + kTN) : min(hi, start(i) + kTN); }
-  // every query sees every key of tile i
-  __device__ __forceinline__ bool full(int i) const {
-    return i < ns ? i * kTN + kTN <= sink : start(i) + kTN <= hi_first && start(i) >= lo_last;
+  __device__ __forceinline__ int start(int i) const { return i < ns ? i * KN : lo + (i - ns) * KN; }
+  __device__ __forceinline__ int end(int i) const { return i < ns ? min(sink, i * KN + KN) : min(hi, start(i) + KN); }
+  // queries with bounds from lo0 .. lo1 and hi0 .. hi1 (first .. last): whether
+  // every one of them sees every key of tile i, and whether any sees any
+  __device__ __forceinline__ bool full(int i, int lo1, int hi0) const {
+    return i < ns ? i * KN + KN <= sink : start(i) + KN <= hi0 && start(i) >= lo1;
+  }
+  __device__ __forceinline__ bool any(int i, int lo0, int hi1, int S) const {
+    return i < ns || (start(i) < hi1 && (start(i) + KN > lo0 || start(i) < S));
   }
 };
 
@@ -209,57 +211,145 @@ __device__ __forceinline__ void give_up(int* status, uint64_t* drain) {
 }
 
 // ---- forward --------------------------------------------------------------------
-// One CTA per (sequence, key head, 128 packed rows[, split of the keys]); thread
-// i owns row i = TMEM lane i. LA score tiles are in flight in tensor memory: in
-// step i the threads wait for S(i), issue the copies of K(i + LA) and V(i), turn
-// S(i) into P(i), and after the step's one barrier thread 0 issues O += P(i) V(i)
-// and S(i + LA) = Q K^T.
-template <int D>
+// One CTA per (sequence, key head, QT x 128 packed rows[, split of the keys]).
+// Warps: QT softmax warpgroups (thread i owns row i of its tile = TMEM lane i),
+// then one warp that issues the products and three that copy K and V.
+//   copies    a ring of NS stages of KN rows, K0 V0 K1 V1 ..., by TMA (one thread);
+//             a tile that runs into padding or past the last token is copied by
+//             the three warps with cp.async and zeros
+//   products  per step, for each query tile t: O_t += P_t(i-1) V(i-1), then
+//             S_t(i) = Q_t K(i)^T; with two tiles, one's products run during the
+//             other's softmax
+//   softmax   S_t from tensor memory, P_t in bf16 back over S_t's columns (the
+//             A operand of the next product is read from tensor memory), O_t
+//             rescaled there when the reference maximum rises
+// Every wait is bounded and watches a shared flag that the first expired wait
+// raises; all warps then leave for the common end.
+// Registers with two query tiles: the softmax keeps a row's 128 scores, so its
+// two warpgroups take over what the service warps do not need. The block is
+// launched with 168 x 384 = 64512 >= 208 x 256 + 80 x 128 (checked at launch).
+constexpr int kSoftmaxRegs = 208, kServiceRegs = 80;
+
+template <int D, int QT>
 struct FwdCfg {
-  static constexpr int LA = D == 64 ? 1 : 2;
-  static constexpr int CTAS = D == 64 ? 4 : 2;
-  static constexpr uint32_t KT = kTN * D * 2;  // bytes of a key tile
-  static constexpr uint32_t OQ = 0, OK = kTM * D * 2, OV = OK + LA * KT, OP = OV + LA * KT;
-  static constexpr uint32_t OBAR = OP + kTM * 128;  // bar_s[2], bar_o, drain
-  static constexpr uint32_t OSLOT = OBAR + 32;
-  static constexpr uint32_t BYTES = OSLOT + 8;  // the base is 1024-byte aligned (extern __shared__ alignment)
-  static constexpr uint32_t COLS = D == 64 ? 128 : 256;
-  static constexpr uint32_t COL_O = LA * kTN;
+  static constexpr int KN = QT == 2 ? 128 : 64;
+  static constexpr int NS = D == 128 ? 5 : 8;
+  static constexpr int CTAS = QT == 2 ? 1 : 2;
+  static constexpr int THREADS = QT * 128 + 128;
+  static constexpr uint32_t QB = kTM * D * 2, SB = KN * D * 2;
+  static constexpr uint32_t OQ = 0, OST = QT * QB, OBAR = OST + NS * SB;
+  static constexpr int NBAR = 2 * NS + 2 * QT + 3;  // full, empty, s_full, p_full, q_full, o_full, drain
+  static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;  // TMEM base, dead flag
+  static constexpr uint32_t COLS = QT == 2 ? 512 : 256;
+  static constexpr uint32_t COL_O = QT * KN;
 };
 
-// SPLIT: the CTA's part of the keys, its unnormalised fp32 rows to the workspace.
-template <int D, bool SPLIT>
-__global__ void __launch_bounds__(kTM, FwdCfg<D>::CTAS) window_fwd_kernel(const __grid_constant__ WindowArgs A) {
-  using C = FwdCfg<D>;
-  constexpr int LA = C::LA;
+// Waits for the barrier's phase; false once `dead` is set or the limit expired
+// (which sets it and the status word).
+__device__ __forceinline__ bool wait_alive(uint64_t* bar, uint32_t parity, volatile int* dead, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*dead) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      *dead = 1;
+      if (status) atomicExch(status, kStatusTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+// Whether the ROWS rows from token j0 on are tokens of the sequence in
+// consecutive rows: then a tensor-map box brings them (rows behind the tile's
+// end are masked, and hold a token's values).
+template <int ROWS>
+__device__ __forceinline__ bool boxed(const Seq& s, int j0) {
+  return j0 + ROWS <= s.total && (s.kb == s.c || j0 + ROWS <= s.c || j0 >= s.c);
+}
+
+// The other tiles: keys [j0, j1) into ROWS rows (the rest zeros), by the three
+// service warps (lt = 0 .. 95); complete and visible to the tensor core when
+// it returns. Every one of the 96 threads calls it; `copy` false: nothing is
+// copied (an expired wait).
+template <int ROWS, int D>
+__device__ __forceinline__ void stage_keys(uint32_t tile, const bf16_t* base, int64_t stride, const Seq& s, int j0,
+                                           int j1, int lt, bool copy) {
+  constexpr int C = D / 8, RP = 96 / C;  // chunks per row, rows per pass
+  if (copy) {
+    const int c = lt % C;
+    const uint32_t dst = tile + (uint32_t)(c >> 3) * (ROWS * 128u);
+#pragma unroll 2
+    for (int r = lt / C; r < ROWS; r += RP) {
+      const int j = j0 + r;
+      const bool valid = j < j1;
+      cp_async16(dst + sw128((uint32_t)r, (uint32_t)(c & 7)),
+                 valid ? base + (int64_t)(j < s.c ? j : j + s.kb - s.c) * stride + c * 8 : base, valid);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+  }
+  fence_proxy_async_smem();
+  asm volatile("bar.sync 1, 96;" ::: "memory");
+}
+
+template <int D, int QT, bool SPLIT>
+__global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
+    window_fwd_kernel(const __grid_constant__ WindowArgs A) {
+  using C = FwdCfg<D, QT>;
+  constexpr int KN = C::KN;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  uint64_t* bar_s = reinterpret_cast<uint64_t*>(smem + C::OBAR);
-  uint64_t* bar_o = bar_s + 2;
-  uint64_t* drain = bar_s + 3;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem + C::OSLOT + 4);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OBAR);
+  uint64_t* empty = full + C::NS;
+  uint64_t* s_full = empty + C::NS;
+  uint64_t* p_full = s_full + QT;
+  uint64_t* q_full = p_full + QT;
+  uint64_t* o_full = q_full + 1;
+  uint64_t* drain = q_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OSLOT);
   const int warp = threadIdx.x >> 5;
+  const int wg = threadIdx.x >> 7;  // 0 .. QT-1: softmax, QT: service
   const int bh = blockIdx.x, b = bh / A.Hk, hk = bh - b * A.Hk;
-  const int m0 = (int)(gridDim.y - 1 - blockIdx.y) * kTM;  // the last tiles see the most keys: first
-  const int m1 = min(A.M, m0 + kTM);
+  const int m0 = (int)(gridDim.y - 1 - blockIdx.y) * (QT * kTM);  // the last tiles see the most keys: first
   const Seq sq = seq_of(A, b);
-  const int m = m0 + (int)threadIdx.x;
-  const int t = group_div(A, min(m, A.M - 1)), hq = hk * A.G + min(m, A.M - 1) - t * A.G;
-  bf16_t* orow = A.o + (((int64_t)b * A.Tq + t) * A.Hq + hq) * D;
-  const int64_t prow = ((int64_t)bh * A.M + m) * A.splits + (SPLIT ? blockIdx.z : 0);
 
+  // the query tiles' tokens and bounds, the CTA's key tiles
+  int lo0[QT], lo1[QT], hi0[QT], hi1[QT];
   int p0, p1, i0 = 0, n = 0;
-  if (token_range(A, sq, m0, m1 - 1, p0, p1)) {
-    const KeyTiles kt(A, sq, p0, p1);
+  const bool some = token_range(A, sq, m0, min(A.M, m0 + QT * kTM) - 1, p0, p1);
+  const KeyTiles<KN> kt(A, sq, some ? p0 : 0, some ? p1 : -1);
+  if (some) {
     n = kt.n;
     if (SPLIT) {
       const int per = (n + A.splits - 1) / A.splits;
       i0 = min(n, (int)blockIdx.z * per);
       n = min(n, i0 + per) - i0;
     }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      int a, z;
+      const int mt = m0 + t * kTM;
+      const bool live = mt < A.M && token_range(A, sq, mt, min(A.M, mt + kTM) - 1, a, z);
+      lo0[t] = live ? low_of(A, sq, a) : 0;
+      lo1[t] = live ? low_of(A, sq, z) : 0;
+      hi0[t] = live ? high_of(sq, a) : 0;
+      hi1[t] = live ? high_of(sq, z) : -1;  // -1: no tile of keys at all
+    }
   }
+  auto needs = [&](int t, int i) { return hi1[t] >= 0 && kt.any(i0 + i, lo0[t], hi1[t], A.S); };
+
+  // this softmax thread's row
+  const int m = m0 + (int)(threadIdx.x % (QT * kTM));
+  const int tq = group_div(A, min(m, A.M - 1)), hq = hk * A.G + min(m, A.M - 1) - tq * A.G;
+  bf16_t* orow = A.o + (((int64_t)b * A.Tq + tq) * A.Hq + hq) * D;
+  const int64_t prow = ((int64_t)bh * A.M + m) * A.splits + (SPLIT ? blockIdx.z : 0);
+  const bool mine = wg < QT && m < A.M;
+  const int p = mine ? token_of(A, sq, tq) : -1;
+
   if (n == 0) {  // nothing to see
-    if (m < A.M) {
+    if (mine) {
       if (SPLIT) {
         A.part_ml[prow] = make_float2(-INFINITY, 0.f);
       } else {
@@ -270,138 +360,227 @@ __global__ void __launch_bounds__(kTM, FwdCfg<D>::CTAS) window_fwd_kernel(const 
     }
     return;
   }
-  const KeyTiles kt(A, sq, p0, p1);
-  const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
-  const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
   if (threadIdx.x == 0) {
-    mbar_init(bar_s, 1);
-    mbar_init(bar_s + 1, 1);
-    mbar_init(bar_o, 1);
+#pragma unroll
+    for (int i = 0; i < C::NS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      mbar_init(s_full + t, 1);
+      mbar_init(p_full + t, 128);
+    }
+    mbar_init(q_full, A.q_maps ? 1 : QT * 128);
+    mbar_init(o_full, 1);
     mbar_init(drain, 1);
     fence_mbar_init();
+    *dead = 0;
   }
-  if (warp == 0) tmem_alloc(slot, C::COLS);
-  load_queries<kTM, kTM, D>(A, base + C::OQ, A.q + (int64_t)b * A.qs[0] + (int64_t)hk * A.G * A.qs[2], A.qs[1], A.qs[2],
-                            sq, m0, m1);
-#pragma unroll
-  for (int i = 0; i < LA; ++i)
-    if (i < n) load_keys<kTM, kTN, D>(base + C::OK + i * C::KT, kb, A.ks[1], sq, kt.start(i0 + i), kt.end(i0 + i));
-  cp_async_commit();
-  const int p = m < A.M ? token_of(A, sq, t) : -1;
-  const int lo = low_of(A, sq, p), hi = high_of(sq, p);
-  constexpr uint32_t kIdS = instr_desc(kTM, kTN, 0, 0);
-  constexpr uint32_t kIdO = instr_desc(kTM, D, 0, 1);
-  cp_async_wait<0>();
-  publish(false);
-  const uint32_t tmem = *slot;
-  const uint32_t lane = tmem + ((uint32_t)(warp * 32) << 16);
-  // failure-detection test hook: the grid's first CTA issues no first product,
-  // so its own wait runs into the limit
-  const bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int i = 0; i < LA; ++i)
-      if (i < n && !(withhold && i == 0)) {
-        mma_kk<D, kTM, kTN>(tmem + i * kTN, base + C::OQ, base + C::OK + i * C::KT, kIdS, 0);
-        umma_commit(bar_s + i);
-      }
-  }
-
-  float m_ref = -INFINITY, l_run = 0.f;
-  bool ok = true;
-  for (int i = 0; i < n; ++i) {
-    const int u = LA == 1 ? 0 : i & 1;
-    bool good = mbar_wait(bar_s + u, (i / LA) & 1);
-    tc_fence_after();
-    // S(i) has read K(i); with S(i), P V of step i - LA is complete as well
-    if (i + LA < n)
-      load_keys<kTM, kTN, D>(base + C::OK + u * C::KT, kb, A.ks[1], sq, kt.start(i0 + i + LA), kt.end(i0 + i + LA));
-    load_keys<kTM, kTN, D>(base + C::OV + u * C::KT, vb, A.vs[1], sq, kt.start(i0 + i), kt.end(i0 + i));
-    cp_async_commit();
-    float s[2][32];
-    tmem_ld32x2(lane + u * kTN, lane + u * kTN + 32, s[0], s[1]);
-    if (!kt.full(i0 + i)) {
-      const int k0 = kt.start(i0 + i);
-      const bool in_sink = i0 + i < kt.ns;
-      // relative bounds: lo <= j < hi, or j < S (a sink tile: j < min(sink, hi))
-      const int rl = in_sink ? kTN : lo - k0, rh = hi - k0, rs = (in_sink ? kt.sink : A.S) - k0;
-#pragma unroll
-      for (int j = 0; j < kTN; ++j)
-        if (!(j < rh && (j >= rl || j < rs))) s[j >> 5][j & 31] = -INFINITY;
-    }
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int j = 0; j < kTN; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j >> 5][j & 31]);
-    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
-    const bool raise = mt > m_ref + kRescaleLog2;
-    const float alpha = raise ? (m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - mt)) : 1.f;
-    if (raise) m_ref = mt;
-    const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen nothing yet: p = 2^-inf = 0
-    if (i > 0) good &= mbar_wait(bar_o, (i - 1) & 1);  // P and O are free
-    tc_fence_after();
-    float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      uint32_t pk[16];
-#pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        const float a = exp2_approx(fmaf(s[hh][j], A.scale_log2, nm));
-        const float c = exp2_approx(fmaf(s[hh][j + 1], A.scale_log2, nm));
-        ls[(j >> 1) & 3] += a + c;
-        pk[j / 2] = pack_bf16x2(a, c);
-      }
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4)
-        st_shared_u4(base + C::OP + sw128(threadIdx.x, (uint32_t)(hh * 4 + c4)),
-                     make_uint4(pk[4 * c4], pk[4 * c4 + 1], pk[4 * c4 + 2], pk[4 * c4 + 3]));
-    }
-    l_run = fmaf(l_run, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
-    if (i > 0 && __any_sync(kFullMask, raise)) {
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float ot[32];
-        tmem_ld32(lane + C::COL_O + c, ot);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) ot[j] *= alpha;
-        tmem_st32(lane + C::COL_O + c, ot);
-      }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-    }
-    cp_async_wait<0>();  // K(i + LA), V(i)
-    if (publish(!good)) {
-      ok = false;
-      break;
-    }
-    if (threadIdx.x == 0) {
-      mma_kn(tmem + C::COL_O, base + C::OP, base + C::OV + u * C::KT, kIdO, i > 0);
-      umma_commit(bar_o);
-      if (i + LA < n) {
-        mma_kk<D, kTM, kTN>(tmem + u * kTN, base + C::OQ, base + C::OK + u * C::KT, kIdS, 0);
-        umma_commit(bar_s + u);
-      }
-    }
-  }
-  cp_async_wait<0>();  // no copy outlives the CTA
-  if (ok) ok = __syncthreads_or(mbar_wait(bar_o, (n - 1) & 1) ? 0 : 1) == 0;
+  if (warp == QT * 4) tmem_alloc(slot, C::COLS);
+  tc_fence_before();
+  __syncthreads();
   tc_fence_after();
-  if (!ok) {
-    give_up(A.status, drain);  // then its rows are NaN
-    if (m < A.M) {
-      if (SPLIT) {
-        A.part_ml[prow] = make_float2(0.f, __int_as_float(0x7fc00000));
-      } else {
+  const uint32_t tmem = *slot;
+  int issued = 0;  // stages that this thread's copies have begun
+
+  if (wg == QT) {
+    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
+    if (warp == QT * 4) {
+      // ---- products (one thread; the warp stays together for the end) ----
+      if ((threadIdx.x & 31) == 0) {
+        constexpr uint32_t kIdS = instr_desc(kTM, KN, 0, 0);
+        constexpr uint32_t kIdO = instr_desc(kTM, D, 0, 1);
+        // failure-detection test hook: the grid's first CTA issues no first
+        // product, so its softmax runs into the limit
+        bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+        uint32_t steps[QT];  // steps of each tile so far
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(orow + 8 * c) = make_uint4(kNan2, kNan2, kNan2, kNan2);
-        if (A.lse) A.lse[(int64_t)bh * A.M + m] = __int_as_float(0x7fc00000);
+        for (int t = 0; t < QT; ++t) steps[t] = 0;
+        bool ok = wait_alive(q_full, 0, dead, A.status);
+        for (int i = 0; i <= n && ok; ++i) {
+          const int sv = 2 * i - 1, sk = 2 * i;  // stages of V(i-1) and K(i) in ring order
+          if (i > 0) ok = wait_alive(full + sv % C::NS, (sv / C::NS) & 1, dead, A.status);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            if (i > 0 && needs(t, i - 1)) {
+              ok = ok && wait_alive(p_full + t, (steps[t] - 1) & 1, dead, A.status);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < KN / 16; ++kk)
+                umma_bf16_ta(tmem + C::COL_O + t * D, tmem + t * KN + kk * 8,
+                             smem_desc(base + C::OST + (sv % C::NS) * C::SB + kk * 2048, KN * 128, 1024), kIdO,
+                             (steps[t] > 1) | (kk > 0));
+            }
+            if (i == n) continue;
+            if (t == 0) ok = ok && wait_alive(full + sk % C::NS, (sk / C::NS) & 1, dead, A.status);
+            if (!ok) break;
+            if (needs(t, i)) {
+              tc_fence_after();
+              ++steps[t];
+              if (withhold) {
+                withhold = false;
+                continue;
+              }
+              mma_kk<D, kTM, KN>(tmem + t * KN, base + C::OQ + t * C::QB, base + C::OST + (sk % C::NS) * C::SB, kIdS, 0);
+              umma_commit(s_full + t);
+            }
+          }
+          if (!ok) break;
+          if (i > 0) umma_commit(empty + sv % C::NS);
+          if (i < n) umma_commit(empty + sk % C::NS);
+        }
+        if (ok) umma_commit(o_full);
+      }
+      __syncwarp();
+    } else {
+      // ---- copies ----
+      const int lt = (int)threadIdx.x - QT * 128 - 32;
+      const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
+      const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
+      if (lt == 0 && A.q_maps) {
+        mbar_arrive_expect_tx(q_full, QT * C::QB);
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(base + C::OQ + t * C::QB + c * (kTM * 128), &A.mq, c * 64, hk * A.G,
+                        (m0 + t * kTM) / A.G, b, q_full);
+      }
+      bool ok = true;
+      for (int s = 0; s < 2 * n; ++s) {  // no early exit: the 96 threads meet in stage_keys
+        if (ok && s >= C::NS) ok = wait_alive(empty + s % C::NS, (s / C::NS - 1) & 1, dead, A.status);
+        if (ok) issued = s + 1;
+        const int i = i0 + (s >> 1), j0 = kt.start(i);
+        const uint32_t stage = base + C::OST + (s % C::NS) * C::SB;
+        if (A.kv_maps && boxed<KN>(sq, j0)) {
+          if (ok && lt == 0) {
+            const int row = j0 < sq.c ? j0 : j0 + sq.kb - sq.c;
+            mbar_arrive_expect_tx(full + s % C::NS, C::SB);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(stage + c * (KN * 128), s & 1 ? &A.mv : &A.mk, c * 64, row, hk, b, full + s % C::NS);
+          }
+        } else {
+          stage_keys<KN, D>(stage, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0, kt.end(i), lt, ok);
+          if (ok && lt == 0) mbar_arrive(full + s % C::NS);
+        }
       }
     }
   } else {
-    const float inv = p < 0 ? 0.f : 1.f / l_run;
+    // ---- softmax of tile wg ----
+    if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = wg, mt = m0 + t * kTM;
+    const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    if (!A.q_maps) {  // Q_t: this warpgroup's 128 rows
+      constexpr int CH = D / 8;
+      const int lt = threadIdx.x & 127, c = lt % CH;
+      const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)hk * A.G * A.qs[2];
+#pragma unroll 4
+      for (int r = lt / CH; r < kTM; r += 128 / CH) {
+        const int mr = mt + r, tr = group_div(A, mr);
+        const bool valid = mr < A.M && token_of(A, sq, tr) >= 0;
+        cp_async16(base + C::OQ + t * C::QB + (uint32_t)(c >> 3) * (kTM * 128u) + sw128((uint32_t)r, (uint32_t)(c & 7)),
+                   valid ? qb + (int64_t)tr * A.qs[1] + (int64_t)(mr - tr * A.G) * A.qs[2] + c * 8 : qb, valid);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+    const int lo = low_of(A, sq, p), hi = high_of(sq, p);
+    float m_ref = -INFINITY, l_run = 0.f;
+    uint32_t steps = 0;
+    bool ok = true;
+    int tl1 = lo1[0], th0 = hi0[0];
+    if (QT == 2 && t == 1) {
+      tl1 = lo1[QT - 1];
+      th0 = hi0[QT - 1];
+    }
+    for (int i = 0; i < n; ++i) {
+      if (!needs(t, i)) continue;
+      ok = __all_sync(kFullMask, wait_alive(s_full + t, steps & 1, dead, A.status));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sr[KN / 32][32];
 #pragma unroll
-    for (int c = 0; c < D; c += 32) {
-      float ot[32];
-      tmem_ld32(lane + C::COL_O + c, ot);
-      if (m < A.M) {
+      for (int c = 0; c < KN / 32; ++c) tmem_ld32_async(lane + t * KN + c * 32, sr[c]);
+      tmem_wait_ld();
+      float s[KN / 32][32];
+#pragma unroll
+      for (int c = 0; c < KN / 32; ++c)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[c][j] = __uint_as_float(sr[c][j]);
+      if (!kt.full(i0 + i, tl1, th0)) {
+        const int k0 = kt.start(i0 + i);
+        const bool in_sink = i0 + i < kt.ns;
+        // relative bounds: lo <= j < hi, or j < S (a sink tile: j < min(sink, hi))
+        const int rl = in_sink ? KN : lo - k0, rh = hi - k0, rs = (in_sink ? kt.sink : A.S) - k0;
+#pragma unroll
+        for (int j = 0; j < KN; ++j)
+          if (!(j < rh && (j >= rl || j < rs))) s[j >> 5][j & 31] = -INFINITY;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < KN; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j >> 5][j & 31]);
+      const float mt_ = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+      const bool raise = mt_ > m_ref + kRescaleLog2;
+      const float alpha = raise ? (m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - mt_)) : 1.f;
+      if (raise) m_ref = mt_;
+      const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen nothing yet: p = 2^-inf = 0
+      const float2 sc2 = make_float2(A.scale_log2, A.scale_log2), nm2 = make_float2(nm, nm);
+      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c = 0; c < KN / 32; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 e = ffma2(make_float2(s[c][j], s[c][j + 1]), sc2, nm2);
+          const float2 pr = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+          ls[(j >> 1) & 1] = fadd2(ls[(j >> 1) & 1], pr);
+          pk[j / 2] = pack_bf16x2(pr.x, pr.y);
+        }
+        tmem_st16(lane + t * KN + c * 16, pk);
+      }
+      const float2 l2 = fadd2(ls[0], ls[1]);
+      l_run = fmaf(l_run, alpha, l2.x + l2.y);
+      if (steps > 0 && __any_sync(kFullMask, raise)) {  // S(i) came behind O's last product
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float ot[32];
+          tmem_ld32(lane + C::COL_O + t * D + c, ot);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) ot[j] *= alpha;
+          tmem_st32(lane + C::COL_O + t * D + c, ot);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_full + t);
+      ++steps;
+    }
+    if (ok && steps > 0) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
+    tc_fence_after();
+    if (!ok) {  // never a plausible wrong number: the row is NaN
+      if (mine) {
+        if (SPLIT) {
+          A.part_ml[prow] = make_float2(0.f, __int_as_float(0x7fc00000));
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint4*>(orow + 8 * c) = make_uint4(kNan2, kNan2, kNan2, kNan2);
+          if (A.lse) A.lse[(int64_t)bh * A.M + m] = __int_as_float(0x7fc00000);
+        }
+      }
+    } else {
+      const bool seen = p >= 0 && l_run != 0.f;  // (a NaN sum is written as it is)
+      const float inv = 1.f / l_run;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float ot[32];
+        tmem_ld32(lane + C::COL_O + t * D + c, ot);
+        if (!mine) continue;
         if (SPLIT) {
           float* pr = A.part_o + prow * D + c;
 #pragma unroll
@@ -409,7 +588,7 @@ __global__ void __launch_bounds__(kTM, FwdCfg<D>::CTAS) window_fwd_kernel(const 
             *reinterpret_cast<float4*>(pr + j) = make_float4(ot[j], ot[j + 1], ot[j + 2], ot[j + 3]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) ot[j] = p < 0 ? 0.f : ot[j] * inv;
+          for (int j = 0; j < 32; ++j) ot[j] = seen ? ot[j] * inv : 0.f;
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
             *reinterpret_cast<uint4*>(orow + c + j) =
@@ -417,18 +596,27 @@ __global__ void __launch_bounds__(kTM, FwdCfg<D>::CTAS) window_fwd_kernel(const 
                            pack_bf16x2(ot[j + 4], ot[j + 5]), pack_bf16x2(ot[j + 6], ot[j + 7]));
         }
       }
-    }
-    if (m < A.M) {
-      if (SPLIT)
-        A.part_ml[prow] = make_float2(m_ref, p < 0 ? 0.f : l_run);
-      else if (A.lse)
-        A.lse[(int64_t)bh * A.M + m] = p < 0 ? -INFINITY : (m_ref + log2f(l_run)) * kLn2;
+      if (mine) {
+        if (SPLIT)
+          A.part_ml[prow] = make_float2(m_ref, p < 0 ? 0.f : l_run);
+        else if (A.lse)
+          A.lse[(int64_t)bh * A.M + m] = seen ? (m_ref + log2f(l_run)) * kLn2 : -INFINITY;
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) tmem_free(tmem, C::COLS);
+  if (*dead) {  // bounded waits for every product and box that was issued
+    if (warp == QT * 4 && (threadIdx.x & 31) == 0) umma_commit(drain);
+    mbar_wait(drain, 0);
+    if (threadIdx.x == QT * 128 + 32) {
+      if (A.q_maps) mbar_wait(q_full, 0);
+      for (int s = max(0, issued - C::NS); s < issued; ++s) mbar_wait(full + s % C::NS, (s / C::NS) & 1);
+    }
+    __syncthreads();
+  }
+  if (warp == QT * 4) tmem_free(tmem, C::COLS);
 }
 
 // Joins the splits of a row: weights 2^(m_z - max m), a warp per packed row.
@@ -544,7 +732,8 @@ __device__ __forceinline__ void window_dq(const WindowArgs& A, int bh, int mt, b
     if (m < A.M) fill_row<D>(drow, half, 0u);
     return;
   }
-  const KeyTiles kt(A, sq, p0, p1);
+  const KeyTiles<kTN> kt(A, sq, p0, p1);
+  const int lo_last = low_of(A, sq, p1), hi_first = high_of(sq, p0);
   const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
   const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
   if (threadIdx.x == 0) {
@@ -598,7 +787,7 @@ __device__ __forceinline__ void window_dq(const WindowArgs& A, int bh, int mt, b
     {
       float sv[32], dp[32];
       tmem_ld32x2(lane + C::COL_S + half * 32, lane + C::COL_P + half * 32, sv, dp);
-      const bool full = kt.full(i);
+      const bool full = kt.full(i, lo_last, hi_first);
       const int k0 = kt.start(i) + half * 32;
       const bool in_sink = i < kt.ns;
       const int rl = in_sink ? kTN : lo - k0, rh = hi - k0, rs = (in_sink ? kt.sink : A.S) - k0;
@@ -835,33 +1024,96 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const __grid_constant
   A.delta[((int64_t)b * A.Hk + hk) * A.M + (int64_t)t * A.G + (h - hk * A.G)] = d;
 }
 
-// Raises a kernel's dynamic shared-memory limit once per device.
+// Raises a kernel's dynamic shared-memory limit once per device; refuses a
+// kernel whose block holds fewer registers than its warps will ask for.
 template <class K>
-cudaError_t allow_smem(K* kernel, uint32_t bytes, std::atomic<unsigned long long>& done) {
+cudaError_t allow_smem(K* kernel, uint32_t bytes, std::atomic<unsigned long long>& done, int regs = 0,
+                       int threads = 0) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned long long bit = 1ull << (dev & 63);
   if (done.load() & bit) return cudaSuccess;
+  if (regs > 0) {
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs * threads < regs) return cudaErrorInvalidConfiguration;
+  }
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) done.fetch_or(bit);
   return e;
 }
 
-template <int D, bool SPLIT>
-cudaError_t fwd_launch(const WindowArgs& A, cudaStream_t st) {
+// cuTensorMapEncodeTiled, through the runtime (the library does not link libcuda).
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// A bf16 tensor of four dimensions (innermost first, contiguous; the others
+// with element strides), 128-byte-swizzled boxes of 64 x b1 x b2 x 1. False
+// where a stride cannot be expressed (the kernels then copy by hand).
+bool make_map(CUtensorMap* map, const bf16_t* p, const int64_t (&dim)[4], const int64_t (&stride)[3], int b1, int b2) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[4], s[3];
+  for (int i = 0; i < 4; ++i) d[i] = (cuuint64_t)dim[i];
+  for (int i = 0; i < 3; ++i) {
+    s[i] = (cuuint64_t)(dim[i + 1] > 1 ? stride[i] : dim[0]) * sizeof(bf16_t);
+    if (s[i] == 0 || s[i] >= (cuuint64_t(1) << 40) || s[i] % 16) return false;
+  }
+  const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, one[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<bf16_t*>(p), d, s, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Keys and values as [D, T, Hk, B], boxes of `rows` tokens.
+void kv_maps(WindowArgs& A, int D, int rows) {
+  const int64_t d[4] = {D, A.Tk, A.Hk, A.B};
+  A.kv_maps = make_map(&A.mk, A.k, d, {A.ks[1], A.ks[2], A.ks[0]}, rows, 1) &&
+              make_map(&A.mv, A.v, d, {A.vs[1], A.vs[2], A.vs[0]}, rows, 1);
+}
+
+// Queries (or dO) as [D, Hq, T, B], boxes of whole tokens' groups: G a power of two.
+bool group_map(CUtensorMap* map, const WindowArgs& A, const bf16_t* p, const int64_t (&s)[3], int D, int rows) {
+  if (A.G > rows || (A.G & (A.G - 1))) return false;
+  const int64_t d[4] = {D, A.Hq, A.Tq, A.B};
+  return make_map(map, p, d, {s[2], s[1], s[0]}, A.G, rows / A.G);
+}
+
+template <int D, int QT, bool SPLIT>
+cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
+  using C = FwdCfg<D, QT>;
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = allow_smem(window_fwd_kernel<D, SPLIT>, FwdCfg<D>::BYTES, done);
+  const cudaError_t e = allow_smem(window_fwd_kernel<D, QT, SPLIT>, C::BYTES, done,
+                                   QT == 2 ? kSoftmaxRegs * 256 + kServiceRegs * 128 : 0, C::THREADS);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(A.B * A.Hk), (unsigned)((A.M + kTM - 1) / kTM), (unsigned)A.splits);
-  window_fwd_kernel<D, SPLIT><<<grid, kTM, FwdCfg<D>::BYTES, st>>>(A);
+  kv_maps(A, D, C::KN);
+  A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
+  const dim3 grid((unsigned)(A.B * A.Hk), (unsigned)((A.M + QT * kTM - 1) / (QT * kTM)), (unsigned)A.splits);
+  window_fwd_kernel<D, QT, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
   return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t fwd_any(const WindowArgs& A, cudaStream_t st) {
-  if (A.splits == 1) return fwd_launch<D, false>(A, st);
-  const cudaError_t e = fwd_launch<D, true>(A, st);
+cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
+  if (A.splits == 1) {
+    const int64_t pairs = (int64_t)A.B * A.Hk * ((A.M + 2 * kTM - 1) / (2 * kTM));
+    return A.M > kTM && pairs >= sms ? fwd_launch<D, 2, false>(A, st) : fwd_launch<D, 1, false>(A, st);
+  }
+  const cudaError_t e = fwd_launch<D, 1, true>(A, st);
   if (e != cudaSuccess) return e;
   const int64_t rows = (int64_t)A.B * A.Hk * A.M;
   window_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(A);
@@ -869,7 +1121,7 @@ cudaError_t fwd_any(const WindowArgs& A, cudaStream_t st) {
 }
 
 template <int D>
-cudaError_t bwd_any(const WindowArgs& A, cudaStream_t st) {
+cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem(window_bwd_kernel<D>, BwdCfg<D>::BYTES, done);
   if (e != cudaSuccess) return e;
@@ -888,15 +1140,15 @@ cudaError_t bwd_any(const WindowArgs& A, cudaStream_t st) {
 // each, from the most keys a query tile can see.
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms) {
   const int64_t tiles = (most_keys + kTN - 1) / kTN + 1;
-  const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64>::CTAS : FwdCfg<128>::CTAS);
+  const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64, 1>::CTAS : FwdCfg<128, 1>::CTAS);
   return (int)std::max<int64_t>(1, std::min<int64_t>(room / std::max<int64_t>(1, ctas), tiles / 2));
 }
 
-cudaError_t window_fwd_launch(const WindowArgs& A, int D, cudaStream_t st) {
-  return D == 64 ? fwd_any<64>(A, st) : fwd_any<128>(A, st);
+cudaError_t window_fwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st) {
+  return D == 64 ? fwd_any<64>(A, sms, st) : fwd_any<128>(A, sms, st);
 }
 
-cudaError_t window_bwd_launch(const WindowArgs& A, int D, cudaStream_t st) {
+cudaError_t window_bwd_launch(WindowArgs& A, int D, cudaStream_t st) {
   return D == 64 ? bwd_any<64>(A, st) : bwd_any<128>(A, st);
 }
 

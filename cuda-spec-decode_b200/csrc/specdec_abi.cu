@@ -1155,6 +1155,13 @@ int window_input(const char* name, const void* p, const int64_t* strides, int32_
   return SPECDEC_OK;
 }
 
+int device_sms(int* sms) {
+  const int dev = current_device();
+  if (dev < 0 || cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return fail(SPECDEC_ERR_CUDA, "device query failed");
+  return SPECDEC_OK;
+}
+
 int64_t window_most_keys(int64_t Tq, int64_t Tk, int64_t n_block, int64_t window, int64_t sinks) {
   return std::min<int64_t>(Tk, window + sinks + Tq + n_block);
 }
@@ -1186,7 +1193,9 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
   A.n_ctx = n_ctx;
   A.status = status;
   A.withhold = take_withhold_stage();
-  const cudaError_t e = window_fwd_launch(A, head_dim, static_cast<cudaStream_t>(stream));
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != SPECDEC_OK) return rc;
+  const cudaError_t e = window_fwd_launch(A, head_dim, sms, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? ok() : cuda_fail(e, "window attention forward launch");
 }
 
@@ -1273,10 +1282,8 @@ int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides,
     return rc;
   if ((rc = window_input("v_cache", v_cache, v_strides, batch, cache_len, k_heads, head_dim, A.vs)) != SPECDEC_OK)
     return rc;
-  const int dev = current_device();
   int sms = 0;
-  if (dev < 0 || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return fail(SPECDEC_ERR_CUDA, "device query failed");
+  if ((rc = device_sms(&sms)) != SPECDEC_OK) return rc;
   const int64_t bh = (int64_t)batch * k_heads;
   A.splits = window_splits(head_dim, bh * ((A.M + 127) / 128),
                            window_most_keys(q_len, cache_len, n_block, window, sinks), sms);
@@ -1296,7 +1303,7 @@ int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides,
   A.cached = 1;
   A.status = status;
   A.withhold = take_withhold_stage();
-  const cudaError_t e = window_fwd_launch(A, head_dim, st);
+  const cudaError_t e = window_fwd_launch(A, head_dim, sms, st);
   return e == cudaSuccess ? ok() : cuda_fail(e, "window attention launch");
 }
 

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "specdec_common.cuh"
@@ -239,10 +240,14 @@ struct WindowArgs {
   bf16_t *dq, *dk, *dv;
   int* status;
   int withhold;
+  // tensor maps, set by the launch: [D, T, Hk, B] with boxes of 64 x rows, and
+  // [D, Hq, T, B] with boxes of 64 x G x (rows / G); the flags say which exist
+  int kv_maps, q_maps;
+  CUtensorMap mk, mv, mq, mg;
 };
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms);
-cudaError_t window_fwd_launch(const WindowArgs& A, int D, cudaStream_t st);
-cudaError_t window_bwd_launch(const WindowArgs& A, int D, cudaStream_t st);
+cudaError_t window_fwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st);
+cudaError_t window_bwd_launch(WindowArgs& A, int D, cudaStream_t st);
 
 // Sets the calling thread's specdec_last_error() text.
 void set_last_error(const char* msg);

@@ -214,6 +214,12 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor shaped as t (empty_like costs the
+    host half of torch.empty)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _strides(t: torch.Tensor):
     """The C ABI's three element strides (None: contiguous)."""
     return None if t.is_contiguous() else (ctypes.c_int64 * 3)(*t.stride()[:3])
@@ -247,7 +253,7 @@ def _rotary(x, positions, inv_freq, interleaved, scale, inverse):
     lib = _lib.load()
     B, T, H, D = x.shape
     x = _strided(x)
-    y = torch.empty((B, T, H, D), dtype=x.dtype, device=x.device)
+    y = _new(x)
     with _lib.on_device(x.device):
         _lib.check(lib.specdec_rotary(
             x.data_ptr(), _strides(x), y.data_ptr(), positions.data_ptr(), _position_stride(positions),
@@ -288,8 +294,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
 def _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale):
     lib = _lib.load()
     B, T, Hq, D = q.shape
-    yq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    yk = torch.empty((B, T, k.shape[2], D), dtype=q.dtype, device=q.device)
+    yq, yk = _new(q), _new(k)
     with _lib.on_device(q.device):
         _lib.check(lib.specdec_qk_norm_rotary_forward(
             q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), yq.data_ptr(),
@@ -318,19 +323,17 @@ class _QKNormRotary(torch.autograd.Function):
         B, T, Hq, D = q.shape
         Hk = k.shape[2]
         dyq, dyk = _strided(dyq), _strided(dyk)
-        dq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-        dk = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
-        dw = torch.empty((2, D), dtype=torch.float32, device=q.device)
+        dq, dk, dwq, dwk = _new(q), _new(k), _new(wq), _new(wk)
         with _lib.on_device(q.device):
             ws_bytes = lib.specdec_qk_norm_rotary_workspace_bytes(B, T, D, q.device.index)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
             _lib.check(lib.specdec_qk_norm_rotary_backward(
                 q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), dyq.data_ptr(),
-                _strides(dyq), dyk.data_ptr(), _strides(dyk), dq.data_ptr(), dk.data_ptr(), dw[0].data_ptr(),
-                dw[1].data_ptr(), positions.data_ptr(), _position_stride(positions), inv_freq.data_ptr(), B, T, Hq, Hk,
+                _strides(dyq), dyk.data_ptr(), _strides(dyk), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
+                dwk.data_ptr(), positions.data_ptr(), _position_stride(positions), inv_freq.data_ptr(), B, T, Hq, Hk,
                 D, 2 * inv_freq.numel(), interleaved, scale, eps, _DTYPES[q.dtype], ws.data_ptr(), ws_bytes,
                 _stream(q)), "specdec_qk_norm_rotary_backward")
-        return dq, dk, dw[0].to(ctx.wdtypes[0]), dw[1].to(ctx.wdtypes[1]), None, None, None, None, None
+        return dq, dk, dwq.to(ctx.wdtypes[0]), dwk.to(ctx.wdtypes[1]), None, None, None, None, None
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -395,7 +398,7 @@ def _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, want_lse):
     lib = _lib.load()
     B, T, Hq, D = q.shape
     Hk = k.shape[2]
-    o = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    o = _new(q)
     lse = torch.empty((B, Hk, T, Hq // Hk), dtype=torch.float32, device=q.device) if want_lse else None
     with _lib.on_device(q.device):
         _lib.check(lib.specdec_window_attention_forward(
@@ -424,8 +427,7 @@ class _WindowAttention(torch.autograd.Function):
         do = do.contiguous()
         if do.data_ptr() % 16:
             do = do.clone()
-        dq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        dq, dk, dv = _new(q), _new(k), _new(v)
         with _lib.on_device(q.device):
             ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
@@ -487,7 +489,7 @@ def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the cache's heads must be contiguous"
     assert 0 <= n_block <= size, f"n_block must be in [0, size of the cache], got {n_block}"
     q = _rows16(q)
-    o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
+    o = _new(q)
     with _lib.on_device(q.device):
         ws_bytes = lib.specdec_window_attention_cached_workspace_bytes(B, Tq, size, Hq, Hk, D, n_block, window, sinks,
                                                                        q.device.index)

@@ -181,6 +181,21 @@ __device__ __forceinline__ void mma_kn(uint32_t d, uint32_t a, uint32_t b, uint3
               accumulate | (kk > 0));
 }
 
+// The same from the operands' descriptor words (a step's offset is one addition).
+template <int D, int RA, int RB>
+__device__ __forceinline__ void issue_kk(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    umma_ss(d, a + (((kk >> 2) * (RA * 128) + (kk & 3) * 32) >> 4), b + (((kk >> 2) * (RB * 128) + (kk & 3) * 32) >> 4),
+            idesc, kk > 0);
+}
+// A in tensor memory [128 x 16 K], B rows along K.
+template <int K>
+__device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+  for (int kk = 0; kk < K; ++kk) umma_ts(d, a + kk * 8, b + ((kk * 2048) >> 4), idesc, accumulate | (kk > 0));
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
                : "memory");
@@ -213,10 +228,10 @@ __device__ __forceinline__ void give_up(int* status, uint64_t* drain) {
 // ---- forward --------------------------------------------------------------------
 // One CTA per (sequence, key head, QT x 128 packed rows[, split of the keys]).
 // Warps: QT softmax warpgroups (thread i owns row i of its tile = TMEM lane i),
-// then one warp that issues the products and three that copy K and V.
+// then one warp that issues the products and three (QT = 1: one) that copy K and V.
 //   copies    a ring of NS stages of KN rows, K0 V0 K1 V1 ..., by TMA (one thread);
 //             a tile that runs into padding or past the last token is copied by
-//             the three warps with cp.async and zeros
+//             the copying warps with cp.async and zeros
 //   products  per step, for each query tile t: O_t += P_t(i-1) V(i-1), then
 //             S_t(i) = Q_t K(i)^T; with two tiles, one's products run during the
 //             other's softmax
@@ -225,22 +240,22 @@ __device__ __forceinline__ void give_up(int* status, uint64_t* drain) {
 //             rescaled there when the reference maximum rises
 // Every wait is bounded and watches a shared flag that the first expired wait
 // raises; all warps then leave for the common end.
-// Registers with two query tiles: the softmax keeps a row's 128 scores, so its
-// two warpgroups take over what the service warps do not need. The block is
-// launched with 168 x 384 = 64512 >= 208 x 256 + 80 x 128 (checked at launch).
-constexpr int kSoftmaxRegs = 208, kServiceRegs = 80;
-
 template <int D, int QT>
 struct FwdCfg {
   static constexpr int KN = QT == 2 ? 128 : 64;
-  static constexpr int NS = D == 128 ? 5 : 8;
+  static constexpr int NS = D == 64 && QT == 2 ? 8 : 5;
   static constexpr int CTAS = QT == 2 ? 1 : 2;
-  static constexpr int THREADS = QT * 128 + 128;
+  static constexpr int COPY = QT == 2 ? 96 : 32;  // threads of the copying warps
+  static constexpr int THREADS = QT * 128 + 32 + COPY;
+  // registers: with two tiles the softmax keeps a row's 128 scores and takes
+  // over what the service warps do not need (0: an even split does)
+  static constexpr int LAUNCH_REGS = QT == 2 ? 168 : 0, SOFTMAX_REGS = 208, SERVICE_REGS = 80;
+  static_assert(LAUNCH_REGS == 0 || LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 256 + SERVICE_REGS * 128, "register split");
   static constexpr uint32_t QB = kTM * D * 2, SB = KN * D * 2;
   static constexpr uint32_t OQ = 0, OST = QT * QB, OBAR = OST + NS * SB;
-  static constexpr int NBAR = 2 * NS + 2 * QT + 3;  // full, empty, s_full, p_full, q_full, o_full, drain
+  static constexpr int NBAR = 2 * NS + 3 * QT + 3;  // full, empty, s_full, p_full (halves), q_full, o_full, drain
   static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;  // TMEM base, dead flag
-  static constexpr uint32_t COLS = QT == 2 ? 512 : 256;
+  static constexpr uint32_t COLS = QT == 2 ? 512 : D == 64 ? 128 : 256;
   static constexpr uint32_t COL_O = QT * KN;
 };
 
@@ -268,14 +283,14 @@ __device__ __forceinline__ bool boxed(const Seq& s, int j0) {
   return j0 + ROWS <= s.total && (s.kb == s.c || j0 + ROWS <= s.c || j0 >= s.c);
 }
 
-// The other tiles: keys [j0, j1) into ROWS rows (the rest zeros), by the three
-// service warps (lt = 0 .. 95); complete and visible to the tensor core when
-// it returns. Every one of the 96 threads calls it; `copy` false: nothing is
-// copied (an expired wait).
-template <int ROWS, int D>
+// The other tiles: keys [j0, j1) into ROWS rows (the rest zeros), by the NT
+// threads of the copying warps (lt = 0 .. NT-1); complete and visible to the
+// tensor core when it returns. Every one of them calls it; `copy` false:
+// nothing is copied (an expired wait).
+template <int NT, int ROWS, int D>
 __device__ __forceinline__ void stage_keys(uint32_t tile, const bf16_t* base, int64_t stride, const Seq& s, int j0,
                                            int j1, int lt, bool copy) {
-  constexpr int C = D / 8, RP = 96 / C;  // chunks per row, rows per pass
+  constexpr int C = D / 8, RP = NT / C;  // chunks per row, rows per pass
   if (copy) {
     const int c = lt % C;
     const uint32_t dst = tile + (uint32_t)(c >> 3) * (ROWS * 128u);
@@ -290,7 +305,7 @@ __device__ __forceinline__ void stage_keys(uint32_t tile, const bf16_t* base, in
     cp_async_wait<0>();
   }
   fence_proxy_async_smem();
-  asm volatile("bar.sync 1, 96;" ::: "memory");
+  asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
 template <int D, int QT, bool SPLIT>
@@ -305,7 +320,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   uint64_t* empty = full + C::NS;
   uint64_t* s_full = empty + C::NS;
   uint64_t* p_full = s_full + QT;
-  uint64_t* q_full = p_full + QT;
+  uint64_t* q_full = p_full + 2 * QT;
   uint64_t* o_full = q_full + 1;
   uint64_t* drain = q_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OSLOT);
@@ -369,7 +384,8 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       mbar_init(s_full + t, 1);
-      mbar_init(p_full + t, 128);
+      mbar_init(p_full + 2 * t, 128);
+      mbar_init(p_full + 2 * t + 1, 128);
     }
     mbar_init(q_full, A.q_maps ? 1 : QT * 128);
     mbar_init(o_full, 1);
@@ -385,54 +401,71 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   int issued = 0;  // stages that this thread's copies have begun
 
   if (wg == QT) {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
+    if constexpr (C::LAUNCH_REGS > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::SERVICE_REGS));
     if (warp == QT * 4) {
-      // ---- products (one thread; the warp stays together for the end) ----
-      if ((threadIdx.x & 31) == 0) {
-        constexpr uint32_t kIdS = instr_desc(kTM, KN, 0, 0);
-        constexpr uint32_t kIdO = instr_desc(kTM, D, 0, 1);
-        // failure-detection test hook: the grid's first CTA issues no first
-        // product, so its softmax runs into the limit
-        bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
-        uint32_t steps[QT];  // steps of each tile so far
+      // ---- products: the warp walks together, one lane issues ----
+      constexpr uint32_t kIdS = instr_desc(kTM, KN, 0, 0);
+      constexpr uint32_t kIdO = instr_desc(kTM, D, 0, 1);
+      // failure-detection test hook: the grid's first CTA issues no first
+      // product, so its softmax runs into the limit
+      bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+      const uint32_t dq = desc_low(base + C::OQ, 16);
+      const uint32_t dk = desc_low(base + C::OST, 16), dv = desc_low(base + C::OST, KN * 128);
+      uint32_t steps[QT];  // steps of each tile so far
 #pragma unroll
-        for (int t = 0; t < QT; ++t) steps[t] = 0;
-        bool ok = wait_alive(q_full, 0, dead, A.status);
-        for (int i = 0; i <= n && ok; ++i) {
-          const int sv = 2 * i - 1, sk = 2 * i;  // stages of V(i-1) and K(i) in ring order
-          if (i > 0) ok = wait_alive(full + sv % C::NS, (sv / C::NS) & 1, dead, A.status);
+      for (int t = 0; t < QT; ++t) steps[t] = 0;
+      uint32_t kslot = 0, kph = 0, vslot = 1, vph = 0;  // ring slots and phases of K(i), V(i-1)
+      bool ok = wait_alive(q_full, 0, dead, A.status);
+      for (int i = 0; i <= n && ok; ++i) {
+        if (i > 0) ok = wait_alive(full + vslot, vph, dead, A.status);
 #pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            if (i > 0 && needs(t, i - 1)) {
-              ok = ok && wait_alive(p_full + t, (steps[t] - 1) & 1, dead, A.status);
+        for (int t = 0; t < QT; ++t) {
+          if (i > 0 && needs(t, i - 1)) {
+            const uint32_t ph = (steps[t] - 1) & 1;
+            const uint32_t v = dv + vslot * (C::SB >> 4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // P arrives in halves
+              ok = ok && wait_alive(p_full + 2 * t + h, ph, dead, A.status);
               if (!ok) break;
               tc_fence_after();
-#pragma unroll
-              for (int kk = 0; kk < KN / 16; ++kk)
-                umma_bf16_ta(tmem + C::COL_O + t * D, tmem + t * KN + kk * 8,
-                             smem_desc(base + C::OST + (sv % C::NS) * C::SB + kk * 2048, KN * 128, 1024), kIdO,
-                             (steps[t] > 1) | (kk > 0));
+              if (elect_one())
+                issue_tn<KN / 32>(tmem + C::COL_O + t * D, tmem + t * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4),
+                                  kIdO, (steps[t] > 1) | (h > 0));
+              __syncwarp();
             }
-            if (i == n) continue;
-            if (t == 0) ok = ok && wait_alive(full + sk % C::NS, (sk / C::NS) & 1, dead, A.status);
             if (!ok) break;
-            if (needs(t, i)) {
-              tc_fence_after();
-              ++steps[t];
-              if (withhold) {
-                withhold = false;
-                continue;
-              }
-              mma_kk<D, kTM, KN>(tmem + t * KN, base + C::OQ + t * C::QB, base + C::OST + (sk % C::NS) * C::SB, kIdS, 0);
+          }
+          if (i == n) continue;
+          if (t == 0) ok = ok && wait_alive(full + kslot, kph, dead, A.status);
+          if (!ok) break;
+          if (needs(t, i)) {
+            tc_fence_after();
+            ++steps[t];
+            if (withhold) {
+              withhold = false;
+              continue;
+            }
+            if (elect_one()) {
+              issue_kk<D, kTM, KN>(tmem + t * KN, dq + t * (C::QB >> 4), dk + kslot * (C::SB >> 4), kIdS);
               umma_commit(s_full + t);
             }
+            __syncwarp();
           }
-          if (!ok) break;
-          if (i > 0) umma_commit(empty + sv % C::NS);
-          if (i < n) umma_commit(empty + sk % C::NS);
         }
-        if (ok) umma_commit(o_full);
+        if (!ok) break;
+        if (elect_one()) {
+          if (i > 0) umma_commit(empty + vslot);
+          if (i < n) umma_commit(empty + kslot);
+        }
+        __syncwarp();
+        kslot += 2;
+        if (kslot >= C::NS) kslot -= C::NS, kph ^= 1;
+        if (i > 0) {
+          vslot += 2;
+          if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
+        }
       }
+      if (ok && elect_one()) umma_commit(o_full);
       __syncwarp();
     } else {
       // ---- copies ----
@@ -449,7 +482,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
                         (m0 + t * kTM) / A.G, b, q_full);
       }
       bool ok = true;
-      for (int s = 0; s < 2 * n; ++s) {  // no early exit: the 96 threads meet in stage_keys
+      for (int s = 0; s < 2 * n; ++s) {  // no early exit: the copying threads meet in stage_keys
         if (ok && s >= C::NS) ok = wait_alive(empty + s % C::NS, (s / C::NS - 1) & 1, dead, A.status);
         if (ok) issued = s + 1;
         const int i = i0 + (s >> 1), j0 = kt.start(i);
@@ -463,14 +496,14 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
               tma_load_4d(stage + c * (KN * 128), s & 1 ? &A.mv : &A.mk, c * 64, row, hk, b, full + s % C::NS);
           }
         } else {
-          stage_keys<KN, D>(stage, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0, kt.end(i), lt, ok);
+          stage_keys<C::COPY, KN, D>(stage, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0, kt.end(i), lt, ok);
           if (ok && lt == 0) mbar_arrive(full + s % C::NS);
         }
       }
     }
   } else {
     // ---- softmax of tile wg ----
-    if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    if constexpr (C::LAUNCH_REGS > 0) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
     const int t = wg, mt = m0 + t * kTM;
     const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     if (!A.q_maps) {  // Q_t: this warpgroup's 128 rows
@@ -523,13 +556,25 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < KN; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j >> 5][j & 31]);
-      const float mt_ = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
-      const bool raise = mt_ > m_ref + kRescaleLog2;
+      for (int j = 0; j < KN; j += 2)
+        mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], s[j >> 5][j & 31], s[j >> 5][(j & 31) + 1]);
+      // a NaN score makes the maximum, and so the whole row, NaN
+      const float mt_ = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * A.scale_log2;
+      const bool raise = !(mt_ <= m_ref + kRescaleLog2) && mt_ != -INFINITY;
       const float alpha = raise ? (m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - mt_)) : 1.f;
       if (raise) m_ref = mt_;
       const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen nothing yet: p = 2^-inf = 0
       const float2 sc2 = make_float2(A.scale_log2, A.scale_log2), nm2 = make_float2(nm, nm);
+      if (steps > 0 && __any_sync(kFullMask, raise)) {  // S(i) came behind O's last product
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t ot[16];
+          tmem_ld16(lane + C::COL_O + t * D + c, ot);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) ot[j] = __float_as_uint(__uint_as_float(ot[j]) * alpha);
+          tmem_st16(lane + C::COL_O + t * D + c, ot);
+        }
+      }
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < KN / 32; ++c) {
@@ -542,22 +587,14 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
           pk[j / 2] = pack_bf16x2(pr.x, pr.y);
         }
         tmem_st16(lane + t * KN + c * 16, pk);
+        if ((c + 1) % (KN / 64) == 0) {  // half of P is there: its product may start
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_full + 2 * t + (c + 1) / (KN / 64) - 1);
+        }
       }
       const float2 l2 = fadd2(ls[0], ls[1]);
       l_run = fmaf(l_run, alpha, l2.x + l2.y);
-      if (steps > 0 && __any_sync(kFullMask, raise)) {  // S(i) came behind O's last product
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float ot[32];
-          tmem_ld32(lane + C::COL_O + t * D + c, ot);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) ot[j] *= alpha;
-          tmem_st32(lane + C::COL_O + t * D + c, ot);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(p_full + t);
       ++steps;
     }
     if (ok && steps > 0) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
@@ -1098,7 +1135,7 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   using C = FwdCfg<D, QT>;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(window_fwd_kernel<D, QT, SPLIT>, C::BYTES, done,
-                                   QT == 2 ? kSoftmaxRegs * 256 + kServiceRegs * 128 : 0, C::THREADS);
+                                   C::LAUNCH_REGS * C::THREADS, C::THREADS);
   if (e != cudaSuccess) return e;
   kv_maps(A, D, C::KN);
   A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
@@ -1110,8 +1147,13 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
 template <int D>
 cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
   if (A.splits == 1) {
+    // Two query tiles per CTA share the key tiles and hide one another's softmax,
+    // one tile per CTA fills the device with less: us with one / two at D = 128,
+    // 512 pairs of tiles: 1024 keys seen 101 / 102, 2048 keys 160 / 145, 4096 keys
+    // 232 / 188, 512 keys 71 / 80; at D = 64: 84 / 85, 135 / 125, 199 / 169, 57 / 66.
     const int64_t pairs = (int64_t)A.B * A.Hk * ((A.M + 2 * kTM - 1) / (2 * kTM));
-    return A.M > kTM && pairs >= sms ? fwd_launch<D, 2, false>(A, st) : fwd_launch<D, 1, false>(A, st);
+    const int64_t seen = std::min<int64_t>(A.Tk, (int64_t)A.W + A.S);
+    return pairs >= sms && seen >= 1536 ? fwd_launch<D, 2, false>(A, st) : fwd_launch<D, 1, false>(A, st);
   }
   const cudaError_t e = fwd_launch<D, 1, true>(A, st);
   if (e != cudaSuccess) return e;

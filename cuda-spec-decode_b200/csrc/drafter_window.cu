@@ -16,10 +16,13 @@
 // products as zeros) and its outputs and gradients are zero. In a cache the
 // block follows the context directly and the queries are the last Tq tokens.
 //
-// Shared heads. The G = Hq / Hk query heads of a key head are packed into one
-// tile: packed row m is token m / G, head m % G of the group. A key tile is
-// loaded once for the group, and a group's sums for dK and dV happen inside
-// the product.
+// Shared heads. Query heads of one key head are packed into a tile: packed row
+// m is token m / G, head m % G of the group, so a key tile is loaded once for
+// the group and the group's sums for dK and dV happen inside the product. In
+// a training batch G is the largest power of two in Hq / Hk (at most 64): 64
+// packed rows are then a box of a tensor map; `nsub` such groups ("virtual
+// heads") share a key head. In the cached form, bound by reading the cache,
+// G = Hq / Hk.
 //
 // Softmax: one pass, p = 2^(s - m_ref) with the row's reference maximum raised
 // only when a tile exceeds it by more than 2^8 (then O is rescaled in tensor
@@ -125,63 +128,10 @@ struct KeyTiles {
 
 // ---- tiles in shared memory ---------------------------------------------------
 // A tile of ROWS rows of D bf16 is D / 64 column blocks of ROWS x 128 bytes in
-// the 128-byte-swizzled layout. `row(r)` gives row r's first element, or null
-// for a zero row.
-template <int NT, int ROWS, int D, class F>
-__device__ __forceinline__ void load_tile(uint32_t tile, const bf16_t* any, F row) {
-  constexpr int C = D / 8;  // 16-byte chunks per row
-#pragma unroll
-  for (int j = 0; j < ROWS * C / NT; ++j) {
-    const int idx = threadIdx.x + j * NT;
-    const int r = idx / C, c = idx % C;
-    const bf16_t* p = row(r);
-    cp_async16(tile + (uint32_t)(c >> 3) * (ROWS * 128u) + sw128((uint32_t)r, (uint32_t)(c & 7)),
-               p ? p + c * 8 : any, p != nullptr);
-  }
-}
+// the 128-byte-swizzled layout.
 
-// Keys [j0, j1) of a sequence (rows of the batch: the block starts at row kb).
-template <int NT, int ROWS, int D>
-__device__ __forceinline__ void load_keys(uint32_t tile, const bf16_t* base, int64_t stride, const Seq& s, int j0,
-                                          int j1) {
-  load_tile<NT, ROWS, D>(tile, base, [&](int r) -> const bf16_t* {
-    const int j = j0 + r;
-    if (j >= j1) return nullptr;
-    return base + (int64_t)(j < s.c ? j : j + s.kb - s.c) * stride;
-  });
-}
-
-// Packed query rows [m0, m1) of key head hk, padding as zeros.
-template <int NT, int ROWS, int D>
-__device__ __forceinline__ void load_queries(const WindowArgs& A, uint32_t tile, const bf16_t* base, int64_t ts,
-                                             int64_t hs, const Seq& s, int m0, int m1) {
-  load_tile<NT, ROWS, D>(tile, base, [&](int r) -> const bf16_t* {
-    const int m = m0 + r;
-    if (m >= m1) return nullptr;
-    const int t = group_div(A, m);
-    if (token_of(A, s, t) < 0) return nullptr;
-    return base + (int64_t)t * ts + (int64_t)(m - t * A.G) * hs;
-  });
-}
-
-// Both operands K-major (64 columns of K per block of ROWSx x 128 bytes):
-// D[128 x N] (+)= A[128 x D] B[N x D]^T.
-template <int D, int RA, int RB>
-__device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-#pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk)
-    umma_bf16(d, smem_desc(a + (kk >> 2) * (RA * 128) + (kk & 3) * 32, 16, 1024),
-              smem_desc(b + (kk >> 2) * (RB * 128) + (kk & 3) * 32, 16, 1024), idesc, accumulate | (kk > 0));
-}
-// A K-major [128 x 64], B rows along K: D[128 x N] (+)= A B[64 x N].
-__device__ __forceinline__ void mma_kn(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-#pragma unroll
-  for (int kk = 0; kk < kTN / 16; ++kk)
-    umma_bf16(d, smem_desc(a + kk * 32, 16, 1024), smem_desc(b + kk * 2048, kTN * 128, 1024), idesc,
-              accumulate | (kk > 0));
-}
-
-// The same from the operands' descriptor words (a step's offset is one addition).
+// Both operands K-major, from their descriptor words (a step's offset is one
+// addition): D[128 x N] = A[RA x D] B[RB x D]^T.
 template <int D, int RA, int RB>
 __device__ __forceinline__ void issue_kk(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
 #pragma unroll
@@ -203,26 +153,6 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
 }
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
-}
-
-// The CTA's shared-memory writes and copies become visible to the tensor core;
-// true in every thread if any passes true.
-__device__ __forceinline__ bool publish(bool failed) {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  tc_fence_before();
-  const bool any = __syncthreads_or(failed ? 1 : 0) != 0;
-  tc_fence_after();
-  return any;
-}
-
-// After an expired wait: the status word, and a bounded wait for every product
-// that thread 0 has issued (a commit completes behind all of them).
-__device__ __forceinline__ void give_up(int* status, uint64_t* drain) {
-  if (threadIdx.x == 0) {
-    if (status) atomicExch(status, kStatusTimeout);
-    umma_commit(drain);
-  }
-  mbar_wait(drain, 0);
 }
 
 // ---- forward --------------------------------------------------------------------
@@ -326,7 +256,8 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OSLOT);
   const int warp = threadIdx.x >> 5;
   const int wg = threadIdx.x >> 7;  // 0 .. QT-1: softmax, QT: service
-  const int bh = blockIdx.x, b = bh / A.Hk, hk = bh - b * A.Hk;
+  const int hv_n = A.Hk * A.nsub;  // virtual heads: A.G query heads of one key head
+  const int bh = blockIdx.x, b = bh / hv_n, hv = bh - b * hv_n, hk = hv / A.nsub;
   const int m0 = (int)(gridDim.y - 1 - blockIdx.y) * (QT * kTM);  // the last tiles see the most keys: first
   const Seq sq = seq_of(A, b);
 
@@ -357,7 +288,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
 
   // this softmax thread's row
   const int m = m0 + (int)(threadIdx.x % (QT * kTM));
-  const int tq = group_div(A, min(m, A.M - 1)), hq = hk * A.G + min(m, A.M - 1) - tq * A.G;
+  const int tq = group_div(A, min(m, A.M - 1)), hq = hv * A.G + min(m, A.M - 1) - tq * A.G;
   bf16_t* orow = A.o + (((int64_t)b * A.Tq + tq) * A.Hq + hq) * D;
   const int64_t prow = ((int64_t)bh * A.M + m) * A.splits + (SPLIT ? blockIdx.z : 0);
   const bool mine = wg < QT && m < A.M;
@@ -478,7 +409,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
         for (int t = 0; t < QT; ++t)
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(base + C::OQ + t * C::QB + c * (kTM * 128), &A.mq, c * 64, hk * A.G,
+            tma_load_4d(base + C::OQ + t * C::QB + c * (kTM * 128), &A.mq, c * 64, hv * A.G,
                         (m0 + t * kTM) / A.G, b, q_full);
       }
       bool ok = true;
@@ -509,7 +440,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     if (!A.q_maps) {  // Q_t: this warpgroup's 128 rows
       constexpr int CH = D / 8;
       const int lt = threadIdx.x & 127, c = lt % CH;
-      const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)hk * A.G * A.qs[2];
+      const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)hv * A.G * A.qs[2];
 #pragma unroll 4
       for (int r = lt / CH; r < kTM; r += 128 / CH) {
         const int mr = mt + r, tr = group_div(A, mr);
@@ -688,368 +619,541 @@ __global__ void __launch_bounds__(128) window_join_kernel(const __grid_constant_
 }
 
 // ---- backward -------------------------------------------------------------------
-// No atomics: a kernel forms delta = sum_d dO o per packed row; then one grid
-// holds both roles. dq: a CTA per 128 packed rows walks its key tiles
-// (S = Q K^T, dP = dO V^T, dS = p (dP - delta) scale, dQ += dS K). dk/dv: a CTA
-// per 128 key rows walks the packed query rows that see them (S^T = K Q^T,
-// dP^T = V dO^T, dV += P^T dO, dK += dS^T Q); the group's heads are rows of the
-// same walk. 8 warps: warps w and w + 4 share TMEM lanes and split the columns.
-constexpr int kBT = 256;
-
-template <int D>
-struct DqCfg {
-  static constexpr uint32_t QT = kTM * D * 2, KT = kTN * D * 2;
-  static constexpr uint32_t OQ = 0, OG = QT, OK = 2 * QT, OV = OK + 2 * KT, OS = OV + KT;
-  static constexpr uint32_t OBAR = OS + kTM * 128, BYTES = OBAR + 32;
-  static constexpr uint32_t COL_S = 0, COL_P = 64, COL_ACC = 128;
-};
-template <int D>
-struct DkvCfg {
-  static constexpr uint32_t KT = kTM * D * 2, QT = kTN * D * 2;
-  static constexpr uint32_t OK = 0, OV = KT, OQ = 2 * KT, OG = OQ + 2 * QT, OP = OG + 2 * QT, OS = OP + kTM * 128;
-  static constexpr uint32_t OROW = OS + kTM * 128;  // two sets of lse, delta, lo, hi of 64 rows
-  static constexpr uint32_t OBAR = OROW + 2 * 4 * kTN * 4, BYTES = OBAR + 32;
-  static constexpr uint32_t COL_S = 0, COL_P = 64, COL_V = 128, COL_K = 128 + D;
-};
+// No atomics: a kernel forms, per packed row, -lse log2 e and -delta (delta =
+// sum_d dO o); then one grid holds two roles of the same shape. A CTA keeps 128
+// rows X1, X2 in shared memory and streams tiles of 64 rows Y1, Y2:
+//   dq      X = Q, dO of 128 packed rows;  Y = K, V of the keys they see
+//             S = Q K^T, dP = dO V^T, dS = P (dP - delta);  dQ += dS K
+//   dk/dv   X = K, V of 128 key rows;  Y = Q, dO of the packed rows that see them
+//             S^T = K Q^T, dP^T = V dO^T;  dV += P^T dO, dK += dS^T Q
+// (the scale is applied once, to dQ and dK at the end). One warp issues the
+// products, three copy (TMA; cp.async where a tile runs into padding), two
+// warpgroups take the steps in turn: step i's scores sit in tensor-memory buffer
+// i & 1, its P and dS go back over them in bf16 as the next product's A operand,
+// and S, dP of step i + 1 are computed meanwhile. Tensor memory: 2 x (64 + 64)
+// columns of scores, then the accumulators.
+//
+// The first key tile holds the sinks: every later context query sees them, far
+// more than see any other tile. Tiles with sinks are split over their queries
+// into `sink_splits` CTAs that leave fp32 partials, joined in order by a kernel.
 template <int D>
 struct BwdCfg {
-  static constexpr uint32_t BYTES = DqCfg<D>::BYTES > DkvCfg<D>::BYTES ? DqCfg<D>::BYTES : DkvCfg<D>::BYTES;
-  static constexpr uint32_t COLS = D == 64 ? 256 : 512;
-  static constexpr int CTAS = D == 64 ? 2 : 1;
+  static constexpr int NS = D == 128 ? 4 : 6;
+  static constexpr int THREADS = 384;
+  static constexpr uint32_t XB = kTM * D * 2, YB = kTN * D * 2;
+  static constexpr uint32_t OX = 0, OY = 2 * XB, OROW = OY + NS * 2 * YB;  // rows: 64 x (-lse2, -delta, lo, hi) per stage
+  static constexpr uint32_t OBAR = OROW + NS * kTN * 16;
+  static constexpr int NBAR = 3 * NS + 7;  // full, empty, r_full; s_full[2], p_full[2], x_full, o_full, drain
+  static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;
+  static constexpr uint32_t COLS = 512, COL_A = 256, COL_B = 256 + D;  // dQ or dV; dK
 };
 
-// Writes 32 bf16 values (16 words) of row r at columns [32 hh, 32 hh + 32) of a 64-column tile.
-__device__ __forceinline__ void st_half_row(uint32_t tile, uint32_t r, int hh, const uint32_t (&w)[16]) {
-#pragma unroll
-  for (int c4 = 0; c4 < 4; ++c4)
-    st_shared_u4(tile + sw128(r, (uint32_t)(hh * 4 + c4)),
-                 make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]));
+// Packed query rows that see a key of the 128 key rows from k0 on: context
+// tokens [a0, a1) and block rows [b0, b1), for each of the A.nsub sub-groups.
+struct QueryTiles {
+  int a0 = 0, a1 = 0, b0 = 0, b1 = 0, na, per, n;
+  __device__ __forceinline__ QueryTiles(const WindowArgs& A, const Seq& s, int k0) {
+    const int jmax = min(k0 + kTM, s.c) - 1;  // last context key of the tile
+    if (k0 < s.c) {
+      a0 = k0;
+      a1 = k0 < A.S ? s.c : min(s.c, jmax + A.W);  // W <= 2^30: no overflow
+    }
+    if (A.n_block > 0 && (min(k0 + kTM, A.Tq) > A.n_ctx || (k0 < s.c && (jmax >= s.c - A.W || k0 < A.S)))) {
+      b0 = A.n_ctx;
+      b1 = A.Tq;
+    }
+    na = ((a1 - a0) * A.G + kTN - 1) / kTN;
+    per = na + ((b1 - b0) * A.G + kTN - 1) / kTN;
+    n = per * A.nsub;
+  }
+  __device__ __forceinline__ int first(const WindowArgs& A, int r) const {
+    return r < na ? a0 * A.G + r * kTN : b0 * A.G + (r - na) * kTN;
+  }
+  __device__ __forceinline__ int last(const WindowArgs& A, int r) const {
+    return min(first(A, r) + kTN, (r < na ? a1 : b1) * A.G);
+  }
+};
+
+// 64 packed rows [m0, m1) (padding and the rest as zeros) by the copying warps,
+// as stage_keys.
+template <int NT, int D>
+__device__ __forceinline__ void stage_queries(const WindowArgs& A, uint32_t tile, const bf16_t* base, int64_t ts, int64_t hs,
+                                              const Seq& s, int m0, int m1, int rows, int lt, bool copy) {
+  constexpr int C = D / 8, RP = NT / C;
+  if (copy) {
+    const int c = lt % C;
+    const uint32_t dst = tile + (uint32_t)(c >> 3) * (uint32_t)(rows * 128);
+#pragma unroll 2
+    for (int r = lt / C; r < rows; r += RP) {
+      const int m = m0 + r, t = group_div(A, m);
+      const bool valid = m < m1 && token_of(A, s, t) >= 0;
+      cp_async16(dst + sw128((uint32_t)r, (uint32_t)(c & 7)),
+                 valid ? base + (int64_t)t * ts + (int64_t)(m - t * A.G) * hs + c * 8 : base, valid);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+  }
+  fence_proxy_async_smem();
+  asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-// One row's D / 2 columns of half `half` from tensor memory to global memory.
+// This thread's D / 2 columns (half `half`) of an accumulator row, times `f`.
 template <int D>
-__device__ __forceinline__ void store_acc(bf16_t* row, uint32_t col, int half, bool write, bool zero) {
+__device__ __forceinline__ void store_acc(bf16_t* row, float* part, uint32_t col, int half, float f, bool write, bool zero) {
 #pragma unroll
   for (int c = 0; c < D / 2; c += 32) {
     float a[32];
     tmem_ld32(col + half * (D / 2) + c, a);
     if (!write) continue;
+    const int at = half * (D / 2) + c;
 #pragma unroll
-    for (int j = 0; j < 32; j += 8)
-      *reinterpret_cast<uint4*>(row + half * (D / 2) + c + j) =
-          zero ? make_uint4(0, 0, 0, 0)
-               : make_uint4(pack_bf16x2(a[j], a[j + 1]), pack_bf16x2(a[j + 2], a[j + 3]),
-                            pack_bf16x2(a[j + 4], a[j + 5]), pack_bf16x2(a[j + 6], a[j + 7]));
+    for (int j = 0; j < 32; ++j) a[j] = zero ? 0.f : a[j] * f;
+    if (part) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        *reinterpret_cast<float4*>(part + at + j) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j += 8)
+        *reinterpret_cast<uint4*>(row + at + j) =
+            make_uint4(pack_bf16x2(a[j], a[j + 1]), pack_bf16x2(a[j + 2], a[j + 3]),
+                       pack_bf16x2(a[j + 4], a[j + 5]), pack_bf16x2(a[j + 6], a[j + 7]));
+    }
   }
 }
+// The same half row filled with one value: zeros, or NaN after an expired wait.
 template <int D>
-__device__ __forceinline__ void fill_row(bf16_t* row, int half, uint32_t word) {
+__device__ __forceinline__ void fill_row(bf16_t* row, float* part, int half, bool nan) {
+  const uint32_t w = nan ? kNan2 : 0u;
+  const float v = nan ? __int_as_float(0x7fc00000) : 0.f;
 #pragma unroll
-  for (int c = 0; c < D / 2; c += 8)
-    *reinterpret_cast<uint4*>(row + half * (D / 2) + c) = make_uint4(word, word, word, word);
+  for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 8) {
+    if (part) {
+      *reinterpret_cast<float4*>(part + c) = make_float4(v, v, v, v);
+      *reinterpret_cast<float4*>(part + c + 4) = make_float4(v, v, v, v);
+    } else {
+      *reinterpret_cast<uint4*>(row + c) = make_uint4(w, w, w, w);
+    }
+  }
 }
 
-template <int D>
-__device__ __forceinline__ void window_dq(const WindowArgs& A, int bh, int mt, bool fail_first) {
-  using C = DqCfg<D>;
+// P and dS of 32 columns: pr = 2^(s sl2 + nl), ds = pr (dp + nd).
+__device__ __forceinline__ void grad_pair(float2 s, float2 dp, float sl2, float2 nl, float2 nd, float2& pr, float2& ds) {
+  const float2 e = ffma2(s, make_float2(sl2, sl2), nl);
+  pr = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+  ds = fmul2(pr, fadd2(dp, nd));
+}
+
+template <int D, bool DKV>
+__device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int head, int tile, int split, bool withhold) {
+  using C = BwdCfg<D>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OBAR);
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OBAR + 16);
-  const int warp = threadIdx.x >> 5;
-  const int b = bh / A.Hk, hk = bh - b * A.Hk;
-  const int m0 = mt * kTM, m1 = min(A.M, m0 + kTM);
-  const int r_in = threadIdx.x & (kTM - 1), half = threadIdx.x >> 7;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem + C::OSLOT + 4);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OSLOT);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OBAR);
+  uint64_t* empty = full + C::NS;
+  uint64_t* r_full = empty + C::NS;
+  uint64_t* s_full = r_full + C::NS;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* x_full = p_full + 2;
+  uint64_t* o_full = x_full + 1;
+  uint64_t* drain = x_full + 2;
+  const int warp = threadIdx.x >> 5, wg = threadIdx.x >> 7;
   const Seq sq = seq_of(A, b);
-  const int m = m0 + r_in;
-  const int t = group_div(A, min(m, A.M - 1)), g = min(m, A.M - 1) - t * A.G;
-  bf16_t* drow = A.dq + (((int64_t)b * A.Tq + t) * A.Hq + hk * A.G + g) * D;
-  int p0, p1;
-  if (!token_range(A, sq, m0, m1 - 1, p0, p1)) {  // padding only
-    if (m < A.M) fill_row<D>(drow, half, 0u);
+  // dq: head = virtual head (A.G query heads), its key head; dk/dv: head = key head
+  const int hk = DKV ? head : head / A.nsub;
+  const int x0 = tile * kTM;  // packed row (dq) or key row (dk/dv) of X's first row
+
+  // steps [i0, i0 + n)
+  int p0 = 0, p1 = -1, i0 = 0, n = 0;
+  const bool some = DKV || token_range(A, sq, x0, min(A.M, x0 + kTM) - 1, p0, p1);
+  const KeyTiles<kTN> kt(A, sq, some ? p0 : 0, some ? p1 : -1);
+  const QueryTiles qt(A, sq, x0);
+  if (some) n = DKV ? qt.n : kt.n;
+  const bool partial = DKV && A.sink_splits > 1 && tile < A.sink_tiles;
+  if (partial) {
+    const int each = (n + A.sink_splits - 1) / A.sink_splits;
+    i0 = min(n, split * each);
+    n = min(n, i0 + each) - i0;
+  }
+
+  // this thread's output row: lane r of X
+  const int r = threadIdx.x & (kTM - 1), half = wg & 1;
+  const int xr = x0 + r;
+  bf16_t *row_a, *row_b = nullptr;  // dQ; or dV and dK
+  float *part_a = nullptr, *part_b = nullptr;
+  int token = -1;
+  bool mine = wg < 2;
+  if (DKV) {
+    mine = mine && xr < A.Tq;
+    token = mine ? token_of(A, sq, xr) : -1;
+    const int64_t at = (((int64_t)b * A.Tq + min(xr, A.Tq - 1)) * A.Hk + hk) * D;
+    row_a = A.dv + at;
+    row_b = A.dk + at;
+    if (partial) {  // [B Hk, sink tile, split, dV | dK, row, D]
+      part_a = A.sink_part +
+               (((((int64_t)b * A.Hk + hk) * A.sink_tiles + tile) * A.sink_splits + split) * 2 * kTM + r) * D;
+      part_b = part_a + (int64_t)kTM * D;
+    }
+  } else {
+    mine = mine && xr < A.M;
+    const int m = min(xr, A.M - 1), t = group_div(A, m);
+    token = mine ? token_of(A, sq, t) : -1;
+    row_a = A.dq + (((int64_t)b * A.Tq + t) * A.Hq + head * A.G + m - t * A.G) * D;
+  }
+  if (n == 0) {  // padding only, or no step left for this split
+    if (mine) {
+      fill_row<D>(row_a, part_a, half, false);
+      if (DKV) fill_row<D>(row_b, part_b, half, false);
+    }
     return;
   }
-  const KeyTiles<kTN> kt(A, sq, p0, p1);
-  const int lo_last = low_of(A, sq, p1), hi_first = high_of(sq, p0);
-  const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
-  const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
+
+  const bool x_boxes = DKV ? A.kv_maps : A.q_maps, y_boxes = DKV ? A.q_maps : A.kv_maps;
   if (threadIdx.x == 0) {
-    mbar_init(bar, 1);
-    mbar_init(bar + 1, 1);
+#pragma unroll
+    for (int i = 0; i < C::NS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+      mbar_init(r_full + i, 128);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+    }
+    mbar_init(x_full, 1);
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
     fence_mbar_init();
+    *dead = 0;
   }
-  if (warp == 0) tmem_alloc(slot, BwdCfg<D>::COLS);
-  load_queries<kBT, kTM, D>(A, base + C::OQ, A.q + (int64_t)b * A.qs[0] + (int64_t)hk * A.G * A.qs[2], A.qs[1], A.qs[2],
-                            sq, m0, m1);
-  load_queries<kBT, kTM, D>(A, base + C::OG, A.dO + ((int64_t)b * A.Tq * A.Hq + (int64_t)hk * A.G) * D,
-                            (int64_t)A.Hq * D, D, sq, m0, m1);
-  load_keys<kBT, kTN, D>(base + C::OK, kb, A.ks[1], sq, kt.start(0), kt.end(0));
-  load_keys<kBT, kTN, D>(base + C::OV, vb, A.vs[1], sq, kt.start(0), kt.end(0));
-  cp_async_commit();
-  const int p = m < A.M ? token_of(A, sq, t) : -1;
-  const int lo = low_of(A, sq, p), hi = high_of(sq, p);
-  float delta = 0.f, lse2 = 0.f;
-  if (p >= 0) {
-    delta = A.delta[(int64_t)bh * A.M + m];
-    lse2 = A.lse[(int64_t)bh * A.M + m] * kLog2e;
-  }
-  constexpr uint32_t kIdS = instr_desc(kTM, kTN, 0, 0);
-  constexpr uint32_t kIdQ = instr_desc(kTM, D, 0, 1);
-  uint32_t ph = 0, tmem = 0, lane = 0;
-  bool ok = true;
-  for (int i = 0; i < kt.n; ++i) {
-    const uint32_t kcur = C::OK + (i & 1) * C::KT, knext = C::OK + ((i & 1) ^ 1) * C::KT;
-    cp_async_wait<0>();  // this K and V tile
-    publish(false);
-    if (i == 0) {
-      tmem = *slot;
-      lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  if (warp == 8) tmem_alloc(slot, C::COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  int issued = 0;  // stages that this thread's copies have begun
+
+  if (wg == 2) {
+    if (warp == 8) {
+      // ---- products: the warp walks together, one lane issues ----
+      constexpr uint32_t kIdS = instr_desc(kTM, kTN, 0, 0);
+      constexpr uint32_t kIdA = instr_desc(kTM, D, 0, 1);
+      const uint32_t x1 = desc_low(base + C::OX, 16), x2 = desc_low(base + C::OX + C::XB, 16);
+      const uint32_t yk = desc_low(base + C::OY, 16), yn = desc_low(base + C::OY, kTN * 128);
+      uint32_t slot_s = 0, ph_s = 0, slot_a = 0;  // ring slots of step i and of step i - 1
+      bool ok = wait_alive(x_full, 0, dead, A.status);
+      for (int i = 0; i <= n && ok; ++i) {
+        if (i < n) {
+          ok = wait_alive(full + slot_s, ph_s, dead, A.status);
+          if (!ok) break;
+          tc_fence_after();
+          // the buffer's previous P and dS were read by products issued before
+          // (failure-detection test hook: the first step's products are withheld)
+          if (!(withhold && i == 0)) {
+            if (elect_one()) {
+              const uint32_t y = yk + slot_s * (2 * C::YB >> 4), d = tmem + (i & 1) * 128;
+              issue_kk<D, kTM, kTN>(d, x1, y, kIdS);
+              issue_kk<D, kTM, kTN>(d + 64, x2, y + (C::YB >> 4), kIdS);
+              umma_commit(s_full + (i & 1));
+            }
+            __syncwarp();
+          }
+          if (++slot_s == C::NS) slot_s = 0, ph_s ^= 1;
+        }
+        if (i > 0) {
+          const int j = i - 1;
+          ok = wait_alive(p_full + (j & 1), (j >> 1) & 1, dead, A.status);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t y = yn + slot_a * (2 * C::YB >> 4), d = tmem + (j & 1) * 128;
+            if (DKV) {
+              issue_tn<kTN / 16>(tmem + C::COL_A, d, y + (C::YB >> 4), kIdA, j > 0);  // dV += P^T dO
+              issue_tn<kTN / 16>(tmem + C::COL_B, d + 64, y, kIdA, j > 0);            // dK += dS^T Q
+            } else {
+              issue_tn<kTN / 16>(tmem + C::COL_A, d + 64, y, kIdA, j > 0);            // dQ += dS K
+            }
+            umma_commit(empty + slot_a);
+          }
+          __syncwarp();
+          if (++slot_a == C::NS) slot_a = 0;
+        }
+      }
+      if (ok && elect_one()) umma_commit(o_full);
+      __syncwarp();
+    } else {
+      // ---- copies ----
+      const int lt = (int)threadIdx.x - 288;
+      const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
+      const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
+      const int q_head = DKV ? hk * A.nsub * A.G : head * A.G;  // first query head (of sub-group 0)
+      const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)q_head * A.qs[2];
+      const bf16_t* gb = A.dO + ((int64_t)b * A.Tq * A.Hq + q_head) * D;
+      const int64_t gts = (int64_t)A.Hq * D;
+      if (x_boxes) {
+        if (lt == 0) {
+          mbar_arrive_expect_tx(x_full, 2 * C::XB);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {
+                const uint32_t dst = base + C::OX + x * C::XB + c * (kTM * 128) + h * (64 * 128);
+                if (DKV)
+                  tma_load_4d(dst, x ? &A.mv : &A.mk, c * 64, x0 + h * 64, hk, b, x_full);
+                else
+                  tma_load_4d(dst, x ? &A.mg : &A.mq, c * 64, q_head, (x0 + h * 64) / A.G, b, x_full);
+              }
+        }
+      } else {
+        if (DKV) {  // key rows [x0, x0 + 128) of the batch: tokens or padding (zeros)
+#pragma unroll 1
+          for (int x = 0; x < 2; ++x) {
+            constexpr int CH = D / 8;
+            const int c = lt % CH;
+            const bf16_t* src = x ? vb : kb;
+            const int64_t ts = x ? A.vs[1] : A.ks[1];
+            for (int q = lt / CH; q < kTM; q += 96 / CH) {
+              const bool valid = x0 + q < A.Tq && token_of(A, sq, x0 + q) >= 0;
+              cp_async16(base + C::OX + x * C::XB + (uint32_t)(c >> 3) * (kTM * 128u) + sw128((uint32_t)q, (uint32_t)(c & 7)),
+                         valid ? src + (int64_t)(x0 + q) * ts + c * 8 : src, valid);
+            }
+          }
+          cp_async_commit();
+          cp_async_wait<0>();
+          fence_proxy_async_smem();
+          asm volatile("bar.sync 1, 96;" ::: "memory");
+        } else {
+          stage_queries<96, D>(A, base + C::OX, qb, A.qs[1], A.qs[2], sq, x0, A.M, kTM, lt, true);
+          stage_queries<96, D>(A, base + C::OX + C::XB, gb, gts, D, sq, x0, A.M, kTM, lt, true);
+        }
+        if (lt == 0) mbar_arrive(x_full);
+      }
+      bool ok = true;
+      int sub = 0, rr = 0;  // dk/dv: sub-group and tile of the step
+      if (DKV) {
+        sub = i0 / qt.per;
+        rr = i0 - sub * qt.per;
+      }
+      uint32_t sl = 0, ph = 1;  // the ring's first pass finds every slot free
+      for (int i = 0; i < n; ++i) {  // no early exit: the copying threads meet in stage_*
+        if (ok) ok = wait_alive(empty + sl, ph, dead, A.status);
+        if (ok) issued = i + 1;
+        const uint32_t y1 = base + C::OY + sl * 2 * C::YB, y2 = y1 + C::YB;
+        if (DKV) {
+          const int f = qt.first(A, rr), l = qt.last(A, rr);
+          const int t0 = f / A.G, t1 = t0 + kTN / A.G;
+          if (lt < kTN) {  // -lse2, -delta and the bounds of the keys that row f + lt sees
+            const uint32_t rowp = base + C::OROW + (sl * kTN + lt) * 16;
+            const int m = f + lt;
+            if (ok) {
+              const float2* src = A.rows + ((int64_t)b * A.Hk * A.nsub + hk * A.nsub + sub) * A.M + (m < l ? m : f);
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(rowp), "l"(src), "r"(m < l ? 8 : 0) : "memory");
+              const int p = m < l ? token_of(A, sq, group_div(A, m)) : -1;
+              asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(rowp + 8), "r"(low_of(A, sq, p)), "r"(high_of(sq, p))
+                           : "memory");
+              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(r_full + sl)) : "memory");
+              mbar_arrive(r_full + sl);
+            }
+          }
+          if (y_boxes && (t1 <= sq.c || t0 >= A.n_ctx || sq.c == A.n_ctx)) {
+            if (ok && lt == 0) {
+              mbar_arrive_expect_tx(full + sl, 2 * C::YB);
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {
+                tma_load_4d(y1 + c * (kTN * 128), &A.mq, c * 64, q_head + sub * A.G, t0, b, full + sl);
+                tma_load_4d(y2 + c * (kTN * 128), &A.mg, c * 64, q_head + sub * A.G, t0, b, full + sl);
+              }
+            }
+          } else {
+            stage_queries<96, D>(A, y1, qb + (int64_t)sub * A.G * A.qs[2], A.qs[1], A.qs[2], sq, f, l, kTN, lt, ok);
+            stage_queries<96, D>(A, y2, gb + (int64_t)sub * A.G * D, gts, D, sq, f, l, kTN, lt, ok);
+            if (ok && lt == 0) mbar_arrive(full + sl);
+          }
+          if (++rr == qt.per) rr = 0, ++sub;
+        } else {
+          const int j0 = kt.start(i);
+          if (y_boxes && boxed<kTN>(sq, j0)) {
+            if (ok && lt == 0) {
+              const int row = j0 < sq.c ? j0 : j0 + sq.kb - sq.c;
+              mbar_arrive_expect_tx(full + sl, 2 * C::YB);
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {
+                tma_load_4d(y1 + c * (kTN * 128), &A.mk, c * 64, row, hk, b, full + sl);
+                tma_load_4d(y2 + c * (kTN * 128), &A.mv, c * 64, row, hk, b, full + sl);
+              }
+            }
+          } else {
+            stage_keys<96, kTN, D>(y1, kb, A.ks[1], sq, j0, kt.end(i), lt, ok);
+            stage_keys<96, kTN, D>(y2, vb, A.vs[1], sq, j0, kt.end(i), lt, ok);
+            if (ok && lt == 0) mbar_arrive(full + sl);
+          }
+        }
+        if (++sl == C::NS) sl = 0, ph ^= 1;
+      }
+      cp_async_wait<0>();  // no copy outlives the CTA
     }
-    // the other K buffer was last read by the previous step's dQ product
-    if (i + 1 < kt.n) load_keys<kBT, kTN, D>(base + knext, kb, A.ks[1], sq, kt.start(i + 1), kt.end(i + 1));
-    cp_async_commit();
-    if (threadIdx.x == 0 && !(fail_first && i == 0)) {
-      mma_kk<D, kTM, kTN>(tmem + C::COL_S, base + C::OQ, base + kcur, kIdS, 0);
-      mma_kk<D, kTM, kTN>(tmem + C::COL_P, base + C::OG, base + C::OV, kIdS, 0);
-      umma_commit(bar);
+  } else {
+    // ---- P and dS of steps wg, wg + 2, ... ----
+    const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t buf = lane + wg * 128;
+    const int lo = low_of(A, sq, token), hi = high_of(sq, token);
+    const int lo_last = low_of(A, sq, p1), hi_first = high_of(sq, p0);
+    float2 nl = make_float2(0.f, 0.f), nd = nl;
+    if (!DKV && token >= 0) {
+      const float2 v = A.rows[((int64_t)b * A.Hk * A.nsub + head) * A.M + xr];
+      nl = make_float2(v.x, v.x);
+      nd = make_float2(v.y, v.y);
     }
-    if (__syncthreads_or(!mbar_wait(bar, ph) ? 1 : 0)) {
-      ok = false;
-      break;
-    }
-    ph ^= 1u;
-    tc_fence_after();
-    if (i + 1 < kt.n) load_keys<kBT, kTN, D>(base + C::OV, vb, A.vs[1], sq, kt.start(i + 1), kt.end(i + 1));
-    cp_async_commit();
-    {
-      float sv[32], dp[32];
-      tmem_ld32x2(lane + C::COL_S + half * 32, lane + C::COL_P + half * 32, sv, dp);
-      const bool full = kt.full(i, lo_last, hi_first);
-      const int k0 = kt.start(i) + half * 32;
+    bool ok = true;
+    uint32_t k = 0, sl = wg % C::NS, rph = 0;
+    for (int i = wg; i < n; i += 2, ++k) {
+      ok = __all_sync(kFullMask, wait_alive(s_full + wg, k & 1, dead, A.status));
+      if (DKV) ok = ok && __all_sync(kFullMask, wait_alive(r_full + sl, rph, dead, A.status));
+      if (!ok) break;
+      tc_fence_after();
+      const float4* rows = reinterpret_cast<const float4*>(smem + C::OROW + sl * (kTN * 16));  // (-lse2, -delta, lo, hi)
+      bool whole;  // every row of X sees (is seen by) every row of Y
+      if (DKV) {
+        const float4 ra = rows[0], rz = rows[kTN - 1];
+        whole = x0 + kTM <= sq.c && __float_as_int(ra.w) >= x0 + kTM && __float_as_int(rz.w) > 0 &&
+                __float_as_int(rz.z) <= x0;
+      } else {
+        whole = kt.full(i, lo_last, hi_first);
+      }
+      const int j0 = kt.start(DKV ? 0 : i);
       const bool in_sink = i < kt.ns;
-      const int rl = in_sink ? kTN : lo - k0, rh = hi - k0, rs = (in_sink ? kt.sink : A.S) - k0;
-      uint32_t w[16];
+      const int rl = in_sink ? kTN : lo - j0, rh = hi - j0, rs = (in_sink ? kt.sink : A.S) - j0;
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        float d[2];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sr[32], dr[32];
+        tmem_ld32_async(buf + h * 32, sr);
+        tmem_ld32_async(buf + 64 + h * 32, dr);
+        tmem_wait_ld();
+        uint32_t wp[16], wd[16];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float pr = exp2_approx(fmaf(sv[j + e], A.scale_log2, -lse2));
-          d[e] = pr * (dp[j + e] - delta) * A.scale;
-          if (!full && !(j + e < rh && (j + e >= rl || j + e < rs))) d[e] = 0.f;
+        for (int j = 0; j < 32; j += 2) {
+          float2 pr, ds;
+          float4 ra, rb;
+          if (DKV) {
+            ra = rows[h * 32 + j];
+            rb = rows[h * 32 + j + 1];
+            nl = make_float2(ra.x, rb.x);
+            nd = make_float2(ra.y, rb.y);
+          }
+          grad_pair(make_float2(__uint_as_float(sr[j]), __uint_as_float(sr[j + 1])),
+                    make_float2(__uint_as_float(dr[j]), __uint_as_float(dr[j + 1])), A.scale_log2, nl, nd, pr, ds);
+          if (!whole) {
+            bool va, vb;
+            if (DKV) {
+              va = token >= 0 && token < __float_as_int(ra.w) && (token >= __float_as_int(ra.z) || token < A.S);
+              vb = token >= 0 && token < __float_as_int(rb.w) && (token >= __float_as_int(rb.z) || token < A.S);
+            } else {
+              const int e = h * 32 + j;
+              va = e < rh && (e >= rl || e < rs);
+              vb = e + 1 < rh && (e + 1 >= rl || e + 1 < rs);
+            }
+            if (!va) pr.x = ds.x = 0.f;
+            if (!vb) pr.y = ds.y = 0.f;
+          }
+          if (DKV) wp[j / 2] = pack_bf16x2(pr.x, pr.y);
+          wd[j / 2] = pack_bf16x2(ds.x, ds.y);
         }
-        w[j / 2] = pack_bf16x2(d[0], d[1]);
+        // the 32 columns read so far are free: P over S, dS over dP
+        if (DKV) tmem_st16(buf + h * 16, wp);
+        tmem_st16(buf + 64 + h * 16, wd);
       }
-      st_half_row(base + C::OS, (uint32_t)r_in, half, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_full + wg);
+      sl += 2;
+      if (sl >= C::NS) sl -= C::NS, rph ^= 1;
     }
-    publish(false);
-    if (threadIdx.x == 0) {
-      mma_kn(tmem + C::COL_ACC, base + C::OS, base + kcur, kIdQ, i > 0);
-      umma_commit(bar);
-    }
-    if (__syncthreads_or(!mbar_wait(bar, ph) ? 1 : 0)) {
-      ok = false;
-      break;
-    }
-    ph ^= 1u;
-  }
-  cp_async_wait<0>();  // no copy outlives the CTA
-  tc_fence_after();
-  if (!ok) {
-    give_up(A.status, bar + 1);
-    if (m < A.M) fill_row<D>(drow, half, kNan2);
-  } else {
-    store_acc<D>(drow, lane + C::COL_ACC, half, m < A.M, p < 0);
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (warp == 0) tmem_free(tmem, BwdCfg<D>::COLS);
-}
-
-template <int D>
-__device__ __forceinline__ void window_dkv(const WindowArgs& A, int bh, int ktile, bool fail_first) {
-  using C = DkvCfg<D>;
-  extern __shared__ __align__(1024) unsigned char smem[];
-  const uint32_t base = smem_u32(smem);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OBAR);
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OBAR + 16);
-  const int warp = threadIdx.x >> 5;
-  const int b = bh / A.Hk, hk = bh - b * A.Hk;
-  const int r_in = threadIdx.x & (kTM - 1), half = threadIdx.x >> 7;
-  const Seq sq = seq_of(A, b);
-  const int T = A.Tq, k0 = ktile * kTM, krow = k0 + r_in;  // key row of the batch
-  const int key = krow < T ? token_of(A, sq, krow) : -1;     // its token, -1: padding
-  bf16_t* kr = A.dk + (((int64_t)b * T + min(krow, T - 1)) * A.Hk + hk) * D;
-  bf16_t* vr = A.dv + (((int64_t)b * T + min(krow, T - 1)) * A.Hk + hk) * D;
-  // query rows that see a key of this tile: context rows [a0, a1), block rows [b0, b1)
-  int a0 = 0, a1 = 0, b0 = 0, b1 = 0;
-  const int jmax = min(k0 + kTM, sq.c) - 1;  // last context key of the tile
-  if (k0 < sq.c) {
-    a0 = k0;
-    a1 = k0 < A.S ? sq.c : min(sq.c, jmax + A.W);  // W <= 2^30: no overflow
-  }
-  if (A.n_block > 0 && (min(k0 + kTM, T) > A.n_ctx || (k0 < sq.c && (jmax >= sq.c - A.W || k0 < A.S)))) {
-    b0 = A.n_ctx;
-    b1 = T;
-  }
-  const int na = ((a1 - a0) * A.G + kTN - 1) / kTN, n = na + ((b1 - b0) * A.G + kTN - 1) / kTN;
-  if (n == 0) {  // padding only
-    if (krow < T) {
-      fill_row<D>(kr, half, 0u);
-      fill_row<D>(vr, half, 0u);
-    }
-    return;
-  }
-  const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)hk * A.G * A.qs[2];
-  const bf16_t* gb = A.dO + ((int64_t)b * T * A.Hq + (int64_t)hk * A.G) * D;
-  // packed rows [first, last) of query tile i
-  auto first_of = [&](int i) { return i < na ? a0 * A.G + i * kTN : b0 * A.G + (i - na) * kTN; };
-  auto last_of = [&](int i) { return min(first_of(i) + kTN, (i < na ? a1 : b1) * A.G); };
-  auto load_query_tile = [&](int i, int set) {
-    const int f = first_of(i), l = last_of(i);
-    load_queries<kBT, kTN, D>(A, base + C::OQ + set * C::QT, qb, A.qs[1], A.qs[2], sq, f, l);
-    load_queries<kBT, kTN, D>(A, base + C::OG + set * C::QT, gb, (int64_t)A.Hq * D, D, sq, f, l);
-    const uint32_t rows = base + C::OROW + set * (4 * kTN * 4);
-    if (r_in < kTN) {  // half 0 copies lse of row f + r_in, half 1 its delta
-      const int mq = f + r_in;
-      cp_async4(rows + 4u * (half * kTN + r_in), (half ? A.delta : A.lse) + (int64_t)bh * A.M + (mq < l ? mq : f),
-                mq < l);
-    } else {  // bounds of the rows' visible keys (nothing for rows past the end)
-      const int mq = f + r_in - kTN;
-      const int p = mq < l ? token_of(A, sq, group_div(A, mq)) : -1;
-      int* bounds = reinterpret_cast<int*>(smem + C::OROW + set * (4 * kTN * 4)) + (2 + half) * kTN;
-      bounds[r_in - kTN] = half ? high_of(sq, p) : low_of(A, sq, p);
-    }
-  };
-  auto load_key_rows = [&](uint32_t tile, const bf16_t* src, int64_t ts) {
-    load_tile<kBT, kTM, D>(tile, src, [&](int r) -> const bf16_t* {
-      const int row = k0 + r;
-      return row < T && token_of(A, sq, row) >= 0 ? src + (int64_t)row * ts : nullptr;
-    });
-  };
-  if (threadIdx.x == 0) {
-    mbar_init(bar, 1);
-    mbar_init(bar + 1, 1);
-    fence_mbar_init();
-  }
-  if (warp == 0) tmem_alloc(slot, BwdCfg<D>::COLS);
-  load_key_rows(base + C::OK, A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2], A.ks[1]);
-  load_key_rows(base + C::OV, A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2], A.vs[1]);
-  load_query_tile(0, 0);
-  cp_async_commit();
-  constexpr uint32_t kIdS = instr_desc(kTM, kTN, 0, 0);
-  constexpr uint32_t kIdKV = instr_desc(kTM, D, 0, 1);
-  uint32_t ph = 0, tmem = 0, lane = 0;
-  bool ok = true;
-  for (int i = 0; i < n; ++i) {
-    const int set = i & 1;
-    const uint32_t offq = C::OQ + set * C::QT, offg = C::OG + set * C::QT;
-    const float* sh_lse = reinterpret_cast<const float*>(smem + C::OROW + set * (4 * kTN * 4));
-    const float* sh_delta = sh_lse + kTN;
-    const int* sh_lo = reinterpret_cast<const int*>(sh_lse + 2 * kTN);
-    const int* sh_hi = sh_lo + kTN;
-    cp_async_wait<0>();  // this query tile
-    publish(false);
-    if (i == 0) {
-      tmem = *slot;
-      lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    }
-    // the other set was last read by the previous step's products
-    if (i + 1 < n) load_query_tile(i + 1, set ^ 1);
-    cp_async_commit();
-    if (threadIdx.x == 0 && !(fail_first && i == 0)) {
-      mma_kk<D, kTM, kTN>(tmem + C::COL_S, base + C::OK, base + offq, kIdS, 0);
-      mma_kk<D, kTM, kTN>(tmem + C::COL_P, base + C::OV, base + offg, kIdS, 0);
-      umma_commit(bar);
-    }
-    if (__syncthreads_or(!mbar_wait(bar, ph) ? 1 : 0)) {
-      ok = false;
-      break;
-    }
-    ph ^= 1u;
+    if (ok) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
     tc_fence_after();
-    {
-      float sv[32], dp[32];
-      tmem_ld32x2(lane + C::COL_S + half * 32, lane + C::COL_P + half * 32, sv, dp);
-      // every query of the tile sees every (context) key of this CTA's tile
-      const bool full = last_of(i) - first_of(i) == kTN && k0 + kTM <= sq.c && sh_hi[0] >= k0 + kTM &&
-                        sh_lo[kTN - 1] <= k0;
-      uint32_t wp[16], wd[16];
-#pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        float pr[2], d[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = half * 32 + j + e;
-          pr[e] = exp2_approx(fmaf(sv[j + e], A.scale_log2, -sh_lse[c] * kLog2e));
-          d[e] = pr[e] * (dp[j + e] - sh_delta[c]) * A.scale;
-          if (!full && !(key >= 0 && key < sh_hi[c] && (key >= sh_lo[c] || key < A.S))) pr[e] = d[e] = 0.f;
-        }
-        wp[j / 2] = pack_bf16x2(pr[0], pr[1]);
-        wd[j / 2] = pack_bf16x2(d[0], d[1]);
+    if (!ok) {  // never a plausible wrong number
+      if (mine) {
+        fill_row<D>(row_a, part_a, half, true);
+        if (DKV) fill_row<D>(row_b, part_b, half, true);
       }
-      st_half_row(base + C::OP, (uint32_t)r_in, half, wp);
-      st_half_row(base + C::OS, (uint32_t)r_in, half, wd);
+    } else {
+      store_acc<D>(row_a, part_a, lane + C::COL_A, half, DKV ? 1.f : A.scale, mine, token < 0);
+      if (DKV) store_acc<D>(row_b, part_b, lane + C::COL_B, half, A.scale, mine, token < 0);
     }
-    publish(false);
-    if (threadIdx.x == 0) {
-      mma_kn(tmem + C::COL_V, base + C::OP, base + offg, kIdKV, i > 0);
-      mma_kn(tmem + C::COL_K, base + C::OS, base + offq, kIdKV, i > 0);
-      umma_commit(bar);
-    }
-    if (__syncthreads_or(!mbar_wait(bar, ph) ? 1 : 0)) {
-      ok = false;
-      break;
-    }
-    ph ^= 1u;
-  }
-  cp_async_wait<0>();  // no copy outlives the CTA
-  tc_fence_after();
-  if (!ok) {
-    give_up(A.status, bar + 1);
-    if (krow < T) {
-      fill_row<D>(kr, half, kNan2);
-      fill_row<D>(vr, half, kNan2);
-    }
-  } else {
-    store_acc<D>(vr, lane + C::COL_V, half, krow < T, key < 0);
-    store_acc<D>(kr, lane + C::COL_K, half, krow < T, key < 0);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) tmem_free(tmem, BwdCfg<D>::COLS);
+  if (*dead) {  // bounded waits for every product and box that was issued
+    if (warp == 8 && (threadIdx.x & 31) == 0) umma_commit(drain);
+    mbar_wait(drain, 0);
+    if (threadIdx.x == 288) {
+      mbar_wait(x_full, 0);
+      for (int i = max(0, issued - C::NS); i < issued; ++i) mbar_wait(full + i % C::NS, (i / C::NS) & 1);
+    }
+    __syncthreads();
+  }
+  if (warp == 8) tmem_free(tmem, C::COLS);
 }
 
-// Blocks in dispatch order: the dk/dv tiles (longer by the group's heads), then
-// the dq tiles, each from the first key tile / the last query tile on.
+// Blocks in dispatch order: the parts of the sink tiles, the other dk/dv tiles
+// (longer than the dq tiles by the group's heads), the dq tiles from the last on.
 template <int D>
-__global__ void __launch_bounds__(kBT, BwdCfg<D>::CTAS) window_bwd_kernel(const __grid_constant__ WindowArgs A) {
-  const int bhs = A.B * A.Hk;
-  const int tile = (int)(blockIdx.x / bhs), bh = (int)(blockIdx.x - (unsigned)tile * bhs);
+__global__ void __launch_bounds__(BwdCfg<D>::THREADS, 1) window_bwd_kernel(const __grid_constant__ WindowArgs A) {
   const int nk = (A.Tq + kTM - 1) / kTM, nq = (A.M + kTM - 1) / kTM;
-  const bool fail_first = A.withhold && bh == 0 && (tile == 0 || tile == nk);
-  if (tile < nk)
-    window_dkv<D>(A, bh, tile, fail_first);
-  else
-    window_dq<D>(A, bh, nq - 1 - (tile - nk), fail_first);
+  const int sinks = A.sink_tiles * A.sink_splits, bk = A.B * A.Hk, bv = bk * A.nsub;
+  const int64_t dkv = (int64_t)(sinks + nk - A.sink_tiles) * bk;
+  const int64_t i = blockIdx.x;
+  if (i < dkv) {
+    const int job = (int)(i / bk), bh = (int)(i - (int64_t)job * bk), b = bh / A.Hk;
+    const int tile = job < sinks ? job / A.sink_splits : job - sinks + A.sink_tiles;
+    const int split = job < sinks ? job - tile * A.sink_splits : 0;
+    window_bwd_role<D, true>(A, b, bh - b * A.Hk, tile, split, A.withhold && i == 0);
+  } else {
+    const int64_t q = i - dkv;
+    const int tile = nq - 1 - (int)(q / bv), bh = (int)(q % bv), hv = A.Hk * A.nsub, b = bh / hv;
+    window_bwd_role<D, false>(A, b, bh - b * hv, tile, 0, A.withhold && q == 0);
+  }
 }
 
-// delta[bh, m] = sum_d dO o of every packed row (fp32, in order); a thread per
-// row, rows in the tensors' order.
+// Sums a sink tile's partials in split order: a thread per 4 elements of a row.
 template <int D>
-__global__ void __launch_bounds__(256) window_delta_kernel(const __grid_constant__ WindowArgs A) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;  // over [B, Tq, Hq]
-  if (i >= (int64_t)A.B * A.Tq * A.Hq) return;
-  const int h = (int)(i % A.Hq), t = (int)((i / A.Hq) % A.Tq), b = (int)(i / ((int64_t)A.Hq * A.Tq));
-  const bf16_t* orow = A.o + i * D;
-  const bf16_t* grow = A.dO + i * D;
+__global__ void __launch_bounds__(256) window_sink_join_kernel(const __grid_constant__ WindowArgs A) {
+  constexpr int Q = D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // [B Hk, sink tile, dV | dK, row, D / 4]
+  const int64_t per = (int64_t)A.sink_tiles * 2 * kTM * Q;
+  if (i >= per * A.B * A.Hk) return;
+  const int c = (int)(i % Q) * 4, r = (int)(i / Q % kTM), which = (int)(i / (Q * kTM) % 2);
+  const int tile = (int)(i / (2 * Q * kTM) % A.sink_tiles);
+  const int64_t bh = i / per;
+  const int row = tile * kTM + r, b = (int)(bh / A.Hk), hk = (int)(bh % A.Hk);
+  if (row >= A.Tq) return;
+  const float* p = A.sink_part + ((((bh * A.sink_tiles + tile) * A.sink_splits) * 2 + which) * kTM + r) * D + c;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int z = 0; z < A.sink_splits; ++z, p += 2 * kTM * D) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  bf16_t* out = (which ? A.dk : A.dv) + (((int64_t)b * A.Tq + row) * A.Hk + hk) * D + c;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+}
+
+// rows[b, virtual head, m] = (-lse log2 e, -sum_d dO o) of every packed row;
+// D / 8 lanes per row, rows in the tensors' order. Padding: (0, 0), masked later.
+template <int D>
+__global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant__ WindowArgs A) {
+  constexpr int L = D / 8;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;  // over [B, Tq, Hq]
+  const int c = threadIdx.x % L;
+  const bool on = i < (int64_t)A.B * A.Tq * A.Hq;
   float d = 0.f;
-#pragma unroll
-  for (int c = 0; c < D / 8; ++c) {
-    const uint4 a = *reinterpret_cast<const uint4*>(orow + 8 * c);
-    const uint4 g = *reinterpret_cast<const uint4*>(grow + 8 * c);
+  if (on) {
+    const uint4 a = *reinterpret_cast<const uint4*>(A.o + i * D + 8 * c);
+    const uint4 g = *reinterpret_cast<const uint4*>(A.dO + i * D + 8 * c);
     const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1057,8 +1161,14 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const __grid_constant
       d = fmaf(bf16_hi(aw[j]), bf16_hi(gw[j]), d);
     }
   }
-  const int hk = h / A.G;
-  A.delta[((int64_t)b * A.Hk + hk) * A.M + (int64_t)t * A.G + (h - hk * A.G)] = d;
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) d += __shfl_xor_sync(kFullMask, d, o);
+  if (!on || c != 0) return;
+  const int h = (int)(i % A.Hq), t = (int)((i / A.Hq) % A.Tq), b = (int)(i / ((int64_t)A.Hq * A.Tq));
+  const int hv = h / A.G;
+  const int64_t at = ((int64_t)b * A.Hk * A.nsub + hv) * A.M + (int64_t)t * A.G + (h - hv * A.G);
+  const float lse = A.lse[at];
+  A.rows[at] = lse == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-lse * kLog2e, -d);
 }
 
 // Raises a kernel's dynamic shared-memory limit once per device; refuses a
@@ -1139,7 +1249,7 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   kv_maps(A, D, C::KN);
   A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
-  const dim3 grid((unsigned)(A.B * A.Hk), (unsigned)((A.M + QT * kTM - 1) / (QT * kTM)), (unsigned)A.splits);
+  const dim3 grid((unsigned)(A.B * A.Hk * A.nsub), (unsigned)((A.M + QT * kTM - 1) / (QT * kTM)), (unsigned)A.splits);
   window_fwd_kernel<D, QT, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
   return cudaGetLastError();
 }
@@ -1151,7 +1261,7 @@ cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
     // one tile per CTA fills the device with less: us with one / two at D = 128,
     // 512 pairs of tiles: 1024 keys seen 101 / 102, 2048 keys 160 / 145, 4096 keys
     // 232 / 188, 512 keys 71 / 80; at D = 64: 84 / 85, 135 / 125, 199 / 169, 57 / 66.
-    const int64_t pairs = (int64_t)A.B * A.Hk * ((A.M + 2 * kTM - 1) / (2 * kTM));
+    const int64_t pairs = (int64_t)A.B * A.Hk * A.nsub * ((A.M + 2 * kTM - 1) / (2 * kTM));
     const int64_t seen = std::min<int64_t>(A.Tk, (int64_t)A.W + A.S);
     return pairs >= sms && seen >= 1536 ? fwd_launch<D, 2, false>(A, st) : fwd_launch<D, 1, false>(A, st);
   }
@@ -1164,19 +1274,51 @@ cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
 
 template <int D>
 cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
+  using C = BwdCfg<D>;
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = allow_smem(window_bwd_kernel<D>, BwdCfg<D>::BYTES, done);
+  cudaError_t e = allow_smem(window_bwd_kernel<D>, C::BYTES, done);
   if (e != cudaSuccess) return e;
-  const int64_t rows = (int64_t)A.B * A.Tq * A.Hq;
-  window_delta_kernel<D><<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(A);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const int64_t tiles = (A.Tq + kTM - 1) / kTM + (A.M + kTM - 1) / kTM;
-  window_bwd_kernel<D><<<(unsigned)(tiles * A.B * A.Hk), kBT, BwdCfg<D>::BYTES, st>>>(A);
-  return cudaGetLastError();
+  const int64_t lanes = (int64_t)A.B * A.Tq * A.Hq * (D / 8);
+  window_rows_kernel<D><<<(unsigned)((lanes + 255) / 256), 256, 0, st>>>(A);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  kv_maps(A, D, kTN);
+  A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTN) &&
+             group_map(&A.mg, A, A.dO, {(int64_t)A.Tq * A.Hq * D, (int64_t)A.Hq * D, D}, D, kTN);
+  const int64_t nk = (A.Tq + kTM - 1) / kTM, nq = (A.M + kTM - 1) / kTM;
+  const int64_t bk = (int64_t)A.B * A.Hk;
+  const int64_t grid = ((int64_t)A.sink_tiles * (A.sink_splits - 1) + nk + nq * A.nsub) * bk;
+  window_bwd_kernel<D><<<(unsigned)grid, C::THREADS, C::BYTES, st>>>(A);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (A.sink_splits > 1) {
+    const int64_t threads = bk * A.sink_tiles * 2 * kTM * (D / 4);
+    window_sink_join_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(A);
+    e = cudaGetLastError();
+  }
+  return e;
 }
 
 }  // namespace
+
+// How the backward splits the key tiles that hold sinks (see above): as many
+// parts as make a part no longer than an ordinary tile. More than four such
+// tiles (512 sinks) are many tiles, not one long one: no split.
+void window_sink_shape(WindowArgs& A) {
+  A.sink_tiles = 0;
+  A.sink_splits = 1;
+  if (A.W >= A.n_ctx) A.S = 0;  // the window reaches every context token: no sink lies outside it
+  const int tiles = (std::min(A.S, A.n_ctx) + kTM - 1) / kTM;
+  if (tiles == 0 || tiles > 4) return;
+  const int64_t longest = ((int64_t)A.n_ctx * A.G + kTN - 1) / kTN, usual = ((int64_t)(A.W + kTM) * A.G + kTN - 1) / kTN;
+  A.sink_tiles = tiles;
+  A.sink_splits = (int)std::max<int64_t>(1, std::min<int64_t>(64, (longest + usual - 1) / usual));
+}
+
+size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at) {
+  const size_t rows = (size_t)A.B * A.Tq * A.Hq * sizeof(float2);
+  *sink_at = (rows + 255) & ~size_t(255);
+  return *sink_at +
+         (A.sink_splits > 1 ? (size_t)A.B * A.Hk * A.sink_tiles * A.sink_splits * 2 * kTM * D * sizeof(float) : 0);
+}
 
 // Splits of the keys: enough CTAs to fill the device, at least two key tiles
 // each, from the most keys a query tile can see.

@@ -1108,7 +1108,7 @@ namespace {
 
 // Checks shared by the window attention entry points, and the fields they share.
 int window_args(WindowArgs& A, int32_t batch, int32_t Tq, int32_t Tk, int32_t q_heads, int32_t k_heads, int32_t D,
-                int32_t n_block, int32_t window, int32_t sinks, float scale) {
+                int32_t n_block, int32_t window, int32_t sinks, float scale, bool cached) {
   if (D != 64 && D != 128) return fail(SPECDEC_ERR_ARGUMENT, "head_dim must be 64 or 128, got %d", D);
   if (batch < 0 || Tq < 0 || Tk < 0 || q_heads < 1 || k_heads < 1) return fail(SPECDEC_ERR_ARGUMENT, "bad shape");
   if (q_heads % k_heads)
@@ -1116,11 +1116,18 @@ int window_args(WindowArgs& A, int32_t batch, int32_t Tq, int32_t Tk, int32_t q_
   if (window < 1) return fail(SPECDEC_ERR_ARGUMENT, "window must be >= 1, got %d", window);
   if (sinks < 0) return fail(SPECDEC_ERR_ARGUMENT, "sinks must be >= 0, got %d", sinks);
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(SPECDEC_ERR_VALUE, "scale must be > 0 and finite");
-  const int64_t G = q_heads / k_heads, M = (int64_t)Tq * G;
+  int64_t G = q_heads / k_heads, nsub = 1;
+  if (!cached) {  // see drafter_window.cu: whole tokens' groups in 64 packed rows
+    int64_t p = 1;
+    while (p < 64 && G % (2 * p) == 0) p *= 2;
+    nsub = G / p;
+    G = p;
+  }
+  const int64_t M = (int64_t)Tq * G;
   if (Tk > (1 << 30) || M > INT32_MAX - 256) return fail(SPECDEC_ERR_ARGUMENT, "too many tokens");
   if ((M + 127) / 128 > 65535) return fail(SPECDEC_ERR_ARGUMENT, "at most 65535 * 128 query rows per key head");
-  if ((int64_t)batch * k_heads * ((M + 127) / 128 + (Tq + 127) / 128) > INT32_MAX ||
-      (int64_t)batch * Tq * q_heads / 4 >= INT32_MAX)
+  if ((int64_t)batch * k_heads * (nsub * ((M + 127) / 128) + (Tq + 127) / 128 + 256) > INT32_MAX ||
+      (int64_t)batch * Tq * q_heads / 8 >= INT32_MAX)
     return fail(SPECDEC_ERR_ARGUMENT, "too many rows");
   A = WindowArgs{};
   A.B = batch;
@@ -1129,6 +1136,7 @@ int window_args(WindowArgs& A, int32_t batch, int32_t Tq, int32_t Tk, int32_t q_
   A.Hq = q_heads;
   A.Hk = k_heads;
   A.G = (int)G;
+  A.nsub = (int)nsub;
   A.M = (int)M;
   int l = 0;
   while ((int64_t(1) << l) < G) ++l;
@@ -1178,7 +1186,7 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
   WindowArgs A;
   if (n_ctx < 0 || n_ctx > T)
     return fail(SPECDEC_ERR_ARGUMENT, "n_ctx must be in [0, T] (n_ctx=%d, T=%d)", n_ctx, T);
-  int rc = window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, scale);
+  int rc = window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, scale, false);
   if (rc != SPECDEC_OK || batch == 0 || T == 0) return rc;
   if ((rc = window_input("q", q, q_strides, batch, T, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
   if ((rc = window_input("k", k, k_strides, batch, T, k_heads, head_dim, A.ks)) != SPECDEC_OK) return rc;
@@ -1199,9 +1207,16 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
   return e == cudaSuccess ? ok() : cuda_fail(e, "window attention forward launch");
 }
 
-size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads) {
-  if (batch <= 0 || T <= 0 || q_heads <= 0) return 256;
-  return align256((size_t)batch * (size_t)q_heads * (size_t)T * sizeof(float));
+size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads,
+                                                int32_t head_dim, int32_t n_ctx, int32_t window, int32_t sinks) {
+  WindowArgs A;
+  if (n_ctx < 0 || n_ctx > T ||
+      window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, 1.f, false) != SPECDEC_OK)
+    return 256;
+  A.n_ctx = n_ctx;
+  window_sink_shape(A);
+  size_t at;
+  return align256(window_bwd_workspace(A, head_dim, &at));
 }
 
 int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
@@ -1214,7 +1229,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   WindowArgs A;
   if (n_ctx < 0 || n_ctx > T)
     return fail(SPECDEC_ERR_ARGUMENT, "n_ctx must be in [0, T] (n_ctx=%d, T=%d)", n_ctx, T);
-  int rc = window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, scale);
+  int rc = window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, scale, false);
   if (rc != SPECDEC_OK || batch == 0 || T == 0) return rc;
   if ((rc = window_input("q", q, q_strides, batch, T, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
   if ((rc = window_input("k", k, k_strides, batch, T, k_heads, head_dim, A.ks)) != SPECDEC_OK) return rc;
@@ -1223,9 +1238,14 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   const void* ptrs[] = {o, dout, dq, dk, dv};
   for (const void* p : ptrs)
     if (!p || !aligned(p, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o, dout, dq, dk and dv must be 16-byte aligned");
-  const size_t need = (size_t)batch * (size_t)q_heads * (size_t)T * sizeof(float);
-  if (workspace_bytes < need)
-    return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+  A.n_ctx = n_ctx;
+  window_sink_shape(A);
+  size_t sink_at = 0;
+  const size_t need = window_bwd_workspace(A, head_dim, &sink_at);
+  if (workspace_bytes < need || !aligned(workspace, 16))
+    return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
+  A.rows = static_cast<float2*>(workspace);
+  A.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sink_at);
   A.q = q;
   A.k = k;
   A.v = v;
@@ -1235,9 +1255,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   A.dq = dq;
   A.dk = dk;
   A.dv = dv;
-  A.delta = static_cast<float*>(workspace);
   A.ctx_lens = ctx_lens;
-  A.n_ctx = n_ctx;
   A.status = status;
   A.withhold = take_withhold_stage();
   const cudaError_t e = window_bwd_launch(A, head_dim, static_cast<cudaStream_t>(stream));
@@ -1268,7 +1286,7 @@ int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides,
   WindowArgs A;
   if (n_block < 0 || n_block > cache_len)
     return fail(SPECDEC_ERR_ARGUMENT, "n_block must be in [0, cache_len] (n_block=%d, cache_len=%d)", n_block, cache_len);
-  int rc = window_args(A, batch, q_len, cache_len, q_heads, k_heads, head_dim, n_block, window, sinks, scale);
+  int rc = window_args(A, batch, q_len, cache_len, q_heads, k_heads, head_dim, n_block, window, sinks, scale, true);
   if (rc != SPECDEC_OK || batch == 0 || q_len == 0) return rc;
   if (!ctx_lens) return fail(SPECDEC_ERR_ARGUMENT, "null ctx_lens");
   if ((rc = window_input("q", q, q_strides, batch, q_len, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
@@ -1290,8 +1308,9 @@ int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides,
   if (A.splits > 1) {
     const size_t rows = (size_t)bh * A.M * A.splits, at = align256(rows * head_dim * sizeof(float));
     const size_t need = at + rows * sizeof(float2);
-    if (!workspace || workspace_bytes < need)
-      return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace ? workspace_bytes : 0);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+      return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes on a 16-byte boundary, got %zu", need,
+                  workspace ? workspace_bytes : 0);
     A.part_o = static_cast<float*>(workspace);
     A.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + at);
   }

@@ -224,9 +224,10 @@ struct WindowArgs {
   const bf16_t *q, *k, *v;         // [B, Tq | Tk, heads, D], strided
   int64_t qs[3], ks[3], vs[3];     // batch, token, head stride in elements
   bf16_t* o;                       // [B, Tq, Hq, D]
-  float* lse;                      // [B, Hk, M] of packed rows (token * G + head of the group), or null
+  float* lse;                      // [B, Hk * nsub, M] of packed rows (token * G + head of the group), or null
   const int* ctx_lens;             // [B], or null (training: every context is n_ctx long)
-  int B, Tq, Tk, Hq, Hk, G, M;     // M = Tq * G packed rows per key head
+  int B, Tq, Tk, Hq, Hk;
+  int G, nsub, M;                  // Hq = Hk * nsub * G; M = Tq * G packed rows per virtual head
   uint32_t gmul;                   // m / G = (m * gmul) >> gshift
   int gshift;
   int cached;                      // 1: keys are a cache of Tk rows, the queries its last tokens
@@ -236,7 +237,9 @@ struct WindowArgs {
   float* part_o;                   // [B * Hk * M, splits, D]
   float2* part_ml;                 // [B * Hk * M, splits]: reference maximum, sum
   const bf16_t* dO;                // backward: [B, Tq, Hq, D]
-  float* delta;                    // [B, Hk, M]
+  float2* rows;                    // [B, Hk * nsub, M]: -lse log2 e, -delta
+  float* sink_part;                // partials of the key tiles that hold sinks
+  int sink_tiles, sink_splits;
   bf16_t *dq, *dk, *dv;
   int* status;
   int withhold;
@@ -245,6 +248,8 @@ struct WindowArgs {
   int kv_maps, q_maps;
   CUtensorMap mk, mv, mq, mg;
 };
+void window_sink_shape(WindowArgs& A);
+size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at);
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms);
 cudaError_t window_fwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st);
 cudaError_t window_bwd_launch(WindowArgs& A, int D, cudaStream_t st);

@@ -399,7 +399,7 @@ def _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, want_lse):
     B, T, Hq, D = q.shape
     Hk = k.shape[2]
     o = _new(q)
-    lse = torch.empty((B, Hk, T, Hq // Hk), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
     with _lib.on_device(q.device):
         _lib.check(lib.specdec_window_attention_forward(
             q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
@@ -429,7 +429,7 @@ class _WindowAttention(torch.autograd.Function):
             do = do.clone()
         dq, dk, dv = _new(q), _new(k), _new(v)
         with _lib.on_device(q.device):
-            ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq)
+            ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq, Hk, D, *ctx.how[:3])
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
             _lib.check(lib.specdec_window_attention_backward(
                 q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),

@@ -411,8 +411,8 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
  *                 head_dim] bf16 patterns; head h of q reads head
  *                 h / (q_heads / k_heads) of k and v; head_dim 64 or 128;
  *                 q, k, v strided (rows on 16-byte boundaries), o contiguous
- *   lse           [batch, k_heads, T, q_heads / k_heads] fp32, natural log
- *                 (-inf for padding), for the backward; or NULL
+ *   lse           [batch, q_heads, T] values, fp32, natural log (-inf for
+ *                 padding), in the backward's own order; or NULL
  *   window >= 1   (INT32_MAX: no window); sinks >= 0
  *   status        as in specdec_dflash_attention_forward
  * A row's probabilities are rounded to bf16 before the second product, all
@@ -427,7 +427,8 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
                                      int32_t sinks, float scale, int32_t* status, void* stream);
 
 /* Workspace bytes of specdec_window_attention_backward. */
-size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads);
+size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads,
+                                                int32_t head_dim, int32_t n_ctx, int32_t window, int32_t sinks);
 
 /*
  * Its backward: dq, dk, dv (contiguous, shaped as q, k, v) from q, k, v, the

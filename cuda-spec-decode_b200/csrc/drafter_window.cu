@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "bulk_copy.cuh"
 #include "specdec_common.cuh"
@@ -636,16 +637,21 @@ __global__ void __launch_bounds__(128) window_join_kernel(const __grid_constant_
 // The first key tile holds the sinks: every later context query sees them, far
 // more than see any other tile. Tiles with sinks are split over their queries
 // into `sink_splits` CTAs that leave fp32 partials, joined in order by a kernel.
-template <int D>
+// NB score buffers, and as many warpgroups: two hide one another's latency in a
+// CTA that has the SM to itself; with one buffer (heads of 64) two CTAs share it.
+template <int D, int NB>
 struct BwdCfg {
-  static constexpr int NS = D == 128 ? 4 : 6;
-  static constexpr int THREADS = 384;
+  static constexpr int NS = NB == 1 ? 3 : D == 128 ? 4 : 6;
+  static_assert(NB == 1 || NS % 2 == 0, "a warpgroup's steps sit in every other stage");
+  static constexpr int COPY = NB == 1 ? 32 : 96;  // threads of the copying warps
+  static constexpr int THREADS = NB * 128 + 32 + COPY, CTAS = NB == 1 ? 2 : 1;
   static constexpr uint32_t XB = kTM * D * 2, YB = kTN * D * 2;
   static constexpr uint32_t OX = 0, OY = 2 * XB, OROW = OY + NS * 2 * YB;  // rows: 64 x (-lse2, -delta, lo, hi) per stage
   static constexpr uint32_t OBAR = OROW + NS * kTN * 16;
-  static constexpr int NBAR = 3 * NS + 7;  // full, empty, r_full; s_full[2], p_full[2], x_full, o_full, drain
+  static constexpr int NBAR = 3 * NS + 2 * NB + 3;  // full, empty, r_full; s_full, p_full, x_full, o_full, drain
   static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;
-  static constexpr uint32_t COLS = 512, COL_A = 256, COL_B = 256 + D;  // dQ or dV; dK
+  static constexpr uint32_t COL_A = NB * 128, COL_B = COL_A + D;  // dQ or dV; dK
+  static constexpr uint32_t COLS = COL_B + D <= 256 ? 256 : 512;
 };
 
 // Packed query rows that see a key of the 128 key rows from k0 on: context
@@ -697,15 +703,15 @@ __device__ __forceinline__ void stage_queries(const WindowArgs& A, uint32_t tile
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-// This thread's D / 2 columns (half `half`) of an accumulator row, times `f`.
-template <int D>
-__device__ __forceinline__ void store_acc(bf16_t* row, float* part, uint32_t col, int half, float f, bool write, bool zero) {
+// The warpgroup's D / NB columns of an accumulator row, times `f`.
+template <int D, int NB>
+__device__ __forceinline__ void store_acc(bf16_t* row, float* part, uint32_t col, int wg, float f, bool write, bool zero) {
 #pragma unroll
-  for (int c = 0; c < D / 2; c += 32) {
+  for (int c = 0; c < D / NB; c += 32) {
     float a[32];
-    tmem_ld32(col + half * (D / 2) + c, a);
+    tmem_ld32(col + wg * (D / NB) + c, a);
     if (!write) continue;
-    const int at = half * (D / 2) + c;
+    const int at = wg * (D / NB) + c;
 #pragma unroll
     for (int j = 0; j < 32; ++j) a[j] = zero ? 0.f : a[j] * f;
     if (part) {
@@ -721,13 +727,13 @@ __device__ __forceinline__ void store_acc(bf16_t* row, float* part, uint32_t col
     }
   }
 }
-// The same half row filled with one value: zeros, or NaN after an expired wait.
-template <int D>
-__device__ __forceinline__ void fill_row(bf16_t* row, float* part, int half, bool nan) {
+// The same columns filled with one value: zeros, or NaN after an expired wait.
+template <int D, int NB>
+__device__ __forceinline__ void fill_row(bf16_t* row, float* part, int wg, bool nan) {
   const uint32_t w = nan ? kNan2 : 0u;
   const float v = nan ? __int_as_float(0x7fc00000) : 0.f;
 #pragma unroll
-  for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 8) {
+  for (int c = wg * (D / NB); c < (wg + 1) * (D / NB); c += 8) {
     if (part) {
       *reinterpret_cast<float4*>(part + c) = make_float4(v, v, v, v);
       *reinterpret_cast<float4*>(part + c + 4) = make_float4(v, v, v, v);
@@ -744,9 +750,9 @@ __device__ __forceinline__ void grad_pair(float2 s, float2 dp, float sl2, float2
   ds = fmul2(pr, fadd2(dp, nd));
 }
 
-template <int D, bool DKV>
+template <int D, int NB, bool DKV>
 __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int head, int tile, int split, bool withhold) {
-  using C = BwdCfg<D>;
+  using C = BwdCfg<D, NB>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   volatile int* dead = reinterpret_cast<volatile int*>(smem + C::OSLOT + 4);
@@ -755,8 +761,8 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   uint64_t* empty = full + C::NS;
   uint64_t* r_full = empty + C::NS;
   uint64_t* s_full = r_full + C::NS;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* x_full = p_full + 2;
+  uint64_t* p_full = s_full + NB;
+  uint64_t* x_full = p_full + NB;
   uint64_t* o_full = x_full + 1;
   uint64_t* drain = x_full + 2;
   const int warp = threadIdx.x >> 5, wg = threadIdx.x >> 7;
@@ -779,12 +785,12 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   }
 
   // this thread's output row: lane r of X
-  const int r = threadIdx.x & (kTM - 1), half = wg & 1;
+  const int r = threadIdx.x & (kTM - 1);
   const int xr = x0 + r;
   bf16_t *row_a, *row_b = nullptr;  // dQ; or dV and dK
   float *part_a = nullptr, *part_b = nullptr;
   int token = -1;
-  bool mine = wg < 2;
+  bool mine = wg < NB;
   if (DKV) {
     mine = mine && xr < A.Tq;
     token = mine ? token_of(A, sq, xr) : -1;
@@ -804,8 +810,8 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   }
   if (n == 0) {  // padding only, or no step left for this split
     if (mine) {
-      fill_row<D>(row_a, part_a, half, false);
-      if (DKV) fill_row<D>(row_b, part_b, half, false);
+      fill_row<D, NB>(row_a, part_a, wg, false);
+      if (DKV) fill_row<D, NB>(row_b, part_b, wg, false);
     }
     return;
   }
@@ -816,10 +822,10 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     for (int i = 0; i < C::NS; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
-      mbar_init(r_full + i, 128);
+      mbar_init(r_full + i, 2 * C::COPY);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NB; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
     }
@@ -829,64 +835,63 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     fence_mbar_init();
     *dead = 0;
   }
-  if (warp == 8) tmem_alloc(slot, C::COLS);
+  if (warp == NB * 4) tmem_alloc(slot, C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
   int issued = 0;  // stages that this thread's copies have begun
 
-  if (wg == 2) {
-    if (warp == 8) {
+  if (wg == NB) {
+    if (warp == NB * 4) {
       // ---- products: the warp walks together, one lane issues ----
       constexpr uint32_t kIdS = instr_desc(kTM, kTN, 0, 0);
       constexpr uint32_t kIdA = instr_desc(kTM, D, 0, 1);
       const uint32_t x1 = desc_low(base + C::OX, 16), x2 = desc_low(base + C::OX + C::XB, 16);
       const uint32_t yk = desc_low(base + C::OY, 16), yn = desc_low(base + C::OY, kTN * 128);
-      uint32_t slot_s = 0, ph_s = 0, slot_a = 0;  // ring slots of step i and of step i - 1
+      uint32_t slot_s = 0, ph_s = 0, slot_a = 0;  // ring slots of the next scores and of the next accumulation
       bool ok = wait_alive(x_full, 0, dead, A.status);
+      auto scores = [&](int i) {  // S, dP of step i; its buffer's last P and dS were read by products issued before
+        ok = wait_alive(full + slot_s, ph_s, dead, A.status);
+        if (!ok) return;
+        tc_fence_after();
+        // (failure-detection test hook: the first step's products are withheld)
+        if (!(withhold && i == 0) && elect_one()) {
+          const uint32_t y = yk + slot_s * (2 * C::YB >> 4), d = tmem + (i % NB) * 128;
+          issue_kk<D, kTM, kTN>(d, x1, y, kIdS);
+          issue_kk<D, kTM, kTN>(d + 64, x2, y + (C::YB >> 4), kIdS);
+          umma_commit(s_full + i % NB);
+        }
+        __syncwarp();
+        if (++slot_s == C::NS) slot_s = 0, ph_s ^= 1;
+      };
+      auto accumulate = [&](int i) {
+        ok = wait_alive(p_full + i % NB, (i / NB) & 1, dead, A.status);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t y = yn + slot_a * (2 * C::YB >> 4), d = tmem + (i % NB) * 128;
+          if (DKV) {
+            issue_tn<kTN / 16>(tmem + C::COL_A, d, y + (C::YB >> 4), kIdA, i > 0);  // dV += P^T dO
+            issue_tn<kTN / 16>(tmem + C::COL_B, d + 64, y, kIdA, i > 0);            // dK += dS^T Q
+          } else {
+            issue_tn<kTN / 16>(tmem + C::COL_A, d + 64, y, kIdA, i > 0);            // dQ += dS K
+          }
+          umma_commit(empty + slot_a);
+        }
+        __syncwarp();
+        if (++slot_a == C::NS) slot_a = 0;
+      };
       for (int i = 0; i <= n && ok; ++i) {
-        if (i < n) {
-          ok = wait_alive(full + slot_s, ph_s, dead, A.status);
-          if (!ok) break;
-          tc_fence_after();
-          // the buffer's previous P and dS were read by products issued before
-          // (failure-detection test hook: the first step's products are withheld)
-          if (!(withhold && i == 0)) {
-            if (elect_one()) {
-              const uint32_t y = yk + slot_s * (2 * C::YB >> 4), d = tmem + (i & 1) * 128;
-              issue_kk<D, kTM, kTN>(d, x1, y, kIdS);
-              issue_kk<D, kTM, kTN>(d + 64, x2, y + (C::YB >> 4), kIdS);
-              umma_commit(s_full + (i & 1));
-            }
-            __syncwarp();
-          }
-          if (++slot_s == C::NS) slot_s = 0, ph_s ^= 1;
-        }
-        if (i > 0) {
-          const int j = i - 1;
-          ok = wait_alive(p_full + (j & 1), (j >> 1) & 1, dead, A.status);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t y = yn + slot_a * (2 * C::YB >> 4), d = tmem + (j & 1) * 128;
-            if (DKV) {
-              issue_tn<kTN / 16>(tmem + C::COL_A, d, y + (C::YB >> 4), kIdA, j > 0);  // dV += P^T dO
-              issue_tn<kTN / 16>(tmem + C::COL_B, d + 64, y, kIdA, j > 0);            // dK += dS^T Q
-            } else {
-              issue_tn<kTN / 16>(tmem + C::COL_A, d + 64, y, kIdA, j > 0);            // dQ += dS K
-            }
-            umma_commit(empty + slot_a);
-          }
-          __syncwarp();
-          if (++slot_a == C::NS) slot_a = 0;
-        }
+        if (NB == 2 && i < n) scores(i);  // while the warpgroups are at step i - 1
+        if (ok && i > 0) accumulate(i - 1);
+        if (NB == 1 && ok && i < n) scores(i);
       }
       if (ok && elect_one()) umma_commit(o_full);
       __syncwarp();
     } else {
       // ---- copies ----
-      const int lt = (int)threadIdx.x - 288;
+      const int lt = (int)threadIdx.x - NB * 128 - 32;
       const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
       const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
       const int q_head = DKV ? hk * A.nsub * A.G : head * A.G;  // first query head (of sub-group 0)
@@ -917,7 +922,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
             const int c = lt % CH;
             const bf16_t* src = x ? vb : kb;
             const int64_t ts = x ? A.vs[1] : A.ks[1];
-            for (int q = lt / CH; q < kTM; q += 96 / CH) {
+            for (int q = lt / CH; q < kTM; q += C::COPY / CH) {
               const bool valid = x0 + q < A.Tq && token_of(A, sq, x0 + q) >= 0;
               cp_async16(base + C::OX + x * C::XB + (uint32_t)(c >> 3) * (kTM * 128u) + sw128((uint32_t)q, (uint32_t)(c & 7)),
                          valid ? src + (int64_t)(x0 + q) * ts + c * 8 : src, valid);
@@ -926,10 +931,10 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
           cp_async_commit();
           cp_async_wait<0>();
           fence_proxy_async_smem();
-          asm volatile("bar.sync 1, 96;" ::: "memory");
+          asm volatile("bar.sync 1, %0;" ::"n"(C::COPY) : "memory");
         } else {
-          stage_queries<96, D>(A, base + C::OX, qb, A.qs[1], A.qs[2], sq, x0, A.M, kTM, lt, true);
-          stage_queries<96, D>(A, base + C::OX + C::XB, gb, gts, D, sq, x0, A.M, kTM, lt, true);
+          stage_queries<C::COPY, D>(A, base + C::OX, qb, A.qs[1], A.qs[2], sq, x0, A.M, kTM, lt, true);
+          stage_queries<C::COPY, D>(A, base + C::OX + C::XB, gb, gts, D, sq, x0, A.M, kTM, lt, true);
         }
         if (lt == 0) mbar_arrive(x_full);
       }
@@ -947,18 +952,20 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
         if (DKV) {
           const int f = qt.first(A, rr), l = qt.last(A, rr);
           const int t0 = f / A.G, t1 = t0 + kTN / A.G;
-          if (lt < kTN) {  // -lse2, -delta and the bounds of the keys that row f + lt sees
-            const uint32_t rowp = base + C::OROW + (sl * kTN + lt) * 16;
-            const int m = f + lt;
-            if (ok) {
+          // -lse2, -delta and the bounds of the keys that each row sees
+          if (ok) {
+            for (int e = lt; e < kTN; e += C::COPY) {
+              const uint32_t rowp = base + C::OROW + (sl * kTN + e) * 16;
+              const int m = f + e;
               const float2* src = A.rows + ((int64_t)b * A.Hk * A.nsub + hk * A.nsub + sub) * A.M + (m < l ? m : f);
               asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(rowp), "l"(src), "r"(m < l ? 8 : 0) : "memory");
               const int p = m < l ? token_of(A, sq, group_div(A, m)) : -1;
               asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(rowp + 8), "r"(low_of(A, sq, p)), "r"(high_of(sq, p))
                            : "memory");
-              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(r_full + sl)) : "memory");
-              mbar_arrive(r_full + sl);
             }
+            // two arrivals per thread: when its copies have landed, and for its own writes
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(r_full + sl)) : "memory");
+            mbar_arrive(r_full + sl);
           }
           if (y_boxes && (t1 <= sq.c || t0 >= A.n_ctx || sq.c == A.n_ctx)) {
             if (ok && lt == 0) {
@@ -970,8 +977,8 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
               }
             }
           } else {
-            stage_queries<96, D>(A, y1, qb + (int64_t)sub * A.G * A.qs[2], A.qs[1], A.qs[2], sq, f, l, kTN, lt, ok);
-            stage_queries<96, D>(A, y2, gb + (int64_t)sub * A.G * D, gts, D, sq, f, l, kTN, lt, ok);
+            stage_queries<C::COPY, D>(A, y1, qb + (int64_t)sub * A.G * A.qs[2], A.qs[1], A.qs[2], sq, f, l, kTN, lt, ok);
+            stage_queries<C::COPY, D>(A, y2, gb + (int64_t)sub * A.G * D, gts, D, sq, f, l, kTN, lt, ok);
             if (ok && lt == 0) mbar_arrive(full + sl);
           }
           if (++rr == qt.per) rr = 0, ++sub;
@@ -988,8 +995,8 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
               }
             }
           } else {
-            stage_keys<96, kTN, D>(y1, kb, A.ks[1], sq, j0, kt.end(i), lt, ok);
-            stage_keys<96, kTN, D>(y2, vb, A.vs[1], sq, j0, kt.end(i), lt, ok);
+            stage_keys<C::COPY, kTN, D>(y1, kb, A.ks[1], sq, j0, kt.end(i), lt, ok);
+            stage_keys<C::COPY, kTN, D>(y2, vb, A.vs[1], sq, j0, kt.end(i), lt, ok);
             if (ok && lt == 0) mbar_arrive(full + sl);
           }
         }
@@ -998,7 +1005,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
       cp_async_wait<0>();  // no copy outlives the CTA
     }
   } else {
-    // ---- P and dS of steps wg, wg + 2, ... ----
+    // ---- P and dS of steps wg, wg + NB, ... ----
     const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t buf = lane + wg * 128;
     const int lo = low_of(A, sq, token), hi = high_of(sq, token);
@@ -1011,7 +1018,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     }
     bool ok = true;
     uint32_t k = 0, sl = wg % C::NS, rph = 0;
-    for (int i = wg; i < n; i += 2, ++k) {
+    for (int i = wg; i < n; i += NB, ++k) {
       ok = __all_sync(kFullMask, wait_alive(s_full + wg, k & 1, dead, A.status));
       if (DKV) ok = ok && __all_sync(kFullMask, wait_alive(r_full + sl, rph, dead, A.status));
       if (!ok) break;
@@ -1028,8 +1035,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
       const int j0 = kt.start(DKV ? 0 : i);
       const bool in_sink = i < kt.ns;
       const int rl = in_sink ? kTN : lo - j0, rh = hi - j0, rs = (in_sink ? kt.sink : A.S) - j0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      auto half_step = [&](int h, auto masked) {  // 32 columns; no branch inside
         uint32_t sr[32], dr[32];
         tmem_ld32_async(buf + h * 32, sr);
         tmem_ld32_async(buf + 64 + h * 32, dr);
@@ -1038,27 +1044,28 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           float2 pr, ds;
-          float4 ra, rb;
           if (DKV) {
-            ra = rows[h * 32 + j];
-            rb = rows[h * 32 + j + 1];
-            nl = make_float2(ra.x, rb.x);
-            nd = make_float2(ra.y, rb.y);
+            const float2 va = *reinterpret_cast<const float2*>(rows + h * 32 + j);
+            const float2 vb = *reinterpret_cast<const float2*>(rows + h * 32 + j + 1);
+            nl = make_float2(va.x, vb.x);
+            nd = make_float2(va.y, vb.y);
           }
           grad_pair(make_float2(__uint_as_float(sr[j]), __uint_as_float(sr[j + 1])),
                     make_float2(__uint_as_float(dr[j]), __uint_as_float(dr[j + 1])), A.scale_log2, nl, nd, pr, ds);
-          if (!whole) {
+          if constexpr (masked.value) {
             bool va, vb;
             if (DKV) {
-              va = token >= 0 && token < __float_as_int(ra.w) && (token >= __float_as_int(ra.z) || token < A.S);
-              vb = token >= 0 && token < __float_as_int(rb.w) && (token >= __float_as_int(rb.z) || token < A.S);
+              const int2 ba = reinterpret_cast<const int2*>(rows + h * 32 + j)[1];
+              const int2 bb = reinterpret_cast<const int2*>(rows + h * 32 + j + 1)[1];
+              va = (token >= 0) & (token < ba.y) & ((token >= ba.x) | (token < A.S));
+              vb = (token >= 0) & (token < bb.y) & ((token >= bb.x) | (token < A.S));
             } else {
               const int e = h * 32 + j;
-              va = e < rh && (e >= rl || e < rs);
-              vb = e + 1 < rh && (e + 1 >= rl || e + 1 < rs);
+              va = (e < rh) & ((e >= rl) | (e < rs));
+              vb = (e + 1 < rh) & ((e + 1 >= rl) | (e + 1 < rs));
             }
-            if (!va) pr.x = ds.x = 0.f;
-            if (!vb) pr.y = ds.y = 0.f;
+            pr = make_float2(va ? pr.x : 0.f, vb ? pr.y : 0.f);
+            ds = make_float2(va ? ds.x : 0.f, vb ? ds.y : 0.f);
           }
           if (DKV) wp[j / 2] = pack_bf16x2(pr.x, pr.y);
           wd[j / 2] = pack_bf16x2(ds.x, ds.y);
@@ -1066,44 +1073,52 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
         // the 32 columns read so far are free: P over S, dS over dP
         if (DKV) tmem_st16(buf + h * 16, wp);
         tmem_st16(buf + 64 + h * 16, wd);
+      };
+      if (whole) {
+        half_step(0, std::false_type{});
+        half_step(1, std::false_type{});
+      } else {
+        half_step(0, std::true_type{});
+        half_step(1, std::true_type{});
       }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(p_full + wg);
-      sl += 2;
+      sl += NB;
       if (sl >= C::NS) sl -= C::NS, rph ^= 1;
     }
     if (ok) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
     tc_fence_after();
     if (!ok) {  // never a plausible wrong number
       if (mine) {
-        fill_row<D>(row_a, part_a, half, true);
-        if (DKV) fill_row<D>(row_b, part_b, half, true);
+        fill_row<D, NB>(row_a, part_a, wg, true);
+        if (DKV) fill_row<D, NB>(row_b, part_b, wg, true);
       }
     } else {
-      store_acc<D>(row_a, part_a, lane + C::COL_A, half, DKV ? 1.f : A.scale, mine, token < 0);
-      if (DKV) store_acc<D>(row_b, part_b, lane + C::COL_B, half, A.scale, mine, token < 0);
+      store_acc<D, NB>(row_a, part_a, lane + C::COL_A, wg, DKV ? 1.f : A.scale, mine, token < 0);
+      if (DKV) store_acc<D, NB>(row_b, part_b, lane + C::COL_B, wg, A.scale, mine, token < 0);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (*dead) {  // bounded waits for every product and box that was issued
-    if (warp == 8 && (threadIdx.x & 31) == 0) umma_commit(drain);
+    if (warp == NB * 4 && (threadIdx.x & 31) == 0) umma_commit(drain);
     mbar_wait(drain, 0);
-    if (threadIdx.x == 288) {
+    if (threadIdx.x == NB * 128 + 32) {
       mbar_wait(x_full, 0);
       for (int i = max(0, issued - C::NS); i < issued; ++i) mbar_wait(full + i % C::NS, (i / C::NS) & 1);
     }
     __syncthreads();
   }
-  if (warp == 8) tmem_free(tmem, C::COLS);
+  if (warp == NB * 4) tmem_free(tmem, C::COLS);
 }
 
 // Blocks in dispatch order: the parts of the sink tiles, the other dk/dv tiles
 // (longer than the dq tiles by the group's heads), the dq tiles from the last on.
-template <int D>
-__global__ void __launch_bounds__(BwdCfg<D>::THREADS, 1) window_bwd_kernel(const __grid_constant__ WindowArgs A) {
+template <int D, int NB>
+__global__ void __launch_bounds__(BwdCfg<D, NB>::THREADS, BwdCfg<D, NB>::CTAS)
+    window_bwd_kernel(const __grid_constant__ WindowArgs A) {
   const int nk = (A.Tq + kTM - 1) / kTM, nq = (A.M + kTM - 1) / kTM;
   const int sinks = A.sink_tiles * A.sink_splits, bk = A.B * A.Hk, bv = bk * A.nsub;
   const int64_t dkv = (int64_t)(sinks + nk - A.sink_tiles) * bk;
@@ -1112,11 +1127,11 @@ __global__ void __launch_bounds__(BwdCfg<D>::THREADS, 1) window_bwd_kernel(const
     const int job = (int)(i / bk), bh = (int)(i - (int64_t)job * bk), b = bh / A.Hk;
     const int tile = job < sinks ? job / A.sink_splits : job - sinks + A.sink_tiles;
     const int split = job < sinks ? job - tile * A.sink_splits : 0;
-    window_bwd_role<D, true>(A, b, bh - b * A.Hk, tile, split, A.withhold && i == 0);
+    window_bwd_role<D, NB, true>(A, b, bh - b * A.Hk, tile, split, A.withhold && i == 0);
   } else {
     const int64_t q = i - dkv;
     const int tile = nq - 1 - (int)(q / bv), bh = (int)(q % bv), hv = A.Hk * A.nsub, b = bh / hv;
-    window_bwd_role<D, false>(A, b, bh - b * hv, tile, 0, A.withhold && q == 0);
+    window_bwd_role<D, NB, false>(A, b, bh - b * hv, tile, 0, A.withhold && q == 0);
   }
 }
 
@@ -1272,12 +1287,28 @@ cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+// Heads of 64: one score buffer and two CTAs per SM, or two buffers and one CTA.
+// Short walks want the second CTA (its set-up and end hide the first's), long
+// ones the overlap within a CTA; us with one / two: [32, 528, 4] W 128 73 / 91,
+// [8, 2048, 8] W 512 165 / 193, [4, 4096, 8] W 1024 221 / 244, [2, 8192, 8 / 2
+// heads] W 4096 550 / 483.
+bool bwd_one_buffer(const WindowArgs& A) {
+  return std::min<int64_t>(A.Tk, (int64_t)A.W + A.S) < 2048;
+}
+
+template <int D, int NB>
+cudaError_t bwd_launch(const WindowArgs& A, unsigned grid, cudaStream_t st) {
+  using C = BwdCfg<D, NB>;
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(window_bwd_kernel<D, NB>, C::BYTES, done);
+  if (e != cudaSuccess) return e;
+  window_bwd_kernel<D, NB><<<grid, C::THREADS, C::BYTES, st>>>(A);
+  return cudaGetLastError();
+}
+
 template <int D>
 cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
-  using C = BwdCfg<D>;
-  static std::atomic<unsigned long long> done{0};
-  cudaError_t e = allow_smem(window_bwd_kernel<D>, C::BYTES, done);
-  if (e != cudaSuccess) return e;
+  cudaError_t e;
   const int64_t lanes = (int64_t)A.B * A.Tq * A.Hq * (D / 8);
   window_rows_kernel<D><<<(unsigned)((lanes + 255) / 256), 256, 0, st>>>(A);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -1287,8 +1318,13 @@ cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
   const int64_t nk = (A.Tq + kTM - 1) / kTM, nq = (A.M + kTM - 1) / kTM;
   const int64_t bk = (int64_t)A.B * A.Hk;
   const int64_t grid = ((int64_t)A.sink_tiles * (A.sink_splits - 1) + nk + nq * A.nsub) * bk;
-  window_bwd_kernel<D><<<(unsigned)grid, C::THREADS, C::BYTES, st>>>(A);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  bool one = false;
+  if constexpr (D == 64) {
+    one = bwd_one_buffer(A);
+    if (one) e = bwd_launch<D, 1>(A, (unsigned)grid, st);
+  }
+  if (!one) e = bwd_launch<D, 2>(A, (unsigned)grid, st);
+  if (e != cudaSuccess) return e;
   if (A.sink_splits > 1) {
     const int64_t threads = bk * A.sink_tiles * 2 * kTM * (D / 4);
     window_sink_join_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(A);
@@ -1299,18 +1335,24 @@ cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
 
 }  // namespace
 
-// How the backward splits the key tiles that hold sinks (see above): as many
-// parts as make a part no longer than an ordinary tile. More than four such
-// tiles (512 sinks) are many tiles, not one long one: no split.
-void window_sink_shape(WindowArgs& A) {
+// How the backward splits the key tiles that hold sinks (see above): into parts
+// no longer than an ordinary tile's walk or half of what an SM has to do in
+// all, whichever is more. More than four such tiles (512 sinks) are many
+// tiles, not a few long ones: no split.
+void window_sink_shape(WindowArgs& A, int sms) {
   A.sink_tiles = 0;
   A.sink_splits = 1;
   if (A.W >= A.n_ctx) A.S = 0;  // the window reaches every context token: no sink lies outside it
   const int tiles = (std::min(A.S, A.n_ctx) + kTM - 1) / kTM;
   if (tiles == 0 || tiles > 4) return;
-  const int64_t longest = ((int64_t)A.n_ctx * A.G + kTN - 1) / kTN, usual = ((int64_t)(A.W + kTM) * A.G + kTN - 1) / kTN;
+  const int64_t walk = std::min<int64_t>(A.n_ctx, (int64_t)A.W + kTM);  // queries that see an ordinary tile
+  const int64_t usual = (walk * A.G + kTN - 1) / kTN * A.nsub;
+  const int64_t longest = ((int64_t)A.n_ctx * A.G + kTN - 1) / kTN * A.nsub;
+  const int64_t rows = (A.Tq + kTM - 1) / kTM;
+  const int64_t all = 2 * rows * usual * A.B * A.Hk;  // steps: dk/dv, and dq's as many
+  const int64_t part = std::max(usual, all / sms / 2);
   A.sink_tiles = tiles;
-  A.sink_splits = (int)std::max<int64_t>(1, std::min<int64_t>(64, (longest + usual - 1) / usual));
+  A.sink_splits = (int)std::max<int64_t>(1, std::min<int64_t>(64, (longest + part - 1) / part));
 }
 
 size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at) {

@@ -1147,7 +1147,7 @@ int window_args(WindowArgs& A, int32_t batch, int32_t Tq, int32_t Tk, int32_t q_
   A.S = sinks;
   A.scale = scale;
   A.scale_log2 = scale * kLog2e;
-  A.splits = 1;
+  A.splits = A.sink_splits = 1;
   return ok();
 }
 
@@ -1208,13 +1208,15 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
 }
 
 size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads,
-                                                int32_t head_dim, int32_t n_ctx, int32_t window, int32_t sinks) {
+                                                int32_t head_dim, int32_t n_ctx, int32_t window, int32_t sinks,
+                                                int device) {
   WindowArgs A;
-  if (n_ctx < 0 || n_ctx > T ||
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n_ctx < 0 || n_ctx > T ||
       window_args(A, batch, T, T, q_heads, k_heads, head_dim, T - n_ctx, window, sinks, 1.f, false) != SPECDEC_OK)
     return 256;
   A.n_ctx = n_ctx;
-  window_sink_shape(A);
+  window_sink_shape(A, sms);
   size_t at;
   return align256(window_bwd_workspace(A, head_dim, &at));
 }
@@ -1239,9 +1241,14 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   for (const void* p : ptrs)
     if (!p || !aligned(p, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o, dout, dq, dk and dv must be 16-byte aligned");
   A.n_ctx = n_ctx;
-  window_sink_shape(A);
   size_t sink_at = 0;
-  const size_t need = window_bwd_workspace(A, head_dim, &sink_at);
+  size_t need = window_bwd_workspace(A, head_dim, &sink_at);  // without parts of sink tiles
+  int sms = 0;
+  if (workspace_bytes >= need) {
+    if ((rc = device_sms(&sms)) != SPECDEC_OK) return rc;
+    window_sink_shape(A, sms);
+    need = window_bwd_workspace(A, head_dim, &sink_at);
+  }
   if (workspace_bytes < need || !aligned(workspace, 16))
     return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
   A.rows = static_cast<float2*>(workspace);

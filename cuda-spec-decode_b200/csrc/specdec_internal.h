@@ -248,7 +248,7 @@ struct WindowArgs {
   int kv_maps, q_maps;
   CUtensorMap mk, mv, mq, mg;
 };
-void window_sink_shape(WindowArgs& A);
+void window_sink_shape(WindowArgs& A, int sms);
 size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at);
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms);
 cudaError_t window_fwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st);

@@ -429,7 +429,7 @@ class _WindowAttention(torch.autograd.Function):
             do = do.clone()
         dq, dk, dv = _new(q), _new(k), _new(v)
         with _lib.on_device(q.device):
-            ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq, Hk, D, *ctx.how[:3])
+            ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq, Hk, D, *ctx.how[:3], q.device.index)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
             _lib.check(lib.specdec_window_attention_backward(
                 q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),

@@ -426,9 +426,10 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
                                      int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx, int32_t window,
                                      int32_t sinks, float scale, int32_t* status, void* stream);
 
-/* Workspace bytes of specdec_window_attention_backward. */
+/* Workspace bytes of specdec_window_attention_backward on `device`. */
 size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads,
-                                                int32_t head_dim, int32_t n_ctx, int32_t window, int32_t sinks);
+                                                int32_t head_dim, int32_t n_ctx, int32_t window, int32_t sinks,
+                                                int device);
 
 /*
  * Its backward: dq, dk, dv (contiguous, shaped as q, k, v) from q, k, v, the

@@ -559,10 +559,18 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
 #pragma unroll
           for (int j = 0; j < 32; ++j) ot[j] = seen ? ot[j] * inv : 0.f;
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            *reinterpret_cast<uint4*>(orow + c + j) =
-                make_uint4(pack_bf16x2(ot[j], ot[j + 1]), pack_bf16x2(ot[j + 2], ot[j + 3]),
-                           pack_bf16x2(ot[j + 4], ot[j + 5]), pack_bf16x2(ot[j + 6], ot[j + 7]));
+          for (int j = 0; j < 32; j += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(ot[j + 2 * e], ot[j + 2 * e + 1]);
+            *reinterpret_cast<uint4*>(orow + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (A.o_res) {  // what the rounding took away
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_bf16x2(ot[j + 2 * e] - bf16_lo(w[e]), ot[j + 2 * e + 1] - bf16_hi(w[e]));
+              *reinterpret_cast<uint4*>(A.o_res + (orow - A.o) + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
         }
       }
       if (mine) {
@@ -1159,6 +1167,11 @@ __global__ void __launch_bounds__(256) window_sink_join_kernel(const __grid_cons
 
 // rows[b, virtual head, m] = (-lse log2 e, -sum_d dO o) of every packed row;
 // D / 8 lanes per row, rows in the tensors' order. Padding: (0, 0), masked later.
+// o comes as the rounded output and the residual of that rounding (16 bits in
+// all): with o rounded to 8 bits, delta's error is the largest in the gradients
+// of rows that see few keys (dq, dk 1.53 to 1.9 times as far off as one
+// rounding of the result; with the residual 1.41 to 1.5, of which 1.41 is the
+// rounding of dS).
 template <int D>
 __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant__ WindowArgs A) {
   constexpr int L = D / 8;
@@ -1169,11 +1182,12 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
   if (on) {
     const uint4 a = *reinterpret_cast<const uint4*>(A.o + i * D + 8 * c);
     const uint4 g = *reinterpret_cast<const uint4*>(A.dO + i * D + 8 * c);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+    const uint4 e = A.o_res ? *reinterpret_cast<const uint4*>(A.o_res + i * D + 8 * c) : make_uint4(0, 0, 0, 0);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w}, ew[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      d = fmaf(bf16_lo(aw[j]), bf16_lo(gw[j]), d);
-      d = fmaf(bf16_hi(aw[j]), bf16_hi(gw[j]), d);
+      d = fmaf(bf16_lo(aw[j]) + bf16_lo(ew[j]), bf16_lo(gw[j]), d);
+      d = fmaf(bf16_hi(aw[j]) + bf16_hi(ew[j]), bf16_hi(gw[j]), d);
     }
   }
 #pragma unroll

@@ -1180,8 +1180,8 @@ extern "C" {
 
 int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
                                      const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
-                                     uint16_t* o, float* lse, const int32_t* ctx_lens, int32_t batch, int32_t T,
-                                     int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx, int32_t window,
+                                     uint16_t* o, uint16_t* o_residual, float* lse, const int32_t* ctx_lens,
+                                     int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx, int32_t window,
                                      int32_t sinks, float scale, int32_t* status, void* stream) {
   WindowArgs A;
   if (n_ctx < 0 || n_ctx > T)
@@ -1191,11 +1191,13 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
   if ((rc = window_input("q", q, q_strides, batch, T, q_heads, head_dim, A.qs)) != SPECDEC_OK) return rc;
   if ((rc = window_input("k", k, k_strides, batch, T, k_heads, head_dim, A.ks)) != SPECDEC_OK) return rc;
   if ((rc = window_input("v", v, v_strides, batch, T, k_heads, head_dim, A.vs)) != SPECDEC_OK) return rc;
-  if (!o || !aligned(o, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o must be 16-byte aligned");
+  if (!o || !aligned(o, 16) || !aligned(o_residual, 16))
+    return fail(SPECDEC_ERR_ARGUMENT, "o and o_residual must be 16-byte aligned");
   A.q = q;
   A.k = k;
   A.v = v;
   A.o = o;
+  A.o_res = o_residual;
   A.lse = lse;
   A.ctx_lens = ctx_lens;
   A.n_ctx = n_ctx;
@@ -1223,9 +1225,10 @@ size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_
 
 int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
                                       const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
-                                      const uint16_t* o, const float* lse, const uint16_t* dout, uint16_t* dq,
-                                      uint16_t* dk, uint16_t* dv, const int32_t* ctx_lens, int32_t batch, int32_t T,
-                                      int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx,
+                                      const uint16_t* o, const uint16_t* o_residual, const float* lse,
+                                      const uint16_t* dout, uint16_t* dq, uint16_t* dk, uint16_t* dv,
+                                      const int32_t* ctx_lens, int32_t batch, int32_t T, int32_t q_heads,
+                                      int32_t k_heads, int32_t head_dim, int32_t n_ctx,
                                       int32_t window, int32_t sinks, float scale, int32_t* status, void* workspace,
                                       size_t workspace_bytes, void* stream) {
   WindowArgs A;
@@ -1240,6 +1243,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   const void* ptrs[] = {o, dout, dq, dk, dv};
   for (const void* p : ptrs)
     if (!p || !aligned(p, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o, dout, dq, dk and dv must be 16-byte aligned");
+  if (!aligned(o_residual, 16)) return fail(SPECDEC_ERR_ARGUMENT, "o_residual must be 16-byte aligned");
   A.n_ctx = n_ctx;
   size_t sink_at = 0;
   size_t need = window_bwd_workspace(A, head_dim, &sink_at);  // without parts of sink tiles
@@ -1257,6 +1261,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   A.k = k;
   A.v = v;
   A.o = const_cast<uint16_t*>(o);
+  A.o_res = const_cast<uint16_t*>(o_residual);
   A.lse = const_cast<float*>(lse);
   A.dO = dout;
   A.dq = dq;

@@ -224,6 +224,7 @@ struct WindowArgs {
   const bf16_t *q, *k, *v;         // [B, Tq | Tk, heads, D], strided
   int64_t qs[3], ks[3], vs[3];     // batch, token, head stride in elements
   bf16_t* o;                       // [B, Tq, Hq, D]
+  bf16_t* o_res;                   // as o: the residual of its rounding, for the backward, or null
   float* lse;                      // [B, Hk * nsub, M] of packed rows (token * G + head of the group), or null
   const int* ctx_lens;             // [B], or null (training: every context is n_ctx long)
   int B, Tq, Tk, Hq, Hk;

@@ -276,6 +276,11 @@ class _Rotary(torch.autograd.Function):
         return _rotary(dy, positions, inv_freq, *ctx.how, 1), None, None, None, None
 
 
+def rotary_supported(x: torch.Tensor) -> bool:
+    return (ENABLED and x.is_cuda and x.dtype in _DTYPES and x.dim() == 4 and x.shape[3] % 2 == 0
+            and 0 < x.shape[3] <= 512)
+
+
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
            scale: float = 1.0) -> torch.Tensor:
     """Rotary positions of every head of x [B, T, heads, D] (fp32 or bf16, any
@@ -394,26 +399,27 @@ def _check_lens(ctx_lens: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
     return ctx_lens.to(torch.int32).contiguous()
 
 
-def _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, want_lse):
+def _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, train):
     lib = _lib.load()
     B, T, Hq, D = q.shape
     Hk = k.shape[2]
     o = _new(q)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if train else None
+    res = _new(q) if train else None  # what o's rounding took away: the backward's delta needs it
     with _lib.on_device(q.device):
         _lib.check(lib.specdec_window_attention_forward(
             q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
-            _lib.ptr(lse), _lib.ptr(ctx_lens), B, T, Hq, Hk, D, n_ctx, window, sinks, scale, _status(q.device),
+            _lib.ptr(res), _lib.ptr(lse), _lib.ptr(ctx_lens), B, T, Hq, Hk, D, n_ctx, window, sinks, scale, _status(q.device),
             _stream(q)), "specdec_window_attention_forward")
-    return o, lse
+    return o, res, lse
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, ctx_lens, n_ctx, window, sinks, scale):
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        o, lse = _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, ctx_lens)
+        o, res, lse = _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, o, res, lse, ctx_lens)
         ctx.how = n_ctx, window, sinks, scale
         return o
 
@@ -421,7 +427,7 @@ class _WindowAttention(torch.autograd.Function):
     @_once
     def backward(ctx, do):
         lib = _lib.load()
-        q, k, v, o, lse, ctx_lens = ctx.saved_tensors
+        q, k, v, o, res, lse, ctx_lens = ctx.saved_tensors
         B, T, Hq, D = q.shape
         Hk = k.shape[2]
         do = do.contiguous()
@@ -433,7 +439,7 @@ class _WindowAttention(torch.autograd.Function):
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
             _lib.check(lib.specdec_window_attention_backward(
                 q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
-                lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ctx_lens), B, T,
+                res.data_ptr(), lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ctx_lens), B, T,
                 Hq, Hk, D, *ctx.how, _status(q.device), ws.data_ptr(), ws_bytes, _stream(q)),
                 "specdec_window_attention_backward")
         return dq, dk, dv, None, None, None, None, None

@@ -411,6 +411,8 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
  *                 head_dim] bf16 patterns; head h of q reads head
  *                 h / (q_heads / k_heads) of k and v; head_dim 64 or 128;
  *                 q, k, v strided (rows on 16-byte boundaries), o contiguous
+ *   o_residual    as o, or NULL: what o's rounding took away (bf16(x - o)), for
+ *                 the backward, whose gradients it brings closer
  *   lse           [batch, q_heads, T] values, fp32, natural log (-inf for
  *                 padding), in the backward's own order; or NULL
  *   window >= 1   (INT32_MAX: no window); sinks >= 0
@@ -422,9 +424,10 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
  */
 int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
                                      const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
-                                     uint16_t* o, float* lse, const int32_t* ctx_lens, int32_t batch, int32_t T,
-                                     int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx, int32_t window,
-                                     int32_t sinks, float scale, int32_t* status, void* stream);
+                                     uint16_t* o, uint16_t* o_residual, float* lse, const int32_t* ctx_lens,
+                                     int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                     int32_t n_ctx, int32_t window, int32_t sinks, float scale, int32_t* status,
+                                     void* stream);
 
 /* Workspace bytes of specdec_window_attention_backward on `device`. */
 size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_t q_heads, int32_t k_heads,
@@ -433,14 +436,15 @@ size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_
 
 /*
  * Its backward: dq, dk, dv (contiguous, shaped as q, k, v) from q, k, v, the
- * forward's o and lse, and dout (contiguous). dk and dv are sums over the
+ * forward's o, o_residual (or NULL) and lse, and dout (contiguous). dk and dv are sums over the
  * query heads that share a key head. Fixed summation order, no atomics.
  */
 int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
                                       const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
-                                      const uint16_t* o, const float* lse, const uint16_t* dout, uint16_t* dq,
-                                      uint16_t* dk, uint16_t* dv, const int32_t* ctx_lens, int32_t batch, int32_t T,
-                                      int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t n_ctx,
+                                      const uint16_t* o, const uint16_t* o_residual, const float* lse,
+                                      const uint16_t* dout, uint16_t* dq, uint16_t* dk, uint16_t* dv,
+                                      const int32_t* ctx_lens, int32_t batch, int32_t T, int32_t q_heads,
+                                      int32_t k_heads, int32_t head_dim, int32_t n_ctx,
                                       int32_t window, int32_t sinks, float scale, int32_t* status, void* workspace,
                                       size_t workspace_bytes, void* stream);
 

@@ -305,3 +305,17 @@ def test_rotary_refusals(cuda):
     (g,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
     with pytest.raises(RuntimeError):  # no second derivative
         g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_rotary_past_32_bit_offsets(cuda):
+    """2.2e9 elements: the last tokens lie past 2^31."""
+    T, H, D = 262_200, 64, 128
+    x = torch.zeros(1, T, H, D, device="cuda", dtype=torch.bfloat16)
+    assert x.numel() > 2 ** 31
+    x[0, -9:] = _randn(9, H, D, seed=3, dtype=torch.bfloat16)
+    pos = torch.arange(T, device="cuda")
+    y = drafter.rotary(x, pos, _freq(D))
+    want, size = _rot64(x[:, -9:], pos[-9:], _freq(D), False, 1.0)
+    assert bool(((y[:, -9:].double() - want).abs() <= 5e-7 * size + _half(x.dtype) * want.abs()).all())
+    assert not bool(y[:, :-9].any())

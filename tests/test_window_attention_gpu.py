@@ -7,9 +7,9 @@ Tolerances, per element (h = 2^-8, half a step of bf16):
   once (h): |error| <= h sum_j P_j |v_j| + h |o| + 1e-5.
 - dv = P^T do: likewise with sum P |do|.
 - dS = P (dP - delta) scale: P itself is exact to fp32 here, dP to fp32; delta
-  uses the rounded o: at most h sum_d |do_d o_d| off, and the o above is itself
+  uses the forward's sums (o and the residual of its rounding), which are
   h sum P |v| off. dS is rounded once. So each dS element is off by
-  E = h |dS| + scale P h sum_d |do_d| (sum_j P_j |v_jd| + |o_d|), and
+  E = h |dS| + scale P h sum_d |do_d| sum_j P_j |v_jd|, and
   dq is off by sum_j E |k_j| + h |dq|, dk by sum_i E |q_i| + h |dk|.
 fp32 accumulation of a few thousand terms and exp2's 2^-22 are covered by a
 factor of 1.02 and 1e-5.
@@ -65,7 +65,7 @@ def _oracle(q, k, v, vis, do=None, scale=None):
     dp = torch.einsum("thgd,jhd->hgtj", do, v)
     delta = (do * o).sum(-1).permute(1, 2, 0)[..., None]
     ds = p * (dp - delta) * scale
-    off = H * (do.abs() * (oe + o.abs())).sum(-1).permute(1, 2, 0)[..., None]
+    off = H * (do.abs() * oe).sum(-1).permute(1, 2, 0)[..., None]
     e = H * ds.abs() + scale * p * off
     dq = torch.einsum("hgtj,jhd->thgd", ds, k)
     dqe = torch.einsum("hgtj,jhd->thgd", e, k.abs()) + H * dq.abs()
@@ -275,11 +275,11 @@ def test_window_c_argument_checks():
     p = ctypes.c_void_p(256)  # never dereferenced: the checks fail first
 
     def fwd(q=p, B=1, T=8, Hq=2, Hk=1, D=64, n_ctx=4, W=4, S=0, scale=0.125):
-        return lib.specdec_window_attention_forward(q, None, p, None, p, None, p, p, None, B, T, Hq, Hk, D, n_ctx, W, S,
+        return lib.specdec_window_attention_forward(q, None, p, None, p, None, p, p, p, None, B, T, Hq, Hk, D, n_ctx, W, S,
                                                     scale, None, None)
 
     def bwd(B=1, T=8, Hq=2, Hk=1, D=64, n_ctx=4, W=4, S=0, scale=0.125, ws=1 << 20):
-        return lib.specdec_window_attention_backward(p, None, p, None, p, None, p, p, p, p, p, p, None, B, T, Hq, Hk, D,
+        return lib.specdec_window_attention_backward(p, None, p, None, p, None, p, p, p, p, p, p, p, None, B, T, Hq, Hk, D,
                                                      n_ctx, W, S, scale, None, p, ws, None)
 
     def cached(B=1, T=1, size=8, Hq=2, Hk=1, D=64, nb=0, W=4, S=0, scale=0.125, lens=p):
@@ -326,3 +326,90 @@ def test_window_refusals(cuda):
         drafter.window_attention_cached(x.clone().requires_grad_(True), x, x, lens)
     e = drafter.window_attention(x[:, :0], x[:, :0], x[:, :0], 0)
     assert e.shape == (2, 0, 4, 64)
+
+
+def _withheld(fn):
+    """fn() with the next launch's first CTA left without its first products."""
+    from specdec import _lib
+
+    try:
+        _lib.check(_lib.load().specdec_test_withhold_stage(1), "specdec_test_withhold_stage")
+        out = fn()
+    finally:
+        _lib.load().specdec_test_withhold_stage(0)
+    torch.cuda.synchronize()
+    return out
+
+
+def _reported():
+    from specdec import ops
+
+    with pytest.raises(RuntimeError, match="attention"):
+        ops.check_backward()
+    ops.check_backward()  # cleared
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,Hq,Hk,D,W,first", [
+    (2, 300, 2, 1, 64, 40, 256),         # one query tile per CTA: packed rows 512 .. 599 are tokens 256 .. 299
+    (2, 2048, 16, 16, 128, None, 1792),  # two query tiles per CTA
+])
+def test_an_expired_wait_of_the_forward_gives_nan_rows_and_a_report(cuda, B, T, Hq, Hk, D, W, first):
+    q, k, v = _rand(B, T, Hq, D, seed=1), _rand(B, T, Hk, D, seed=2), _rand(B, T, Hk, D, seed=3)
+    want = drafter.window_attention(q, k, v, T, window=W, sinks=2)
+    got = _withheld(lambda: drafter.window_attention(q, k, v, T, window=W, sinks=2))
+    _reported()
+    lost = torch.zeros(B, T, Hq, dtype=torch.bool, device="cuda")
+    lost[0, first:, :Hq // Hk] = True
+    assert bool(torch.isnan(got[lost]).all()) and torch.equal(got[~lost], want[~lost])
+    assert torch.equal(drafter.window_attention(q, k, v, T, window=W, sinks=2), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,n_ctx,D,W,S", [(300, 300, 64, 40, 0), (2300, 2300, 128, 64, 4), (300, 290, 128, 40, 2)])
+def test_an_expired_wait_of_the_backward_gives_nan_rows_and_a_report(cuda, T, n_ctx, D, W, S):
+    x = [_rand(1, T, 2, D, seed=i).requires_grad_(True) for i in range(3)]
+    do = _rand(1, T, 2, D, seed=5)
+    o = drafter.window_attention(*x, n_ctx, window=W, sinks=S)
+    want = torch.autograd.grad(o, x, do, retain_graph=True)
+    got = _withheld(lambda: torch.autograd.grad(o, x, do, retain_graph=True))
+    _reported()
+    last = (T - 1) // 128 * 128
+    for g, w, rows in zip(got, want, (slice(last, T), slice(0, 128), slice(0, 128))):
+        lost = torch.zeros(1, T, 2, dtype=torch.bool, device="cuda")
+        lost[0, rows, 0] = True
+        assert bool(torch.isnan(g[lost]).all()) and torch.equal(g[~lost], w[~lost])
+    for g, w in zip(torch.autograd.grad(o, x, do), want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.gpu
+def test_an_expired_wait_of_the_cached_form_reaches_the_joined_rows(cuda):
+    q, k, v = _rand(2, 5, 4, 64, seed=1), _rand(2, 900, 2, 64, seed=2), _rand(2, 900, 2, 64, seed=3)
+    lens = torch.tensor([880, 500], device="cuda", dtype=torch.int32)
+    run = lambda: drafter.window_attention_cached(q, k, v, lens, n_block=4, window=700, sinks=2)  # noqa: E731
+    want = run()
+    got = _withheld(run)
+    _reported()
+    lost = torch.zeros(2, 5, 4, dtype=torch.bool, device="cuda")
+    lost[0, :, :2] = True
+    assert bool(torch.isnan(got[lost]).all()) and torch.equal(got[~lost], want[~lost])
+
+
+@pytest.mark.gpu
+def test_a_cache_past_32_bit_offsets(cuda):
+    """Keys and values of 2.4e9 elements each; the last sequence's last tokens
+    lie past 2^31 elements."""
+    B, size, Hk, D = 2, 150_000, 64, 128
+    k, v = (torch.zeros(B, size, Hk, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    c = size - 3
+    for i, t in enumerate((k, v)):
+        t[1, c - 70:] = _rand(73, Hk, D, seed=i)
+    q = _rand(B, 4, Hk, D, seed=9)
+    lens = torch.tensor([0, c], device="cuda", dtype=torch.int32)
+    o = drafter.window_attention_cached(q, k, v, lens, n_block=3, window=60)
+    tail = slice(c - 70, size)
+    pk = torch.arange(c - 70, size)
+    vis = _visible(c + 3 - 4 + torch.arange(4), pk, c, 60, 0)
+    _near("o", o[1], _oracle(q[1], k[1, tail], v[1, tail], vis)["o"])

@@ -41,6 +41,7 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
+constexpr int kMaxHead = 512;
 constexpr int kTableFloats = 512;  // a warp's table: at most 32 / lanes * 32 pairs' cos, or the R of one token
 
 // V consecutive elements of a row, as loaded: one element, or a 16-byte vector.
@@ -105,26 +106,78 @@ __device__ __forceinline__ void ld_sh(const float* p, float (&v)[V]) {
   }
 }
 
+// Elementwise on V values, two per instruction (packed fp32 pairs) for V > 1.
+template <int V>
+__device__ __forceinline__ void vmul(float (&o)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) {
+    o[0] = a[0] * b[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 r = fmul2(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]));
+      o[j] = r.x, o[j + 1] = r.y;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void vfma(float (&o)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V == 1) {
+    o[0] = fmaf(a[0], b[0], c[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 r = ffma2(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]), make_float2(c[j], c[j + 1]));
+      o[j] = r.x, o[j + 1] = r.y;
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void vscale(float (&o)[V], const float (&a)[V], float f) {
+  if constexpr (V == 1) {
+    o[0] = a[0] * f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 r = fmul2(make_float2(a[j], a[j + 1]), make_float2(f, f));
+      o[j] = r.x, o[j + 1] = r.y;
+    }
+  }
+}
+// acc += a . b
+template <int V>
+__device__ __forceinline__ void vdot(float2& acc, const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) {
+    acc.x = fmaf(a[0], b[0], acc.x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2)
+      acc = ffma2(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]), acc);
+  }
+}
+
 // Turns a slot's pairs by (cos, sin). INTER with V > 1: pairs are neighbours
 // inside each vector; otherwise element j of one vector pairs with j of the other.
 template <int V, bool INTER>
 __device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
   if constexpr (INTER && V > 1) {
+    // (x, y) -> x (c, s) + y (-s, c)
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
-      const float a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
-      a[2 * j] = a0 * c[j] - a1 * s[j];
-      a[2 * j + 1] = a1 * c[j] + a0 * s[j];
-      b[2 * j] = b0 * c[V / 2 + j] - b1 * s[V / 2 + j];
-      b[2 * j + 1] = b1 * c[V / 2 + j] + b0 * s[V / 2 + j];
+      const float2 ta = fmul2(make_float2(a[2 * j + 1], a[2 * j + 1]), make_float2(-s[j], c[j]));
+      const float2 ra = ffma2(make_float2(a[2 * j], a[2 * j]), make_float2(c[j], s[j]), ta);
+      const float2 tb = fmul2(make_float2(b[2 * j + 1], b[2 * j + 1]), make_float2(-s[V / 2 + j], c[V / 2 + j]));
+      const float2 rb = ffma2(make_float2(b[2 * j], b[2 * j]), make_float2(c[V / 2 + j], s[V / 2 + j]), tb);
+      a[2 * j] = ra.x, a[2 * j + 1] = ra.y;
+      b[2 * j] = rb.x, b[2 * j + 1] = rb.y;
     }
   } else {
+    float bs[V], as[V];
+    vmul<V>(bs, b, s);
+    vmul<V>(as, a, s);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float x = a[j], y = b[j];
-      a[j] = x * c[j] - y * s[j];
-      b[j] = y * c[j] + x * s[j];
-    }
+    for (int j = 0; j < V; ++j) bs[j] = -bs[j];
+    vfma<V>(a, a, c, bs);
+    vfma<V>(b, b, c, as);
   }
 }
 
@@ -220,9 +273,15 @@ __device__ __forceinline__ T* head_ptr(const RotaryTensor& t, const Unit& u, int
   return const_cast<T*>(static_cast<const T*>(t.p)) + u.b * t.s[0] + u.t * t.s[1] + (int64_t)h * t.s[2];
 }
 
+__device__ __forceinline__ void load_weights(const RotaryArgs& A, const Place& P, float* w) {
+  for (int i = threadIdx.x; i < A.D; i += kRotThreads) w[i] = A.w[P.side][i];
+  __syncthreads();
+}
+
 template <class T, int V, int K, bool NORM, bool INTER>
-__global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const __grid_constant__ RotaryArgs A) {
+__global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 2) rotary_fwd_kernel(const __grid_constant__ RotaryArgs A) {
   __shared__ __align__(16) float table[kRotWarps][kTableFloats];
+  __shared__ __align__(16) float w[kMaxHead];  // the side's weights
   float* cs = table[threadIdx.x >> 5];
   const Place P = place_of(A);
   float* sn = cs + P.tw * (A.R / 2);
@@ -235,16 +294,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const __grid_co
     live[k] = slot < slots;
     rot[k] = slot_place<V>(A, slot, ea[k], eb[k]) && live[k];
   }
-  float wa[K][V], wb[K][V];
-  if constexpr (NORM) {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        wa[k][j] = live[k] ? A.w[P.side][ea[k] + j] : 0.f;
-        wb[k][j] = live[k] ? A.w[P.side][eb[k] + j] : 0.f;
-      }
-  }
+  if constexpr (NORM) load_weights(A, P, w);
   for (int64_t u = P.unit; u < P.units; u += P.step) {
     const Unit U = unit_of(A, P, u);
     Raw<T, V> ra[K], rb[K];
@@ -278,11 +328,13 @@ __global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const __grid_co
       }
       load(h + hpw);  // in flight while this group is worked on
       if constexpr (NORM) {
+        float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) ss = fmaf(x[k][j], x[k][j], fmaf(y[k][j], y[k][j], ss));
-        ss = head_sum(ss, A.lg);
+        for (int k = 0; k < K; ++k) {
+          vdot<V>(sq, x[k], x[k]);
+          vdot<V>(sq, y[k], y[k]);
+        }
+        ss = head_sum(sq.x + sq.y, A.lg);
       }
       if (on) {
         T* q = head_ptr<T>(A.y[P.side], U, h);
@@ -291,11 +343,13 @@ __global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const __grid_co
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
           if constexpr (NORM) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              x[k][j] *= r * wa[k][j];
-              y[k][j] *= r * wb[k][j];
-            }
+            float wv[V];
+            ld_sh<V>(w + ea[k], wv);
+            vscale<V>(x[k], x[k], r);
+            vmul<V>(x[k], x[k], wv);
+            ld_sh<V>(w + eb[k], wv);
+            vscale<V>(y[k], y[k], r);
+            vmul<V>(y[k], y[k], wv);
           }
           if (rot[k]) {
             float c[V], s[V];
@@ -317,13 +371,14 @@ template <class T, int V, int K, bool INTER>
 __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_constant__ RotaryArgs A,
                                                                   float* __restrict__ part) {
   __shared__ __align__(16) float table[kRotWarps][kTableFloats];
+  __shared__ __align__(16) float w[kMaxHead];  // the side's weights
   float* cs = table[threadIdx.x >> 5];
   const Place P = place_of(A);
   float* sn = cs + P.tw * (A.R / 2);
   const int hpw = 32 >> A.lg, slots = A.D / (2 * V);
   int ea[K], eb[K];
   bool live[K], rot[K];
-  float wa[K][V], wb[K][V], acca[K][V], accb[K][V];
+  float acca[K][V], accb[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int slot = P.sub + k * 32;
@@ -331,11 +386,10 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
     rot[k] = slot_place<V>(A, slot, ea[k], eb[k]) && live[k];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      wa[k][j] = live[k] ? A.w[P.side][ea[k] + j] : 0.f;
-      wb[k][j] = live[k] ? A.w[P.side][eb[k] + j] : 0.f;
       acca[k][j] = accb[k][j] = 0.f;
     }
   }
+  load_weights(A, P, w);
   for (int64_t u = P.unit; u < P.units; u += P.step) {
     const Unit U = unit_of(A, P, u);
     Raw<T, V> ra[K], rb[K], sa[K], sb[K];
@@ -359,7 +413,7 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
     for (int i = P.tw == 1 ? U.h - P.group : 0, h = U.h; i < hlast; i += hpw, h += hpw) {
       float xa[K][V], xb[K][V], ga[K][V], gb[K][V];
       const bool on = h < U.hend;
-      float ss = 0.f, dot = 0.f;
+      float2 sq = make_float2(0.f, 0.f), gx = sq;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (on && live[k]) {
@@ -382,14 +436,18 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
           ld_sh<V>(sn + at, s);
           turn<V, INTER>(ga[k], gb[k], c, s);  // dn = rot^T(dout): sin is negated in the table
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          ss = fmaf(xa[k][j], xa[k][j], fmaf(xb[k][j], xb[k][j], ss));
-          dot = fmaf(ga[k][j] * wa[k][j], xa[k][j], fmaf(gb[k][j] * wb[k][j], xb[k][j], dot));
-        }
+        vdot<V>(sq, xa[k], xa[k]);
+        vdot<V>(sq, xb[k], xb[k]);
+        if (!live[k]) continue;
+        float wv[V], t[V];  // g = dn w
+        ld_sh<V>(w + ea[k], wv);
+        vmul<V>(t, ga[k], wv);
+        vdot<V>(gx, t, xa[k]);
+        ld_sh<V>(w + eb[k], wv);
+        vmul<V>(t, gb[k], wv);
+        vdot<V>(gx, t, xb[k]);
       }
-      ss = head_sum(ss, A.lg);
-      dot = head_sum(dot, A.lg);
+      const float ss = head_sum(sq.x + sq.y, A.lg), dot = head_sum(gx.x + gx.y, A.lg);
       if (on) {
         const float r = rsqrtf(ss / (float)A.D + A.eps);
         const float m = r * r * r * dot / (float)A.D;
@@ -397,14 +455,17 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float ta = r * ga[k][j], tb = r * gb[k][j];
-            acca[k][j] = fmaf(ta, xa[k][j], acca[k][j]);
-            accb[k][j] = fmaf(tb, xb[k][j], accb[k][j]);
-            xa[k][j] = ta * wa[k][j] - xa[k][j] * m;
-            xb[k][j] = tb * wb[k][j] - xb[k][j] * m;
-          }
+          vscale<V>(ga[k], ga[k], r);
+          vfma<V>(acca[k], ga[k], xa[k], acca[k]);
+          vscale<V>(xa[k], xa[k], -m);
+          float wv[V];
+          ld_sh<V>(w + ea[k], wv);
+          vfma<V>(xa[k], ga[k], wv, xa[k]);
+          vscale<V>(gb[k], gb[k], r);
+          vfma<V>(accb[k], gb[k], xb[k], accb[k]);
+          vscale<V>(xb[k], xb[k], -m);
+          ld_sh<V>(w + eb[k], wv);
+          vfma<V>(xb[k], gb[k], wv, xb[k]);
           st<V>(q + ea[k], xa[k]);
           st<V>(q + eb[k], xb[k]);
         }

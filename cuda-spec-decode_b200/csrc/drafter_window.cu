@@ -156,6 +156,30 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
+// Rows on their way out. A thread holds one row, and storing it from there
+// would touch a cache line per lane and store; so 16-byte chunks go to shared
+// memory (chunk c of row r at c ^ (r % 8)) and out again row by row.
+template <int D>
+__device__ __forceinline__ void put_chunk(uint32_t tile, uint32_t r, uint32_t c, uint4 v) {
+  st_shared_u4(tile + r * (D * 2) + ((c ^ (r & 7u)) << 4), v);
+}
+// NT threads (lt) write rows [0, rows) of the tile to dst(r); NaN if `bad`.
+template <int D, int NT, class F>
+__device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool bad, F dst) {
+  constexpr int CH = D / 8;
+  const int c = lt % CH;
+#pragma unroll 4
+  for (int r = lt / CH; r < rows; r += NT / CH) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(tile + r * (D * 2) + ((c ^ (r & 7)) << 4))
+                 : "memory");
+    if (bad) v = make_uint4(kNan2, kNan2, kNan2, kNan2);
+    *reinterpret_cast<uint4*>(dst(r) + c * 8) = v;
+  }
+}
+
 // ---- forward --------------------------------------------------------------------
 // One CTA per (sequence, key head, QT x 128 packed rows[, split of the keys]).
 // Warps: QT softmax warpgroups (thread i owns row i of its tile = TMEM lane i),
@@ -171,6 +195,10 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
 //             rescaled there when the reference maximum rises
 // Every wait is bounded and watches a shared flag that the first expired wait
 // raises; all warps then leave for the common end.
+// How the parts of a row's keys come together: one part; unnormalised fp32 rows
+// in the workspace and a second kernel; or within a cluster, up to 8 parts.
+constexpr int kSplitNone = 0, kSplitMemory = 1, kSplitCluster = 2, kClusterMost = 8;
+
 template <int D, int QT>
 struct FwdCfg {
   static constexpr int KN = QT == 2 ? 128 : 64;
@@ -185,7 +213,12 @@ struct FwdCfg {
   static constexpr uint32_t QB = kTM * D * 2, SB = KN * D * 2;
   static constexpr uint32_t OQ = 0, OST = QT * QB, OBAR = OST + NS * SB;
   static constexpr int NBAR = 2 * NS + 3 * QT + 3;  // full, empty, s_full, p_full (halves), q_full, o_full, drain
-  static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;  // TMEM base, dead flag
+  static constexpr uint32_t OSLOT = OBAR + NBAR * 8;         // TMEM base, dead flag
+  static constexpr uint32_t BYTES = OSLOT + 8;
+  // a cluster's join, over the queries and the ring: 128 rows of fp32 (padded
+  // against bank conflicts), then their (maximum, sum)
+  static constexpr uint32_t LD = D + 4, OML = kTM * LD * 4;
+  static_assert(QT == 2 || OML + kTM * 8 <= OBAR, "they fit");
   static constexpr uint32_t COLS = QT == 2 ? 512 : D == 64 ? 128 : 256;
   static constexpr uint32_t COL_O = QT * KN;
 };
@@ -239,7 +272,7 @@ __device__ __forceinline__ void stage_keys(uint32_t tile, const bf16_t* base, in
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-template <int D, int QT, bool SPLIT>
+template <int D, int QT, int SPLIT>
 __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     window_fwd_kernel(const __grid_constant__ WindowArgs A) {
   using C = FwdCfg<D, QT>;
@@ -295,9 +328,9 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   const bool mine = wg < QT && m < A.M;
   const int p = mine ? token_of(A, sq, tq) : -1;
 
-  if (n == 0) {  // nothing to see
+  if (n == 0 && SPLIT != kSplitCluster) {  // nothing to see
     if (mine) {
-      if (SPLIT) {
+      if (SPLIT == kSplitMemory) {
         A.part_ml[prow] = make_float2(-INFINITY, 0.f);
       } else {
 #pragma unroll
@@ -307,7 +340,19 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     }
     return;
   }
-  if (threadIdx.x == 0) {
+  float m_ref = -INFINITY, l_run = 0.f;  // a softmax thread's row: reference maximum, sum
+  bool ok_row = true;                    // no wait of this thread expired
+  int issued = 0;  // stages that this thread's copies have begun
+  // a box of K or V, stage s of the ring
+  auto load_box = [&](int s) {
+    const int j0 = kt.start(i0 + (s >> 1)), row = j0 < sq.c ? j0 : j0 + sq.kb - sq.c;
+    mbar_arrive_expect_tx(full + s % C::NS, C::SB);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(base + C::OST + (s % C::NS) * C::SB + c * (KN * 128), s & 1 ? &A.mv : &A.mk, c * 64, row, hk, b,
+                  full + s % C::NS);
+  };
+  if (threadIdx.x == QT * 128 + 32) {  // the first copying thread
 #pragma unroll
     for (int i = 0; i < C::NS; ++i) {
       mbar_init(full + i, 1);
@@ -324,15 +369,25 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     mbar_init(drain, 1);
     fence_mbar_init();
     *dead = 0;
+    // its boxes start before the CTA meets
+    if (A.q_maps && n > 0) {
+      mbar_arrive_expect_tx(q_full, QT * C::QB);
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(base + C::OQ + t * C::QB + c * (kTM * 128), &A.mq, c * 64, hv * A.G, (m0 + t * kTM) / A.G, b, q_full);
+    }
+    while (issued < min(2 * n, C::NS) && A.kv_maps && boxed<KN>(sq, kt.start(i0 + (issued >> 1)))) load_box(issued++);
   }
   if (warp == QT * 4) tmem_alloc(slot, C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
-  int issued = 0;  // stages that this thread's copies have begun
 
-  if (wg == QT) {
+  if (n == 0) {  // (a cluster's CTA without keys still takes part in the join)
+  } else if (wg == QT) {
     if constexpr (C::LAUNCH_REGS > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::SERVICE_REGS));
     if (warp == QT * 4) {
       // ---- products: the warp walks together, one lane issues ----
@@ -404,31 +459,17 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       const int lt = (int)threadIdx.x - QT * 128 - 32;
       const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
       const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
-      if (lt == 0 && A.q_maps) {
-        mbar_arrive_expect_tx(q_full, QT * C::QB);
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(base + C::OQ + t * C::QB + c * (kTM * 128), &A.mq, c * 64, hv * A.G,
-                        (m0 + t * kTM) / A.G, b, q_full);
-      }
+      const int early = issued;
       bool ok = true;
       for (int s = 0; s < 2 * n; ++s) {  // no early exit: the copying threads meet in stage_keys
         if (ok && s >= C::NS) ok = wait_alive(empty + s % C::NS, (s / C::NS - 1) & 1, dead, A.status);
-        if (ok) issued = s + 1;
+        if (ok) issued = max(issued, s + 1);
         const int i = i0 + (s >> 1), j0 = kt.start(i);
-        const uint32_t stage = base + C::OST + (s % C::NS) * C::SB;
         if (A.kv_maps && boxed<KN>(sq, j0)) {
-          if (ok && lt == 0) {
-            const int row = j0 < sq.c ? j0 : j0 + sq.kb - sq.c;
-            mbar_arrive_expect_tx(full + s % C::NS, C::SB);
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(stage + c * (KN * 128), s & 1 ? &A.mv : &A.mk, c * 64, row, hk, b, full + s % C::NS);
-          }
+          if (ok && lt == 0 && s >= early) load_box(s);
         } else {
-          stage_keys<C::COPY, KN, D>(stage, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0, kt.end(i), lt, ok);
+          stage_keys<C::COPY, KN, D>(base + C::OST + (s % C::NS) * C::SB, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0,
+                                     kt.end(i), lt, ok);
           if (ok && lt == 0) mbar_arrive(full + s % C::NS);
         }
       }
@@ -455,7 +496,6 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       mbar_arrive(q_full);
     }
     const int lo = low_of(A, sq, p), hi = high_of(sq, p);
-    float m_ref = -INFINITY, l_run = 0.f;
     uint32_t steps = 0;
     bool ok = true;
     int tl1 = lo1[0], th0 = hi0[0];
@@ -531,31 +571,33 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     }
     if (ok && steps > 0) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
     tc_fence_after();
-    if (!ok) {  // never a plausible wrong number: the row is NaN
-      if (mine) {
-        if (SPLIT) {
-          A.part_ml[prow] = make_float2(0.f, __int_as_float(0x7fc00000));
-        } else {
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            *reinterpret_cast<uint4*>(orow + 8 * c) = make_uint4(kNan2, kNan2, kNan2, kNan2);
-          if (A.lse) A.lse[(int64_t)bh * A.M + m] = __int_as_float(0x7fc00000);
-        }
-      }
-    } else {
-      const bool seen = p >= 0 && l_run != 0.f;  // (a NaN sum is written as it is)
-      const float inv = 1.f / l_run;
+    ok_row = ok;
+    if (SPLIT == kSplitMemory && mine) A.part_ml[prow] =
+        ok ? make_float2(m_ref, p < 0 ? 0.f : l_run) : make_float2(0.f, __int_as_float(0x7fc00000));
+    if (SPLIT == kSplitMemory && ok) {
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float ot[32];
         tmem_ld32(lane + C::COL_O + t * D + c, ot);
         if (!mine) continue;
-        if (SPLIT) {
-          float* pr = A.part_o + prow * D + c;
+        float* pr = A.part_o + prow * D + c;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(pr + j) = make_float4(ot[j], ot[j + 1], ot[j + 2], ot[j + 3]);
-        } else {
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(pr + j) = make_float4(ot[j], ot[j + 1], ot[j + 2], ot[j + 3]);
+      }
+    }
+    if (SPLIT == kSplitNone) {  // (a cluster's rows are joined below)
+      // every product is done: the rows leave through Q_t's place, the residuals
+      // through the ring's
+      const uint32_t out = base + C::OQ + t * C::QB, res = base + C::OST + t * C::QB, r = threadIdx.x & (kTM - 1);
+      static_assert(QT * C::QB <= C::NS * C::SB, "the residuals fit over the ring");
+      const bool seen = p >= 0 && l_run != 0.f;  // (a NaN sum is written as it is)
+      const float inv = 1.f / l_run;
+      if (ok) {
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float ot[32];
+          tmem_ld32(lane + C::COL_O + t * D + c, ot);
 #pragma unroll
           for (int j = 0; j < 32; ++j) ot[j] = seen ? ot[j] * inv : 0.f;
 #pragma unroll
@@ -563,22 +605,28 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(ot[j + 2 * e], ot[j + 2 * e + 1]);
-            *reinterpret_cast<uint4*>(orow + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            put_chunk<D>(out, r, (c + j) / 8, make_uint4(w[0], w[1], w[2], w[3]));
             if (A.o_res) {  // what the rounding took away
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 w[e] = pack_bf16x2(ot[j + 2 * e] - bf16_lo(w[e]), ot[j + 2 * e + 1] - bf16_hi(w[e]));
-              *reinterpret_cast<uint4*>(A.o_res + (orow - A.o) + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+              put_chunk<D>(res, r, (c + j) / 8, make_uint4(w[0], w[1], w[2], w[3]));
             }
           }
         }
       }
-      if (mine) {
-        if (SPLIT)
-          A.part_ml[prow] = make_float2(m_ref, p < 0 ? 0.f : l_run);
-        else if (A.lse)
-          A.lse[(int64_t)bh * A.M + m] = seen ? (m_ref + log2f(l_run)) * kLn2 : -INFINITY;
-      }
+      if (mine && A.lse)
+        A.lse[(int64_t)bh * A.M + m] = !ok ? __int_as_float(0x7fc00000) : seen ? (m_ref + log2f(l_run)) * kLn2 : -INFINITY;
+      // all 128 threads meet, also after an expired wait (then the rows are NaN,
+      // never a plausible wrong number)
+      asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory");
+      const int rows = min(kTM, A.M - mt);
+      auto at = [&](int row) {
+        const int mr = mt + row, tr = group_div(A, mr);
+        return (((int64_t)b * A.Tq + tr) * A.Hq + hv * A.G + mr - tr * A.G) * D;
+      };
+      flush_rows<D, kTM>(out, rows, r, *dead != 0, [&](int row) { return A.o + at(row); });
+      if (A.o_res) flush_rows<D, kTM>(res, rows, r, *dead != 0, [&](int row) { return A.o_res + at(row); });
     }
   }
   tc_fence_before();
@@ -588,10 +636,68 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     if (warp == QT * 4 && (threadIdx.x & 31) == 0) umma_commit(drain);
     mbar_wait(drain, 0);
     if (threadIdx.x == QT * 128 + 32) {
-      if (A.q_maps) mbar_wait(q_full, 0);
+      if (A.q_maps && n > 0) mbar_wait(q_full, 0);
       for (int s = max(0, issued - C::NS); s < issued; ++s) mbar_wait(full + s % C::NS, (s / C::NS) & 1);
     }
     __syncthreads();
+  }
+  if constexpr (SPLIT == kSplitCluster) {
+    // The splits of a row are the CTAs of a cluster: each leaves its fp32 rows
+    // and their (maximum, sum) in its own shared memory, where nothing is in
+    // flight any more, and joins a share of the rows from all of them.
+    constexpr int LD = C::LD;
+    float* po = reinterpret_cast<float*>(smem);
+    float2* ml = reinterpret_cast<float2*>(smem + C::OML);
+    if (wg < QT) {
+      const int r = threadIdx.x;
+      if (n > 0) {
+        const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float ot[32];
+          tmem_ld32(lane + C::COL_O + c, ot);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(po + r * LD + c + j) = make_float4(ot[j], ot[j + 1], ot[j + 2], ot[j + 3]);
+        }
+      }
+      ml[r] = !ok_row ? make_float2(0.f, __int_as_float(0x7fc00000)) : make_float2(m_ref, p < 0 ? 0.f : l_run);
+    }
+    cluster_sync();
+    const int rows = min(kTM, A.M - m0), each = (rows + A.splits - 1) / A.splits;
+    const int r0 = (int)blockIdx.z * each, r1 = min(rows, r0 + each);
+    for (int i = threadIdx.x; i < (r1 - r0) * (D / 4); i += C::THREADS) {
+      const int r = r0 + i / (D / 4), c = i % (D / 4) * 4;
+      float2 v[kClusterMost];
+      float4 o[kClusterMost];
+#pragma unroll
+      for (int z = 0; z < kClusterMost; ++z) {  // all parts' loads in flight at once
+        v[z] = make_float2(-INFINITY, 0.f);
+        if (z < A.splits) {
+          v[z] = ld_cluster_f2(cluster_addr(base + C::OML + r * 8, z));
+          o[z] = ld_cluster_f4(cluster_addr(base + (uint32_t)(r * LD + c) * 4, z));
+        }
+      }
+      float mx = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int z = 0; z < kClusterMost; ++z) mx = fmaxf(mx, v[z].x);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int z = 0; z < kClusterMost; ++z) {
+        if (v[z].y == 0.f) continue;  // this part saw nothing (its rows hold anything)
+        const float w = exp2_approx(v[z].x - mx);
+        l = fmaf(v[z].y, w, l);
+        acc.x = fmaf(o[z].x, w, acc.x), acc.y = fmaf(o[z].y, w, acc.y);
+        acc.z = fmaf(o[z].z, w, acc.z), acc.w = fmaf(o[z].w, w, acc.w);
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int mr = m0 + r, tr = group_div(A, mr);
+      *reinterpret_cast<uint2*>(A.o + (((int64_t)b * A.Tq + tr) * A.Hq + hv * A.G + mr - tr * A.G) * D + c) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    }
+    tc_fence_before();
+    cluster_sync();  // a CTA's shared memory stays until all have read it
+    tc_fence_after();
   }
   if (warp == QT * 4) tmem_free(tmem, C::COLS);
 }
@@ -711,31 +817,33 @@ __device__ __forceinline__ void stage_queries(const WindowArgs& A, uint32_t tile
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-// The warpgroup's D / NB columns of an accumulator row, times `f`.
+// The warpgroup's D / NB columns of an accumulator row, times `f` (zeros if
+// `zero`), as bf16 chunks into the shared tile, or as fp32 to `part`.
 template <int D, int NB>
-__device__ __forceinline__ void store_acc(bf16_t* row, float* part, uint32_t col, int wg, float f, bool write, bool zero) {
+__device__ __forceinline__ void store_acc(uint32_t tile, uint32_t r, float* part, uint32_t col, int wg, float f, bool mine,
+                                          bool zero) {
 #pragma unroll
   for (int c = 0; c < D / NB; c += 32) {
     float a[32];
     tmem_ld32(col + wg * (D / NB) + c, a);
-    if (!write) continue;
     const int at = wg * (D / NB) + c;
 #pragma unroll
     for (int j = 0; j < 32; ++j) a[j] = zero ? 0.f : a[j] * f;
     if (part) {
+      if (!mine) continue;
 #pragma unroll
       for (int j = 0; j < 32; j += 4)
         *reinterpret_cast<float4*>(part + at + j) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
     } else {
 #pragma unroll
       for (int j = 0; j < 32; j += 8)
-        *reinterpret_cast<uint4*>(row + at + j) =
-            make_uint4(pack_bf16x2(a[j], a[j + 1]), pack_bf16x2(a[j + 2], a[j + 3]),
-                       pack_bf16x2(a[j + 4], a[j + 5]), pack_bf16x2(a[j + 6], a[j + 7]));
+        put_chunk<D>(tile, r, (at + j) / 8,
+                     make_uint4(pack_bf16x2(a[j], a[j + 1]), pack_bf16x2(a[j + 2], a[j + 3]),
+                                pack_bf16x2(a[j + 4], a[j + 5]), pack_bf16x2(a[j + 6], a[j + 7])));
     }
   }
 }
-// The same columns filled with one value: zeros, or NaN after an expired wait.
+// The same columns of a row in global memory filled with zeros, or NaN.
 template <int D, int NB>
 __device__ __forceinline__ void fill_row(bf16_t* row, float* part, int wg, bool nan) {
   const uint32_t w = nan ? kNan2 : 0u;
@@ -825,7 +933,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   }
 
   const bool x_boxes = DKV ? A.kv_maps : A.q_maps, y_boxes = DKV ? A.q_maps : A.kv_maps;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == NB * 128 + 32) {  // the first copying thread
 #pragma unroll
     for (int i = 0; i < C::NS; ++i) {
       mbar_init(full + i, 1);
@@ -842,6 +950,22 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     mbar_init(drain, 1);
     fence_mbar_init();
     *dead = 0;
+    if (x_boxes) {  // X starts before the CTA meets
+      const int q_head = DKV ? hk * A.nsub * A.G : head * A.G;
+      mbar_arrive_expect_tx(x_full, 2 * C::XB);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const uint32_t dst = base + C::OX + x * C::XB + c * (kTM * 128) + h * (64 * 128);
+            if (DKV)
+              tma_load_4d(dst, x ? &A.mv : &A.mk, c * 64, x0 + h * 64, hk, b, x_full);
+            else
+              tma_load_4d(dst, x ? &A.mg : &A.mq, c * 64, q_head, (x0 + h * 64) / A.G, b, x_full);
+          }
+    }
   }
   if (warp == NB * 4) tmem_alloc(slot, C::COLS);
   tc_fence_before();
@@ -906,23 +1030,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
       const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)q_head * A.qs[2];
       const bf16_t* gb = A.dO + ((int64_t)b * A.Tq * A.Hq + q_head) * D;
       const int64_t gts = (int64_t)A.Hq * D;
-      if (x_boxes) {
-        if (lt == 0) {
-          mbar_arrive_expect_tx(x_full, 2 * C::XB);
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int c = 0; c < D / 64; ++c) {
-                const uint32_t dst = base + C::OX + x * C::XB + c * (kTM * 128) + h * (64 * 128);
-                if (DKV)
-                  tma_load_4d(dst, x ? &A.mv : &A.mk, c * 64, x0 + h * 64, hk, b, x_full);
-                else
-                  tma_load_4d(dst, x ? &A.mg : &A.mq, c * 64, q_head, (x0 + h * 64) / A.G, b, x_full);
-              }
-        }
-      } else {
+      if (!x_boxes) {
         if (DKV) {  // key rows [x0, x0 + 128) of the batch: tokens or padding (zeros)
 #pragma unroll 1
           for (int x = 0; x < 2; ++x) {
@@ -1097,14 +1205,30 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     }
     if (ok) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
     tc_fence_after();
-    if (!ok) {  // never a plausible wrong number
-      if (mine) {
-        fill_row<D, NB>(row_a, part_a, wg, true);
-        if (DKV) fill_row<D, NB>(row_b, part_b, wg, true);
+    // every product is done: the rows leave through X's place
+    if (ok) {
+      store_acc<D, NB>(base + C::OX, r, part_a, lane + C::COL_A, wg, DKV ? 1.f : A.scale, mine, token < 0);
+      if (DKV) store_acc<D, NB>(base + C::OX + C::XB, r, part_b, lane + C::COL_B, wg, A.scale, mine, token < 0);
+    } else if (partial && mine) {
+      fill_row<D, NB>(row_a, part_a, wg, true);
+      fill_row<D, NB>(row_b, part_b, wg, true);
+    }
+    if (!partial) {
+      // all the threads meet, also after an expired wait (then the rows are NaN,
+      // never a plausible wrong number)
+      asm volatile("bar.sync 2, %0;" ::"n"(NB * 128) : "memory");
+      const bool bad = *dead != 0;
+      if (DKV) {
+        const int rows = min(kTM, A.Tq - x0);
+        const int64_t at = (((int64_t)b * A.Tq + x0) * A.Hk + hk) * D, step = (int64_t)A.Hk * D;
+        flush_rows<D, NB * 128>(base + C::OX, rows, threadIdx.x, bad, [&](int q) { return A.dv + at + q * step; });
+        flush_rows<D, NB * 128>(base + C::OX + C::XB, rows, threadIdx.x, bad, [&](int q) { return A.dk + at + q * step; });
+      } else {
+        flush_rows<D, NB * 128>(base + C::OX, min(kTM, A.M - x0), threadIdx.x, bad, [&](int q) {
+          const int mr = x0 + q, tr = group_div(A, mr);
+          return A.dq + (((int64_t)b * A.Tq + tr) * A.Hq + head * A.G + mr - tr * A.G) * D;
+        });
       }
-    } else {
-      store_acc<D, NB>(row_a, part_a, lane + C::COL_A, wg, DKV ? 1.f : A.scale, mine, token < 0);
-      if (DKV) store_acc<D, NB>(row_b, part_b, lane + C::COL_B, wg, A.scale, mine, token < 0);
     }
   }
   tc_fence_before();
@@ -1269,7 +1393,7 @@ bool group_map(CUtensorMap* map, const WindowArgs& A, const bf16_t* p, const int
   return make_map(map, p, d, {s[2], s[1], s[0]}, A.G, rows / A.G);
 }
 
-template <int D, int QT, bool SPLIT>
+template <int D, int QT, int SPLIT>
 cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   using C = FwdCfg<D, QT>;
   static std::atomic<unsigned long long> done{0};
@@ -1279,8 +1403,22 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   kv_maps(A, D, C::KN);
   A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
   const dim3 grid((unsigned)(A.B * A.Hk * A.nsub), (unsigned)((A.M + QT * kTM - 1) / (QT * kTM)), (unsigned)A.splits);
-  window_fwd_kernel<D, QT, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
-  return cudaGetLastError();
+  if constexpr (SPLIT == kSplitCluster) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {1, 1, (unsigned)A.splits};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::BYTES;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, window_fwd_kernel<D, QT, SPLIT>, (const WindowArgs&)A);
+  } else {
+    window_fwd_kernel<D, QT, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
+    return cudaGetLastError();
+  }
 }
 
 template <int D>
@@ -1292,9 +1430,10 @@ cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
     // 232 / 188, 512 keys 71 / 80; at D = 64: 84 / 85, 135 / 125, 199 / 169, 57 / 66.
     const int64_t pairs = (int64_t)A.B * A.Hk * A.nsub * ((A.M + 2 * kTM - 1) / (2 * kTM));
     const int64_t seen = std::min<int64_t>(A.Tk, (int64_t)A.W + A.S);
-    return pairs >= sms && seen >= 1536 ? fwd_launch<D, 2, false>(A, st) : fwd_launch<D, 1, false>(A, st);
+    return pairs >= sms && seen >= 1536 ? fwd_launch<D, 2, kSplitNone>(A, st) : fwd_launch<D, 1, kSplitNone>(A, st);
   }
-  const cudaError_t e = fwd_launch<D, 1, true>(A, st);
+  if (A.splits <= kClusterMost) return fwd_launch<D, 1, kSplitCluster>(A, st);
+  const cudaError_t e = fwd_launch<D, 1, kSplitMemory>(A, st);
   if (e != cudaSuccess) return e;
   const int64_t rows = (int64_t)A.B * A.Hk * A.M;
   window_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(A);
@@ -1382,6 +1521,13 @@ int window_splits(int D, int64_t ctas, int64_t most_keys, int sms) {
   const int64_t tiles = (most_keys + kTN - 1) / kTN + 1;
   const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64, 1>::CTAS : FwdCfg<128, 1>::CTAS);
   return (int)std::max<int64_t>(1, std::min<int64_t>(room / std::max<int64_t>(1, ctas), tiles / 2));
+}
+
+size_t window_split_workspace(int D, int64_t rows, int splits, size_t* ml_at) {
+  *ml_at = 0;
+  if (splits <= kClusterMost) return 0;  // joined within clusters
+  *ml_at = ((size_t)rows * splits * D * sizeof(float) + 255) & ~size_t(255);
+  return *ml_at + (size_t)rows * splits * sizeof(float2);
 }
 
 cudaError_t window_fwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st) {

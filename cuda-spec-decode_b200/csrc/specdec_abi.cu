@@ -979,7 +979,7 @@ int rotary_args(RotaryArgs& A, const int64_t* positions, int64_t pos_stride, con
                 int32_t T, int32_t q_heads, int32_t k_heads, int32_t D, int32_t R, int32_t interleaved, float scale,
                 float eps, int32_t dtype, int* sms) {
   if (batch < 0 || T < 0 || q_heads < 1 || k_heads < 0) return fail(SPECDEC_ERR_ARGUMENT, "bad shape");
-  if ((int64_t)batch * T > INT32_MAX) return fail(SPECDEC_ERR_ARGUMENT, "batch * T must fit in int32");
+  if ((int64_t)batch * T > INT32_MAX - 64) return fail(SPECDEC_ERR_ARGUMENT, "batch * T must be below 2^31 - 64");
   if ((int64_t)q_heads + k_heads > 65536) return fail(SPECDEC_ERR_ARGUMENT, "at most 65536 heads");
   if (D < 2 || D > 512 || D % 2) return fail(SPECDEC_ERR_ARGUMENT, "head_dim must be even and in [2, 512], got %d", D);
   if (R < 2 || R > D || R % 2)
@@ -1281,12 +1281,12 @@ size_t specdec_window_attention_cached_workspace_bytes(int32_t batch, int32_t q_
   if (batch <= 0 || q_len <= 0 || cache_len <= 0 || q_heads <= 0 || k_heads <= 0 || q_heads % k_heads ||
       (head_dim != 64 && head_dim != 128) || window < 1 || sinks < 0 || n_block < 0 ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return 256;
+    return 0;
   const int64_t M = (int64_t)q_len * (q_heads / k_heads), bh = (int64_t)batch * k_heads;
   const int splits = window_splits(head_dim, bh * ((M + 127) / 128),
                                    window_most_keys(q_len, cache_len, n_block, window, sinks), sms);
-  if (splits == 1) return 256;
-  return align256((size_t)bh * M * splits * head_dim * sizeof(float)) + align256((size_t)bh * M * splits * sizeof(float2));
+  size_t at;
+  return align256(window_split_workspace(head_dim, bh * M, splits, &at));
 }
 
 int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides, const uint16_t* k_cache,
@@ -1317,9 +1317,9 @@ int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides,
   const int64_t bh = (int64_t)batch * k_heads;
   A.splits = window_splits(head_dim, bh * ((A.M + 127) / 128),
                            window_most_keys(q_len, cache_len, n_block, window, sinks), sms);
-  if (A.splits > 1) {
-    const size_t rows = (size_t)bh * A.M * A.splits, at = align256(rows * head_dim * sizeof(float));
-    const size_t need = at + rows * sizeof(float2);
+  size_t at = 0;
+  const size_t need = window_split_workspace(head_dim, bh * A.M, A.splits, &at);
+  if (need > 0) {
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
       return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes on a 16-byte boundary, got %zu", need,
                   workspace ? workspace_bytes : 0);

@@ -372,8 +372,8 @@ _NO_WINDOW = 2 ** 31 - 1
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t itself if every row of a head starts on a 16-byte boundary, else a copy."""
-    if t.data_ptr() % 16 == 0 and t.stride(3) == 1 and all(
-            t.stride(d) % 8 == 0 or t.shape[d] <= 1 for d in range(3)):
+    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or t.stride(3) == 1 and all(
+            t.stride(d) % 8 == 0 or t.shape[d] <= 1 for d in range(3))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -499,9 +499,9 @@ def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     with _lib.on_device(q.device):
         ws_bytes = lib.specdec_window_attention_cached_workspace_bytes(B, Tq, size, Hq, Hk, D, n_block, window, sinks,
                                                                        q.device.index)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
         _lib.check(lib.specdec_window_attention_cached(
             q.data_ptr(), _strides(q), k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
             o.data_ptr(), ctx_lens.data_ptr(), B, Tq, size, Hq, Hk, D, int(n_block), window, sinks, scale,
-            _status(q.device), ws.data_ptr(), ws_bytes, _stream(q)), "specdec_window_attention_cached")
+            _status(q.device), _lib.ptr(ws), ws_bytes, _stream(q)), "specdec_window_attention_cached")
     return o

@@ -362,7 +362,7 @@ int specdec_dflash_attention_backward(const uint16_t* q, const uint16_t* k, cons
  *              (position_stride 0: shared by the sequences)
  *   inv_freq   [rotary_dim / 2] fp64; angles are formed and reduced in fp64
  * head_dim even, <= 512; rotary_dim even, in [2, head_dim]; batch * T must
- * fit in int32. x, y: `dtype` (SPECDEC_DTYPE_*). y may equal x if x is contiguous.
+ * be below 2^31 - 64. x, y: `dtype` (SPECDEC_DTYPE_*). y may equal x if x is contiguous.
  */
 int specdec_rotary(const void* x, const int64_t* x_strides, void* y, const int64_t* positions,
                    int64_t position_stride, const double* inv_freq, int32_t batch, int32_t T, int32_t heads,
@@ -448,7 +448,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
                                       int32_t window, int32_t sinks, float scale, int32_t* status, void* workspace,
                                       size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of specdec_window_attention_cached on `device`. */
+/* Workspace bytes of specdec_window_attention_cached on `device`; 0: it needs none (NULL will do). */
 size_t specdec_window_attention_cached_workspace_bytes(int32_t batch, int32_t q_len, int32_t cache_len,
                                                        int32_t q_heads, int32_t k_heads, int32_t head_dim,
                                                        int32_t n_block, int32_t window, int32_t sinks, int device);

@@ -569,7 +569,9 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       l_run = fmaf(l_run, alpha, l2.x + l2.y);
       ++steps;
     }
-    if (ok && steps > 0) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
+    // also where this tile had no step: the rows leave through memory that the
+    // other tile's products read
+    if (ok) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
     tc_fence_after();
     ok_row = ok;
     if (SPLIT == kSplitMemory && mine) A.part_ml[prow] =

@@ -131,6 +131,42 @@ def test_window_attention_forward_backward(cuda, B, n_ctx, nb, Hq, Hk, D, W, S, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,n_ctx,nb,Hq,Hk,D,W,S,lens", [
+    (2, 1584, 16, 16, 16, 64, 1540, 4, None),         # the last CTA's second query tile is empty
+    (2, 1584, 16, 16, 16, 128, 1540, 4, None),
+    (1, 2000, 7, 40, 20, 128, 1700, 130, None),       # shared heads, two sink tiles
+    (3, 1700, 0, 18, 6, 64, None, 0, (1700, 3, 900)),  # groups of three, padded tiles
+    (3, 1650, 20, 16, 16, 128, 1600, 1, (0, 1650, 1500)),
+])
+def test_window_attention_with_two_query_tiles_per_cta(cuda, B, n_ctx, nb, Hq, Hk, D, W, S, lens):
+    """Sizes that take the forward with two query tiles per CTA (148 of them or
+    more, 1536 visible keys or more); a few heads of each sequence are compared."""
+    T, G = n_ctx + nb, Hq // Hk
+    q, do = _rand(B, T, Hq, D, seed=1), _rand(B, T, Hq, D, seed=2)
+    k, v = _rand(B, T, Hk, D, seed=3), _rand(B, T, Hk, D, seed=4)
+    cs = [n_ctx] * B if lens is None else lens
+    ctx_lens = None if lens is None else torch.tensor(lens, device="cuda", dtype=torch.int32)
+    for b, c in enumerate(cs):
+        for t in (q, k, v, do):
+            t[b, c:n_ctx] = float("nan")
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = drafter.window_attention(*x, n_ctx, window=W, sinks=S, ctx_lens=ctx_lens)
+    got = [o.detach(), *torch.autograd.grad(o, x, do)]
+    with torch.no_grad():
+        assert torch.equal(drafter.window_attention(*x, n_ctx, window=W, sinks=S, ctx_lens=ctx_lens), o)
+    for b, c in enumerate(cs):
+        for t in got:
+            assert bool((t[b, c:n_ctx] == 0).all()) and bool(torch.isfinite(t[b].float()).all())
+        tok = _tokens(T, n_ctx, c)
+        vis = _visible(tok, tok, c, W or 10 ** 9, S)
+        for h in {0, Hk - 1}:
+            qs, ks = slice(h * G, (h + 1) * G), slice(h, h + 1)
+            want = _oracle(q[b, :, qs].detach(), k[b, :, ks].detach(), v[b, :, ks].detach(), vis, do[b, :, qs])
+            for n, t, s in zip(("o", "dq", "dk", "dv"), got, (qs, qs, ks, ks)):
+                _near(n, t[b, :, s], want[n])
+
+
+@pytest.mark.gpu
 def test_without_window_it_is_the_dflash_attention(cuda):
     """window None, no sinks: the mask of dflash_attention; the two kernels
     round the same quantities, in tiles of their own."""

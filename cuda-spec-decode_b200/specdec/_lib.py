@@ -1,7 +1,9 @@
 """ctypes binding of libspecdec.so, the C ABI declared in include/specdec.h.
 
-This module is the only place that touches the shared library. It maps the
-library's status codes onto the exceptions the reference raises
+From Python, this module is the only place that touches the shared library
+(the drafter's long-context operators go through the torch binding
+csrc/drafter_bind.cpp instead, over the same C ABI). It maps the library's
+status codes onto the exceptions the reference raises
 (AssertionError for shape/dtype/contract violations, ValueError for values out
 of domain), and keeps one workspace (scratch + zero-initialised counters) per
 (device, stream, kernel family) so repeated calls allocate nothing.

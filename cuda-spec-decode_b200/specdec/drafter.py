@@ -28,11 +28,9 @@ dtypes above.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -57,17 +55,6 @@ def _status(dev: torch.device) -> int:
     synchronising check (specdec.ops.check_backward, a validating D-PACE
     forward, GraphedStep.check) raises RuntimeError and clears it."""
     return _lib.status_words(dev).data_ptr() + 4 * _lib.STATUS_DRAFTER
-
-
-def _once(fn):
-    """once_differentiable, but only where a graph of the backward is being
-    built: its wrapper costs 20 us per call."""
-    slow = once_differentiable(fn)
-
-    def backward(ctx, *grads):
-        return slow(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
-
-    return backward
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -209,71 +196,22 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str | None = No
     return freq.to(device=device), scale
 
 
-def _strided(t: torch.Tensor) -> torch.Tensor:
-    """A head's elements contiguous; the other dimensions as they are."""
-    return t if t.stride(-1) == 1 else t.contiguous()
+def _ops():
+    """The torch binding of these operators (csrc/drafter_bind.cpp): checks,
+    outputs, streams and autograd in C++ over the same C ABI."""
+    global _torch_ops
+    if _torch_ops is None:
+        _lib.load()  # raises if the library is not built
+        try:
+            from . import _torch_ops as module
+        except ImportError as e:
+            raise ImportError("_torch_ops.so is not built; build it with `make -C cuda-spec-decode_b200/csrc` or "
+                              "__graft_entry__.build()") from e
+        _torch_ops = module
+    return _torch_ops
 
 
-def _new(t: torch.Tensor) -> torch.Tensor:
-    """An uninitialised contiguous tensor shaped as t (empty_like costs the
-    host half of torch.empty)."""
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
-
-
-def _strides(t: torch.Tensor):
-    """The C ABI's three element strides (None: contiguous)."""
-    return None if t.is_contiguous() else (ctypes.c_int64 * 3)(*t.stride()[:3])
-
-
-def _check_heads(name: str, x: torch.Tensor, like: torch.Tensor | None = None) -> None:
-    assert x.is_cuda and x.dim() == 4 and x.dtype in _DTYPES, f"{name} must be cuda float32 or bfloat16 [B, T, heads, D]"
-    if like is not None:
-        assert x.device == like.device and x.dtype == like.dtype and x.shape[:2] == like.shape[:2] \
-            and x.shape[3] == like.shape[3], f"{name} must match q's device, dtype, batch, length and head size"
-
-
-def _check_rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    assert positions.device == x.device and positions.dtype in (torch.int64, torch.int32) \
-        and (positions.shape == x.shape[:2] or positions.shape == x.shape[1:2]), \
-        "positions must be int64 (or int32) [T] or [B, T] on the heads' device"
-    assert inv_freq.device == x.device and inv_freq.dtype == torch.float64 and inv_freq.dim() == 1, \
-        "inv_freq must be float64 [rotary_dim / 2] on the heads' device"
-    assert 0 < 2 * inv_freq.numel() <= x.shape[3], "inv_freq must turn at least one pair and at most the head"
-    positions = positions.long()
-    if positions.stride(-1) != 1 and positions.shape[-1] > 1:
-        positions = positions.contiguous()
-    return positions, inv_freq.contiguous()
-
-
-def _position_stride(positions: torch.Tensor) -> int:
-    return positions.stride(0) if positions.dim() == 2 else 0
-
-
-def _rotary(x, positions, inv_freq, interleaved, scale, inverse):
-    lib = _lib.load()
-    B, T, H, D = x.shape
-    x = _strided(x)
-    y = _new(x)
-    with _lib.on_device(x.device):
-        _lib.check(lib.specdec_rotary(
-            x.data_ptr(), _strides(x), y.data_ptr(), positions.data_ptr(), _position_stride(positions),
-            inv_freq.data_ptr(), B, T, H, D, 2 * inv_freq.numel(), interleaved, scale, inverse, _DTYPES[x.dtype],
-            _stream(x)), "specdec_rotary")
-    return y
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, inv_freq, interleaved, scale):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.how = interleaved, scale
-        return _rotary(x, positions, inv_freq, interleaved, scale, 0)
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        positions, inv_freq = ctx.saved_tensors
-        return _rotary(dy, positions, inv_freq, *ctx.how, 1), None, None, None, None
+_torch_ops = None
 
 
 def rotary_supported(x: torch.Tensor) -> bool:
@@ -289,56 +227,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     position * inv_freq[i] and is multiplied by ``scale``; the rest is copied.
     positions: int64 [T] or [B, T]; inv_freq: fp64 (``rotary_frequencies``).
     Angles are formed in fp64. Differentiable in x."""
-    _check_heads("x", x)
-    positions, inv_freq = _check_rotary(x, positions, inv_freq)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Rotary.apply(x, positions, inv_freq, int(bool(interleaved)), float(scale))
-    return _rotary(x, positions, inv_freq, int(bool(interleaved)), float(scale), 0)
-
-
-def _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale):
-    lib = _lib.load()
-    B, T, Hq, D = q.shape
-    yq, yk = _new(q), _new(k)
-    with _lib.on_device(q.device):
-        _lib.check(lib.specdec_qk_norm_rotary_forward(
-            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), yq.data_ptr(),
-            yk.data_ptr(), positions.data_ptr(), _position_stride(positions), inv_freq.data_ptr(), B, T, Hq, k.shape[2],
-            D, 2 * inv_freq.numel(), interleaved, scale, eps, _DTYPES[q.dtype], _stream(q)),
-            "specdec_qk_norm_rotary_forward")
-    return yq, yk
-
-
-class _QKNormRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, scale):
-        q, k = _strided(q), _strided(k)
-        wq, wk = q_weight.float().contiguous(), k_weight.float().contiguous()
-        ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
-        ctx.how = eps, interleaved, scale
-        ctx.wdtypes = q_weight.dtype, k_weight.dtype
-        return _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, scale)
-
-    @staticmethod
-    @_once
-    def backward(ctx, dyq, dyk):
-        lib = _lib.load()
-        q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
-        eps, interleaved, scale = ctx.how
-        B, T, Hq, D = q.shape
-        Hk = k.shape[2]
-        dyq, dyk = _strided(dyq), _strided(dyk)
-        dq, dk, dwq, dwk = _new(q), _new(k), _new(wq), _new(wk)
-        with _lib.on_device(q.device):
-            ws_bytes = lib.specdec_qk_norm_rotary_workspace_bytes(B, T, D, q.device.index)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-            _lib.check(lib.specdec_qk_norm_rotary_backward(
-                q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), wq.data_ptr(), wk.data_ptr(), dyq.data_ptr(),
-                _strides(dyq), dyk.data_ptr(), _strides(dyk), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
-                dwk.data_ptr(), positions.data_ptr(), _position_stride(positions), inv_freq.data_ptr(), B, T, Hq, Hk,
-                D, 2 * inv_freq.numel(), interleaved, scale, eps, _DTYPES[q.dtype], ws.data_ptr(), ws_bytes,
-                _stream(q)), "specdec_qk_norm_rotary_backward")
-        return dq, dk, dwq.to(ctx.wdtypes[0]), dwk.to(ctx.wdtypes[1]), None, None, None, None, None
+    return _ops().rotary(x, positions, inv_freq, interleaved, scale)
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -350,100 +239,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     any strides (views of one fused projection); fp32 arithmetic, one rounding.
     Differentiable in q, k and the weights (their gradients are summed in a
     fixed order)."""
-    _check_heads("q", q)
-    _check_heads("k", k, q)
-    D = q.shape[3]
-    assert q_weight.shape == (D,) and k_weight.shape == (D,) and q_weight.device == q.device \
-        and k_weight.device == q.device, "weights must be [D] on q's device"
-    positions, inv_freq = _check_rotary(q, positions, inv_freq)
-    e = torch.finfo(q.dtype).eps if eps is None else float(eps)
-    how = e, int(bool(interleaved)), float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
-                                    or k_weight.requires_grad):
-        return _QKNormRotary.apply(q, k, q_weight, k_weight, positions, inv_freq, *how)
-    return _qk_norm_rotary(_strided(q), _strided(k), q_weight.float().contiguous(), k_weight.float().contiguous(),
-                           positions, inv_freq, *how)
+    return _ops().qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, scale)
 
 
 # ---- sliding-window attention with sinks ------------------------------------------
-
-_NO_WINDOW = 2 ** 31 - 1
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t itself if every row of a head starts on a 16-byte boundary, else a copy."""
-    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or t.stride(3) == 1 and all(
-            t.stride(d) % 8 == 0 or t.shape[d] <= 1 for d in range(3))):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _check_window(q, k, v, window, sinks, scale) -> tuple[int, int, float]:
-    assert q.is_cuda and q.dtype == torch.bfloat16 and q.dim() == 4, "q must be cuda bfloat16 [B, T, heads, D]"
-    assert q.shape[3] in (64, 128), f"heads must have 64 or 128 elements, got {q.shape[3]}"
-    assert k.dim() == 4 and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3], \
-        "k and v must be [B, T, k_heads, D] with q's batch and head size"
-    assert k.dtype == q.dtype and v.dtype == q.dtype and k.device == q.device and v.device == q.device, \
-        "k and v must have q's dtype and device"
-    assert k.shape[2] > 0 and q.shape[2] > 0 and q.shape[2] % k.shape[2] == 0, \
-        f"query heads must be a multiple of key heads ({q.shape[2]}, {k.shape[2]})"
-    assert window is None or window >= 1, f"window must be >= 1 or None, got {window}"
-    assert sinks >= 0, f"sinks must be >= 0, got {sinks}"
-    return (_NO_WINDOW if window is None else min(int(window), _NO_WINDOW), min(int(sinks), _NO_WINDOW),
-            q.shape[3] ** -0.5 if scale is None else float(scale))
-
-
-def _check_lens(ctx_lens: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
-    assert ctx_lens.shape == (q.shape[0],) and ctx_lens.dtype in (torch.int32, torch.int64) \
-        and ctx_lens.device == q.device, "ctx_lens must be int32 (or int64) [B] on q's device"
-    return ctx_lens.to(torch.int32).contiguous()
-
-
-def _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, train):
-    lib = _lib.load()
-    B, T, Hq, D = q.shape
-    Hk = k.shape[2]
-    o = _new(q)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if train else None
-    res = _new(q) if train else None  # what o's rounding took away: the backward's delta needs it
-    with _lib.on_device(q.device):
-        _lib.check(lib.specdec_window_attention_forward(
-            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
-            _lib.ptr(res), _lib.ptr(lse), _lib.ptr(ctx_lens), B, T, Hq, Hk, D, n_ctx, window, sinks, scale, _status(q.device),
-            _stream(q)), "specdec_window_attention_forward")
-    return o, res, lse
-
-
-class _WindowAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, ctx_lens, n_ctx, window, sinks, scale):
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        o, res, lse = _window_forward(q, k, v, ctx_lens, n_ctx, window, sinks, scale, True)
-        ctx.save_for_backward(q, k, v, o, res, lse, ctx_lens)
-        ctx.how = n_ctx, window, sinks, scale
-        return o
-
-    @staticmethod
-    @_once
-    def backward(ctx, do):
-        lib = _lib.load()
-        q, k, v, o, res, lse, ctx_lens = ctx.saved_tensors
-        B, T, Hq, D = q.shape
-        Hk = k.shape[2]
-        do = do.contiguous()
-        if do.data_ptr() % 16:
-            do = do.clone()
-        dq, dk, dv = _new(q), _new(k), _new(v)
-        with _lib.on_device(q.device):
-            ws_bytes = lib.specdec_window_attention_workspace_bytes(B, T, Hq, Hk, D, *ctx.how[:3], q.device.index)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-            _lib.check(lib.specdec_window_attention_backward(
-                q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(),
-                res.data_ptr(), lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ctx_lens), B, T,
-                Hq, Hk, D, *ctx.how, _status(q.device), ws.data_ptr(), ws_bytes, _stream(q)),
-                "specdec_window_attention_backward")
-        return dq, dk, dv, None, None, None, None, None
-
 
 def window_attention_supported(q: torch.Tensor) -> bool:
     return ENABLED and q.is_cuda and q.dtype == torch.bfloat16 and q.dim() == 4 and q.shape[-1] in (64, 128)
@@ -463,15 +262,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_ctx: i
     ctx_lens[b] context tokens, in rows 0 .. ctx_lens[b]-1; the rows behind
     them up to n_ctx are padding, never read, with zero outputs and gradients.
     Differentiable in q, k, v; scale None = D^-0.5."""
-    window, sinks, scale = _check_window(q, k, v, window, sinks, scale)
-    assert k.shape[1] == q.shape[1], "k and v must have q's length"
-    assert 0 <= n_ctx <= q.shape[1], f"n_ctx must be in [0, T], got {n_ctx}"
-    if ctx_lens is not None:
-        ctx_lens = _check_lens(ctx_lens, q)
-    how = int(n_ctx), window, sinks, scale
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _WindowAttention.apply(q, k, v, ctx_lens, *how)
-    return _window_forward(_rows16(q), _rows16(k), _rows16(v), ctx_lens, *how, False)[0]
+    return _ops().window_attention(q, k, v, n_ctx, window, sinks, scale, ctx_lens)
 
 
 def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_lens: torch.Tensor, *,
@@ -485,23 +276,4 @@ def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     block together (Tq = 1, n_block = 0: the next token); a query in front of
     the first token gives zeros. The cache is read in place: its rows must start
     on 16-byte boundaries."""
-    window, sinks, scale = _check_window(q, k_cache, v_cache, window, sinks, scale)
-    assert not (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)), \
-        "window_attention_cached has no backward: call it under torch.no_grad()"
-    ctx_lens = _check_lens(ctx_lens, q)
-    lib = _lib.load()
-    B, Tq, Hq, D = q.shape
-    size, Hk = k_cache.shape[1], k_cache.shape[2]
-    assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the cache's heads must be contiguous"
-    assert 0 <= n_block <= size, f"n_block must be in [0, size of the cache], got {n_block}"
-    q = _rows16(q)
-    o = _new(q)
-    with _lib.on_device(q.device):
-        ws_bytes = lib.specdec_window_attention_cached_workspace_bytes(B, Tq, size, Hq, Hk, D, n_block, window, sinks,
-                                                                       q.device.index)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        _lib.check(lib.specdec_window_attention_cached(
-            q.data_ptr(), _strides(q), k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
-            o.data_ptr(), ctx_lens.data_ptr(), B, Tq, size, Hq, Hk, D, int(n_block), window, sinks, scale,
-            _status(q.device), _lib.ptr(ws), ws_bytes, _stream(q)), "specdec_window_attention_cached")
-    return o
+    return _ops().window_attention_cached(q, k_cache, v_cache, ctx_lens, n_block, window, sinks, scale)

@@ -30,6 +30,15 @@
 // dw is summed per thread over the units in order, per CTA through shared
 // memory in warp order, and over CTAs by a second kernel: fixed orders,
 // bitwise repeatable.
+//
+// Measured: rotation of [2, 8191, 16, 128] fp32, interleaved, 46 us (5.9 TB/s);
+// norm and rotation of [1, 32768, 32 + 8, 128] bf16, 122 us (5.5 TB/s) forward,
+// 217 us (4.6 TB/s) backward: there the issue slots (65% and 56% busy) and the
+// wait for shared memory and shuffles bound it as much as HBM does. 16-byte
+// loads of tables and weights in planes without bank conflicts took 8% off
+// (138 and 235 us before). A ring of rows filled with asynchronous copies was
+// slower (179 and 283 us): it spends more instructions. One token of 32
+// sequences takes 3.6 us, the time of a launch and one chain of loads.
 #include <algorithm>
 
 #include "specdec_common.cuh"
@@ -42,7 +51,7 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kMaxHead = 512;
-constexpr int kTableFloats = 512;  // a warp's table: at most 32 / lanes * 32 pairs' cos, or the R of one token
+constexpr int kTableFloats = 512;  // a warp's table: cos, sin and -sin of at most 256 pairs
 
 // V consecutive elements of a row, as loaded: one element, or a 16-byte vector.
 template <class T, int V>
@@ -92,15 +101,22 @@ __device__ __forceinline__ void st(bf16_t* p, const float (&v)[V]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
                                               pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
-// V consecutive fp32 values of shared memory (16-byte aligned when V > 1).
+// V consecutive values of an array of n floats in shared memory, from element e
+// on (a multiple of V). With V = 8 the array is kept in two planes, the first
+// and the last four of every eight: a warp's 16-byte loads then touch
+// consecutive chunks (together they would collide in pairs of banks).
 template <int V>
-__device__ __forceinline__ void ld_sh(const float* p, float (&v)[V]) {
+__device__ __forceinline__ int plane_at(int e, int n) {
+  return V == 8 ? (e >> 3) * 4 + (e & 3) + (e & 4 ? n >> 1 : 0) : e;
+}
+template <int V>
+__device__ __forceinline__ void ld_sh(const float* p, int n, int e, float (&v)[V]) {
   if constexpr (V == 1) {
-    v[0] = *p;
+    v[0] = p[e];
   } else {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-      const float4 q = *reinterpret_cast<const float4*>(p + i);
+      const float4 q = *reinterpret_cast<const float4*>(p + plane_at<V>(e + i, n));
       v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
     }
   }
@@ -206,7 +222,7 @@ struct Place {
   int side, H, groups_per_token;
   int group, sub;      // head group of the lane, lane within it
   int tw;              // tokens per unit
-  int64_t unit, step, units;
+  uint32_t unit, step, units;
 };
 
 __device__ __forceinline__ Place place_of(const RotaryArgs& A) {
@@ -218,32 +234,33 @@ __device__ __forceinline__ Place place_of(const RotaryArgs& A) {
   p.group = lane >> A.lg;
   p.sub = lane & ((1 << A.lg) - 1);
   p.tw = p.H < hpw ? hpw / p.H : 1;
-  p.step = (int64_t)A.ctas[p.side] * kRotWarps;
-  p.unit = ((int64_t)blockIdx.x - (p.side ? A.ctas[0] : 0)) * kRotWarps + (threadIdx.x >> 5);
-  p.units = (A.N + p.tw - 1) / p.tw * A.nchunk[p.side];
+  p.step = (uint32_t)A.ctas[p.side] * kRotWarps;
+  p.unit = (blockIdx.x - (p.side ? A.ctas[0] : 0)) * kRotWarps + (threadIdx.x >> 5);
+  p.units = (uint32_t)((A.N + p.tw - 1) / p.tw) * (uint32_t)A.nchunk[p.side];
   return p;
 }
 
 // What this lane touches in a unit: token n (or none) and its heads h, h + hpw, ... < hend.
 struct Unit {
-  int64_t n0, b, t;  // first token; the lane's token as (sequence, row)
+  int n0;            // first token
+  int64_t b, t;      // the lane's token as (sequence, row)
   int h, hend, tok;  // tok: the lane's token within the unit
 };
 
-__device__ __forceinline__ Unit unit_of(const RotaryArgs& A, const Place& p, int64_t u) {
+__device__ __forceinline__ Unit unit_of(const RotaryArgs& A, const Place& p, uint32_t u) {
   Unit r;
   const int nch = A.nchunk[p.side];
-  const int64_t tile = nch == 1 ? u : u / nch;
-  r.n0 = tile * p.tw;
+  const uint32_t tile = nch == 1 ? u : u / (uint32_t)nch;
+  r.n0 = (int)(tile * (uint32_t)p.tw);
   if (p.tw == 1) {
-    const int ch = (int)(u - tile * nch);
+    const int ch = (int)(u - tile * (uint32_t)nch);
     r.tok = 0;
     r.h = ch * A.hchunk[p.side] + p.group;
     r.hend = min(p.H, (ch + 1) * A.hchunk[p.side]);
   } else {
     r.tok = p.group / p.H;
     r.h = p.group - r.tok * p.H;
-    r.hend = r.tok < p.tw && r.n0 + r.tok < A.N ? r.h + 1 : 0;
+    r.hend = r.tok < p.tw && (int64_t)r.n0 + r.tok < A.N ? r.h + 1 : 0;
   }
   const uint32_t n = (uint32_t)(r.n0 + r.tok);  // N fits in int32
   const uint32_t b = n / (uint32_t)A.T;
@@ -253,8 +270,9 @@ __device__ __forceinline__ Unit unit_of(const RotaryArgs& A, const Place& p, int
 }
 
 // cos and sin (times scale) of the unit's tokens and pairs, by the whole warp.
-__device__ __forceinline__ void build_table(const RotaryArgs& A, const Place& p, int64_t n0, float* cs, float* sn) {
-  const int half = A.R / 2, toks = (int)min((int64_t)p.tw, A.N - n0);
+template <int V>
+__device__ __forceinline__ void build_table(const RotaryArgs& A, const Place& p, int n0, float* cs, float* sn) {
+  const int half = A.R / 2, toks = min(p.tw, (int)A.N - n0);
   __syncwarp();  // the previous unit's table has been read
   for (int i = threadIdx.x & 31; i < toks * half; i += 32) {
     const int tok = p.tw == 1 ? 0 : i / half, f = i - tok * half;
@@ -262,19 +280,23 @@ __device__ __forceinline__ void build_table(const RotaryArgs& A, const Place& p,
     const double turns = (double)A.positions[(int64_t)b * A.pos_stride + t] * A.inv_freq[f] * 0.15915494309189533577;
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-    cs[i] = c * A.scale;
-    sn[i] = s * A.sin_scale;
+    const int at = tok * half + plane_at<V>(f, half);
+    s *= A.sin_scale;
+    cs[at] = c * A.scale;
+    sn[at] = s;
   }
   __syncwarp();
 }
 
+// The lane's first head of a unit; its later ones lie t.s[2] * (heads per warp) apart.
 template <class T>
-__device__ __forceinline__ T* head_ptr(const RotaryTensor& t, const Unit& u, int h) {
-  return const_cast<T*>(static_cast<const T*>(t.p)) + u.b * t.s[0] + u.t * t.s[1] + (int64_t)h * t.s[2];
+__device__ __forceinline__ T* head_ptr(const RotaryTensor& t, const Unit& u) {
+  return const_cast<T*>(static_cast<const T*>(t.p)) + u.b * t.s[0] + u.t * t.s[1] + (int64_t)u.h * t.s[2];
 }
 
+template <int V>
 __device__ __forceinline__ void load_weights(const RotaryArgs& A, const Place& P, float* w) {
-  for (int i = threadIdx.x; i < A.D; i += kRotThreads) w[i] = A.w[P.side][i];
+  for (int i = threadIdx.x; i < A.D; i += kRotThreads) w[plane_at<V>(i, A.D)] = A.w[P.side][i];
   __syncthreads();
 }
 
@@ -294,13 +316,15 @@ __global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 2) rotary_fwd_kernel(
     live[k] = slot < slots;
     rot[k] = slot_place<V>(A, slot, ea[k], eb[k]) && live[k];
   }
-  if constexpr (NORM) load_weights(A, P, w);
-  for (int64_t u = P.unit; u < P.units; u += P.step) {
+  if constexpr (NORM) load_weights<V>(A, P, w);
+  const int64_t xstep = hpw * A.x[P.side].s[2], ystep = hpw * A.y[P.side].s[2];
+  for (uint32_t u = P.unit; u < P.units; u += P.step) {
     const Unit U = unit_of(A, P, u);
     Raw<T, V> ra[K], rb[K];
+    const T* p = head_ptr<T>(A.x[P.side], U);
+    T* q = head_ptr<T>(A.y[P.side], U);
     auto load = [&](int h) {
       if (h < U.hend) {
-        const T* p = head_ptr<T>(A.x[P.side], U, h);
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (live[k]) {
@@ -310,7 +334,7 @@ __global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 2) rotary_fwd_kernel(
       }
     };
     load(U.h);
-    build_table(A, P, U.n0, cs, sn);
+    build_table<V>(A, P, U.n0, cs, sn);
     const int hlast = P.tw == 1 ? U.hend : 1;  // uniform over the warp
     for (int i = P.tw == 1 ? U.h - P.group : 0, h = U.h; i < hlast; i += hpw, h += hpw) {
       float x[K][V], y[K][V];
@@ -326,6 +350,7 @@ __global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 2) rotary_fwd_kernel(
           for (int j = 0; j < V; ++j) x[k][j] = y[k][j] = 0.f;
         }
       }
+      p += xstep;
       load(h + hpw);  // in flight while this group is worked on
       if constexpr (NORM) {
         float2 sq = make_float2(0.f, 0.f);
@@ -337,31 +362,31 @@ __global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 2) rotary_fwd_kernel(
         ss = head_sum(sq.x + sq.y, A.lg);
       }
       if (on) {
-        T* q = head_ptr<T>(A.y[P.side], U, h);
         const float r = NORM ? rsqrtf(ss / (float)A.D + A.eps) : 1.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
           if constexpr (NORM) {
             float wv[V];
-            ld_sh<V>(w + ea[k], wv);
+            ld_sh<V>(w, A.D, ea[k], wv);
             vscale<V>(x[k], x[k], r);
             vmul<V>(x[k], x[k], wv);
-            ld_sh<V>(w + eb[k], wv);
+            ld_sh<V>(w, A.D, eb[k], wv);
             vscale<V>(y[k], y[k], r);
             vmul<V>(y[k], y[k], wv);
           }
           if (rot[k]) {
             float c[V], s[V];
-            const int at = U.tok * (A.R / 2) + (P.sub + k * 32) * V;
-            ld_sh<V>(cs + at, c);
-            ld_sh<V>(sn + at, s);
+            const int half = A.R / 2, at = (P.sub + k * 32) * V;
+            ld_sh<V>(cs + U.tok * half, half, at, c);
+            ld_sh<V>(sn + U.tok * half, half, at, s);
             turn<V, INTER>(x[k], y[k], c, s);
           }
           st<V>(q + ea[k], x[k]);
           st<V>(q + eb[k], y[k]);
         }
       }
+      q += ystep;
     }
   }
 }
@@ -389,14 +414,16 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
       acca[k][j] = accb[k][j] = 0.f;
     }
   }
-  load_weights(A, P, w);
-  for (int64_t u = P.unit; u < P.units; u += P.step) {
+  load_weights<V>(A, P, w);
+  const int64_t xstep = hpw * A.x[P.side].s[2], gstep = hpw * A.dy[P.side].s[2], ystep = hpw * A.y[P.side].s[2];
+  for (uint32_t u = P.unit; u < P.units; u += P.step) {
     const Unit U = unit_of(A, P, u);
     Raw<T, V> ra[K], rb[K], sa[K], sb[K];
+    const T* p = head_ptr<T>(A.x[P.side], U);
+    const T* g = head_ptr<T>(A.dy[P.side], U);
+    T* q = head_ptr<T>(A.y[P.side], U);
     auto load = [&](int h) {
       if (h < U.hend) {
-        const T* p = head_ptr<T>(A.x[P.side], U, h);
-        const T* g = head_ptr<T>(A.dy[P.side], U, h);
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (live[k]) {
@@ -408,7 +435,7 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
       }
     };
     load(U.h);
-    build_table(A, P, U.n0, cs, sn);
+    build_table<V>(A, P, U.n0, cs, sn);
     const int hlast = P.tw == 1 ? U.hend : 1;
     for (int i = P.tw == 1 ? U.h - P.group : 0, h = U.h; i < hlast; i += hpw, h += hpw) {
       float xa[K][V], xb[K][V], ga[K][V], gb[K][V];
@@ -426,24 +453,26 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
           for (int j = 0; j < V; ++j) xa[k][j] = xb[k][j] = ga[k][j] = gb[k][j] = 0.f;
         }
       }
+      p += xstep;
+      g += gstep;
       load(h + hpw);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (rot[k]) {
           float c[V], s[V];
-          const int at = U.tok * (A.R / 2) + (P.sub + k * 32) * V;
-          ld_sh<V>(cs + at, c);
-          ld_sh<V>(sn + at, s);
+          const int half = A.R / 2, at = (P.sub + k * 32) * V;
+          ld_sh<V>(cs + U.tok * half, half, at, c);
+          ld_sh<V>(sn + U.tok * half, half, at, s);
           turn<V, INTER>(ga[k], gb[k], c, s);  // dn = rot^T(dout): sin is negated in the table
         }
         vdot<V>(sq, xa[k], xa[k]);
         vdot<V>(sq, xb[k], xb[k]);
         if (!live[k]) continue;
         float wv[V], t[V];  // g = dn w
-        ld_sh<V>(w + ea[k], wv);
+        ld_sh<V>(w, A.D, ea[k], wv);
         vmul<V>(t, ga[k], wv);
         vdot<V>(gx, t, xa[k]);
-        ld_sh<V>(w + eb[k], wv);
+        ld_sh<V>(w, A.D, eb[k], wv);
         vmul<V>(t, gb[k], wv);
         vdot<V>(gx, t, xb[k]);
       }
@@ -451,7 +480,6 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
       if (on) {
         const float r = rsqrtf(ss / (float)A.D + A.eps);
         const float m = r * r * r * dot / (float)A.D;
-        T* q = head_ptr<T>(A.y[P.side], U, h);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
@@ -459,17 +487,18 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
           vfma<V>(acca[k], ga[k], xa[k], acca[k]);
           vscale<V>(xa[k], xa[k], -m);
           float wv[V];
-          ld_sh<V>(w + ea[k], wv);
+          ld_sh<V>(w, A.D, ea[k], wv);
           vfma<V>(xa[k], ga[k], wv, xa[k]);
           vscale<V>(gb[k], gb[k], r);
           vfma<V>(accb[k], gb[k], xb[k], accb[k]);
           vscale<V>(xb[k], xb[k], -m);
-          ld_sh<V>(w + eb[k], wv);
+          ld_sh<V>(w, A.D, eb[k], wv);
           vfma<V>(xb[k], gb[k], wv, xb[k]);
           st<V>(q + ea[k], xa[k]);
           st<V>(q + eb[k], xb[k]);
         }
       }
+      q += ystep;
     }
   }
   // over the warp's head groups (butterfly), then over the warps in order

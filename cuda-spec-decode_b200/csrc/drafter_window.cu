@@ -14,7 +14,8 @@
 // 0 .. c_b-1 (c_b = ctx_lens[b], or n_ctx), rows c_b .. n_ctx-1 are padding and
 // rows n_ctx .. T-1 the block. Padding is never read (its rows enter the
 // products as zeros) and its outputs and gradients are zero. In a cache the
-// block follows the context directly and the queries are the last Tq tokens.
+// block follows the context directly and the queries are the last Tq tokens;
+// rows behind the last token and rows that no query sees may hold anything.
 //
 // Shared heads. Query heads of one key head are packed into a tile: packed row
 // m is token m / G, head m % G of the group, so a key tile is loaded once for
@@ -346,10 +347,12 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   // a box of K or V, stage s of the ring
   auto load_box = [&](int s) {
     const int j0 = kt.start(i0 + (s >> 1)), row = j0 < sq.c ? j0 : j0 + sq.kb - sq.c;
+    const bool sink = i0 + (s >> 1) < kt.ns;
+    const CUtensorMap *mk = sink ? &A.mks : &A.mk, *mv = sink ? &A.mvs : &A.mv;
     mbar_arrive_expect_tx(full + s % C::NS, C::SB);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
-      tma_load_4d(base + C::OST + (s % C::NS) * C::SB + c * (KN * 128), s & 1 ? &A.mv : &A.mk, c * 64, row, hk, b,
+      tma_load_4d(base + C::OST + (s % C::NS) * C::SB + c * (KN * 128), s & 1 ? mv : mk, c * 64, row, hk, b,
                   full + s % C::NS);
   };
   if (threadIdx.x == QT * 128 + 32) {  // the first copying thread
@@ -1388,6 +1391,19 @@ void kv_maps(WindowArgs& A, int D, int rows) {
               make_map(&A.mv, A.v, d, {A.vs[1], A.vs[2], A.vs[0]}, rows, 1);
 }
 
+// The same for the tiles of sinks. In a cache a token between the sinks and the
+// window is seen by no query, and its row may hold anything by now: maps that
+// end behind the sinks fill its place with zeros. (In a batch every token sees
+// itself, so there are no such rows.)
+void sink_maps(WindowArgs& A, int D, int rows) {
+  A.mks = A.mk;
+  A.mvs = A.mv;
+  if (!A.cached || !A.kv_maps || A.S == 0 || A.S >= A.Tk) return;
+  const int64_t d[4] = {D, A.S, A.Hk, A.B};
+  A.kv_maps = make_map(&A.mks, A.k, d, {A.ks[1], A.ks[2], A.ks[0]}, rows, 1) &&
+              make_map(&A.mvs, A.v, d, {A.vs[1], A.vs[2], A.vs[0]}, rows, 1);
+}
+
 // Queries (or dO) as [D, Hq, T, B], boxes of whole tokens' groups: G a power of two.
 bool group_map(CUtensorMap* map, const WindowArgs& A, const bf16_t* p, const int64_t (&s)[3], int D, int rows) {
   if (A.G > rows || (A.G & (A.G - 1))) return false;
@@ -1403,6 +1419,7 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
                                    C::LAUNCH_REGS * C::THREADS, C::THREADS);
   if (e != cudaSuccess) return e;
   kv_maps(A, D, C::KN);
+  sink_maps(A, D, C::KN);
   A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
   const dim3 grid((unsigned)(A.B * A.Hk * A.nsub), (unsigned)((A.M + QT * kTM - 1) / (QT * kTM)), (unsigned)A.splits);
   if constexpr (SPLIT == kSplitCluster) {

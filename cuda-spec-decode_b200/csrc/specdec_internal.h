@@ -247,7 +247,7 @@ struct WindowArgs {
   // tensor maps, set by the launch: [D, T, Hk, B] with boxes of 64 x rows, and
   // [D, Hq, T, B] with boxes of 64 x G x (rows / G); the flags say which exist
   int kv_maps, q_maps;
-  CUtensorMap mk, mv, mq, mg;
+  CUtensorMap mk, mv, mq, mg, mks, mvs;  // mks, mvs: k and v for tiles of sinks
 };
 void window_sink_shape(WindowArgs& A, int sms);
 size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at);

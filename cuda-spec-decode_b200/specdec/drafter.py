@@ -271,9 +271,10 @@ def window_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """``window_attention`` of the last tokens of each sequence against a cache,
     forward only. k_cache, v_cache bf16 [B, size, Hk, D] hold sequence b's
     ctx_lens[b] context tokens (int32 [B], at most size - n_block) in rows
-    0, 1, ... and its n_block block tokens right behind them; later rows are
-    never read. q [B, Tq, Hq, D] are the sequence's last Tq tokens, context and
-    block together (Tq = 1, n_block = 0: the next token); a query in front of
-    the first token gives zeros. The cache is read in place: its rows must start
-    on 16-byte boundaries."""
+    0, 1, ... and its n_block block tokens right behind them; later rows, and
+    rows that no query sees (between the sinks and the first query's window),
+    may hold anything. q [B, Tq, Hq, D] are the sequence's last Tq tokens,
+    context and block together (Tq = 1, n_block = 0: the next token); a query in
+    front of the first token gives zeros. The cache is read in place: its rows
+    must start on 16-byte boundaries."""
     return _ops().window_attention_cached(q, k_cache, v_cache, ctx_lens, n_block, window, sinks, scale)

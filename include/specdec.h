@@ -457,9 +457,10 @@ size_t specdec_window_attention_cached_workspace_bytes(int32_t batch, int32_t q_
  * The same attention from a cache, forward only: k_cache, v_cache [batch,
  * cache_len, k_heads, head_dim] hold sequence b's ctx_lens[b] context tokens
  * (clamped to [0, cache_len - n_block]) in rows 0, 1, ... and its n_block block
- * tokens right behind them; later rows are never read. q [batch, q_len, ...]
- * are the sequence's last q_len tokens (context and block together); queries
- * in front of the first token see nothing and give zeros. workspace needs no
+ * tokens right behind them; later rows, and rows that no query sees (between
+ * the sinks and the first query's window), may hold anything. q [batch, q_len,
+ * ...] are the sequence's last q_len tokens (context and block together);
+ * queries in front of the first token see nothing and give zeros. workspace needs no
  * initialisation; calls that may run at the same time must not share it.
  */
 int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides, const uint16_t* k_cache,

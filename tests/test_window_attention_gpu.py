@@ -449,3 +449,58 @@ def test_a_cache_past_32_bit_offsets(cuda):
     pk = torch.arange(c - 70, size)
     vis = _visible(c + 3 - 4 + torch.arange(4), pk, c, 60, 0)
     _near("o", o[1], _oracle(q[1], k[1, tail], v[1, tail], vis)["o"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n_ctx,nb,H,D,W,S,lens", [
+    (2, 300, 7, 4, 64, 60, 3, (300, 101)), (2, 300, 7, 4, 128, 60, 70, None), (1, 90, 0, 3, 64, None, 0, None),
+    (2, 1584, 16, 16, 64, 1540, 4, (1584, 1500)),  # two query tiles per CTA
+    (2, 1584, 16, 16, 128, None, 0, None),
+])
+def test_expanded_inputs_equal_their_copies(cuda, B, n_ctx, nb, H, D, W, S, lens):
+    """Strides of zero (a head, a batch or a token broadcast) are read without
+    tensor maps; the arithmetic is the same."""
+    T = n_ctx + nb
+    q, k, v, do = (_rand(B, T, H, D, seed=i) for i in range(4))
+    ctx_lens = None if lens is None else torch.tensor(lens, device="cuda", dtype=torch.int32)
+    for x in ((q, k[:, :, :1].expand_as(k), v[:, :, :1].expand_as(v)), (q[:1].expand_as(q), k[:1].expand_as(k), v),
+              (q[:, :1].expand_as(q), k, v[:, :1].expand_as(v)), (k, k, k)):
+        got = []
+        for y in (x, [t.contiguous().clone() for t in x]):
+            y = [t.detach().requires_grad_(True) for t in y]
+            o = drafter.window_attention(*y, n_ctx, window=W, sinks=S, ctx_lens=ctx_lens)
+            got.append([o.detach(), *torch.autograd.grad(o, y, do)])
+        for a, b in zip(*got):
+            assert bool(torch.isfinite(a.float()).all()) and torch.equal(a, b)
+
+
+UNSEEN = [  # B, Tq, nb, Hq, Hk, D, size, W, S, lens; splits of the keys
+    (2, 1, 0, 4, 2, 64, 900, 300, 4, (900, 640)),        # in a cluster
+    (1, 3, 3, 8, 1, 128, 4000, 3000, 70, (3990,)),       # in the workspace
+    (40, 2, 0, 16, 16, 64, 500, 100, 33, None),          # none
+    (1, 40, 3, 4, 2, 64, 2000, None, 0, (20,)),          # more queries than tokens, empty splits
+    (3, 9, 5, 6, 2, 128, 600, 50, 130, (590, 300, 20)),  # groups of three: no map for the queries
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Tq,nb,Hq,Hk,D,size,W,S,lens", UNSEEN)
+def test_cache_rows_that_no_query_sees_may_hold_anything(cuda, B, Tq, nb, Hq, Hk, D, size, W, S, lens):
+    if lens is None:
+        lens = [(size - 13 * b) % (size - nb + 1) for b in range(B)]
+    q, k, v = _rand(B, Tq, Hq, D, seed=1), _rand(B, size, Hk, D, seed=2), _rand(B, size, Hk, D, seed=3)
+    ctx = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    sees = []
+    for b, c in enumerate(lens):
+        pk = torch.arange(size)
+        sees.append(_visible(c + nb - Tq + torch.arange(Tq), torch.where(pk < c + nb, pk, -1), c, W or 10 ** 9, S))
+        k[b, ~sees[b].any(0)] = float("nan")
+        v[b, ~sees[b].any(0)] = float("inf")
+    o = drafter.window_attention_cached(q, k, v, ctx, n_block=nb, window=W, sinks=S)
+    for b in range(B):
+        _near("o", o[b], _oracle(q[b], k[b], v[b], sees[b])["o"])
+    # one key head broadcast to all: no map for the keys
+    k1, v1 = k[:, :, :1].expand_as(k), v[:, :, :1].expand_as(v)
+    a, b = (drafter.window_attention_cached(q, x, y, ctx, n_block=nb, window=W, sinks=S)
+            for x, y in ((k1, v1), (k1.contiguous(), v1.contiguous())))
+    assert bool(torch.isfinite(a.float()).all()) and torch.equal(a, b)

@@ -188,9 +188,10 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 //   copies    a ring of NS stages of KN rows, K0 V0 K1 V1 ..., by TMA (one thread);
 //             a tile that runs into padding or past the last token is copied by
 //             the copying warps with cp.async and zeros
-//   products  per step, for each query tile t: O_t += P_t(i-1) V(i-1), then
-//             S_t(i) = Q_t K(i)^T; with two tiles, one's products run during the
-//             other's softmax
+//   products  two tiles: per step, for each query tile t: O_t += P_t(i-1) V(i-1),
+//             then S_t(i) = Q_t K(i)^T; one's products run during the other's
+//             softmax. One tile: S(i) into the other one of two buffers, then
+//             O += P(i-1) V(i-1); both run during the softmax of the other buffer
 //   softmax   S_t from tensor memory, P_t in bf16 back over S_t's columns (the
 //             A operand of the next product is read from tensor memory), O_t
 //             rescaled there when the reference maximum rises
@@ -213,15 +214,15 @@ struct FwdCfg {
   static_assert(LAUNCH_REGS == 0 || LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 256 + SERVICE_REGS * 128, "register split");
   static constexpr uint32_t QB = kTM * D * 2, SB = KN * D * 2;
   static constexpr uint32_t OQ = 0, OST = QT * QB, OBAR = OST + NS * SB;
-  static constexpr int NBAR = 2 * NS + 3 * QT + 3;  // full, empty, s_full, p_full (halves), q_full, o_full, drain
+  static constexpr int NBAR = 2 * NS + 10;  // full, empty; s_full, p_full (halves) of 2 buffers; o_step, q_full, o_full, drain
   static constexpr uint32_t OSLOT = OBAR + NBAR * 8;         // TMEM base, dead flag
   static constexpr uint32_t BYTES = OSLOT + 8;
   // a cluster's join, over the queries and the ring: 128 rows of fp32 (padded
   // against bank conflicts), then their (maximum, sum)
   static constexpr uint32_t LD = D + 4, OML = kTM * LD * 4;
   static_assert(QT == 2 || OML + kTM * 8 <= OBAR, "they fit");
-  static constexpr uint32_t COLS = QT == 2 ? 512 : D == 64 ? 128 : 256;
-  static constexpr uint32_t COL_O = QT * KN;
+  static constexpr uint32_t COLS = QT == 2 ? 512 : 256;
+  static constexpr uint32_t COL_O = 2 * KN;  // behind two buffers of scores
 };
 
 // Waits for the barrier's phase; false once `dead` is set or the limit expired
@@ -284,8 +285,9 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OBAR);
   uint64_t* empty = full + C::NS;
   uint64_t* s_full = empty + C::NS;
-  uint64_t* p_full = s_full + QT;
-  uint64_t* q_full = p_full + 2 * QT;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_step = p_full + 4;
+  uint64_t* q_full = o_step + 1;
   uint64_t* o_full = q_full + 1;
   uint64_t* drain = q_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OSLOT);
@@ -362,11 +364,12 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       mbar_init(empty + i, 1);
     }
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
+    for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + t, 1);
       mbar_init(p_full + 2 * t, 128);
       mbar_init(p_full + 2 * t + 1, 128);
     }
+    mbar_init(o_step, 1);
     mbar_init(q_full, A.q_maps ? 1 : QT * 128);
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
@@ -401,58 +404,99 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
       const uint32_t dq = desc_low(base + C::OQ, 16);
       const uint32_t dk = desc_low(base + C::OST, 16), dv = desc_low(base + C::OST, KN * 128);
-      uint32_t steps[QT];  // steps of each tile so far
-#pragma unroll
-      for (int t = 0; t < QT; ++t) steps[t] = 0;
       uint32_t kslot = 0, kph = 0, vslot = 1, vph = 0;  // ring slots and phases of K(i), V(i-1)
       bool ok = wait_alive(q_full, 0, dead, A.status);
-      for (int i = 0; i <= n && ok; ++i) {
-        if (i > 0) ok = wait_alive(full + vslot, vph, dead, A.status);
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          if (i > 0 && needs(t, i - 1)) {
-            const uint32_t ph = (steps[t] - 1) & 1;
+      if constexpr (QT == 1) {
+        for (int i = 0; i <= n && ok; ++i) {
+          if (i < n) {  // S(i) while the softmax is at step i - 1; its buffer's last P was read by the product before
+            ok = wait_alive(full + kslot, kph, dead, A.status);
+            if (!ok) break;
+            tc_fence_after();
+            if (!(withhold && i == 0) && elect_one()) {
+              issue_kk<D, kTM, KN>(tmem + (i & 1) * KN, dq, dk + kslot * (C::SB >> 4), kIdS);
+              umma_commit(s_full + (i & 1));
+              umma_commit(empty + kslot);
+            }
+            __syncwarp();
+            kslot += 2;
+            if (kslot >= C::NS) kslot -= C::NS, kph ^= 1;
+          }
+          if (i > 0) {
+            const int j = i - 1;
+            ok = wait_alive(full + vslot, vph, dead, A.status);
             const uint32_t v = dv + vslot * (C::SB >> 4);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // P arrives in halves
-              ok = ok && wait_alive(p_full + 2 * t + h, ph, dead, A.status);
+              ok = ok && wait_alive(p_full + 2 * (j & 1) + h, (j >> 1) & 1, dead, A.status);
               if (!ok) break;
               tc_fence_after();
               if (elect_one())
-                issue_tn<KN / 32>(tmem + C::COL_O + t * D, tmem + t * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4),
-                                  kIdO, (steps[t] > 1) | (h > 0));
+                issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4), kIdO,
+                                  (j > 0) | (h > 0));
               __syncwarp();
             }
             if (!ok) break;
-          }
-          if (i == n) continue;
-          if (t == 0) ok = ok && wait_alive(full + kslot, kph, dead, A.status);
-          if (!ok) break;
-          if (needs(t, i)) {
-            tc_fence_after();
-            ++steps[t];
-            if (withhold) {
-              withhold = false;
-              continue;
-            }
             if (elect_one()) {
-              issue_kk<D, kTM, KN>(tmem + t * KN, dq + t * (C::QB >> 4), dk + kslot * (C::SB >> 4), kIdS);
-              umma_commit(s_full + t);
+              umma_commit(o_step);
+              umma_commit(empty + vslot);
             }
             __syncwarp();
+            vslot += 2;
+            if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
           }
         }
-        if (!ok) break;
-        if (elect_one()) {
-          if (i > 0) umma_commit(empty + vslot);
-          if (i < n) umma_commit(empty + kslot);
-        }
-        __syncwarp();
-        kslot += 2;
-        if (kslot >= C::NS) kslot -= C::NS, kph ^= 1;
-        if (i > 0) {
-          vslot += 2;
-          if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
+      } else {
+        uint32_t steps[QT];  // steps of each tile so far
+#pragma unroll
+        for (int t = 0; t < QT; ++t) steps[t] = 0;
+        for (int i = 0; i <= n && ok; ++i) {
+          if (i > 0) ok = wait_alive(full + vslot, vph, dead, A.status);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            if (i > 0 && needs(t, i - 1)) {
+              const uint32_t ph = (steps[t] - 1) & 1;
+              const uint32_t v = dv + vslot * (C::SB >> 4);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {  // P arrives in halves
+                ok = ok && wait_alive(p_full + 2 * t + h, ph, dead, A.status);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one())
+                  issue_tn<KN / 32>(tmem + C::COL_O + t * D, tmem + t * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4),
+                                    kIdO, (steps[t] > 1) | (h > 0));
+                __syncwarp();
+              }
+              if (!ok) break;
+            }
+            if (i == n) continue;
+            if (t == 0) ok = ok && wait_alive(full + kslot, kph, dead, A.status);
+            if (!ok) break;
+            if (needs(t, i)) {
+              tc_fence_after();
+              ++steps[t];
+              if (withhold) {
+                withhold = false;
+                continue;
+              }
+              if (elect_one()) {
+                issue_kk<D, kTM, KN>(tmem + t * KN, dq + t * (C::QB >> 4), dk + kslot * (C::SB >> 4), kIdS);
+                umma_commit(s_full + t);
+              }
+              __syncwarp();
+            }
+          }
+          if (!ok) break;
+          if (elect_one()) {
+            if (i > 0) umma_commit(empty + vslot);
+            if (i < n) umma_commit(empty + kslot);
+          }
+          __syncwarp();
+          kslot += 2;
+          if (kslot >= C::NS) kslot -= C::NS, kph ^= 1;
+          if (i > 0) {
+            vslot += 2;
+            if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
+          }
         }
       }
       if (ok && elect_one()) umma_commit(o_full);
@@ -507,13 +551,15 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       th0 = hi0[QT - 1];
     }
     for (int i = 0; i < n; ++i) {
-      if (!needs(t, i)) continue;
-      ok = __all_sync(kFullMask, wait_alive(s_full + t, steps & 1, dead, A.status));
+      if (QT == 2 && !needs(t, i)) continue;
+      // one tile: two buffers in turn; two tiles: a buffer each
+      const int buf = QT == 1 ? (int)(steps & 1) : t;
+      ok = __all_sync(kFullMask, wait_alive(s_full + buf, QT == 1 ? (steps >> 1) & 1 : steps & 1, dead, A.status));
       if (!ok) break;
       tc_fence_after();
       uint32_t sr[KN / 32][32];
 #pragma unroll
-      for (int c = 0; c < KN / 32; ++c) tmem_ld32_async(lane + t * KN + c * 32, sr[c]);
+      for (int c = 0; c < KN / 32; ++c) tmem_ld32_async(lane + buf * KN + c * 32, sr[c]);
       tmem_wait_ld();
       float s[KN / 32][32];
 #pragma unroll
@@ -540,7 +586,13 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       if (raise) m_ref = mt_;
       const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen nothing yet: p = 2^-inf = 0
       const float2 sc2 = make_float2(A.scale_log2, A.scale_log2), nm2 = make_float2(nm, nm);
-      if (steps > 0 && __any_sync(kFullMask, raise)) {  // S(i) came behind O's last product
+      if (steps > 0 && __any_sync(kFullMask, raise)) {
+        // one tile: O's last product may still run (two: S(i) came behind it)
+        if (QT == 1) {
+          ok = __all_sync(kFullMask, wait_alive(o_step, (steps - 1) & 1, dead, A.status));
+          if (!ok) break;
+          tc_fence_after();
+        }
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
           uint32_t ot[16];
@@ -561,11 +613,11 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
           ls[(j >> 1) & 1] = fadd2(ls[(j >> 1) & 1], pr);
           pk[j / 2] = pack_bf16x2(pr.x, pr.y);
         }
-        tmem_st16(lane + t * KN + c * 16, pk);
+        tmem_st16(lane + buf * KN + c * 16, pk);
         if ((c + 1) % (KN / 64) == 0) {  // half of P is there: its product may start
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(p_full + 2 * t + (c + 1) / (KN / 64) - 1);
+          mbar_arrive(p_full + 2 * buf + (c + 1) / (KN / 64) - 1);
         }
       }
       const float2 l2 = fadd2(ls[0], ls[1]);

@@ -118,13 +118,9 @@ struct KeyTiles {
   }
   __device__ __forceinline__ int start(int i) const { return i < ns ? i * KN : lo + (i - ns) * KN; }
   __device__ __forceinline__ int end(int i) const { return i < ns ? min(sink, i * KN + KN) : min(hi, start(i) + KN); }
-  // queries with bounds from lo0 .. lo1 and hi0 .. hi1 (first .. last): whether
-  // every one of them sees every key of tile i, and whether any sees any
+  // whether every query sees every key of tile i: lo1 the last query's lo, hi0 the first one's hi
   __device__ __forceinline__ bool full(int i, int lo1, int hi0) const {
     return i < ns ? i * KN + KN <= sink : start(i) + KN <= hi0 && start(i) >= lo1;
-  }
-  __device__ __forceinline__ bool any(int i, int lo0, int hi1, int S) const {
-    return i < ns || (start(i) < hi1 && (start(i) + KN > lo0 || start(i) < S));
   }
 };
 
@@ -182,18 +178,16 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 }
 
 // ---- forward --------------------------------------------------------------------
-// One CTA per (sequence, key head, QT x 128 packed rows[, split of the keys]).
-// Warps: QT softmax warpgroups (thread i owns row i of its tile = TMEM lane i),
-// then one warp that issues the products and three (QT = 1: one) that copy K and V.
-//   copies    a ring of NS stages of KN rows, K0 V0 K1 V1 ..., by TMA (one thread);
+// One CTA per (sequence, key head, 128 packed rows[, split of the keys]), two
+// CTAs per SM. Warps: a softmax warpgroup (thread i owns row i = TMEM lane i),
+// one warp that issues the products and one that copies K and V.
+//   copies    a ring of 5 stages of 64 rows, K0 V0 K1 V1 ..., by TMA (one thread);
 //             a tile that runs into padding or past the last token is copied by
-//             the copying warps with cp.async and zeros
-//   products  two tiles: per step, for each query tile t: O_t += P_t(i-1) V(i-1),
-//             then S_t(i) = Q_t K(i)^T; one's products run during the other's
-//             softmax. One tile: S(i) into the other one of two buffers, then
-//             O += P(i-1) V(i-1); both run during the softmax of the other buffer
-//   softmax   S_t from tensor memory, P_t in bf16 back over S_t's columns (the
-//             A operand of the next product is read from tensor memory), O_t
+//             the whole warp with cp.async and zeros
+//   products  S(i) = Q K(i)^T into one of two buffers, then O += P(i-1) V(i-1)
+//             from the other: both run during a softmax
+//   softmax   S(i) from tensor memory, P(i) in bf16 back over S(i)'s columns (the
+//             A operand of the next product is read from tensor memory), O
 //             rescaled there when the reference maximum rises
 // Every wait is bounded and watches a shared flag that the first expired wait
 // raises; all warps then leave for the common end.
@@ -201,28 +195,19 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 // in the workspace and a second kernel; or within a cluster, up to 8 parts.
 constexpr int kSplitNone = 0, kSplitMemory = 1, kSplitCluster = 2, kClusterMost = 8;
 
-template <int D, int QT>
+template <int D>
 struct FwdCfg {
-  static constexpr int KN = QT == 2 ? 128 : 64;
-  static constexpr int NS = D == 64 && QT == 2 ? 8 : 5;
-  static constexpr int CTAS = QT == 2 ? 1 : 2;
-  static constexpr int COPY = QT == 2 ? 96 : 32;  // threads of the copying warps
-  static constexpr int THREADS = QT * 128 + 32 + COPY;
-  // registers: with two tiles the softmax keeps a row's 128 scores and takes
-  // over what the service warps do not need (0: an even split does)
-  static constexpr int LAUNCH_REGS = QT == 2 ? 168 : 0, SOFTMAX_REGS = 208, SERVICE_REGS = 80;
-  static_assert(LAUNCH_REGS == 0 || LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 256 + SERVICE_REGS * 128, "register split");
-  static constexpr uint32_t QB = kTM * D * 2, SB = KN * D * 2;
-  static constexpr uint32_t OQ = 0, OST = QT * QB, OBAR = OST + NS * SB;
+  static constexpr int NS = 5, CTAS = 2, THREADS = 192;
+  static constexpr uint32_t QB = kTM * D * 2, SB = kTN * D * 2;
+  static constexpr uint32_t OQ = 0, OST = QB, OBAR = OST + NS * SB;
   static constexpr int NBAR = 2 * NS + 10;  // full, empty; s_full, p_full (halves) of 2 buffers; o_step, q_full, o_full, drain
-  static constexpr uint32_t OSLOT = OBAR + NBAR * 8;         // TMEM base, dead flag
+  static constexpr uint32_t OSLOT = OBAR + NBAR * 8;  // TMEM base, dead flag
   static constexpr uint32_t BYTES = OSLOT + 8;
   // a cluster's join, over the queries and the ring: 128 rows of fp32 (padded
   // against bank conflicts), then their (maximum, sum)
   static constexpr uint32_t LD = D + 4, OML = kTM * LD * 4;
-  static_assert(QT == 2 || OML + kTM * 8 <= OBAR, "they fit");
-  static constexpr uint32_t COLS = QT == 2 ? 512 : 256;
-  static constexpr uint32_t COL_O = 2 * KN;  // behind two buffers of scores
+  static_assert(OML + kTM * 8 <= OBAR, "they fit");
+  static constexpr uint32_t COLS = 256, COL_O = 2 * kTN;  // O behind two buffers of scores
 };
 
 // Waits for the barrier's phase; false once `dead` is set or the limit expired
@@ -274,11 +259,11 @@ __device__ __forceinline__ void stage_keys(uint32_t tile, const bf16_t* base, in
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-template <int D, int QT, int SPLIT>
-__global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
+template <int D, int SPLIT>
+__global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
     window_fwd_kernel(const __grid_constant__ WindowArgs A) {
-  using C = FwdCfg<D, QT>;
-  constexpr int KN = C::KN;
+  using C = FwdCfg<D>;
+  constexpr int KN = kTN;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   volatile int* dead = reinterpret_cast<volatile int*>(smem + C::OSLOT + 4);
@@ -292,16 +277,15 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   uint64_t* drain = q_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::OSLOT);
   const int warp = threadIdx.x >> 5;
-  const int wg = threadIdx.x >> 7;  // 0 .. QT-1: softmax, QT: service
+  const bool service = threadIdx.x >= kTM;  // product and copying warps
   const int hv_n = A.Hk * A.nsub;  // virtual heads: A.G query heads of one key head
   const int bh = blockIdx.x, b = bh / hv_n, hv = bh - b * hv_n, hk = hv / A.nsub;
-  const int m0 = (int)(gridDim.y - 1 - blockIdx.y) * (QT * kTM);  // the last tiles see the most keys: first
+  const int m0 = (int)(gridDim.y - 1 - blockIdx.y) * kTM;  // the last tiles see the most keys: first
   const Seq sq = seq_of(A, b);
 
-  // the query tiles' tokens and bounds, the CTA's key tiles
-  int lo0[QT], lo1[QT], hi0[QT], hi1[QT];
+  // the query tile's tokens, the CTA's key tiles
   int p0, p1, i0 = 0, n = 0;
-  const bool some = token_range(A, sq, m0, min(A.M, m0 + QT * kTM) - 1, p0, p1);
+  const bool some = token_range(A, sq, m0, min(A.M, m0 + kTM) - 1, p0, p1);
   const KeyTiles<KN> kt(A, sq, some ? p0 : 0, some ? p1 : -1);
   if (some) {
     n = kt.n;
@@ -310,25 +294,14 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       i0 = min(n, (int)blockIdx.z * per);
       n = min(n, i0 + per) - i0;
     }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      int a, z;
-      const int mt = m0 + t * kTM;
-      const bool live = mt < A.M && token_range(A, sq, mt, min(A.M, mt + kTM) - 1, a, z);
-      lo0[t] = live ? low_of(A, sq, a) : 0;
-      lo1[t] = live ? low_of(A, sq, z) : 0;
-      hi0[t] = live ? high_of(sq, a) : 0;
-      hi1[t] = live ? high_of(sq, z) : -1;  // -1: no tile of keys at all
-    }
   }
-  auto needs = [&](int t, int i) { return hi1[t] >= 0 && kt.any(i0 + i, lo0[t], hi1[t], A.S); };
 
   // this softmax thread's row
-  const int m = m0 + (int)(threadIdx.x % (QT * kTM));
+  const int m = m0 + (int)(threadIdx.x & (kTM - 1));
   const int tq = group_div(A, min(m, A.M - 1)), hq = hv * A.G + min(m, A.M - 1) - tq * A.G;
   bf16_t* orow = A.o + (((int64_t)b * A.Tq + tq) * A.Hq + hq) * D;
   const int64_t prow = ((int64_t)bh * A.M + m) * A.splits + (SPLIT ? blockIdx.z : 0);
-  const bool mine = wg < QT && m < A.M;
+  const bool mine = !service && m < A.M;
   const int p = mine ? token_of(A, sq, tq) : -1;
 
   if (n == 0 && SPLIT != kSplitCluster) {  // nothing to see
@@ -357,7 +330,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       tma_load_4d(base + C::OST + (s % C::NS) * C::SB + c * (KN * 128), s & 1 ? mv : mk, c * 64, row, hk, b,
                   full + s % C::NS);
   };
-  if (threadIdx.x == QT * 128 + 32) {  // the first copying thread
+  if (threadIdx.x == kTM + 32) {  // the first copying thread
 #pragma unroll
     for (int i = 0; i < C::NS; ++i) {
       mbar_init(full + i, 1);
@@ -370,140 +343,82 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       mbar_init(p_full + 2 * t + 1, 128);
     }
     mbar_init(o_step, 1);
-    mbar_init(q_full, A.q_maps ? 1 : QT * 128);
+    mbar_init(q_full, A.q_maps ? 1 : kTM);
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
     fence_mbar_init();
     *dead = 0;
     // its boxes start before the CTA meets
     if (A.q_maps && n > 0) {
-      mbar_arrive_expect_tx(q_full, QT * C::QB);
+      mbar_arrive_expect_tx(q_full, C::QB);
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(base + C::OQ + t * C::QB + c * (kTM * 128), &A.mq, c * 64, hv * A.G, (m0 + t * kTM) / A.G, b, q_full);
+      for (int c = 0; c < D / 64; ++c)
+        tma_load_4d(base + C::OQ + c * (kTM * 128), &A.mq, c * 64, hv * A.G, m0 / A.G, b, q_full);
     }
     while (issued < min(2 * n, C::NS) && A.kv_maps && boxed<KN>(sq, kt.start(i0 + (issued >> 1)))) load_box(issued++);
   }
-  if (warp == QT * 4) tmem_alloc(slot, C::COLS);
+  if (warp == 4) tmem_alloc(slot, C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
 
   if (n == 0) {  // (a cluster's CTA without keys still takes part in the join)
-  } else if (wg == QT) {
-    if constexpr (C::LAUNCH_REGS > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::SERVICE_REGS));
-    if (warp == QT * 4) {
+  } else if (service) {
+    if (warp == 4) {
       // ---- products: the warp walks together, one lane issues ----
       constexpr uint32_t kIdS = instr_desc(kTM, KN, 0, 0);
       constexpr uint32_t kIdO = instr_desc(kTM, D, 0, 1);
       // failure-detection test hook: the grid's first CTA issues no first
       // product, so its softmax runs into the limit
-      bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+      const bool withhold = A.withhold && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
       const uint32_t dq = desc_low(base + C::OQ, 16);
       const uint32_t dk = desc_low(base + C::OST, 16), dv = desc_low(base + C::OST, KN * 128);
       uint32_t kslot = 0, kph = 0, vslot = 1, vph = 0;  // ring slots and phases of K(i), V(i-1)
       bool ok = wait_alive(q_full, 0, dead, A.status);
-      if constexpr (QT == 1) {
-        for (int i = 0; i <= n && ok; ++i) {
-          if (i < n) {  // S(i) while the softmax is at step i - 1; its buffer's last P was read by the product before
-            ok = wait_alive(full + kslot, kph, dead, A.status);
-            if (!ok) break;
-            tc_fence_after();
-            if (!(withhold && i == 0) && elect_one()) {
-              issue_kk<D, kTM, KN>(tmem + (i & 1) * KN, dq, dk + kslot * (C::SB >> 4), kIdS);
-              umma_commit(s_full + (i & 1));
-              umma_commit(empty + kslot);
-            }
-            __syncwarp();
-            kslot += 2;
-            if (kslot >= C::NS) kslot -= C::NS, kph ^= 1;
-          }
-          if (i > 0) {
-            const int j = i - 1;
-            ok = wait_alive(full + vslot, vph, dead, A.status);
-            const uint32_t v = dv + vslot * (C::SB >> 4);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // P arrives in halves
-              ok = ok && wait_alive(p_full + 2 * (j & 1) + h, (j >> 1) & 1, dead, A.status);
-              if (!ok) break;
-              tc_fence_after();
-              if (elect_one())
-                issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4), kIdO,
-                                  (j > 0) | (h > 0));
-              __syncwarp();
-            }
-            if (!ok) break;
-            if (elect_one()) {
-              umma_commit(o_step);
-              umma_commit(empty + vslot);
-            }
-            __syncwarp();
-            vslot += 2;
-            if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
-          }
-        }
-      } else {
-        uint32_t steps[QT];  // steps of each tile so far
-#pragma unroll
-        for (int t = 0; t < QT; ++t) steps[t] = 0;
-        for (int i = 0; i <= n && ok; ++i) {
-          if (i > 0) ok = wait_alive(full + vslot, vph, dead, A.status);
-#pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            if (i > 0 && needs(t, i - 1)) {
-              const uint32_t ph = (steps[t] - 1) & 1;
-              const uint32_t v = dv + vslot * (C::SB >> 4);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {  // P arrives in halves
-                ok = ok && wait_alive(p_full + 2 * t + h, ph, dead, A.status);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one())
-                  issue_tn<KN / 32>(tmem + C::COL_O + t * D, tmem + t * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4),
-                                    kIdO, (steps[t] > 1) | (h > 0));
-                __syncwarp();
-              }
-              if (!ok) break;
-            }
-            if (i == n) continue;
-            if (t == 0) ok = ok && wait_alive(full + kslot, kph, dead, A.status);
-            if (!ok) break;
-            if (needs(t, i)) {
-              tc_fence_after();
-              ++steps[t];
-              if (withhold) {
-                withhold = false;
-                continue;
-              }
-              if (elect_one()) {
-                issue_kk<D, kTM, KN>(tmem + t * KN, dq + t * (C::QB >> 4), dk + kslot * (C::SB >> 4), kIdS);
-                umma_commit(s_full + t);
-              }
-              __syncwarp();
-            }
-          }
+      for (int i = 0; i <= n && ok; ++i) {
+        if (i < n) {  // S(i) while the softmax is at step i - 1; its buffer's last P was read by the product before
+          ok = wait_alive(full + kslot, kph, dead, A.status);
           if (!ok) break;
-          if (elect_one()) {
-            if (i > 0) umma_commit(empty + vslot);
-            if (i < n) umma_commit(empty + kslot);
+          tc_fence_after();
+          if (!(withhold && i == 0) && elect_one()) {
+            issue_kk<D, kTM, KN>(tmem + (i & 1) * KN, dq, dk + kslot * (C::SB >> 4), kIdS);
+            umma_commit(s_full + (i & 1));
+            umma_commit(empty + kslot);
           }
           __syncwarp();
           kslot += 2;
           if (kslot >= C::NS) kslot -= C::NS, kph ^= 1;
-          if (i > 0) {
-            vslot += 2;
-            if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
+        }
+        if (i > 0) {
+          const int j = i - 1;
+          ok = wait_alive(full + vslot, vph, dead, A.status);
+          const uint32_t v = dv + vslot * (C::SB >> 4);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // P arrives in halves
+            ok = ok && wait_alive(p_full + 2 * (j & 1) + h, (j >> 1) & 1, dead, A.status);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one())
+              issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4), kIdO,
+                                (j > 0) | (h > 0));
+            __syncwarp();
           }
+          if (!ok) break;
+          if (elect_one()) {
+            umma_commit(o_step);
+            umma_commit(empty + vslot);
+          }
+          __syncwarp();
+          vslot += 2;
+          if (vslot >= C::NS) vslot -= C::NS, vph ^= 1;
         }
       }
       if (ok && elect_one()) umma_commit(o_full);
       __syncwarp();
     } else {
       // ---- copies ----
-      const int lt = (int)threadIdx.x - QT * 128 - 32;
+      const int lt = (int)threadIdx.x - kTM - 32;
       const bf16_t* kb = A.k + (int64_t)b * A.ks[0] + (int64_t)hk * A.ks[2];
       const bf16_t* vb = A.v + (int64_t)b * A.vs[0] + (int64_t)hk * A.vs[2];
       const int early = issued;
@@ -515,26 +430,24 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
         if (A.kv_maps && boxed<KN>(sq, j0)) {
           if (ok && lt == 0 && s >= early) load_box(s);
         } else {
-          stage_keys<C::COPY, KN, D>(base + C::OST + (s % C::NS) * C::SB, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0,
+          stage_keys<32, KN, D>(base + C::OST + (s % C::NS) * C::SB, s & 1 ? vb : kb, s & 1 ? A.vs[1] : A.ks[1], sq, j0,
                                      kt.end(i), lt, ok);
           if (ok && lt == 0) mbar_arrive(full + s % C::NS);
         }
       }
     }
   } else {
-    // ---- softmax of tile wg ----
-    if constexpr (C::LAUNCH_REGS > 0) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
-    const int t = wg, mt = m0 + t * kTM;
-    const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    if (!A.q_maps) {  // Q_t: this warpgroup's 128 rows
+    // ---- softmax ----
+    const uint32_t lane = tmem + ((uint32_t)(warp * 32) << 16);
+    if (!A.q_maps) {  // Q: this warpgroup's 128 rows
       constexpr int CH = D / 8;
-      const int lt = threadIdx.x & 127, c = lt % CH;
+      const int lt = threadIdx.x, c = lt % CH;
       const bf16_t* qb = A.q + (int64_t)b * A.qs[0] + (int64_t)hv * A.G * A.qs[2];
 #pragma unroll 4
       for (int r = lt / CH; r < kTM; r += 128 / CH) {
-        const int mr = mt + r, tr = group_div(A, mr);
+        const int mr = m0 + r, tr = group_div(A, mr);
         const bool valid = mr < A.M && token_of(A, sq, tr) >= 0;
-        cp_async16(base + C::OQ + t * C::QB + (uint32_t)(c >> 3) * (kTM * 128u) + sw128((uint32_t)r, (uint32_t)(c & 7)),
+        cp_async16(base + C::OQ + (uint32_t)(c >> 3) * (kTM * 128u) + sw128((uint32_t)r, (uint32_t)(c & 7)),
                    valid ? qb + (int64_t)tr * A.qs[1] + (int64_t)(mr - tr * A.G) * A.qs[2] + c * 8 : qb, valid);
       }
       cp_async_commit();
@@ -543,18 +456,11 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       mbar_arrive(q_full);
     }
     const int lo = low_of(A, sq, p), hi = high_of(sq, p);
-    uint32_t steps = 0;
+    const int lo_last = low_of(A, sq, p1), hi_first = high_of(sq, p0);
     bool ok = true;
-    int tl1 = lo1[0], th0 = hi0[0];
-    if (QT == 2 && t == 1) {
-      tl1 = lo1[QT - 1];
-      th0 = hi0[QT - 1];
-    }
     for (int i = 0; i < n; ++i) {
-      if (QT == 2 && !needs(t, i)) continue;
-      // one tile: two buffers in turn; two tiles: a buffer each
-      const int buf = QT == 1 ? (int)(steps & 1) : t;
-      ok = __all_sync(kFullMask, wait_alive(s_full + buf, QT == 1 ? (steps >> 1) & 1 : steps & 1, dead, A.status));
+      const int buf = i & 1;
+      ok = __all_sync(kFullMask, wait_alive(s_full + buf, (i >> 1) & 1, dead, A.status));
       if (!ok) break;
       tc_fence_after();
       uint32_t sr[KN / 32][32];
@@ -566,7 +472,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       for (int c = 0; c < KN / 32; ++c)
 #pragma unroll
         for (int j = 0; j < 32; ++j) s[c][j] = __uint_as_float(sr[c][j]);
-      if (!kt.full(i0 + i, tl1, th0)) {
+      if (!kt.full(i0 + i, lo_last, hi_first)) {
         const int k0 = kt.start(i0 + i);
         const bool in_sink = i0 + i < kt.ns;
         // relative bounds: lo <= j < hi, or j < S (a sink tile: j < min(sink, hi))
@@ -586,20 +492,17 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       if (raise) m_ref = mt_;
       const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen nothing yet: p = 2^-inf = 0
       const float2 sc2 = make_float2(A.scale_log2, A.scale_log2), nm2 = make_float2(nm, nm);
-      if (steps > 0 && __any_sync(kFullMask, raise)) {
-        // one tile: O's last product may still run (two: S(i) came behind it)
-        if (QT == 1) {
-          ok = __all_sync(kFullMask, wait_alive(o_step, (steps - 1) & 1, dead, A.status));
-          if (!ok) break;
-          tc_fence_after();
-        }
+      if (i > 0 && __any_sync(kFullMask, raise)) {  // O's last product may still run
+        ok = __all_sync(kFullMask, wait_alive(o_step, (i - 1) & 1, dead, A.status));
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
           uint32_t ot[16];
-          tmem_ld16(lane + C::COL_O + t * D + c, ot);
+          tmem_ld16(lane + C::COL_O + c, ot);
 #pragma unroll
           for (int j = 0; j < 16; ++j) ot[j] = __float_as_uint(__uint_as_float(ot[j]) * alpha);
-          tmem_st16(lane + C::COL_O + t * D + c, ot);
+          tmem_st16(lane + C::COL_O + c, ot);
         }
       }
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -622,10 +525,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       }
       const float2 l2 = fadd2(ls[0], ls[1]);
       l_run = fmaf(l_run, alpha, l2.x + l2.y);
-      ++steps;
     }
-    // also where this tile had no step: the rows leave through memory that the
-    // other tile's products read
     if (ok) ok = __all_sync(kFullMask, wait_alive(o_full, 0, dead, A.status));
     tc_fence_after();
     ok_row = ok;
@@ -635,7 +535,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float ot[32];
-        tmem_ld32(lane + C::COL_O + t * D + c, ot);
+        tmem_ld32(lane + C::COL_O + c, ot);
         if (!mine) continue;
         float* pr = A.part_o + prow * D + c;
 #pragma unroll
@@ -644,17 +544,17 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
       }
     }
     if (SPLIT == kSplitNone) {  // (a cluster's rows are joined below)
-      // every product is done: the rows leave through Q_t's place, the residuals
+      // every product is done: the rows leave through Q's place, the residuals
       // through the ring's
-      const uint32_t out = base + C::OQ + t * C::QB, res = base + C::OST + t * C::QB, r = threadIdx.x & (kTM - 1);
-      static_assert(QT * C::QB <= C::NS * C::SB, "the residuals fit over the ring");
+      const uint32_t out = base + C::OQ, res = base + C::OST, r = threadIdx.x;
+      static_assert(C::QB <= C::NS * C::SB, "the residuals fit over the ring");
       const bool seen = p >= 0 && l_run != 0.f;  // (a NaN sum is written as it is)
       const float inv = 1.f / l_run;
       if (ok) {
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           float ot[32];
-          tmem_ld32(lane + C::COL_O + t * D + c, ot);
+          tmem_ld32(lane + C::COL_O + c, ot);
 #pragma unroll
           for (int j = 0; j < 32; ++j) ot[j] = seen ? ot[j] * inv : 0.f;
 #pragma unroll
@@ -676,10 +576,10 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
         A.lse[(int64_t)bh * A.M + m] = !ok ? __int_as_float(0x7fc00000) : seen ? (m_ref + log2f(l_run)) * kLn2 : -INFINITY;
       // all 128 threads meet, also after an expired wait (then the rows are NaN,
       // never a plausible wrong number)
-      asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory");
-      const int rows = min(kTM, A.M - mt);
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+      const int rows = min(kTM, A.M - m0);
       auto at = [&](int row) {
-        const int mr = mt + row, tr = group_div(A, mr);
+        const int mr = m0 + row, tr = group_div(A, mr);
         return (((int64_t)b * A.Tq + tr) * A.Hq + hv * A.G + mr - tr * A.G) * D;
       };
       flush_rows<D, kTM>(out, rows, r, *dead != 0, [&](int row) { return A.o + at(row); });
@@ -690,9 +590,9 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
   __syncthreads();
   tc_fence_after();
   if (*dead) {  // bounded waits for every product and box that was issued
-    if (warp == QT * 4 && (threadIdx.x & 31) == 0) umma_commit(drain);
+    if (warp == 4 && (threadIdx.x & 31) == 0) umma_commit(drain);
     mbar_wait(drain, 0);
-    if (threadIdx.x == QT * 128 + 32) {
+    if (threadIdx.x == kTM + 32) {
       if (A.q_maps && n > 0) mbar_wait(q_full, 0);
       for (int s = max(0, issued - C::NS); s < issued; ++s) mbar_wait(full + s % C::NS, (s / C::NS) & 1);
     }
@@ -705,10 +605,10 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     constexpr int LD = C::LD;
     float* po = reinterpret_cast<float*>(smem);
     float2* ml = reinterpret_cast<float2*>(smem + C::OML);
-    if (wg < QT) {
+    if (!service) {
       const int r = threadIdx.x;
       if (n > 0) {
-        const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t lane = tmem + ((uint32_t)(warp * 32) << 16);
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           float ot[32];
@@ -756,7 +656,7 @@ __global__ void __launch_bounds__(FwdCfg<D, QT>::THREADS, FwdCfg<D, QT>::CTAS)
     cluster_sync();  // a CTA's shared memory stays until all have read it
     tc_fence_after();
   }
-  if (warp == QT * 4) tmem_free(tmem, C::COLS);
+  if (warp == 4) tmem_free(tmem, C::COLS);
 }
 
 // Joins the splits of a row: weights 2^(m_z - max m), a warp per packed row.
@@ -1381,22 +1281,14 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
   A.rows[at] = lse == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-lse * kLog2e, -d);
 }
 
-// Raises a kernel's dynamic shared-memory limit once per device; refuses a
-// kernel whose block holds fewer registers than its warps will ask for.
+// Raises a kernel's dynamic shared-memory limit once per device.
 template <class K>
-cudaError_t allow_smem(K* kernel, uint32_t bytes, std::atomic<unsigned long long>& done, int regs = 0,
-                       int threads = 0) {
+cudaError_t allow_smem(K* kernel, uint32_t bytes, std::atomic<unsigned long long>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned long long bit = 1ull << (dev & 63);
   if (done.load() & bit) return cudaSuccess;
-  if (regs > 0) {
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, kernel);
-    if (e != cudaSuccess) return e;
-    if (fa.numRegs * threads < regs) return cudaErrorInvalidConfiguration;
-  }
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) done.fetch_or(bit);
   return e;
@@ -1463,17 +1355,16 @@ bool group_map(CUtensorMap* map, const WindowArgs& A, const bf16_t* p, const int
   return make_map(map, p, d, {s[2], s[1], s[0]}, A.G, rows / A.G);
 }
 
-template <int D, int QT, int SPLIT>
+template <int D, int SPLIT>
 cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
-  using C = FwdCfg<D, QT>;
+  using C = FwdCfg<D>;
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = allow_smem(window_fwd_kernel<D, QT, SPLIT>, C::BYTES, done,
-                                   C::LAUNCH_REGS * C::THREADS, C::THREADS);
+  const cudaError_t e = allow_smem(window_fwd_kernel<D, SPLIT>, C::BYTES, done);
   if (e != cudaSuccess) return e;
-  kv_maps(A, D, C::KN);
-  sink_maps(A, D, C::KN);
+  kv_maps(A, D, kTN);
+  sink_maps(A, D, kTN);
   A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
-  const dim3 grid((unsigned)(A.B * A.Hk * A.nsub), (unsigned)((A.M + QT * kTM - 1) / (QT * kTM)), (unsigned)A.splits);
+  const dim3 grid((unsigned)(A.B * A.Hk * A.nsub), (unsigned)((A.M + kTM - 1) / kTM), (unsigned)A.splits);
   if constexpr (SPLIT == kSplitCluster) {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1485,26 +1376,18 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, window_fwd_kernel<D, QT, SPLIT>, (const WindowArgs&)A);
+    return cudaLaunchKernelEx(&cfg, window_fwd_kernel<D, SPLIT>, (const WindowArgs&)A);
   } else {
-    window_fwd_kernel<D, QT, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
+    window_fwd_kernel<D, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
     return cudaGetLastError();
   }
 }
 
 template <int D>
-cudaError_t fwd_any(WindowArgs& A, int sms, cudaStream_t st) {
-  if (A.splits == 1) {
-    // Two query tiles per CTA share the key tiles and hide one another's softmax,
-    // one tile per CTA fills the device with less: us with one / two at D = 128,
-    // 512 pairs of tiles: 1024 keys seen 101 / 102, 2048 keys 160 / 145, 4096 keys
-    // 232 / 188, 512 keys 71 / 80; at D = 64: 84 / 85, 135 / 125, 199 / 169, 57 / 66.
-    const int64_t pairs = (int64_t)A.B * A.Hk * A.nsub * ((A.M + 2 * kTM - 1) / (2 * kTM));
-    const int64_t seen = std::min<int64_t>(A.Tk, (int64_t)A.W + A.S);
-    return pairs >= sms && seen >= 1536 ? fwd_launch<D, 2, kSplitNone>(A, st) : fwd_launch<D, 1, kSplitNone>(A, st);
-  }
-  if (A.splits <= kClusterMost) return fwd_launch<D, 1, kSplitCluster>(A, st);
-  const cudaError_t e = fwd_launch<D, 1, kSplitMemory>(A, st);
+cudaError_t fwd_any(WindowArgs& A, cudaStream_t st) {
+  if (A.splits == 1) return fwd_launch<D, kSplitNone>(A, st);
+  if (A.splits <= kClusterMost) return fwd_launch<D, kSplitCluster>(A, st);
+  const cudaError_t e = fwd_launch<D, kSplitMemory>(A, st);
   if (e != cudaSuccess) return e;
   const int64_t rows = (int64_t)A.B * A.Hk * A.M;
   window_join_kernel<D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(A);
@@ -1590,7 +1473,7 @@ size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at) {
 // each, from the most keys a query tile can see.
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms) {
   const int64_t tiles = (most_keys + kTN - 1) / kTN + 1;
-  const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64, 1>::CTAS : FwdCfg<128, 1>::CTAS);
+  const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64>::CTAS : FwdCfg<128>::CTAS);
   return (int)std::max<int64_t>(1, std::min<int64_t>(room / std::max<int64_t>(1, ctas), tiles / 2));
 }
 
@@ -1601,8 +1484,8 @@ size_t window_split_workspace(int D, int64_t rows, int splits, size_t* ml_at) {
   return *ml_at + (size_t)rows * splits * sizeof(float2);
 }
 
-cudaError_t window_fwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st) {
-  return D == 64 ? fwd_any<64>(A, sms, st) : fwd_any<128>(A, sms, st);
+cudaError_t window_fwd_launch(WindowArgs& A, int D, cudaStream_t st) {
+  return D == 64 ? fwd_any<64>(A, st) : fwd_any<128>(A, st);
 }
 
 cudaError_t window_bwd_launch(WindowArgs& A, int D, cudaStream_t st) {

@@ -1203,9 +1203,7 @@ int specdec_window_attention_forward(const uint16_t* q, const int64_t* q_strides
   A.n_ctx = n_ctx;
   A.status = status;
   A.withhold = take_withhold_stage();
-  int sms = 0;
-  if ((rc = device_sms(&sms)) != SPECDEC_OK) return rc;
-  const cudaError_t e = window_fwd_launch(A, head_dim, sms, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = window_fwd_launch(A, head_dim, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? ok() : cuda_fail(e, "window attention forward launch");
 }
 
@@ -1334,7 +1332,7 @@ int specdec_window_attention_cached(const uint16_t* q, const int64_t* q_strides,
   A.cached = 1;
   A.status = status;
   A.withhold = take_withhold_stage();
-  const cudaError_t e = window_fwd_launch(A, head_dim, sms, st);
+  const cudaError_t e = window_fwd_launch(A, head_dim, st);
   return e == cudaSuccess ? ok() : cuda_fail(e, "window attention launch");
 }
 

@@ -132,15 +132,15 @@ def test_window_attention_forward_backward(cuda, B, n_ctx, nb, Hq, Hk, D, W, S, 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,n_ctx,nb,Hq,Hk,D,W,S,lens", [
-    (2, 1584, 16, 16, 16, 64, 1540, 4, None),         # the last CTA's second query tile is empty
+    (2, 1584, 16, 16, 16, 64, 1540, 4, None),
     (2, 1584, 16, 16, 16, 128, 1540, 4, None),
     (1, 2000, 7, 40, 20, 128, 1700, 130, None),       # shared heads, two sink tiles
     (3, 1700, 0, 18, 6, 64, None, 0, (1700, 3, 900)),  # groups of three, padded tiles
     (3, 1650, 20, 16, 16, 128, 1600, 1, (0, 1650, 1500)),
 ])
-def test_window_attention_with_two_query_tiles_per_cta(cuda, B, n_ctx, nb, Hq, Hk, D, W, S, lens):
-    """Sizes that take the forward with two query tiles per CTA (148 of them or
-    more, 1536 visible keys or more); a few heads of each sequence are compared."""
+def test_window_attention_of_long_windows(cuda, B, n_ctx, nb, Hq, Hk, D, W, S, lens):
+    """More tiles than the device holds at once, windows of many key tiles; a few
+    heads of each sequence are compared."""
     T, G = n_ctx + nb, Hq // Hk
     q, do = _rand(B, T, Hq, D, seed=1), _rand(B, T, Hq, D, seed=2)
     k, v = _rand(B, T, Hk, D, seed=3), _rand(B, T, Hk, D, seed=4)
@@ -387,8 +387,8 @@ def _reported():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,T,Hq,Hk,D,W,first", [
-    (2, 300, 2, 1, 64, 40, 256),         # one query tile per CTA: packed rows 512 .. 599 are tokens 256 .. 299
-    (2, 2048, 16, 16, 128, None, 1792),  # two query tiles per CTA
+    (2, 300, 2, 1, 64, 40, 256),  # packed rows 512 .. 599 are tokens 256 .. 299
+    (2, 2048, 16, 16, 128, None, 1920),
 ])
 def test_an_expired_wait_of_the_forward_gives_nan_rows_and_a_report(cuda, B, T, Hq, Hk, D, W, first):
     q, k, v = _rand(B, T, Hq, D, seed=1), _rand(B, T, Hk, D, seed=2), _rand(B, T, Hk, D, seed=3)
@@ -454,7 +454,7 @@ def test_a_cache_past_32_bit_offsets(cuda):
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,n_ctx,nb,H,D,W,S,lens", [
     (2, 300, 7, 4, 64, 60, 3, (300, 101)), (2, 300, 7, 4, 128, 60, 70, None), (1, 90, 0, 3, 64, None, 0, None),
-    (2, 1584, 16, 16, 64, 1540, 4, (1584, 1500)),  # two query tiles per CTA
+    (2, 1584, 16, 16, 64, 1540, 4, (1584, 1500)),
     (2, 1584, 16, 16, 128, None, 0, None),
 ])
 def test_expanded_inputs_equal_their_copies(cuda, B, n_ctx, nb, H, D, W, S, lens):

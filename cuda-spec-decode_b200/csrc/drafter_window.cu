@@ -124,6 +124,13 @@ struct KeyTiles {
   }
 };
 
+// Bits 0 .. n-1 (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int n) {
+  uint32_t r;
+  asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(0xFFFFFFFFu), "r"(32 - min(max(n, 0), 32)));  // 32 places: 0
+  return r;
+}
+
 // ---- tiles in shared memory ---------------------------------------------------
 // A tile of ROWS rows of D bf16 is D / 64 column blocks of ROWS x 128 bytes in
 // the 128-byte-swizzled layout.
@@ -348,14 +355,14 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
     mbar_init(drain, 1);
     fence_mbar_init();
     *dead = 0;
-    // its boxes start before the CTA meets
+    // Q and the first K start before the CTA meets
     if (A.q_maps && n > 0) {
       mbar_arrive_expect_tx(q_full, C::QB);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
         tma_load_4d(base + C::OQ + c * (kTM * 128), &A.mq, c * 64, hv * A.G, m0 / A.G, b, q_full);
     }
-    while (issued < min(2 * n, C::NS) && A.kv_maps && boxed<KN>(sq, kt.start(i0 + (issued >> 1)))) load_box(issued++);
+    if (n > 0 && A.kv_maps && boxed<KN>(sq, kt.start(i0))) load_box(issued++);
   }
   if (warp == 4) tmem_alloc(slot, C::COLS);
   tc_fence_before();
@@ -478,8 +485,12 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
         // relative bounds: lo <= j < hi, or j < S (a sink tile: j < min(sink, hi))
         const int rl = in_sink ? KN : lo - k0, rh = hi - k0, rs = (in_sink ? kt.sink : A.S) - k0;
 #pragma unroll
-        for (int j = 0; j < KN; ++j)
-          if (!(j < rh && (j >= rl || j < rs))) s[j >> 5][j & 31] = -INFINITY;
+        for (int c = 0; c < KN / 32; ++c) {
+          const uint32_t sees = below(rh - c * 32) & (~below(rl - c * 32) | below(rs - c * 32));
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (!(sees & (1u << j))) s[c][j] = -INFINITY;
+        }
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

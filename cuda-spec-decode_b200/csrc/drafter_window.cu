@@ -31,6 +31,7 @@
 // type; its relative error, half a step, equals that of the rounded output).
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cstdint>
 #include <type_traits>
 
@@ -728,8 +729,8 @@ struct BwdCfg {
   static constexpr int COPY = NB == 1 ? 32 : 96;  // threads of the copying warps
   static constexpr int THREADS = NB * 128 + 32 + COPY, CTAS = NB == 1 ? 2 : 1;
   static constexpr uint32_t XB = kTM * D * 2, YB = kTN * D * 2;
-  static constexpr uint32_t OX = 0, OY = 2 * XB, OROW = OY + NS * 2 * YB;  // rows: 64 x (-lse2, -delta, lo, hi) per stage
-  static constexpr uint32_t OBAR = OROW + NS * kTN * 16;
+  static constexpr uint32_t OX = 0, OY = 2 * XB, OROW = OY + NS * 2 * YB;  // rows: 64 x -lse2, 64 x -delta per stage
+  static constexpr uint32_t OBAR = OROW + NS * kTN * 8;
   static constexpr int NBAR = 3 * NS + 2 * NB + 3;  // full, empty, r_full; s_full, p_full, x_full, o_full, drain
   static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;
   static constexpr uint32_t COL_A = NB * 128, COL_B = COL_A + D;  // dQ or dV; dK
@@ -906,7 +907,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     for (int i = 0; i < C::NS; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
-      mbar_init(r_full + i, 2 * C::COPY);
+      mbar_init(r_full + i, C::COPY);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
@@ -1036,20 +1037,14 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
         if (DKV) {
           const int f = qt.first(A, rr), l = qt.last(A, rr);
           const int t0 = f / A.G, t1 = t0 + kTN / A.G;
-          // -lse2, -delta and the bounds of the keys that each row sees
-          if (ok) {
-            for (int e = lt; e < kTN; e += C::COPY) {
-              const uint32_t rowp = base + C::OROW + (sl * kTN + e) * 16;
-              const int m = f + e;
-              const float2* src = A.rows + ((int64_t)b * A.Hk * A.nsub + hk * A.nsub + sub) * A.M + (m < l ? m : f);
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(rowp), "l"(src), "r"(m < l ? 8 : 0) : "memory");
-              const int p = m < l ? token_of(A, sq, group_div(A, m)) : -1;
-              asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(rowp + 8), "r"(low_of(A, sq, p)), "r"(high_of(sq, p))
-                           : "memory");
+          if (ok) {  // -lse2 and -delta of the rows (zeros behind the last)
+            for (int e = lt; e < 2 * kTN; e += C::COPY) {
+              const int m = f + (e & (kTN - 1));
+              const float* src = A.rows + (int64_t)(e / kTN) * A.rows_plane +
+                                 ((int64_t)b * A.Hk * A.nsub + hk * A.nsub + sub) * A.M + (m < l ? m : f);
+              cp_async4(base + C::OROW + (sl * 2 * kTN + e) * 4, src, m < l);
             }
-            // two arrivals per thread: when its copies have landed, and for its own writes
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(r_full + sl)) : "memory");
-            mbar_arrive(r_full + sl);
           }
           if (y_boxes && (t1 <= sq.c || t0 >= A.n_ctx || sq.c == A.n_ctx)) {
             if (ok && lt == 0) {
@@ -1093,13 +1088,17 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     const uint32_t lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t buf = lane + wg * 128;
     const int lo = low_of(A, sq, token), hi = high_of(sq, token);
-    const int lo_last = low_of(A, sq, p1), hi_first = high_of(sq, p0);
     float2 nl = make_float2(0.f, 0.f), nd = nl;
     if (!DKV && token >= 0) {
-      const float2 v = A.rows[((int64_t)b * A.Hk * A.nsub + head) * A.M + xr];
-      nl = make_float2(v.x, v.x);
-      nd = make_float2(v.y, v.y);
+      const float* v = A.rows + ((int64_t)b * A.Hk * A.nsub + head) * A.M + xr;
+      nl = make_float2(v[0], v[0]);
+      nd = make_float2(v[A.rows_plane], v[A.rows_plane]);
     }
+    // dk/dv: this key's first and last context query as packed rows, and whether the block sees it
+    const bool key = DKV && token >= 0, ctx_key = key && token < sq.c;
+    const int q_lo = ctx_key ? token * A.G : INT_MAX, q_hi = token < A.S ? INT_MAX : min(token + A.W, sq.c) * A.G;
+    const bool in_block = key && (token >= sq.c || sq.c - token <= A.W || token < A.S);
+    int rr = DKV ? (i0 + wg) % qt.per : 0;
     bool ok = true;
     uint32_t k = 0, sl = wg % C::NS, rph = 0;
     for (int i = wg; i < n; i += NB, ++k) {
@@ -1107,47 +1106,54 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
       if (DKV) ok = ok && __all_sync(kFullMask, wait_alive(r_full + sl, rph, dead, A.status));
       if (!ok) break;
       tc_fence_after();
-      const float4* rows = reinterpret_cast<const float4*>(smem + C::OROW + sl * (kTN * 16));  // (-lse2, -delta, lo, hi)
-      bool whole;  // every row of X sees (is seen by) every row of Y
+      const float4* rows = reinterpret_cast<const float4*>(smem + C::OROW + sl * (2 * kTN * 4));  // -lse2, -delta
+      // the columns that this thread's row sees, 32 in a word
+      int ca, cb, cs;  // [ca, cb), and [0, min(cs, cb))
       if (DKV) {
-        const float4 ra = rows[0], rz = rows[kTN - 1];
-        whole = x0 + kTM <= sq.c && __float_as_int(ra.w) >= x0 + kTM && __float_as_int(rz.w) > 0 &&
-                __float_as_int(rz.z) <= x0;
+        const int f = qt.first(A, rr), l = qt.last(A, rr) - f;
+        cs = 0;
+        if (rr < qt.na) {
+          ca = q_lo == INT_MAX ? kTN : q_lo - f;
+          cb = min(l, q_hi == INT_MAX ? kTN : q_hi - f);
+        } else {
+          ca = 0;
+          cb = in_block ? l : 0;
+        }
+        rr += NB;
+        while (rr >= qt.per) rr -= qt.per;
       } else {
-        whole = kt.full(i, lo_last, hi_first);
+        const int j0 = kt.start(i);
+        ca = i < kt.ns ? kTN : lo - j0;
+        cb = hi - j0;
+        cs = (i < kt.ns ? kt.sink : A.S) - j0;
       }
-      const int j0 = kt.start(DKV ? 0 : i);
-      const bool in_sink = i < kt.ns;
-      const int rl = in_sink ? kTN : lo - j0, rh = hi - j0, rs = (in_sink ? kt.sink : A.S) - j0;
+      uint32_t sees[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sees[h] = below(cb - h * 32) & (~below(ca - h * 32) | below(cs - h * 32));
+      const bool whole = __all_sync(kFullMask, (sees[0] & sees[1]) == 0xFFFFFFFFu);
       auto half_step = [&](int h, auto masked) {  // 32 columns; no branch inside
         uint32_t sr[32], dr[32];
         tmem_ld32_async(buf + h * 32, sr);
         tmem_ld32_async(buf + 64 + h * 32, dr);
         tmem_wait_ld();
         uint32_t wp[16], wd[16];
+        float2 nl_next, nd_next;
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           float2 pr, ds;
           if (DKV) {
-            const float2 va = *reinterpret_cast<const float2*>(rows + h * 32 + j);
-            const float2 vb = *reinterpret_cast<const float2*>(rows + h * 32 + j + 1);
-            nl = make_float2(va.x, vb.x);
-            nd = make_float2(va.y, vb.y);
+            if (j % 4 == 0) {
+              const float4 a = rows[(h * 32 + j) / 4], d = rows[(kTN + h * 32 + j) / 4];
+              nl = make_float2(a.x, a.y), nl_next = make_float2(a.z, a.w);
+              nd = make_float2(d.x, d.y), nd_next = make_float2(d.z, d.w);
+            } else {
+              nl = nl_next, nd = nd_next;
+            }
           }
           grad_pair(make_float2(__uint_as_float(sr[j]), __uint_as_float(sr[j + 1])),
                     make_float2(__uint_as_float(dr[j]), __uint_as_float(dr[j + 1])), A.scale_log2, nl, nd, pr, ds);
           if constexpr (masked.value) {
-            bool va, vb;
-            if (DKV) {
-              const int2 ba = reinterpret_cast<const int2*>(rows + h * 32 + j)[1];
-              const int2 bb = reinterpret_cast<const int2*>(rows + h * 32 + j + 1)[1];
-              va = (token >= 0) & (token < ba.y) & ((token >= ba.x) | (token < A.S));
-              vb = (token >= 0) & (token < bb.y) & ((token >= bb.x) | (token < A.S));
-            } else {
-              const int e = h * 32 + j;
-              va = (e < rh) & ((e >= rl) | (e < rs));
-              vb = (e + 1 < rh) & ((e + 1 >= rl) | (e + 1 < rs));
-            }
+            const bool va = sees[h] & (1u << j), vb = sees[h] & (2u << j);
             pr = make_float2(va ? pr.x : 0.f, vb ? pr.y : 0.f);
             ds = make_float2(va ? ds.x : 0.f, vb ? ds.y : 0.f);
           }
@@ -1257,8 +1263,8 @@ __global__ void __launch_bounds__(256) window_sink_join_kernel(const __grid_cons
   *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
 }
 
-// rows[b, virtual head, m] = (-lse log2 e, -sum_d dO o) of every packed row;
-// D / 8 lanes per row, rows in the tensors' order. Padding: (0, 0), masked later.
+// rows[0 | 1][b, virtual head, m] = -lse log2 e | -sum_d dO o of every packed row;
+// D / 8 lanes per row, rows in the tensors' order. Padding: zeros, masked later.
 // o comes as the rounded output and the residual of that rounding (16 bits in
 // all): with o rounded to 8 bits, delta's error is the largest in the gradients
 // of rows that see few keys (dq, dk 1.53 to 1.9 times as far off as one
@@ -1289,7 +1295,8 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
   const int hv = h / A.G;
   const int64_t at = ((int64_t)b * A.Hk * A.nsub + hv) * A.M + (int64_t)t * A.G + (h - hv * A.G);
   const float lse = A.lse[at];
-  A.rows[at] = lse == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-lse * kLog2e, -d);
+  A.rows[at] = lse == -INFINITY ? 0.f : -lse * kLog2e;
+  A.rows[A.rows_plane + at] = lse == -INFINITY ? 0.f : -d;
 }
 
 // Raises a kernel's dynamic shared-memory limit once per device.
@@ -1427,6 +1434,7 @@ cudaError_t bwd_launch(const WindowArgs& A, unsigned grid, cudaStream_t st) {
 template <int D>
 cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
   cudaError_t e;
+  A.rows_plane = (int64_t)A.B * A.Tq * A.Hq;
   const int64_t lanes = (int64_t)A.B * A.Tq * A.Hq * (D / 8);
   window_rows_kernel<D><<<(unsigned)((lanes + 255) / 256), 256, 0, st>>>(A);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -1474,7 +1482,7 @@ void window_sink_shape(WindowArgs& A, int sms) {
 }
 
 size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at) {
-  const size_t rows = (size_t)A.B * A.Tq * A.Hq * sizeof(float2);
+  const size_t rows = (size_t)A.B * A.Tq * A.Hq * 2 * sizeof(float);
   *sink_at = (rows + 255) & ~size_t(255);
   return *sink_at +
          (A.sink_splits > 1 ? (size_t)A.B * A.Hk * A.sink_tiles * A.sink_splits * 2 * kTM * D * sizeof(float) : 0);

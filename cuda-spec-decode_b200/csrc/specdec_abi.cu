@@ -1253,7 +1253,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   }
   if (workspace_bytes < need || !aligned(workspace, 16))
     return fail(SPECDEC_ERR_WORKSPACE, "workspace needs %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
-  A.rows = static_cast<float2*>(workspace);
+  A.rows = static_cast<float*>(workspace);
   A.sink_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sink_at);
   A.q = q;
   A.k = k;

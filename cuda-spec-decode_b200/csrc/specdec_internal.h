@@ -238,7 +238,8 @@ struct WindowArgs {
   float* part_o;                   // [B * Hk * M, splits, D]
   float2* part_ml;                 // [B * Hk * M, splits]: reference maximum, sum
   const bf16_t* dO;                // backward: [B, Tq, Hq, D]
-  float2* rows;                    // [B, Hk * nsub, M]: -lse log2 e, -delta
+  float* rows;                     // [2, B, Hk * nsub, M]: -lse log2 e, -delta
+  int64_t rows_plane;              // B * Tq * Hq
   float* sink_part;                // partials of the key tiles that hold sinks
   int sink_tiles, sink_splits;
   bf16_t *dq, *dk, *dv;

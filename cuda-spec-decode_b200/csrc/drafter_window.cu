@@ -145,6 +145,13 @@ __device__ __forceinline__ void issue_kk(uint32_t d, uint32_t a, uint32_t b, uin
     umma_ss(d, a + (((kk >> 2) * (RA * 128) + (kk & 3) * 32) >> 4), b + (((kk >> 2) * (RB * 128) + (kk & 3) * 32) >> 4),
             idesc, kk > 0);
 }
+// The same with A in tensor memory: two elements of a row per column.
+template <int D, int RB>
+__device__ __forceinline__ void issue_tk(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    umma_ts(d, a + kk * 8, b + (((kk >> 2) * (RB * 128) + (kk & 3) * 32) >> 4), idesc, kk > 0);
+}
 // A in tensor memory [128 x 16 K], B rows along K.
 template <int K>
 __device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -705,7 +712,7 @@ __global__ void __launch_bounds__(128) window_join_kernel(const __grid_constant_
 // ---- backward -------------------------------------------------------------------
 // No atomics: a kernel forms, per packed row, -lse log2 e and -delta (delta =
 // sum_d dO o); then one grid holds two roles of the same shape. A CTA keeps 128
-// rows X1, X2 in shared memory and streams tiles of 64 rows Y1, Y2:
+// rows X1, X2 and streams tiles of 64 rows Y1, Y2:
 //   dq      X = Q, dO of 128 packed rows;  Y = K, V of the keys they see
 //             S = Q K^T, dP = dO V^T, dS = P (dP - delta);  dQ += dS K
 //   dk/dv   X = K, V of 128 key rows;  Y = Q, dO of the packed rows that see them
@@ -715,7 +722,11 @@ __global__ void __launch_bounds__(128) window_join_kernel(const __grid_constant_
 // warpgroups take the steps in turn: step i's scores sit in tensor-memory buffer
 // i & 1, its P and dS go back over them in bf16 as the next product's A operand,
 // and S, dP of step i + 1 are computed meanwhile. Tensor memory: 2 x (64 + 64)
-// columns of scores, then the accumulators.
+// columns of scores, then the accumulators. A product of 128 x 64 reads more
+// operand bytes from shared memory than it has cycles for (192 of 128 bytes a
+// cycle), so the dq role, whose accumulator leaves room, keeps X in tensor
+// memory: [1, 8208, 32 / 8 heads, 128] W 2048 took 793 us with X in shared memory
+// in both roles, 751 so.
 //
 // The first key tile holds the sinks: every later context query sees them, far
 // more than see any other tile. Tiles with sinks are split over their queries
@@ -731,9 +742,9 @@ struct BwdCfg {
   static constexpr uint32_t XB = kTM * D * 2, YB = kTN * D * 2;
   static constexpr uint32_t OX = 0, OY = 2 * XB, OROW = OY + NS * 2 * YB;  // rows: 64 x -lse2, 64 x -delta per stage
   static constexpr uint32_t OBAR = OROW + NS * kTN * 8;
-  static constexpr int NBAR = 3 * NS + 2 * NB + 3;  // full, empty, r_full; s_full, p_full, x_full, o_full, drain
+  static constexpr int NBAR = 3 * NS + 2 * NB + 4;  // full, empty, r_full; s_full, p_full, x_full, xt_full, o_full, drain
   static constexpr uint32_t OSLOT = OBAR + NBAR * 8, BYTES = OSLOT + 8;
-  static constexpr uint32_t COL_A = NB * 128, COL_B = COL_A + D;  // dQ or dV; dK
+  static constexpr uint32_t COL_A = NB * 128, COL_B = COL_A + D;  // dQ or dV; X = Q, dO or dK
   static constexpr uint32_t COLS = COL_B + D <= 256 ? 256 : 512;
 };
 
@@ -848,8 +859,9 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   uint64_t* s_full = r_full + C::NS;
   uint64_t* p_full = s_full + NB;
   uint64_t* x_full = p_full + NB;
-  uint64_t* o_full = x_full + 1;
-  uint64_t* drain = x_full + 2;
+  uint64_t* xt_full = x_full + 1;
+  uint64_t* o_full = x_full + 2;
+  uint64_t* drain = x_full + 3;
   const int warp = threadIdx.x >> 5, wg = threadIdx.x >> 7;
   const Seq sq = seq_of(A, b);
   // dq: head = virtual head (A.G query heads), its key head; dk/dv: head = key head
@@ -915,6 +927,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
       mbar_init(p_full + i, 128);
     }
     mbar_init(x_full, 1);
+    mbar_init(xt_full, NB * 128);
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
     fence_mbar_init();
@@ -951,7 +964,8 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
       const uint32_t x1 = desc_low(base + C::OX, 16), x2 = desc_low(base + C::OX + C::XB, 16);
       const uint32_t yk = desc_low(base + C::OY, 16), yn = desc_low(base + C::OY, kTN * 128);
       uint32_t slot_s = 0, ph_s = 0, slot_a = 0;  // ring slots of the next scores and of the next accumulation
-      bool ok = wait_alive(x_full, 0, dead, A.status);
+      bool ok = wait_alive(DKV ? x_full : xt_full, 0, dead, A.status);
+      tc_fence_after();
       auto scores = [&](int i) {  // S, dP of step i; its buffer's last P and dS were read by products issued before
         ok = wait_alive(full + slot_s, ph_s, dead, A.status);
         if (!ok) return;
@@ -959,8 +973,13 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
         // (failure-detection test hook: the first step's products are withheld)
         if (!(withhold && i == 0) && elect_one()) {
           const uint32_t y = yk + slot_s * (2 * C::YB >> 4), d = tmem + (i % NB) * 128;
-          issue_kk<D, kTM, kTN>(d, x1, y, kIdS);
-          issue_kk<D, kTM, kTN>(d + 64, x2, y + (C::YB >> 4), kIdS);
+          if (DKV) {
+            issue_kk<D, kTM, kTN>(d, x1, y, kIdS);
+            issue_kk<D, kTM, kTN>(d + 64, x2, y + (C::YB >> 4), kIdS);
+          } else {
+            issue_tk<D, kTN>(d, tmem + C::COL_B, y, kIdS);
+            issue_tk<D, kTN>(d + 64, tmem + C::COL_B + D / 2, y + (C::YB >> 4), kIdS);
+          }
           umma_commit(s_full + i % NB);
         }
         __syncwarp();
@@ -1100,8 +1119,30 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
     const bool in_block = key && (token >= sq.c || sq.c - token <= A.W || token < A.S);
     int rr = DKV ? (i0 + wg) % qt.per : 0;
     bool ok = true;
+    if (!DKV) {  // X to tensor memory, its half by each warpgroup
+      ok = __all_sync(kFullMask, wait_alive(x_full, 0, dead, A.status));
+#pragma unroll
+      for (int x = wg; x < 2; x += NB) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int ch = c * 4 + q;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[4 * q]), "=r"(w[4 * q + 1]), "=r"(w[4 * q + 2]), "=r"(w[4 * q + 3])
+                         : "r"(base + C::OX + x * C::XB + (uint32_t)(ch >> 3) * (kTM * 128u) + sw128((uint32_t)r, (uint32_t)(ch & 7)))
+                         : "memory");
+          }
+          tmem_st16(lane + C::COL_B + x * (D / 2) + c * 16, w);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      if (ok) mbar_arrive(xt_full);
+    }
     uint32_t k = 0, sl = wg % C::NS, rph = 0;
-    for (int i = wg; i < n; i += NB, ++k) {
+    for (int i = wg; i < n && ok; i += NB, ++k) {
       ok = __all_sync(kFullMask, wait_alive(s_full + wg, k & 1, dead, A.status));
       if (DKV) ok = ok && __all_sync(kFullMask, wait_alive(r_full + sl, rph, dead, A.status));
       if (!ok) break;
@@ -1291,7 +1332,13 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant_
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) d += __shfl_xor_sync(kFullMask, d, o);
   if (!on || c != 0) return;
-  const int h = (int)(i % A.Hq), t = (int)((i / A.Hq) % A.Tq), b = (int)(i / ((int64_t)A.Hq * A.Tq));
+  int h, t, b;
+  if ((int64_t)A.B * A.Tq * A.Hq <= UINT_MAX) {  // (64-bit divisions cost as much as the rest)
+    const uint32_t u = (uint32_t)i, v = u / (uint32_t)A.Hq;
+    h = (int)(u - v * A.Hq), b = (int)(v / (uint32_t)A.Tq), t = (int)(v - (uint32_t)b * A.Tq);
+  } else {
+    h = (int)(i % A.Hq), t = (int)((i / A.Hq) % A.Tq), b = (int)(i / ((int64_t)A.Hq * A.Tq));
+  }
   const int hv = h / A.G;
   const int64_t at = ((int64_t)b * A.Hk * A.nsub + hv) * A.M + (int64_t)t * A.G + (h - hv * A.G);
   const float lse = A.lse[at];
@@ -1412,13 +1459,25 @@ cudaError_t fwd_any(WindowArgs& A, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+// Steps of a dk/dv tile: the tiles of packed rows that see 128 keys.
+int64_t walk_steps(const WindowArgs& A) {
+  const int64_t walk = std::min<int64_t>(A.n_ctx, (int64_t)A.W + kTM);  // queries that see an ordinary tile
+  return (walk * A.G + kTN - 1) / kTN * A.nsub;
+}
+
 // Heads of 64: one score buffer and two CTAs per SM, or two buffers and one CTA.
-// Short walks want the second CTA (its set-up and end hide the first's), long
-// ones the overlap within a CTA; us with one / two: [32, 528, 4] W 128 73 / 91,
-// [8, 2048, 8] W 512 165 / 193, [4, 4096, 8] W 1024 221 / 244, [2, 8192, 8 / 2
-// heads] W 4096 550 / 483.
-bool bwd_one_buffer(const WindowArgs& A) {
-  return std::min<int64_t>(A.Tk, (int64_t)A.W + A.S) < 2048;
+// Two CTAs hide each other's set-up and end; two buffers make the single walk
+// faster, which counts where few long ones take all the time: from 32 steps on
+// with at most three dk/dv tiles per SM. us with one / two, (steps, tiles):
+// [32, 528, 4] W 128 (4, 640) 54 / 66, [2, 2048, 8] W 256 (6, 256) 32 / 37,
+// [5, 1228, 6 / 2 heads] W 200 (18, 100) 36.4 / 35.5, [8, 2048, 8] W 512 (10,
+// 1024) 135 / 158, [4, 4096, 8] W 2048 (34, 1024) 280 / 298; [1, 3000, 32 / 8]
+// W 512 (40, 192) 101 / 99, [1, 32768, 4 / 1] W 1024 (72, 256) 204 / 210,
+// [1, 8192, 16 / 2] W 512 (80, 128) 157 / 133, [1, 6000, 8] (94, 376) 204 / 185,
+// [1, 6000, 8 / 4] (188, 188) 255 / 176, [1, 16384, 8] (256, 1024) 1137 / 1144.
+bool bwd_one_buffer(const WindowArgs& A, int sms) {
+  const int64_t tiles = (int64_t)(A.Tq + kTM - 1) / kTM * A.B * A.Hk;
+  return walk_steps(A) < 32 || tiles > 3 * (int64_t)sms;
 }
 
 template <int D, int NB>
@@ -1432,7 +1491,7 @@ cudaError_t bwd_launch(const WindowArgs& A, unsigned grid, cudaStream_t st) {
 }
 
 template <int D>
-cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
+cudaError_t bwd_any(WindowArgs& A, int sms, cudaStream_t st) {
   cudaError_t e;
   A.rows_plane = (int64_t)A.B * A.Tq * A.Hq;
   const int64_t lanes = (int64_t)A.B * A.Tq * A.Hq * (D / 8);
@@ -1446,7 +1505,7 @@ cudaError_t bwd_any(WindowArgs& A, cudaStream_t st) {
   const int64_t grid = ((int64_t)A.sink_tiles * (A.sink_splits - 1) + nk + nq * A.nsub) * bk;
   bool one = false;
   if constexpr (D == 64) {
-    one = bwd_one_buffer(A);
+    one = bwd_one_buffer(A, sms);
     if (one) e = bwd_launch<D, 1>(A, (unsigned)grid, st);
   }
   if (!one) e = bwd_launch<D, 2>(A, (unsigned)grid, st);
@@ -1471,8 +1530,7 @@ void window_sink_shape(WindowArgs& A, int sms) {
   if (A.W >= A.n_ctx) A.S = 0;  // the window reaches every context token: no sink lies outside it
   const int tiles = (std::min(A.S, A.n_ctx) + kTM - 1) / kTM;
   if (tiles == 0 || tiles > 4) return;
-  const int64_t walk = std::min<int64_t>(A.n_ctx, (int64_t)A.W + kTM);  // queries that see an ordinary tile
-  const int64_t usual = (walk * A.G + kTN - 1) / kTN * A.nsub;
+  const int64_t usual = walk_steps(A);
   const int64_t longest = ((int64_t)A.n_ctx * A.G + kTN - 1) / kTN * A.nsub;
   const int64_t rows = (A.Tq + kTM - 1) / kTM;
   const int64_t all = 2 * rows * usual * A.B * A.Hk;  // steps: dk/dv, and dq's as many
@@ -1507,8 +1565,8 @@ cudaError_t window_fwd_launch(WindowArgs& A, int D, cudaStream_t st) {
   return D == 64 ? fwd_any<64>(A, st) : fwd_any<128>(A, st);
 }
 
-cudaError_t window_bwd_launch(WindowArgs& A, int D, cudaStream_t st) {
-  return D == 64 ? bwd_any<64>(A, st) : bwd_any<128>(A, st);
+cudaError_t window_bwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st) {
+  return D == 64 ? bwd_any<64>(A, sms, st) : bwd_any<128>(A, sms, st);
 }
 
 }  // namespace specdec

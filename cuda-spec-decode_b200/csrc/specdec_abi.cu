@@ -1268,7 +1268,7 @@ int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_stride
   A.ctx_lens = ctx_lens;
   A.status = status;
   A.withhold = take_withhold_stage();
-  const cudaError_t e = window_bwd_launch(A, head_dim, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = window_bwd_launch(A, head_dim, sms, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? ok() : cuda_fail(e, "window attention backward launch");
 }
 

@@ -255,7 +255,7 @@ size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at);
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms);
 size_t window_split_workspace(int D, int64_t rows, int splits, size_t* ml_at);
 cudaError_t window_fwd_launch(WindowArgs& A, int D, cudaStream_t st);
-cudaError_t window_bwd_launch(WindowArgs& A, int D, cudaStream_t st);
+cudaError_t window_bwd_launch(WindowArgs& A, int D, int sms, cudaStream_t st);
 
 // Sets the calling thread's specdec_last_error() text.
 void set_last_error(const char* msg);

@@ -82,10 +82,8 @@ __device__ __forceinline__ int low_of(const WindowArgs& A, const Seq& s, int p) 
 }
 __device__ __forceinline__ int high_of(const Seq& s, int p) { return p < s.c ? p + 1 : s.total; }  // -1 -> 0
 
-// m / G for m < 2^31 (G's reciprocal, rounded up, in 31 + ceil(log2 G) bits).
-__device__ __forceinline__ int group_div(const WindowArgs& A, int m) {
-  return (int)(((uint64_t)(uint32_t)m * A.gmul) >> A.gshift);
-}
+__device__ __forceinline__ int div(const Div& d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
+__device__ __forceinline__ int group_div(const WindowArgs& A, int m) { return div(A.by_g, m); }
 
 // First and last token of the packed rows [m0, m1]; false: padding only.
 __device__ __forceinline__ bool token_range(const WindowArgs& A, const Seq& s, int m0, int m1, int& p0, int& p1) {
@@ -294,7 +292,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
   const int warp = threadIdx.x >> 5;
   const bool service = threadIdx.x >= kTM;  // product and copying warps
   const int hv_n = A.Hk * A.nsub;  // virtual heads: A.G query heads of one key head
-  const int bh = blockIdx.x, b = bh / hv_n, hv = bh - b * hv_n, hk = hv / A.nsub;
+  const int bh = blockIdx.x, b = div(A.by_hv, bh), hv = bh - b * hv_n, hk = div(A.by_sub, hv);
   const int m0 = (int)(gridDim.y - 1 - blockIdx.y) * kTM;  // the last tiles see the most keys: first
   const Seq sq = seq_of(A, b);
 
@@ -305,7 +303,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
   if (some) {
     n = kt.n;
     if (SPLIT) {
-      const int per = (n + A.splits - 1) / A.splits;
+      const int per = div(A.by_split, n + A.splits - 1);
       i0 = min(n, (int)blockIdx.z * per);
       n = min(n, i0 + per) - i0;
     }
@@ -368,7 +366,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
       mbar_arrive_expect_tx(q_full, C::QB);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
-        tma_load_4d(base + C::OQ + c * (kTM * 128), &A.mq, c * 64, hv * A.G, m0 / A.G, b, q_full);
+        tma_load_4d(base + C::OQ + c * (kTM * 128), &A.mq, c * 64, hv * A.G, group_div(A, m0), b, q_full);
     }
     if (n > 0 && A.kv_maps && boxed<KN>(sq, kt.start(i0))) load_box(issued++);
   }
@@ -640,7 +638,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
       ml[r] = !ok_row ? make_float2(0.f, __int_as_float(0x7fc00000)) : make_float2(m_ref, p < 0 ? 0.f : l_run);
     }
     cluster_sync();
-    const int rows = min(kTM, A.M - m0), each = (rows + A.splits - 1) / A.splits;
+    const int rows = min(kTM, A.M - m0), each = div(A.by_split, rows + A.splits - 1);
     const int r0 = (int)blockIdx.z * each, r1 = min(rows, r0 + each);
     for (int i = threadIdx.x; i < (r1 - r0) * (D / 4); i += C::THREADS) {
       const int r = r0 + i / (D / 4), c = i % (D / 4) * 4;
@@ -865,7 +863,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   const int warp = threadIdx.x >> 5, wg = threadIdx.x >> 7;
   const Seq sq = seq_of(A, b);
   // dq: head = virtual head (A.G query heads), its key head; dk/dv: head = key head
-  const int hk = DKV ? head : head / A.nsub;
+  const int hk = DKV ? head : div(A.by_sub, head);
   const int x0 = tile * kTM;  // packed row (dq) or key row (dk/dv) of X's first row
 
   // steps [i0, i0 + n)
@@ -876,7 +874,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
   if (some) n = DKV ? qt.n : kt.n;
   const bool partial = DKV && A.sink_splits > 1 && tile < A.sink_tiles;
   if (partial) {
-    const int each = (n + A.sink_splits - 1) / A.sink_splits;
+    const int each = div(A.by_split, n + A.sink_splits - 1);
     i0 = min(n, split * each);
     n = min(n, i0 + each) - i0;
   }
@@ -945,7 +943,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
             if (DKV)
               tma_load_4d(dst, x ? &A.mv : &A.mk, c * 64, x0 + h * 64, hk, b, x_full);
             else
-              tma_load_4d(dst, x ? &A.mg : &A.mq, c * 64, q_head, (x0 + h * 64) / A.G, b, x_full);
+              tma_load_4d(dst, x ? &A.mg : &A.mq, c * 64, q_head, group_div(A, x0 + h * 64), b, x_full);
           }
     }
   }
@@ -1055,7 +1053,7 @@ __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int 
         const uint32_t y1 = base + C::OY + sl * 2 * C::YB, y2 = y1 + C::YB;
         if (DKV) {
           const int f = qt.first(A, rr), l = qt.last(A, rr);
-          const int t0 = f / A.G, t1 = t0 + kTN / A.G;
+          const int t0 = group_div(A, f), t1 = t0 + group_div(A, kTN);
           if (ok) {  // -lse2 and -delta of the rows (zeros behind the last)
             for (int e = lt; e < 2 * kTN; e += C::COPY) {
               const int m = f + (e & (kTN - 1));
@@ -1268,16 +1266,15 @@ __global__ void __launch_bounds__(BwdCfg<D, NB>::THREADS, BwdCfg<D, NB>::CTAS)
     window_bwd_kernel(const __grid_constant__ WindowArgs A) {
   const int nk = (A.Tq + kTM - 1) / kTM, nq = (A.M + kTM - 1) / kTM;
   const int sinks = A.sink_tiles * A.sink_splits, bk = A.B * A.Hk, bv = bk * A.nsub;
-  const int64_t dkv = (int64_t)(sinks + nk - A.sink_tiles) * bk;
-  const int64_t i = blockIdx.x;
+  const int dkv = (sinks + nk - A.sink_tiles) * bk, i = blockIdx.x;  // (the grid is below 2^31)
   if (i < dkv) {
-    const int job = (int)(i / bk), bh = (int)(i - (int64_t)job * bk), b = bh / A.Hk;
-    const int tile = job < sinks ? job / A.sink_splits : job - sinks + A.sink_tiles;
+    const int job = div(A.by_bk, i), bh = i - job * bk, b = div(A.by_hk, bh);
+    const int tile = job < sinks ? div(A.by_split, job) : job - sinks + A.sink_tiles;
     const int split = job < sinks ? job - tile * A.sink_splits : 0;
     window_bwd_role<D, NB, true>(A, b, bh - b * A.Hk, tile, split, A.withhold && i == 0);
   } else {
-    const int64_t q = i - dkv;
-    const int tile = nq - 1 - (int)(q / bv), bh = (int)(q % bv), hv = A.Hk * A.nsub, b = bh / hv;
+    const int q = i - dkv, back = div(A.by_bv, q), tile = nq - 1 - back, bh = q - back * bv;
+    const int hv = A.Hk * A.nsub, b = div(A.by_hv, bh);
     window_bwd_role<D, NB, false>(A, b, bh - b * hv, tile, 0, A.withhold && q == 0);
   }
 }
@@ -1426,6 +1423,9 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(window_fwd_kernel<D, SPLIT>, C::BYTES, done);
   if (e != cudaSuccess) return e;
+  A.by_hv = make_div(A.Hk * A.nsub);
+  A.by_sub = make_div(A.nsub);
+  A.by_split = make_div(A.splits);
   kv_maps(A, D, kTN);
   sink_maps(A, D, kTN);
   A.q_maps = group_map(&A.mq, A, A.q, A.qs, D, kTM);
@@ -1502,6 +1502,12 @@ cudaError_t bwd_any(WindowArgs& A, int sms, cudaStream_t st) {
              group_map(&A.mg, A, A.dO, {(int64_t)A.Tq * A.Hq * D, (int64_t)A.Hq * D, D}, D, kTN);
   const int64_t nk = (A.Tq + kTM - 1) / kTM, nq = (A.M + kTM - 1) / kTM;
   const int64_t bk = (int64_t)A.B * A.Hk;
+  A.by_hk = make_div(A.Hk);
+  A.by_sub = make_div(A.nsub);
+  A.by_hv = make_div(A.Hk * A.nsub);
+  A.by_bk = make_div(bk);
+  A.by_bv = make_div(bk * A.nsub);
+  A.by_split = make_div(A.sink_splits);
   const int64_t grid = ((int64_t)A.sink_tiles * (A.sink_splits - 1) + nk + nq * A.nsub) * bk;
   bool one = false;
   if constexpr (D == 64) {

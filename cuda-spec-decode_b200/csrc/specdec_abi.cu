@@ -1138,10 +1138,7 @@ int window_args(WindowArgs& A, int32_t batch, int32_t Tq, int32_t Tk, int32_t q_
   A.G = (int)G;
   A.nsub = (int)nsub;
   A.M = (int)M;
-  int l = 0;
-  while ((int64_t(1) << l) < G) ++l;
-  A.gshift = 31 + l;
-  A.gmul = (uint32_t)(((uint64_t(1) << (31 + l)) + G - 1) / G);
+  A.by_g = make_div(G);
   A.n_block = n_block;
   A.W = std::min(window, 1 << 30);
   A.S = sinks;

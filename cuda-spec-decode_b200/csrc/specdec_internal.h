@@ -220,6 +220,19 @@ cudaError_t dflash_attn_bwd_launch(const void* q, const void* k, const void* v, 
                                    int n_ctx, float scale, int* status, int withhold, cudaStream_t st);
 
 // Sliding-window attention with sinks (drafter_window.cu).
+// Division by a number known before the launch, for 0 <= n < 2^31: its
+// reciprocal, rounded up, in 31 + ceil(log2 d) bits. (A division by a variable
+// is some forty dependent instructions; a CTA's place in the grid takes several.)
+struct Div {
+  uint32_t mul;
+  int shift;
+};
+inline Div make_div(int64_t d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return {(uint32_t)(((uint64_t(1) << (31 + l)) + d - 1) / d), 31 + l};
+}
+
 struct WindowArgs {
   const bf16_t *q, *k, *v;         // [B, Tq | Tk, heads, D], strided
   int64_t qs[3], ks[3], vs[3];     // batch, token, head stride in elements
@@ -229,8 +242,8 @@ struct WindowArgs {
   const int* ctx_lens;             // [B], or null (training: every context is n_ctx long)
   int B, Tq, Tk, Hq, Hk;
   int G, nsub, M;                  // Hq = Hk * nsub * G; M = Tq * G packed rows per virtual head
-  uint32_t gmul;                   // m / G = (m * gmul) >> gshift
-  int gshift;
+  Div by_g, by_hv, by_sub, by_split;  // G, Hk * nsub, nsub, splits (of the keys, or of sink tiles)
+  Div by_bk, by_bv, by_hk;            // backward's grid: B * Hk, B * Hk * nsub, Hk
   int cached;                      // 1: keys are a cache of Tk rows, the queries its last tokens
   int n_ctx, n_block, W, S;        // W <= 2^30
   float scale, scale_log2;

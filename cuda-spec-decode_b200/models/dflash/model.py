@@ -361,7 +361,9 @@ class DFlashSpeculator(nn.Module):
         With a cache (``new_cache``), target_features are only the features that
         follow those already in it -- the tokens accepted since the last draft --
         and ctx_lens int [batch] says how many of them each sequence has: its
-        last ctx_lens[b] rows (None: all). Their keys and values join the cache."""
+        last ctx_lens[b] rows (None: all). Their keys and values join the cache.
+        Without room for them ValueError; in a replayed graph, where the host does
+        not look, the sequence keeps what it has and its logits are NaN."""
         if cache is None:
             logits = self.forward(target_features, ctx_lens)
             return logits.argmax(dim=-1), logits
@@ -374,10 +376,12 @@ class DFlashSpeculator(nn.Module):
         lens = cache.lens + new
         i = torch.arange(n_new + self.block_size, device=cache.lens.device)
         positions = lens.long()[:, None] + i - n_new
-        rows = torch.where(i >= n_new - new[:, None], positions, cache.size)
+        # a captured draft is replayed without the host's check: what has no room goes to the last row
+        fits = lens + self.block_size <= cache.size
+        rows = torch.where((i >= n_new - new[:, None]) & fits[:, None], positions, cache.size)
         h = self._embed(target_features)
         for layer, k, v in zip(self.layers, cache.k, cache.v):
             h = layer.forward_cached(h, k, v, positions, rows, lens, self.block_size)
-        cache.lens.add_(new)
-        logits = self._block_logits(h)
+        cache.lens.copy_(torch.where(fits, lens, cache.lens))
+        logits = self._block_logits(torch.where(fits[:, None, None], h, float("nan")))
         return logits.argmax(dim=-1), logits

@@ -139,6 +139,26 @@ def test_cache_is_refused_when_full_or_for_another_batch():
     assert isinstance(cache, DraftCache) and cache.lens.tolist() == [5, 6]
 
 
+def test_a_draft_that_does_not_fit_gives_nan_and_leaves_the_cache():
+    """Replays of a captured draft pass by the host's check: a sequence without
+    room keeps its tokens and gets NaN, the others go on."""
+    m = _model(dict(rotary={}, window=6, sinks=1))
+    cache = m.new_cache(2, 12, dtype=torch.float32)
+    x = torch.randn(2, 20, 48)
+    m.draft(x[:, :7], ctx_lens=torch.tensor([2, 7]), cache=cache)
+    kept = [t[1, :7].clone() for t in cache.k + cache.v]
+    cache.longest = 0  # as if the host had not seen the steps before
+    new = torch.stack([x[0, 2:5], x[1, 7:10]])
+    tok, logits = m.draft(new, cache=cache)
+    assert cache.lens.tolist() == [5, 7] and bool(torch.isnan(logits[1]).all())
+    want = m.draft(torch.cat([x[:1, 5:7], x[:1, 2:5]], 1))[1]  # the last two rows, then three more
+    assert float((logits[0] - want[0]).abs().max()) < 1e-5
+    for a, t in zip(kept, cache.k + cache.v):
+        assert torch.equal(a, t[1, :7])
+    again = m.draft(x[:, :0], cache=cache)[1]
+    assert float((again[1] - m.draft(x[1:, :7])[1][0]).abs().max()) < 1e-5
+
+
 def test_option_refusals():
     for bad in (dict(num_kv_heads=3), dict(num_kv_heads=0), dict(window=0), dict(sinks=-1), dict(rotary=dict(dim=18))):
         with pytest.raises(AssertionError):
@@ -342,3 +362,6 @@ def test_captured_draft_from_the_cache(cuda):
                 want = m.draft(x[:, at:at + 3], cache=ref)[1]
                 assert torch.equal(out, want)
     assert cache.lens.tolist() == ref.lens.tolist() == [49, 49]
+    for _ in range(20):  # room for 11 more: the last replays give NaN and write nothing
+        g.replay()
+    assert cache.lens.tolist() == [82, 82] and bool(torch.isnan(out).all())

@@ -202,6 +202,16 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 //   softmax   S(i) from tensor memory, P(i) in bf16 back over S(i)'s columns (the
 //             A operand of the next product is read from tensor memory), O
 //             rescaled there when the reference maximum rises
+// Two buffers of scores took [2, 4096, 16 heads, 128] W 1024 from 108 to 87 us
+// (83 with masks as bit words and the later boxes requested after the CTA has
+// met), [1, 8208, 32 / 8, 128] W 2048 to 235 us (1.03 PFLOP/s of the visible
+// pairs), one token of 16 sequences over 24576 cached rows from 249 to 220-228 us
+// (7 TB/s of them), the drafter's [32, 528, 4, 64] W 128 from 30 to 25 us. What
+// bounds it with heads of 128 is the operands' way from shared memory (S reads Q
+// and K, 192 bytes a cycle of 128); with short walks a CTA's set-up and end
+// (a third of 17 thousand cycles). Slower at every size were two query tiles per
+// CTA (268 us for the second), two softmax warpgroups in turn (89 for the first),
+// a part of the exponentials as polynomials (1 to 6% behind).
 // Every wait is bounded and watches a shared flag that the first expired wait
 // raises; all warps then leave for the common end.
 // How the parts of a row's keys come together: one part; unnormalised fp32 rows
@@ -1552,12 +1562,23 @@ size_t window_bwd_workspace(const WindowArgs& A, int D, size_t* sink_at) {
          (A.sink_splits > 1 ? (size_t)A.B * A.Hk * A.sink_tiles * A.sink_splits * 2 * kTM * D * sizeof(float) : 0);
 }
 
-// Splits of the keys: enough CTAs to fill the device, at least two key tiles
-// each, from the most keys a query tile can see.
+// Splits of the keys, from the most keys a query tile can see: up to a cluster's
+// eight while the device has room for their CTAs; more, joined through memory by
+// a second kernel, where there is room for sixteen and eight would walk more than
+// 16 tiles each. One token, us with 1 / 2 / 4 / 8 in a cluster | 8 / 16 / 37 in memory:
+//   4 heads of 64, 512 keys 9.4 / 7.3 / 5.9 / 5.2 | 7.9; 2048 25 / 15 / 10 / 7.4 |
+//   10.0 / 10.1; 4096 47 / 26 / 16 / 10.0 | 12.6 / 11.5 / 13.4; 16384 174 / 91 / 48 /
+//   27 | 30 / 20.5 / 18.2
+//   8 heads of 128, 4096 keys 52 / 29 / 18 / 11.8 | 15 / 15 / 21; 8192 99 / 52 / 29 /
+//   17.7 | 21 / 18.1 / 24; 32768 383 / 193 / 101 / 54 | 58 / 38 / 39
+// and with no room for the CTAs, 128 tiles of 128 rows: 2048 keys 32 / 26 / 31 / 41.
 int window_splits(int D, int64_t ctas, int64_t most_keys, int sms) {
   const int64_t tiles = (most_keys + kTN - 1) / kTN + 1;
-  const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64>::CTAS : FwdCfg<128>::CTAS);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(room / std::max<int64_t>(1, ctas), tiles / 2));
+  const int64_t room = (int64_t)sms * (D == 64 ? FwdCfg<64>::CTAS : FwdCfg<128>::CTAS) / std::max<int64_t>(1, ctas);
+  const int64_t splits = room >= 2 * kClusterMost && tiles > 16 * kClusterMost
+                             ? std::min(room, tiles / kClusterMost)
+                             : std::min({room, tiles, (int64_t)kClusterMost});
+  return (int)std::max<int64_t>(1, splits);
 }
 
 size_t window_split_workspace(int D, int64_t rows, int splits, size_t* ml_at) {

@@ -420,10 +420,11 @@ def test_an_expired_wait_of_the_backward_gives_nan_rows_and_a_report(cuda, T, n_
 
 
 @pytest.mark.gpu
-def test_an_expired_wait_of_the_cached_form_reaches_the_joined_rows(cuda):
-    q, k, v = _rand(2, 5, 4, 64, seed=1), _rand(2, 900, 2, 64, seed=2), _rand(2, 900, 2, 64, seed=3)
-    lens = torch.tensor([880, 500], device="cuda", dtype=torch.int32)
-    run = lambda: drafter.window_attention_cached(q, k, v, lens, n_block=4, window=700, sinks=2)  # noqa: E731
+@pytest.mark.parametrize("size,c,W", [(900, 880, 700), (9500, 9400, 9300)])  # joined in a cluster, in the workspace
+def test_an_expired_wait_of_the_cached_form_reaches_the_joined_rows(cuda, size, c, W):
+    q, k, v = _rand(2, 5, 4, 64, seed=1), _rand(2, size, 2, 64, seed=2), _rand(2, size, 2, 64, seed=3)
+    lens = torch.tensor([c, 500], device="cuda", dtype=torch.int32)
+    run = lambda: drafter.window_attention_cached(q, k, v, lens, n_block=4, window=W, sinks=2)  # noqa: E731
     want = run()
     got = _withheld(run)
     _reported()
@@ -476,9 +477,11 @@ def test_expanded_inputs_equal_their_copies(cuda, B, n_ctx, nb, H, D, W, S, lens
 
 UNSEEN = [  # B, Tq, nb, Hq, Hk, D, size, W, S, lens; splits of the keys
     (2, 1, 0, 4, 2, 64, 900, 300, 4, (900, 640)),        # in a cluster
-    (1, 3, 3, 8, 1, 128, 4000, 3000, 70, (3990,)),       # in the workspace
+    (1, 3, 3, 8, 1, 128, 9500, 9000, 70, (9490,)),       # in the workspace
+    (2, 1, 0, 4, 2, 64, 9000, None, 0, (9000, 100)),     # the same, most of the second's splits empty
     (40, 2, 0, 16, 16, 64, 500, 100, 33, None),          # none
     (1, 40, 3, 4, 2, 64, 2000, None, 0, (20,)),          # more queries than tokens, empty splits
+    (1, 40, 3, 4, 2, 64, 9000, None, 0, (20,)),
     (3, 9, 5, 6, 2, 128, 600, 50, 130, (590, 300, 20)),  # groups of three: no map for the queries
 ]
 

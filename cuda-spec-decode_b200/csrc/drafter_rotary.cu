@@ -32,13 +32,12 @@
 // bitwise repeatable.
 //
 // Measured: rotation of [2, 8191, 16, 128] fp32, interleaved, 46 us (5.9 TB/s);
-// norm and rotation of [1, 32768, 32 + 8, 128] bf16, 122 us (5.5 TB/s) forward,
-// 217 us (4.6 TB/s) backward: there the issue slots (65% and 56% busy) and the
-// wait for shared memory and shuffles bound it as much as HBM does. 16-byte
-// loads of tables and weights in planes without bank conflicts took 8% off
-// (138 and 235 us before). A ring of rows filled with asynchronous copies was
-// slower (179 and 283 us): it spends more instructions. One token of 32
-// sequences takes 3.6 us, the time of a launch and one chain of loads.
+// norm and rotation of [1, 32768, 32 + 8, 128] bf16, 114 us (5.9 TB/s) forward,
+// 199 us (5.1 TB/s) backward, bound by issue slots and the wait for shared memory
+// and shuffles as much as by HBM. 16-byte loads of tables and weights in planes
+// without bank conflicts took 8% off. A ring of rows filled with asynchronous
+// copies was a quarter slower: it spends more instructions. One token of 32
+// sequences takes 3.5 us, the time of a launch and one chain of loads.
 #include <algorithm>
 
 #include "specdec_common.cuh"
@@ -570,14 +569,20 @@ bool vec_ok(const RotaryArgs& A, bool bwd) {
   return true;
 }
 
-// Lanes per head, heads per unit, CTAs per tensor (at most `most` in all).
-void shape_launch(RotaryArgs& A, bool vec, int sms, int most) {
+// Lanes per head, heads per unit, CTAs per tensor (`most` in all, where more
+// than `limit` would be wanted). A unit costs its groups of heads and about two
+// groups' worth of table, place and first loads; split by the heads alone, the
+// tensor with fewer heads finished last: us of the backward of [1, 32768, 32 + 8,
+// 128] bf16 239 by heads, 199 so ([2, 8191, 12 + 1, 128]: 104, 71; the forwards 127,
+// 114 and 40, 35). Few tokens spread a token's heads over several warps: 3.5 us
+// against 6.6 for one token of 32 sequences with 32 + 8 heads.
+void shape_launch(RotaryArgs& A, bool vec, int sms, int most, int limit) {
   const int es = A.dtype == kDtypeBF16 ? 2 : 4;
   const int slots = vec ? A.D / (2 * (16 / es)) : 32;
   A.lg = 0;
   while ((1 << A.lg) < slots) ++A.lg;
   const int hpw = 32 >> A.lg;
-  int64_t want[2] = {0, 0};
+  int64_t want[2] = {0, 0}, cost[2] = {0, 0};
   for (int s = 0; s < 2; ++s) {
     const int H = A.heads[s];
     A.nchunk[s] = A.hchunk[s] = 1;
@@ -592,10 +597,10 @@ void shape_launch(RotaryArgs& A, bool vec, int sms, int most) {
       A.nchunk[s] = (H + A.hchunk[s] - 1) / A.hchunk[s];
     }
     want[s] = (tiles * A.nchunk[s] + kRotWarps - 1) / kRotWarps;
+    cost[s] = tiles * ((H + hpw - 1) / hpw + 2);
   }
-  // over the limit: each tensor by its share of the heads
-  const int64_t k = want[1] ? std::max<int64_t>(1, (int64_t)most * A.heads[1] / A.H) : 0;
-  const bool over = want[0] + want[1] > most;
+  const int64_t k = want[1] ? std::max<int64_t>(1, (most * cost[1] + (cost[0] + cost[1]) / 2) / (cost[0] + cost[1])) : 0;
+  const bool over = want[0] + want[1] > limit;
   A.ctas[0] = (int)(over ? std::min<int64_t>(want[0], std::max<int64_t>(1, most - k)) : want[0]);
   A.ctas[1] = (int)(over ? std::min<int64_t>(want[1], k) : want[1]);
 }
@@ -644,7 +649,7 @@ void dispatch_bwd(const RotaryArgs& A, bool vec, float* part, cudaStream_t st) {
 
 cudaError_t rotary_fwd_launch(RotaryArgs A, bool norm, int sms, cudaStream_t st) {
   const bool vec = vec_ok(A, false);
-  shape_launch(A, vec, sms, 8 * sms);
+  shape_launch(A, vec, sms, 8 * sms, 8 * sms);
   if (A.dtype == kDtypeBF16)
     norm ? dispatch_fwd<bf16_t, true>(A, vec, st) : dispatch_fwd<bf16_t, false>(A, vec, st);
   else
@@ -652,12 +657,16 @@ cudaError_t rotary_fwd_launch(RotaryArgs A, bool norm, int sms, cudaStream_t st)
   return cudaGetLastError();
 }
 
-// Partial weight-gradient rows: one per CTA of the backward.
+// Partial weight-gradient rows: one per CTA of the backward, at most. Two CTAs per
+// SM are resident; where there is a unit for each warp of four, four run (the
+// second two as the first end), else two, which reduce and begin once: [32, 528,
+// 4 + 4, 64] bf16 27.6 us with two, 32 with four, 42 with eight; [4, 512, 32 + 8,
+// 128] fp32, a unit per warp, 38 and 33.
 int qk_norm_bwd_ctas(int sms) { return 4 * sms; }
 
 cudaError_t qk_norm_bwd_launch(RotaryArgs A, float* part, float* dwq, float* dwk, int sms, cudaStream_t st) {
   const bool vec = vec_ok(A, true);
-  shape_launch(A, vec, sms, qk_norm_bwd_ctas(sms));
+  shape_launch(A, vec, sms, 2 * sms, qk_norm_bwd_ctas(sms));
   if (A.dtype == kDtypeBF16)
     dispatch_bwd<bf16_t>(A, vec, part, st);
   else

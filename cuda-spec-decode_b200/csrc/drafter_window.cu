@@ -1539,7 +1539,11 @@ cudaError_t bwd_any(WindowArgs& A, int sms, cudaStream_t st) {
 // How the backward splits the key tiles that hold sinks (see above): into parts
 // no longer than an ordinary tile's walk or half of what an SM has to do in
 // all, whichever is more. More than four such tiles (512 sinks) are many
-// tiles, not a few long ones: no split.
+// tiles, not a few long ones: no split. us of the backward without / with it, S 4:
+// [5, 1228, 6 / 2 heads, 64] W 200 88 / 38, [1, 8192, 16 / 2, 64] W 512 770 / 133,
+// [1, 8208, 32 / 8, 128] W 512 474 / 328, W 2048 747 / 752, [1, 2048, 8 / 2, 128] W 128
+// 119 / 28, [16, 2048, 8, 128] W 128 274 / 273; shorter parts (an eighth of an SM's
+// steps): 38, 133, 334, 752, 28, 310.
 void window_sink_shape(WindowArgs& A, int sms) {
   A.sink_tiles = 0;
   A.sink_splits = 1;

@@ -998,7 +998,6 @@ int rotary_args(RotaryArgs& A, const int64_t* positions, int64_t pos_stride, con
   A.dtype = dtype;
   A.heads[0] = q_heads;
   A.heads[1] = k_heads;
-  A.H = q_heads + k_heads;
   A.scale = A.sin_scale = scale;
   A.eps = eps;
   if (A.N == 0) return ok();

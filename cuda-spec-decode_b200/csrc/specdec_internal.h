@@ -200,7 +200,7 @@ struct RotaryArgs {
   const double* inv_freq;          // [R / 2]
   int64_t N;                       // batch * T
   int T, D, R, interleaved, dtype;
-  int heads[2], H;                 // H = heads[0] + heads[1]
+  int heads[2];
   float scale, sin_scale, eps;     // sin_scale = -scale turns the other way
   // set by the launch
   int lg;                          // log2 lanes per head

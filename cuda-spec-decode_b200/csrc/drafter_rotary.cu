@@ -261,10 +261,9 @@ __device__ __forceinline__ Unit unit_of(const RotaryArgs& A, const Place& p, uin
     r.h = p.group - r.tok * p.H;
     r.hend = r.tok < p.tw && (int64_t)r.n0 + r.tok < A.N ? r.h + 1 : 0;
   }
-  const uint32_t n = (uint32_t)(r.n0 + r.tok);  // N fits in int32
-  const uint32_t b = n / (uint32_t)A.T;
-  r.b = b;
-  r.t = n - b * (uint32_t)A.T;
+  const int n = r.n0 + r.tok;  // (below 2^31: N is below 2^31 - 64)
+  r.b = div(A.by_t, n);
+  r.t = n - r.b * A.T;
   return r;
 }
 
@@ -274,9 +273,9 @@ __device__ __forceinline__ void build_table(const RotaryArgs& A, const Place& p,
   const int half = A.R / 2, toks = min(p.tw, (int)A.N - n0);
   __syncwarp();  // the previous unit's table has been read
   for (int i = threadIdx.x & 31; i < toks * half; i += 32) {
-    const int tok = p.tw == 1 ? 0 : i / half, f = i - tok * half;
-    const uint32_t n = (uint32_t)(n0 + tok), b = n / (uint32_t)A.T, t = n - b * (uint32_t)A.T;
-    const double turns = (double)A.positions[(int64_t)b * A.pos_stride + t] * A.inv_freq[f] * 0.15915494309189533577;
+    const int tok = p.tw == 1 ? 0 : div(A.by_half, i), f = i - tok * half;
+    const int n = n0 + tok, b = div(A.by_t, n), t = n - b * A.T;
+    const double turns = (double)A.positions[b * A.pos_stride + t] * A.inv_freq[f] * 0.15915494309189533577;
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     const int at = tok * half + plane_at<V>(f, half);
@@ -361,7 +360,7 @@ __global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 2) rotary_fwd_kernel(
         ss = head_sum(sq.x + sq.y, A.lg);
       }
       if (on) {
-        const float r = NORM ? rsqrtf(ss / (float)A.D + A.eps) : 1.f;
+        const float r = NORM ? rsqrtf(ss * A.inv_d + A.eps) : 1.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
@@ -477,8 +476,8 @@ __global__ void __launch_bounds__(kRotThreads) qk_norm_bwd_kernel(const __grid_c
       }
       const float ss = head_sum(sq.x + sq.y, A.lg), dot = head_sum(gx.x + gx.y, A.lg);
       if (on) {
-        const float r = rsqrtf(ss / (float)A.D + A.eps);
-        const float m = r * r * r * dot / (float)A.D;
+        const float r = rsqrtf(ss * A.inv_d + A.eps);
+        const float m = r * r * r * dot * A.inv_d;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k]) continue;
@@ -581,6 +580,8 @@ void shape_launch(RotaryArgs& A, bool vec, int sms, int most, int limit) {
   const int slots = vec ? A.D / (2 * (16 / es)) : 32;
   A.lg = 0;
   while ((1 << A.lg) < slots) ++A.lg;
+  A.by_t = make_div(A.T);
+  A.by_half = make_div(A.R / 2);
   const int hpw = 32 >> A.lg;
   int64_t want[2] = {0, 0}, cost[2] = {0, 0};
   for (int s = 0; s < 2; ++s) {

@@ -82,7 +82,6 @@ __device__ __forceinline__ int low_of(const WindowArgs& A, const Seq& s, int p) 
 }
 __device__ __forceinline__ int high_of(const Seq& s, int p) { return p < s.c ? p + 1 : s.total; }  // -1 -> 0
 
-__device__ __forceinline__ int div(const Div& d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
 __device__ __forceinline__ int group_div(const WindowArgs& A, int m) { return div(A.by_g, m); }
 
 // First and last token of the packed rows [m0, m1]; false: padding only.

@@ -1000,6 +1000,7 @@ int rotary_args(RotaryArgs& A, const int64_t* positions, int64_t pos_stride, con
   A.heads[1] = k_heads;
   A.scale = A.sin_scale = scale;
   A.eps = eps;
+  A.inv_d = 1.f / (float)D;
   if (A.N == 0) return ok();
   if (!positions || !inv_freq) return fail(SPECDEC_ERR_ARGUMENT, "null positions or inv_freq");
   const int dev = current_device();

@@ -192,6 +192,22 @@ struct RotaryTensor {
   int64_t s[3] = {0, 0, 0};        // batch, token, head stride in elements
 };
 
+// Division by a number known before the launch, for 0 <= n < 2^31: its
+// reciprocal, rounded up, in 31 + ceil(log2 d) bits. (A division by a variable
+// is some forty dependent instructions; a CTA's place in the grid takes several.)
+struct Div {
+  uint32_t mul;
+  int shift;
+};
+#ifdef __CUDACC__
+__device__ __forceinline__ int div(const Div& d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
+#endif
+inline Div make_div(int64_t d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return {(uint32_t)(((uint64_t(1) << (31 + l)) + d - 1) / d), 31 + l};
+}
+
 struct RotaryArgs {
   RotaryTensor x[2], dy[2], y[2];  // inputs, output gradients (backward), outputs (y or dx)
   const float* w[2] = {nullptr, nullptr};  // [D] norm weights
@@ -201,10 +217,11 @@ struct RotaryArgs {
   int64_t N;                       // batch * T
   int T, D, R, interleaved, dtype;
   int heads[2];
-  float scale, sin_scale, eps;     // sin_scale = -scale turns the other way
+  float scale, sin_scale, eps, inv_d;  // sin_scale = -scale turns the other way; inv_d = 1 / D
   // set by the launch
   int lg;                          // log2 lanes per head
   int ctas[2], nchunk[2], hchunk[2];  // per tensor: CTAs, units per token, heads per unit
+  Div by_t, by_half;               // T, R / 2
 };
 cudaError_t rotary_fwd_launch(RotaryArgs A, bool norm, int sms, cudaStream_t st);
 int qk_norm_bwd_ctas(int sms);
@@ -220,19 +237,6 @@ cudaError_t dflash_attn_bwd_launch(const void* q, const void* k, const void* v, 
                                    int n_ctx, float scale, int* status, int withhold, cudaStream_t st);
 
 // Sliding-window attention with sinks (drafter_window.cu).
-// Division by a number known before the launch, for 0 <= n < 2^31: its
-// reciprocal, rounded up, in 31 + ceil(log2 d) bits. (A division by a variable
-// is some forty dependent instructions; a CTA's place in the grid takes several.)
-struct Div {
-  uint32_t mul;
-  int shift;
-};
-inline Div make_div(int64_t d) {
-  int l = 0;
-  while ((int64_t(1) << l) < d) ++l;
-  return {(uint32_t)(((uint64_t(1) << (31 + l)) + d - 1) / d), 31 + l};
-}
-
 struct WindowArgs {
   const bf16_t *q, *k, *v;         // [B, Tq | Tk, heads, D], strided
   int64_t qs[3], ks[3], vs[3];     // batch, token, head stride in elements

@@ -229,7 +229,14 @@ struct FwdCfg {
   // against bank conflicts), then their (maximum, sum)
   static constexpr uint32_t LD = D + 4, OML = kTM * LD * 4;
   static_assert(OML + kTM * 8 <= OBAR, "they fit");
+  // A cluster's CTAs wait for one another while they hold tensor memory, so none
+  // of them may have to wait for tensor memory that another cluster's CTA holds:
+  // two fit an SM (256 of 512 columns each), and a request of more than a third
+  // of an SM's 228 KB (1 KB per block is the system's) keeps it at two.
+  static constexpr uint32_t CLUSTER_BYTES = BYTES > 77 * 1024 ? BYTES : 77 * 1024;
+  static_assert(3 * (CLUSTER_BYTES + 1024) > 228 * 1024, "two clusters' CTAs per SM at most");
   static constexpr uint32_t COLS = 256, COL_O = 2 * kTN;  // O behind two buffers of scores
+  static_assert(COL_O + D <= COLS, "tensor memory");
 };
 
 // Waits for the barrier's phase; false once `dead` is set or the limit expired
@@ -1430,7 +1437,8 @@ template <int D, int SPLIT>
 cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   using C = FwdCfg<D>;
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = allow_smem(window_fwd_kernel<D, SPLIT>, C::BYTES, done);
+  constexpr uint32_t bytes = SPLIT == kSplitCluster ? C::CLUSTER_BYTES : C::BYTES;
+  const cudaError_t e = allow_smem(window_fwd_kernel<D, SPLIT>, bytes, done);
   if (e != cudaSuccess) return e;
   A.by_hv = make_div(A.Hk * A.nsub);
   A.by_sub = make_div(A.nsub);
@@ -1446,13 +1454,13 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::BYTES;
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, window_fwd_kernel<D, SPLIT>, (const WindowArgs&)A);
   } else {
-    window_fwd_kernel<D, SPLIT><<<grid, C::THREADS, C::BYTES, st>>>(A);
+    window_fwd_kernel<D, SPLIT><<<grid, C::THREADS, bytes, st>>>(A);
     return cudaGetLastError();
   }
 }

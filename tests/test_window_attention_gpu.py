@@ -507,3 +507,24 @@ def test_cache_rows_that_no_query_sees_may_hold_anything(cuda, B, Tq, nb, Hq, Hk
     a, b = (drafter.window_attention_cached(q, x, y, ctx, n_block=nb, window=W, sinks=S)
             for x, y in ((k1, v1), (k1.contiguous(), v1.contiguous())))
     assert bool(torch.isfinite(a.float()).all()) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_cached_calls_on_several_streams(cuda):
+    """More CTAs of clusters at once than the device holds."""
+    calls = []
+    for i, (B, Hq, Hk, D, size) in enumerate([(8, 4, 4, 64, 700), (4, 8, 8, 64, 1500), (4, 16, 8, 128, 900), (2, 4, 4, 64, 600)]):
+        q, k, v = _rand(B, 1, Hq, D, seed=i), _rand(B, size, Hk, D, seed=i + 10), _rand(B, size, Hk, D, seed=i + 20)
+        lens = torch.full((B,), size, device="cuda", dtype=torch.int32)
+        calls.append(lambda q=q, k=k, v=v, lens=lens: drafter.window_attention_cached(q, k, v, lens, window=600, sinks=4))
+    want = [f() for f in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[] for _ in calls]
+    for _ in range(30):
+        for i, (f, st) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(f())
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)

@@ -32,8 +32,8 @@
 // bitwise repeatable.
 //
 // Measured: rotation of [2, 8191, 16, 128] fp32, interleaved, 46 us (5.9 TB/s);
-// norm and rotation of [1, 32768, 32 + 8, 128] bf16, 114 us (5.9 TB/s) forward,
-// 199 us (5.1 TB/s) backward, bound by issue slots and the wait for shared memory
+// norm and rotation of [1, 32768, 32 + 8, 128] bf16, 111 us (6.0 TB/s) forward,
+// 191 us (5.3 TB/s) backward, bound by issue slots and the wait for shared memory
 // and shuffles as much as by HBM. 16-byte loads of tables and weights in planes
 // without bank conflicts took 8% off. A ring of rows filled with asynchronous
 // copies was a quarter slower: it spends more instructions. One token of 32

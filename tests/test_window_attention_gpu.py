@@ -528,3 +528,27 @@ def test_cached_calls_on_several_streams(cuda):
     torch.cuda.synchronize()
     for w, outs in zip(want, got):
         assert all(torch.equal(w, o) for o in outs)
+
+
+@pytest.mark.gpu
+def test_a_training_batch_past_32_bit_offsets(cuda):
+    """Queries of 2.16e9 elements; the last tokens of the last sequence lie past
+    2^31 of them and see only one another (window 64)."""
+    B, T, Hq, Hk, D, W, n = 2, 66_000, 128, 2, 128, 64, 200
+    q = torch.zeros(B, T, Hq, D, device="cuda", dtype=torch.bfloat16)
+    k, v = (torch.zeros(B, T, Hk, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    assert q.numel() > 2 ** 31
+    do = torch.zeros_like(q)
+    m = n + W
+    for i, t in enumerate((q, k, v, do)):
+        t[1, T - m:] = _rand(m, t.shape[2], D, seed=i)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = drafter.window_attention(*x, T, window=W)
+    grads = torch.autograd.grad(o, x, do)
+    p = torch.arange(m) + 1000  # the first W rows see tokens in front of these: not compared
+    qs, ks = slice(Hq // 2, Hq), slice(1, 2)
+    want = _oracle(q[1, T - m:, qs].detach(), k[1, T - m:, ks].detach(), v[1, T - m:, ks].detach(),
+                   _visible(p, p, 10 ** 6, W, 0), do[1, T - m:, qs])
+    for name, t, h in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads), (qs, qs, ks, ks)):
+        _near(name, t[1, T - n:, h], tuple(w[m - n:] for w in want[name]))
+    assert float(o[0].abs().max()) == 0.0 and float(grads[0][0].abs().max()) == 0.0

@@ -216,6 +216,8 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 // How the parts of a row's keys come together: one part; unnormalised fp32 rows
 // in the workspace and a second kernel; or within a cluster, up to 8 parts.
 constexpr int kSplitNone = 0, kSplitMemory = 1, kSplitCluster = 2, kClusterMost = 8;
+// A batch of few tokens, no splits (see two_p).
+constexpr int kFewTokens = 3;
 
 template <int D>
 struct FwdCfg {
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
   const KeyTiles<KN> kt(A, sq, some ? p0 : 0, some ? p1 : -1);
   if (some) {
     n = kt.n;
-    if (SPLIT) {
+    if (SPLIT == kSplitMemory || SPLIT == kSplitCluster) {
       const int per = div(A.by_split, n + A.splits - 1);
       i0 = min(n, (int)blockIdx.z * per);
       n = min(n, i0 + per) - i0;
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
   const int m = m0 + (int)(threadIdx.x & (kTM - 1));
   const int tq = group_div(A, min(m, A.M - 1)), hq = hv * A.G + min(m, A.M - 1) - tq * A.G;
   bf16_t* orow = A.o + (((int64_t)b * A.Tq + tq) * A.Hq + hq) * D;
-  const int64_t prow = ((int64_t)bh * A.M + m) * A.splits + (SPLIT ? blockIdx.z : 0);
+  const int64_t prow = ((int64_t)bh * A.M + m) * A.splits + (SPLIT == kSplitMemory ? blockIdx.z : 0);
   const bool mine = !service && m < A.M;
   const int p = mine ? token_of(A, sq, tq) : -1;
 
@@ -345,6 +347,13 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
     }
     return;
   }
+  // A batch of at most 64 tokens, all keys in one tile: what P's rounding takes
+  // away goes through a second product, from the other buffer's place. With few keys that rounding is
+  // the largest part of delta's error: dq, dk 1.5 to 1.66 times as far off as one
+  // rounding of the result with 3 to 6 tokens, 1.41 (dS's rounding) so; with more
+  // keys it averages out (1.48 with 80 tokens, 1.44 with hundreds). (In the other
+  // kernels the branch alone would cost the long windows 7%.)
+  const bool two_p = SPLIT == kFewTokens && n == 1;
   float m_ref = -INFINITY, l_run = 0.f;  // a softmax thread's row: reference maximum, sum
   bool ok_row = true;                    // no wait of this thread expired
   int issued = 0;  // stages that this thread's copies have begun
@@ -428,9 +437,11 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
             ok = ok && wait_alive(p_full + 2 * (j & 1) + h, (j >> 1) & 1, dead, A.status);
             if (!ok) break;
             tc_fence_after();
-            if (elect_one())
-              issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + h * (KN / 4), v + h * ((KN / 32 * 2048) >> 4), kIdO,
-                                (j > 0) | (h > 0));
+            if (elect_one()) {
+              const uint32_t vh = v + h * ((KN / 32 * 2048) >> 4);
+              issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + h * (KN / 4), vh, kIdO, (j > 0) | (h > 0));
+              if (two_p) issue_tn<KN / 32>(tmem + C::COL_O, tmem + KN + h * (KN / 4), vh, kIdO, 1);
+            }
             __syncwarp();
           }
           if (!ok) break;
@@ -539,23 +550,29 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
         }
       }
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      auto exponentials = [&](auto both) {
 #pragma unroll
-      for (int c = 0; c < KN / 32; ++c) {
-        uint32_t pk[16];
+        for (int c = 0; c < KN / 32; ++c) {
+          uint32_t pk[16], lo_bits[16];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float2 e = ffma2(make_float2(s[c][j], s[c][j + 1]), sc2, nm2);
-          const float2 pr = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-          ls[(j >> 1) & 1] = fadd2(ls[(j >> 1) & 1], pr);
-          pk[j / 2] = pack_bf16x2(pr.x, pr.y);
-        }
-        tmem_st16(lane + buf * KN + c * 16, pk);
-        if ((c + 1) % (KN / 64) == 0) {  // half of P is there: its product may start
-          tmem_wait_st();
+          for (int j = 0; j < 32; j += 2) {
+            const float2 e = ffma2(make_float2(s[c][j], s[c][j + 1]), sc2, nm2);
+            const float2 pr = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+            ls[(j >> 1) & 1] = fadd2(ls[(j >> 1) & 1], pr);
+            pk[j / 2] = pack_bf16x2(pr.x, pr.y);
+            if constexpr (both.value) lo_bits[j / 2] = pack_bf16x2(pr.x - bf16_lo(pk[j / 2]), pr.y - bf16_hi(pk[j / 2]));
+          }
+          tmem_st16(lane + buf * KN + c * 16, pk);
+          if constexpr (both.value) tmem_st16(lane + KN + c * 16, lo_bits);
+          tmem_wait_st();  // half of P is there: its product may start
           tc_fence_before();
-          mbar_arrive(p_full + 2 * buf + (c + 1) / (KN / 64) - 1);
+          mbar_arrive(p_full + 2 * buf + c);
         }
+      };
+      if constexpr (SPLIT == kFewTokens) {
+        if (two_p) exponentials(std::true_type{});
       }
+      if (SPLIT != kFewTokens || !two_p) exponentials(std::false_type{});
       const float2 l2 = fadd2(ls[0], ls[1]);
       l_run = fmaf(l_run, alpha, l2.x + l2.y);
     }
@@ -576,7 +593,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
           *reinterpret_cast<float4*>(pr + j) = make_float4(ot[j], ot[j + 1], ot[j + 2], ot[j + 3]);
       }
     }
-    if (SPLIT == kSplitNone) {  // (a cluster's rows are joined below)
+    if (SPLIT == kSplitNone || SPLIT == kFewTokens) {  // (a cluster's rows are joined below)
       // every product is done: the rows leave through Q's place, the residuals
       // through the ring's
       const uint32_t out = base + C::OQ, res = base + C::OST, r = threadIdx.x;
@@ -1467,6 +1484,7 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
 
 template <int D>
 cudaError_t fwd_any(WindowArgs& A, cudaStream_t st) {
+  if (!A.cached && A.Tk <= kTN) return fwd_launch<D, kFewTokens>(A, st);
   if (A.splits == 1) return fwd_launch<D, kSplitNone>(A, st);
   if (A.splits <= kClusterMost) return fwd_launch<D, kSplitCluster>(A, st);
   const cudaError_t e = fwd_launch<D, kSplitMemory>(A, st);

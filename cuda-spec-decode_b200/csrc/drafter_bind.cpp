@@ -124,6 +124,15 @@ variable_list once(variable_list grads, const char* name) {
   return (*error)(std::move(grads));
 }
 
+// Forward mode: the kernels compute no tangents. A dual tensor does not require
+// a gradient, so without this check its tangent would be lost without a word.
+// Raises as torch.autograd.Function (the other operators) does.
+template <class... T>
+void refuse_tangents(const char* name, const T&... inputs) {
+  if ((... || inputs._fw_grad(0).defined()))
+    raise(PyExc_NotImplementedError, std::string(name) + " has no forward-mode derivative");
+}
+
 // ---- rotary positions, norms of queries and keys ------------------------------
 
 struct Turn {  // how to turn: positions, frequencies, layout, factor
@@ -181,15 +190,18 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
     Tensor dx;
-    if (g[0].defined())
+    if (g[0].defined()) {
+      refuse_tangents("the gradient of rotary", g[0]);
       dx = rotary_run(g[0], {saved[0], saved[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble()},
                       true);
+    }
     return once({dx, Tensor(), Tensor(), Tensor(), Tensor()}, "rotary");
   }
 };
 
 Tensor rotary(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, bool interleaved, double scale) {
   check_heads("x", x, nullptr);
+  refuse_tangents("rotary", x, inv_freq);
   const Turn how = check_turn(x, positions, inv_freq, interleaved, scale);
   if (at::GradMode::is_enabled() && x.requires_grad())
     return RotaryFn::apply(x, how.positions, how.inv_freq, interleaved, scale);
@@ -233,6 +245,8 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3];
     const Turn how{saved[4], saved[5], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble()};
     const On on(q);
+    for (const Tensor& t : g)
+      if (t.defined()) refuse_tangents("the gradient of qk_norm_rotary", t);
     // an output that nothing depends on brings no gradient: zeros
     const Tensor dyq = g[0].defined() ? heads_contiguous(g[0]) : at::zeros_like(q);
     const Tensor dyk = g[1].defined() ? heads_contiguous(g[1]) : at::zeros_like(k);
@@ -262,6 +276,7 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, cons
   require(q_weight.dim() == 1 && q_weight.size(0) == D && k_weight.dim() == 1 && k_weight.size(0) == D &&
               q_weight.device() == q.device() && k_weight.device() == q.device(),
           "weights must be [D] on q's device");
+  refuse_tangents("qk_norm_rotary", q, k, q_weight, k_weight, inv_freq);
   const Turn how = check_turn(q, positions, inv_freq, interleaved, scale);
   const double e = eps ? *eps
                        : q.scalar_type() == at::kFloat ? (double)std::numeric_limits<float>::epsilon()
@@ -347,6 +362,7 @@ struct WindowFn : torch::autograd::Function<WindowFn> {
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lens = saved[6];
     Tensor dq, dk, dv;
     if (g[0].defined()) {
+      refuse_tangents("the gradient of window_attention", g[0]);
       const On on(q);
       Tensor dout = g[0].contiguous();
       if (reinterpret_cast<uintptr_t>(dout.const_data_ptr()) % 16) dout = dout.clone();
@@ -373,6 +389,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
   const Window w = check_window(q, k, v, window, sinks, scale);
   require(k.size(1) == q.size(1), "k and v must have q's length");
   require(n_ctx >= 0 && n_ctx <= q.size(1), "n_ctx must be in [0, T]");
+  refuse_tangents("window_attention", q, k, v);
   std::optional<Tensor> lens;
   if (ctx_lens) lens = check_lens(*ctx_lens, q);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
@@ -385,6 +402,7 @@ Tensor window_attention_cached(const Tensor& q_in, const Tensor& k_cache, const 
   const Window w = check_window(q_in, k_cache, v_cache, window, sinks, scale);
   require(!(at::GradMode::is_enabled() && (q_in.requires_grad() || k_cache.requires_grad() || v_cache.requires_grad())),
           "window_attention_cached has no backward: call it under torch.no_grad()");
+  refuse_tangents("window_attention_cached", q_in, k_cache, v_cache);
   const Tensor lens = check_lens(ctx_lens, q_in);
   require(k_cache.stride(3) == 1 && v_cache.stride(3) == 1, "the cache's heads must be contiguous");
   const int32_t B = i32(q_in.size(0)), Tq = i32(q_in.size(1)), Hq = i32(q_in.size(2)), D = i32(q_in.size(3)),

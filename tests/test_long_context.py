@@ -365,3 +365,42 @@ def test_captured_draft_from_the_cache(cuda):
     for _ in range(20):  # room for 11 more: the last replays give NaN and write nothing
         g.replay()
     assert cache.lens.tolist() == [82, 82] and bool(torch.isnan(out).all())
+
+
+@pytest.mark.gpu
+def test_forward_mode_raises(cuda):
+    """None of the four has a forward-mode derivative: a tangent on any input, or
+    on the gradient that comes back, is refused instead of lost."""
+    import torch.autograd.forward_ad as fwAD
+
+    from specdec import drafter
+
+    x = torch.randn(2, 6, 4, 64, device="cuda").bfloat16()
+    w, pos = torch.ones(64, device="cuda"), torch.arange(6, device="cuda")
+    f, _ = drafter.rotary_frequencies(64, device="cuda")
+    lens = torch.full((2,), 6, device="cuda", dtype=torch.int32)
+    calls = [
+        (lambda x: drafter.rotary(x, pos, f), (x,)),
+        (lambda f: drafter.rotary(x, pos, f), (f,)),
+        (lambda q, k, a, b: drafter.qk_norm_rotary(q, k, a, b, pos, f, eps=1e-6), (x, x.clone(), w, w.clone())),
+        (lambda f: drafter.qk_norm_rotary(x, x, w, w, pos, f, eps=1e-6), (f,)),
+        (lambda q, k, v: drafter.window_attention(q, k, v, 6), (x, x.clone(), x.clone())),
+        (lambda q, k, v: drafter.window_attention_cached(q, k, v, lens), (x, x.clone(), x.clone())),
+    ]
+    for fn, args in calls:
+        fn(*args)
+        for i in range(len(args)):
+            for grad in (True, False):
+                with fwAD.dual_level(), torch.set_grad_enabled(grad):
+                    dual = [fwAD.make_dual(a, torch.ones_like(a)) if j == i else a for j, a in enumerate(args)]
+                    with pytest.raises(NotImplementedError):
+                        fn(*dual)
+    for fn, args in (calls[0], calls[2], calls[4]):
+        leaves = [a.clone().requires_grad_(True) for a in args]
+        y = fn(*leaves)
+        y = y if torch.is_tensor(y) else y[0]
+        with fwAD.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
+            torch.autograd.grad(y, leaves[0], fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        y = fn(*leaves)
+        y = y if torch.is_tensor(y) else y[0]
+        assert bool(torch.isfinite(torch.autograd.grad(y, leaves[0], torch.ones_like(y))[0].float()).all())

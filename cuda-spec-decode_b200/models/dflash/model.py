@@ -168,7 +168,9 @@ class DFlashAttention(nn.Module):
         over the context; the block queries over all keys), which the fused
         SDPA kernels handle without reading a [T, T] mask. With n_ctx, ctx_lens
         int [B] gives each sequence's own context length (the rows behind it up
-        to n_ctx are padding), and the options above apply."""
+        to n_ctx are padding: no other row sees them, but the projections' weight
+        gradients multiply them by zero, so they have to be finite), and the
+        options above apply."""
         b, s, _ = x.shape
         if self.extended or ctx_lens is not None:
             if attn_mask is not None or n_ctx is None:
@@ -328,8 +330,13 @@ class DFlashSpeculator(nn.Module):
 
     def forward(self, target_features: torch.Tensor, ctx_lens: torch.Tensor | None = None) -> torch.Tensor:
         """target_features [batch, S_ctx, d_target] -> draft logits [batch, block_size, V].
-        ctx_lens int [batch]: sequence b's context is its first ctx_lens[b] features."""
+        ctx_lens int [batch]: sequence b's context is its first ctx_lens[b] features; the
+        others may hold anything (they enter as zeros: a weight's gradient is a product
+        with them too)."""
         s_ctx = target_features.shape[1]
+        if ctx_lens is not None:
+            live = torch.arange(s_ctx, device=target_features.device) < ctx_lens.to(target_features.device)[:, None]
+            target_features = torch.where(live[:, :, None], target_features, 0)
         h = self._embed(target_features)
         # the _build_dflash_mask rule, applied by structure (no [T, T] mask tensor)
         for layer in self.layers:

@@ -177,6 +177,30 @@ def test_frequencies_survive_a_change_of_dtype():
     assert f.dtype == torch.float64 and float(f[1]) == 10000.0 ** (-2.0 / 16)
 
 
+@pytest.mark.parametrize("options", OPTIONS + [None])
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), 3.0])
+def test_gradients_do_not_depend_on_the_padding(options, fill):
+    """Weights' and features' gradients of a padded batch: finite whatever the
+    padding holds, those of zero padding, and zero for the padding itself."""
+    m = _model(options)
+    x = torch.randn(3, 20, 48)
+    lens = torch.tensor([20, 7, 0])
+    pad = torch.arange(20)[None] >= lens[:, None]
+    tokens = torch.randint(0, 50, (3, 4))
+    got = []
+    for value in (fill, 0.0):
+        feats = x.clone()
+        feats[pad] = value
+        feats.requires_grad_(True)
+        m.zero_grad(set_to_none=True)
+        loss = m.compute_loss(feats, tokens, ctx_lens=lens)
+        loss.backward()
+        got.append([loss.detach(), feats.grad] + [p.grad for p in m.parameters() if p.grad is not None])
+    assert bool((got[0][1][pad] == 0).all()) and len(got[0]) > 2 + len(m.layers)
+    for a, b in zip(*got):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
 # ---- on the GPU ------------------------------------------------------------------
 
 GPU_OPTIONS = [

@@ -122,7 +122,9 @@ class DFlashAttention(nn.Module):
             if not 2 <= self.rotary[0] <= self.head_dim:
                 raise AssertionError("rotary dim must be in [2, head_dim]")
             # fp64, kept apart from the module's buffers: .to(dtype) must not round it
-            self._freq = {torch.device("cpu"): _kernels.rotary_frequencies(self.rotary[0], **opts)}
+            with torch.inference_mode(False), torch.device("cpu"):
+                self._freq = {torch.device("cpu"): _kernels.rotary_frequencies(self.rotary[0], **opts)}
+            self._frequencies(self.q_proj.weight.device)
         self.extended = (qk_norm or rotary is not None or window is not None or sinks > 0
                          or self.num_kv_heads != num_heads)
 
@@ -131,11 +133,22 @@ class DFlashAttention(nn.Module):
         return t.view(b, s, self.num_heads, self.head_dim).transpose(1, 2)
 
     def _frequencies(self, device: torch.device):
+        """(inv_freq, scale) on ``device``: a copy kept for the module's life, so
+        never an inference tensor (a later training step saves it for its
+        backward). Made when the module moves there: a first use inside a graph
+        capture could not copy from the host."""
         got = self._freq.get(device)
         if got is None:
             freq, scale = self._freq[torch.device("cpu")]
-            got = self._freq[device] = (freq.to(device), scale)
+            with torch.inference_mode(False):
+                got = self._freq[device] = (freq.to(device), scale)
         return got
+
+    def _apply(self, fn, *args, **kwargs):  # .to(), .cuda(), ...
+        super()._apply(fn, *args, **kwargs)
+        if self.rotary is not None:
+            self._frequencies(self.q_proj.weight.device)
+        return self
 
     def _project(self, x: torch.Tensor, positions: torch.Tensor):
         """Queries, keys and values [B, T, heads, D], normalised and rotated."""

@@ -201,6 +201,32 @@ def test_gradients_do_not_depend_on_the_padding(options, fill):
         assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
 
 
+def test_frequencies_are_never_inference_tensors():
+    """A copy that is made while drafting in inference mode is kept: the next
+    training step has to be able to save it."""
+    m = _model(dict(rotary={}))
+    at = m.layers[0].attn
+    with torch.inference_mode():
+        assert not at._frequencies(torch.device("meta"))[0].is_inference()
+        m.draft(torch.randn(1, 5, 48))
+        born = DFlashAttention(64, 4, rotary={})
+    assert not at._frequencies(torch.device("cpu"))[0].is_inference()
+    assert not born._frequencies(torch.device("cpu"))[0].is_inference()
+
+
+def test_frequencies_follow_the_module():
+    """They are there before the first call: one inside a capture could not copy them."""
+    at = DFlashAttention(64, 4, rotary={})
+    want = at._frequencies(torch.device("cpu"))[0]
+    at.to("meta")
+    assert torch.device("meta") in at._freq
+    with torch.device("meta"):
+        born = DFlashAttention(64, 4, rotary={})
+    assert torch.device("meta") in born._freq
+    back = born.to_empty(device="cpu")._frequencies(torch.device("cpu"))[0]
+    assert back.device.type == "cpu" and torch.equal(back, want)
+
+
 # ---- on the GPU ------------------------------------------------------------------
 
 GPU_OPTIONS = [
@@ -428,3 +454,23 @@ def test_forward_mode_raises(cuda):
         y = fn(*leaves)
         y = y if torch.is_tensor(y) else y[0]
         assert bool(torch.isfinite(torch.autograd.grad(y, leaves[0], torch.ones_like(y))[0].float()).all())
+
+
+@pytest.mark.gpu
+def test_training_after_a_draft_in_inference_mode(cuda):
+    """The frequencies' device copy is the module's, not the first call's; and a
+    draft may be captured as the first call."""
+    case = GPU_OPTIONS[1]
+    m, again = _gpu_model(**case), _gpu_model(**case)
+    x, tokens = torch.randn(2, 40, 256, device="cuda"), torch.randint(0, 500, (2, 16), device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+        with torch.inference_mode():
+            m.draft(x)
+        losses = []
+        for model in (m, again):
+            loss = model.compute_loss(x, tokens)
+            loss.backward()
+            losses.append(loss.detach())
+        assert torch.equal(*losses)
+        device = m.layers[0].attn.q_proj.weight.device
+        assert all(device in layer.attn._freq for layer in _gpu_model(**case).layers)

@@ -200,7 +200,8 @@ class Workspace:
         if self.scratch is None or self.scratch.numel() < scratch_bytes:
             self.scratch = torch.empty(max(scratch_bytes, 256), dtype=torch.uint8, device=device)
         if self.counters is None or self.counters.numel() < counter_bytes:
-            self.counters = torch.zeros(max(counter_bytes, 256), dtype=torch.uint8, device=device)
+            with torch.inference_mode(False):  # kept, and zeroed again outside of it
+                self.counters = torch.zeros(max(counter_bytes, 256), dtype=torch.uint8, device=device)
         return self.scratch, self.counters
 
     def reset_counters(self):
@@ -233,5 +234,6 @@ def status_words(device: torch.device) -> torch.Tensor:
     key = (device.index, stream_handle(device))
     t = _status.get(key)
     if t is None:
-        t = _status[key] = torch.zeros(4, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # kept, and cleared outside of it
+            t = _status[key] = torch.zeros(4, dtype=torch.int32, device=device)
     return t

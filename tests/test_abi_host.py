@@ -156,3 +156,18 @@ def test_dflash_objective_binds_target_logits():
     finally:
         L.dflash_loss = orig
     assert seen == {"lg": "DRAFT", "tl": "VERIFIER", "kw": {"gamma": 2.0, "kind": "ce"}}
+
+
+def test_kept_buffers_are_never_inference_tensors(monkeypatch):
+    """Status words and counters outlive a first call in inference mode: they are
+    zeroed in place later, which an inference tensor refuses."""
+    monkeypatch.setattr(_lib, "stream_handle", lambda device: 0)
+    monkeypatch.setattr(_lib, "_status", {})
+    cpu = torch.device("cpu")
+    with torch.inference_mode():
+        words = _lib.status_words(cpu)
+        ws = _lib.Workspace()
+        _, counters = ws.ensure(cpu, 256, 256)
+    assert not words.is_inference() and not counters.is_inference()
+    words[3:4].zero_()
+    ws.reset_counters()

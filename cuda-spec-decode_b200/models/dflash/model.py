@@ -284,15 +284,18 @@ class DraftCache:
         self.lens = torch.zeros(batch, device=device, dtype=torch.int32)
         self.longest = 0  # on the host: no sequence is longer
 
-    def reserve(self, tokens: int, block: int) -> None:
-        """Room for ``tokens`` more and a block, or ValueError (synchronises only
-        when the host's bound does not already show it)."""
-        if self.longest + tokens + block > self.size:
-            self.longest = int(self.lens.max()) if self.lens.numel() else 0
-            if self.longest + tokens + block > self.size:
-                raise ValueError(f"the cache holds {self.size} tokens: {self.longest} are there, {tokens} and a block "
-                                 f"of {block} do not fit")
-        self.longest += tokens
+    def reserve(self, tokens: int, block: int, new: torch.Tensor | None = None) -> None:
+        """Room for ``tokens`` more per sequence (``new`` [B]: for so many of them)
+        and a block, or ValueError (synchronises only when the host's bound does
+        not already show it)."""
+        longest = self.longest + tokens
+        if longest + block > self.size:
+            lens = self.lens + (tokens if new is None else new)
+            longest = int(lens.max()) if lens.numel() else 0
+            if longest + block > self.size:
+                raise ValueError(f"the cache holds {self.size} tokens: a sequence of {longest} with the new ones and a "
+                                 f"block of {block} do not fit")
+        self.longest = longest
 
 
 class DFlashSpeculator(nn.Module):
@@ -390,9 +393,9 @@ class DFlashSpeculator(nn.Module):
         b, n_new, _ = target_features.shape
         if b != cache.lens.shape[0]:
             raise ValueError(f"the cache is for {cache.lens.shape[0]} sequences, got {b}")
-        cache.reserve(n_new, self.block_size)
         new = torch.full((b,), n_new, device=cache.lens.device, dtype=torch.int32) if ctx_lens is None else \
-            ctx_lens.to(device=cache.lens.device, dtype=torch.int32).clamp(0, n_new)
+            ctx_lens.to(device=cache.lens.device).clamp(0, n_new).to(torch.int32)
+        cache.reserve(n_new, self.block_size, None if ctx_lens is None else new)
         lens = cache.lens + new
         i = torch.arange(n_new + self.block_size, device=cache.lens.device)
         positions = lens.long()[:, None] + i - n_new

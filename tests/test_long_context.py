@@ -227,6 +227,27 @@ def test_frequencies_follow_the_module():
     assert back.device.type == "cpu" and torch.equal(back, want)
 
 
+def test_a_cache_counts_the_new_tokens_not_the_width():
+    """Five tokens there, one more each in features five wide, a block of four:
+    ten of twelve places."""
+    m = _model(dict(rotary={}))
+    cache = m.new_cache(2, 12, dtype=torch.float32)
+    x = torch.randn(2, 9, 48)
+    m.draft(x[:, :5], cache=cache)
+    wide = torch.cat([torch.full((2, 4, 48), float("nan")), x[:, 5:6]], 1)
+    _, logits = m.draft(wide, ctx_lens=torch.tensor([1, 1]), cache=cache)
+    assert cache.lens.tolist() == [6, 6] and cache.longest == 6
+    assert float((logits - m.draft(x[:, :6])[1]).abs().max()) < 1e-5
+    m.draft(x[:, 6:8], ctx_lens=torch.tensor([2, 0]), cache=cache)  # eight and six: full
+    with pytest.raises(ValueError):
+        m.draft(x[:, :2], ctx_lens=torch.tensor([1, 2]), cache=cache)
+    assert cache.lens.tolist() == [8, 6]
+    m.draft(x[:, 6:9], ctx_lens=torch.tensor([0, 2], dtype=torch.int64), cache=cache)
+    assert cache.lens.tolist() == [8, 8] and cache.longest == 8
+    m.draft(x[:, :3], ctx_lens=torch.tensor([-1, -2 ** 33]), cache=cache)  # clamped: none
+    assert cache.lens.tolist() == [8, 8]
+
+
 # ---- on the GPU ------------------------------------------------------------------
 
 GPU_OPTIONS = [

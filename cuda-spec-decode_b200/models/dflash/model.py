@@ -270,6 +270,10 @@ class DFlashTransformerLayer(nn.Module):
         return x + self.mlp(self.norm2(x))
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class DraftCache:
     """Keys and values of the context tokens drafted from so far, per layer
     [B, size + 1, kv_heads, head_dim]: sequence b's ``lens[b]`` tokens in rows 0,
@@ -282,14 +286,19 @@ class DraftCache:
         self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
         self.size = size
         self.lens = torch.zeros(batch, device=device, dtype=torch.int32)
-        self.longest = 0  # on the host: no sequence is longer
+        self.longest = 0  # on the host: no sequence is longer, unless
+        self.captured = False  # a draft was captured: its replays add tokens without the host
 
     def reserve(self, tokens: int, block: int, new: torch.Tensor | None = None) -> None:
         """Room for ``tokens`` more per sequence (``new`` [B]: for so many of them)
         and a block, or ValueError (synchronises only when the host's bound does
-        not already show it)."""
+        not already show it, or no longer holds). A capture is let through: it adds
+        nothing by itself, its replays look after themselves."""
+        if _capturing(self.lens):
+            self.captured = True
+            return
         longest = self.longest + tokens
-        if longest + block > self.size:
+        if self.captured or longest + block > self.size:
             lens = self.lens + (tokens if new is None else new)
             longest = int(lens.max()) if lens.numel() else 0
             if longest + block > self.size:

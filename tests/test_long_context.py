@@ -248,6 +248,29 @@ def test_a_cache_counts_the_new_tokens_not_the_width():
     assert cache.lens.tolist() == [8, 8]
 
 
+def test_a_draft_after_replays_is_checked_against_the_real_lengths(monkeypatch):
+    """A captured draft's replays add tokens behind the host's back: later eager
+    drafts look at the lengths again."""
+    from models.dflash import model
+
+    m = _model(dict(rotary={}))
+    cache = m.new_cache(2, 12, dtype=torch.float32)
+    x = torch.randn(2, 12, 48)
+    m.draft(x[:, :1], cache=cache)
+    with monkeypatch.context() as patch:
+        patch.setattr(model, "_capturing", lambda t: True)  # every call like a replay: it adds, the host does not look
+        for i in range(1, 4):
+            m.draft(x[:, 2 * i - 1:2 * i + 1], cache=cache)
+    assert cache.lens.tolist() == [7, 7]
+    with pytest.raises(ValueError):
+        m.draft(x[:, :2], cache=cache)
+    assert cache.lens.tolist() == [7, 7]
+    _, logits = m.draft(x[:, 7:8], cache=cache)
+    assert float((logits - m.draft(x[:, :8])[1]).abs().max()) < 1e-5
+    with pytest.raises(ValueError):
+        m.draft(x[:, 8:9], cache=cache)
+
+
 # ---- on the GPU ------------------------------------------------------------------
 
 GPU_OPTIONS = [
@@ -495,3 +518,26 @@ def test_training_after_a_draft_in_inference_mode(cuda):
         assert torch.equal(*losses)
         device = m.layers[0].attn.q_proj.weight.device
         assert all(device in layer.attn._freq for layer in _gpu_model(**case).layers)
+
+
+@pytest.mark.gpu
+def test_an_eager_draft_after_replays(cuda):
+    m = _gpu_model(**GPU_OPTIONS[0])
+    x = torch.randn(2, 40, 256, device="cuda")
+    side = torch.cuda.Stream()
+    with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False), torch.cuda.stream(side):
+        cache, ref = m.new_cache(2, 30), m.new_cache(2, 30)
+        for c in (m.new_cache(2, 30), cache, ref):
+            m.draft(x[:, :3], cache=c)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            m.draft(x[:, 3:6], cache=cache)
+        assert cache.lens.tolist() == [3, 3] and cache.longest == 3
+        for _ in range(3):
+            g.replay()
+            m.draft(x[:, 3:6], cache=ref)
+        with pytest.raises(ValueError):
+            m.draft(x[:, :3], cache=cache)
+        assert torch.equal(m.draft(x[:, 6:8], cache=cache)[1], m.draft(x[:, 6:8], cache=ref)[1])
+        assert cache.lens.tolist() == ref.lens.tolist() == [14, 14]

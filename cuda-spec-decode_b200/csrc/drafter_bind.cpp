@@ -278,9 +278,8 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, cons
           "weights must be [D] on q's device");
   refuse_tangents("qk_norm_rotary", q, k, q_weight, k_weight, inv_freq);
   const Turn how = check_turn(q, positions, inv_freq, interleaved, scale);
-  const double e = eps ? *eps
-                       : q.scalar_type() == at::kFloat ? (double)std::numeric_limits<float>::epsilon()
-                                                       : 0.0078125;  // finfo(bfloat16).eps
+  // as torch's rms_norm, which takes fp32's for bf16 inputs too
+  const double e = eps ? *eps : (double)std::numeric_limits<float>::epsilon();
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || q_weight.requires_grad() || k_weight.requires_grad())) {
     const auto y = NormFn::apply(q, k, q_weight, k_weight, how.positions, how.inv_freq, e, interleaved, scale);

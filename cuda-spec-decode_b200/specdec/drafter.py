@@ -234,8 +234,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
                    positions: torch.Tensor, inv_freq: torch.Tensor, *, eps: float | None = None,
                    interleaved: bool = False, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """RMSNorm over the elements of every head of q [B, T, Hq, D] and k
-    [B, T, Hk, D] (weights [D]; eps None = finfo(dtype).eps), then ``rotary`` of
-    both, in one pass: x / sqrt(mean(x^2) + eps) * weight, rotated. fp32 or bf16,
+    [B, T, Hk, D] (weights [D]; eps None: fp32's 2^-23 for both types, as torch's
+    rms_norm takes it), then ``rotary`` of both, in one pass: x / sqrt(mean(x^2) + eps) * weight, rotated. fp32 or bf16,
     any strides (views of one fused projection); fp32 arithmetic, one rounding.
     Differentiable in q, k and the weights (their gradients are summed in a
     fixed order)."""

@@ -319,3 +319,24 @@ def test_rotary_past_32_bit_offsets(cuda):
     want, size = _rot64(x[:, -9:], pos[-9:], _freq(D), False, 1.0)
     assert bool(((y[:, -9:].double() - want).abs() <= 5e-7 * size + _half(x.dtype) * want.abs()).all())
     assert not bool(y[:, :-9].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_default_eps_is_torchs(cuda, dtype):
+    """Small inputs, where eps counts: 2^-7 (bf16's own) would halve the constant
+    0.05. Against the formula as above (3e-6, and half a step), and against
+    torch's own with weights rounded to the type: three roundings at most."""
+    D = 64
+    pos = torch.zeros(3, device="cuda", dtype=torch.int64)  # no rotation: cos 1, sin 0
+    f, _ = drafter.rotary_frequencies(D, device="cuda")
+    w = torch.linspace(0.5, 2.0, D, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for size in (0.05, 3e-4):
+        x = (size * torch.randn(2, 3, 4, D, device="cuda", generator=g)).to(dtype)
+        y, z = drafter.qk_norm_rotary(x, x[:, :, :2], w, w, pos, f)
+        want = x.double() / torch.sqrt(x.double().square().mean(-1, keepdim=True) + 2.0 ** -23) * w.double()
+        assert bool(((y.double() - want).abs() <= (3e-6 + _half(dtype)) * want.abs()).all())
+        assert torch.equal(z, y[:, :, :2])
+        torchs = torch.nn.functional.rms_norm(x, (D,), w.to(dtype), None).double()
+        assert float((y.double() - torchs).norm() / torchs.norm()) <= 3 * _half(dtype) + 1e-5

@@ -40,11 +40,12 @@ from specdec import drafter as _kernels
 
 class RMSNorm(nn.RMSNorm):
     """torch.nn.RMSNorm (same parameters and state-dict keys) whose forward
-    runs the library's RMSNorm kernels on CUDA tensors."""
+    runs the library's RMSNorm kernels on CUDA tensors. eps None: fp32's, which
+    torch takes for bf16 inputs too."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if len(self.normalized_shape) == 1 and _kernels.rms_norm_supported(x, self.weight):
-            return _kernels.rms_norm(x, self.weight, self.eps)
+            return _kernels.rms_norm(x, self.weight, torch.finfo(torch.float32).eps if self.eps is None else self.eps)
         return super().forward(x)
 
 
@@ -110,7 +111,6 @@ class DFlashAttention(nn.Module):
         self.k_proj = nn.Linear(d_model, kv, bias=qkv_bias)
         self.v_proj = nn.Linear(d_model, kv, bias=qkv_bias)
         self.out_proj = nn.Linear(d_model, d_model, bias=qkv_bias)
-        # an eps of their own: the default, the activation type's, would weigh 0.8% of the mean square in bf16
         self.q_norm = RMSNorm(self.head_dim, eps=1e-6) if qk_norm else None
         self.k_norm = RMSNorm(self.head_dim, eps=1e-6) if qk_norm else None
         self.window, self.sinks = window, sinks

@@ -98,7 +98,8 @@ def rms_norm_supported(x: torch.Tensor, weight: torch.Tensor | None) -> bool:
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float | None = None) -> torch.Tensor:
-    """RMSNorm of the last dimension; eps None = finfo(x.dtype).eps (torch's default)."""
+    """RMSNorm of the last dimension; eps None = finfo(x.dtype).eps. (torch's own
+    rms_norm takes fp32's eps for bf16 inputs: the drafter's modules pass that.)"""
     e = torch.finfo(x.dtype).eps if eps is None else float(eps)
     return _RMSNorm.apply(x, weight, e)
 

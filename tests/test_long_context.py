@@ -541,3 +541,20 @@ def test_an_eager_draft_after_replays(cuda):
             m.draft(x[:, :3], cache=cache)
         assert torch.equal(m.draft(x[:, 6:8], cache=cache)[1], m.draft(x[:, 6:8], cache=ref)[1])
         assert cache.lens.tolist() == ref.lens.tolist() == [14, 14]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_modules_norm_has_torchs_default_eps(cuda, dtype):
+    """The drafter's norms are made without an eps. Three roundings to the type at
+    most lie between the two (torch's x / rms before the weight, both results)."""
+    from models.dflash.model import RMSNorm
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a, b = RMSNorm(256).cuda(), nn.RMSNorm(256).cuda()
+    with torch.no_grad():
+        b.weight.copy_(a.weight.copy_(1 + 0.2 * torch.randn(256, device="cuda", generator=g)))
+    for size in (1.0, 0.05, 3e-4):
+        x = (size * torch.randn(5, 7, 256, device="cuda", generator=g)).to(dtype)
+        got, want = a(x).double(), b(x).double()
+        assert float((got - want).norm() / want.norm()) <= 3 * torch.finfo(dtype).eps / 2 + 1e-5

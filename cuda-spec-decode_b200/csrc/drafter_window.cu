@@ -216,8 +216,8 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 // How the parts of a row's keys come together: one part; unnormalised fp32 rows
 // in the workspace and a second kernel; or within a cluster, up to 8 parts.
 constexpr int kSplitNone = 0, kSplitMemory = 1, kSplitCluster = 2, kClusterMost = 8;
-// A batch of few tokens, no splits (see two_p).
-constexpr int kFewTokens = 3;
+// Queries that see few keys, no splits (see few_keys).
+constexpr int kFewKeys = 3;
 
 template <int D>
 struct FwdCfg {
@@ -347,13 +347,9 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
     }
     return;
   }
-  // A batch of at most 64 tokens, all keys in one tile: what P's rounding takes
-  // away goes through a second product, from the other buffer's place. With few keys that rounding is
-  // the largest part of delta's error: dq, dk 1.5 to 1.66 times as far off as one
-  // rounding of the result with 3 to 6 tokens, 1.41 (dS's rounding) so; with more
-  // keys it averages out (1.48 with 80 tokens, 1.44 with hundreds). (In the other
-  // kernels the branch alone would cost the long windows 7%.)
-  const bool two_p = SPLIT == kFewTokens && n == 1;
+  // Few keys (see few_keys): what P's rounding takes away goes through a second
+  // product, from the half of the scores' columns that P itself leaves free.
+  constexpr bool two_p = SPLIT == kFewKeys;
   float m_ref = -INFINITY, l_run = 0.f;  // a softmax thread's row: reference maximum, sum
   bool ok_row = true;                    // no wait of this thread expired
   int issued = 0;  // stages that this thread's copies have begun
@@ -440,7 +436,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
             if (elect_one()) {
               const uint32_t vh = v + h * ((KN / 32 * 2048) >> 4);
               issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + h * (KN / 4), vh, kIdO, (j > 0) | (h > 0));
-              if (two_p) issue_tn<KN / 32>(tmem + C::COL_O, tmem + KN + h * (KN / 4), vh, kIdO, 1);
+              if (two_p) issue_tn<KN / 32>(tmem + C::COL_O, tmem + (j & 1) * KN + KN / 2 + h * (KN / 4), vh, kIdO, 1);
             }
             __syncwarp();
           }
@@ -550,29 +546,24 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
         }
       }
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto exponentials = [&](auto both) {
 #pragma unroll
-        for (int c = 0; c < KN / 32; ++c) {
-          uint32_t pk[16], lo_bits[16];
+      for (int c = 0; c < KN / 32; ++c) {
+        uint32_t pk[16];
+        [[maybe_unused]] uint32_t rest[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 e = ffma2(make_float2(s[c][j], s[c][j + 1]), sc2, nm2);
-            const float2 pr = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-            ls[(j >> 1) & 1] = fadd2(ls[(j >> 1) & 1], pr);
-            pk[j / 2] = pack_bf16x2(pr.x, pr.y);
-            if constexpr (both.value) lo_bits[j / 2] = pack_bf16x2(pr.x - bf16_lo(pk[j / 2]), pr.y - bf16_hi(pk[j / 2]));
-          }
-          tmem_st16(lane + buf * KN + c * 16, pk);
-          if constexpr (both.value) tmem_st16(lane + KN + c * 16, lo_bits);
-          tmem_wait_st();  // half of P is there: its product may start
-          tc_fence_before();
-          mbar_arrive(p_full + 2 * buf + c);
+        for (int j = 0; j < 32; j += 2) {
+          const float2 e = ffma2(make_float2(s[c][j], s[c][j + 1]), sc2, nm2);
+          const float2 pr = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+          ls[(j >> 1) & 1] = fadd2(ls[(j >> 1) & 1], pr);
+          pk[j / 2] = pack_bf16x2(pr.x, pr.y);
+          if constexpr (two_p) rest[j / 2] = pack_bf16x2(pr.x - bf16_lo(pk[j / 2]), pr.y - bf16_hi(pk[j / 2]));
         }
-      };
-      if constexpr (SPLIT == kFewTokens) {
-        if (two_p) exponentials(std::true_type{});
+        tmem_st16(lane + buf * KN + c * 16, pk);
+        if constexpr (two_p) tmem_st16(lane + buf * KN + KN / 2 + c * 16, rest);  // (all scores have been read)
+        tmem_wait_st();  // half of P is there: its product may start
+        tc_fence_before();
+        mbar_arrive(p_full + 2 * buf + c);
       }
-      if (SPLIT != kFewTokens || !two_p) exponentials(std::false_type{});
       const float2 l2 = fadd2(ls[0], ls[1]);
       l_run = fmaf(l_run, alpha, l2.x + l2.y);
     }
@@ -593,7 +584,7 @@ __global__ void __launch_bounds__(FwdCfg<D>::THREADS, FwdCfg<D>::CTAS)
           *reinterpret_cast<float4*>(pr + j) = make_float4(ot[j], ot[j + 1], ot[j + 2], ot[j + 3]);
       }
     }
-    if (SPLIT == kSplitNone || SPLIT == kFewTokens) {  // (a cluster's rows are joined below)
+    if (SPLIT == kSplitNone || SPLIT == kFewKeys) {  // (a cluster's rows are joined below)
       // every product is done: the rows leave through Q's place, the residuals
       // through the ring's
       const uint32_t out = base + C::OQ, res = base + C::OST, r = threadIdx.x;
@@ -877,10 +868,8 @@ __device__ __forceinline__ void grad_pair(float2 s, float2 dp, float sl2, float2
   ds = fmul2(pr, fadd2(dp, nd));
 }
 
-// FEW: dS enters its product with what its rounding takes away, as a second
-// operand. Over few tokens a handful of elements decide the gradients, and dS's
-// rounding shows: dq, dk were 1.3 to 1.6 times as far off as one rounding of the
-// result (with hundreds of tokens 1.41 to 1.45, always).
+// FEW (see few_keys): dS enters its product with what its rounding takes away, as
+// a second operand.
 template <int D, int NB, bool DKV, bool FEW>
 __device__ __forceinline__ void window_bwd_role(const WindowArgs& A, int b, int head, int tile, int split, bool withhold) {
   using C = BwdCfg<D, NB>;
@@ -1351,8 +1340,7 @@ __global__ void __launch_bounds__(256) window_sink_join_kernel(const __grid_cons
 // o comes as the rounded output and the residual of that rounding (16 bits in
 // all): with o rounded to 8 bits, delta's error is the largest in the gradients
 // of rows that see few keys (dq, dk 1.53 to 1.9 times as far off as one
-// rounding of the result; with the residual 1.41 to 1.5, of which 1.41 is the
-// rounding of dS).
+// rounding of the result; with the residual as few_keys says).
 template <int D>
 __global__ void __launch_bounds__(256) window_rows_kernel(const __grid_constant__ WindowArgs A) {
   constexpr int L = D / 8;
@@ -1494,9 +1482,26 @@ cudaError_t fwd_launch(WindowArgs& A, cudaStream_t st) {
   }
 }
 
+// Whether no query can see more than kFewKeysMost keys (of a batch whose contexts
+// are n_ctx long: shorter ctx_lens are on the device). Then what the roundings of
+// P in the forward and of dS in the backward take away goes through products of
+// its own. P's rounding reaches delta as the mean of n errors of a row's n keys,
+// so it counts the more the fewer they are. Aggregate error over that of one rounding
+// of the result, dq (o), without: [8, 1000 + 16, 4, 64] S 4, W 2 1.52 (1.22), 8
+// 1.50 (1.31), 16 1.48 (1.34), 44 1.46 (1.36), 128 1.44 (1.35); 3 tokens 1.48 (1.05),
+// 80 1.45 (1.20); from there on 1.44 (1.2 to 1.36), of which 1.41 is dS's and the
+// result's own rounding. With them 1.00 (1.00) everywhere. us of forward + backward
+// without / with: [4, 40, 4, 64] 16.8 / 17.5, [8, 1000 + 16, 4, 64] W 16 41.5 / 46.0,
+// [2, 4096, 16, 128] W 64 182 / 196, and, not taken, [32, 512 + 16, 4, 64] W 128
+// 82 / 94, [2, 4096, 16, 128] W 1024 352 / 416.
+constexpr int kFewKeysMost = 64;
+bool few_keys(const WindowArgs& A) {
+  return std::min<int64_t>(A.Tk, (int64_t)std::min(A.W, A.n_ctx) + std::min(A.S, A.n_ctx) + A.n_block) <= kFewKeysMost;
+}
+
 template <int D>
 cudaError_t fwd_any(WindowArgs& A, cudaStream_t st) {
-  if (!A.cached && A.Tk <= kTN) return fwd_launch<D, kFewTokens>(A, st);
+  if (!A.cached && few_keys(A)) return fwd_launch<D, kFewKeys>(A, st);
   if (A.splits == 1) return fwd_launch<D, kSplitNone>(A, st);
   if (A.splits <= kClusterMost) return fwd_launch<D, kSplitCluster>(A, st);
   const cudaError_t e = fwd_launch<D, kSplitMemory>(A, st);
@@ -1537,12 +1542,6 @@ cudaError_t bwd_launch(const WindowArgs& A, unsigned grid, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Up to here dS's rounding is made good (see window_bwd_role): us with / without,
-// [32, 200, 4, 64] 21.8 / 19.2, [16, 250, 32 / 8, 128] 88.6 / 80.0, [4, 40, 4, 64] 7.8 /
-// 7.2; dq, dk 1.00 to 1.05 times as far off as one rounding of the result / 1.18 to
-// 1.66. With 300 tokens and more it is 1.41 to 1.46 without, whatever the inputs.
-constexpr int kFewKeys = 256;
-
 template <int D>
 cudaError_t bwd_any(WindowArgs& A, int sms, cudaStream_t st) {
   cudaError_t e;
@@ -1562,7 +1561,7 @@ cudaError_t bwd_any(WindowArgs& A, int sms, cudaStream_t st) {
   A.by_bv = make_div(bk * A.nsub);
   A.by_split = make_div(A.sink_splits);
   const int64_t grid = ((int64_t)A.sink_tiles * (A.sink_splits - 1) + nk + nq * A.nsub) * bk;
-  const bool few = A.Tk <= kFewKeys;
+  const bool few = few_keys(A);
   bool one = false;
   if constexpr (D == 64) {
     one = bwd_one_buffer(A, sms);

@@ -418,7 +418,8 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
  *   window >= 1   (INT32_MAX: no window); sinks >= 0
  *   status        as in specdec_dflash_attention_forward
  * A row's probabilities are rounded to bf16 before the second product, all
- * sums are fp32. A NaN or infinity in v of a token of the sequence may reach
+ * sums are fp32; where no query can see more than 64 keys (min(T, window +
+ * sinks + block tokens), whatever ctx_lens) they enter it in two bf16 parts. A NaN or infinity in v of a token of the sequence may reach
  * queries whose mask excludes that token (as 0 * inf does in a masked dense
  * product); masked scores may hold anything.
  */
@@ -437,7 +438,9 @@ size_t specdec_window_attention_workspace_bytes(int32_t batch, int32_t T, int32_
 /*
  * Its backward: dq, dk, dv (contiguous, shaped as q, k, v) from q, k, v, the
  * forward's o, o_residual (or NULL) and lse, and dout (contiguous). dk and dv are sums over the
- * query heads that share a key head. Fixed summation order, no atomics.
+ * query heads that share a key head. Fixed summation order, no atomics. The
+ * probabilities (for dv) and the scores' gradients are rounded to bf16 for their
+ * products; the latter enter in two parts where the forward's probabilities do.
  */
 int specdec_window_attention_backward(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
                                       const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,

@@ -552,3 +552,75 @@ def test_a_training_batch_past_32_bit_offsets(cuda):
     for name, t, h in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads), (qs, qs, ks, ks)):
         _near(name, t[1, T - n:, h], tuple(w[m - n:] for w in want[name]))
     assert float(o[0].abs().max()) == 0.0 and float(grads[0][0].abs().max()) == 0.0
+
+
+# Aggregate errors: |got - exact| / |bf16(exact) - exact| in norm. Where no query
+# sees more than 64 keys, P (for o and delta), dS and o (for delta) enter their
+# products in two bf16 parts, 16 bits: what is left of their rounding, 2^-17
+# relative to each term, is 2^-7.7 of one rounding of the result (2^-9.3 in the
+# mean), times at most 8 for terms that cancel: 1 + 0.0007. So 1.05 there; one missing
+# second product makes it sqrt(2) and more (below). Elsewhere dS's rounding and the
+# result's are sqrt(2) together, P's adds its square over the number of keys: 1.6.
+# dv = P^T dO has P rounded once everywhere: 1.6.
+ACCURATE = [  # B, n_ctx, n_block, Hq, Hk, D, W, S
+    (6, 3, 0, 4, 4, 64, None, 0), (6, 5, 0, 4, 2, 128, None, 0), (4, 64, 0, 4, 4, 64, None, 0), (4, 48, 16, 8, 2, 128, None, 0),
+    (4, 64, 0, 8, 2, 64, 10, 3),                                        # two query tiles, the second with a tile of sinks
+    (1, 1000, 0, 4, 4, 64, 2, 0), (1, 700, 0, 2, 2, 128, 3, 0), (2, 300, 16, 4, 2, 64, 16, 4), (1, 300, 16, 8, 2, 128, 44, 4),
+    (1, 300, 0, 16, 1, 64, 60, 4),                                      # two score buffers in the backward
+    (1, 900, 0, 8, 1, 128, 30, 1), (1, 900, 0, 6, 2, 64, 30, 34),       # parts of sink tiles, groups of three
+]
+ROUNDED = [(4, 65, 0, 4, 4, 64, None, 0), (2, 256, 0, 4, 4, 64, None, 0), (2, 257, 0, 4, 2, 128, None, 0),
+           (1, 400, 16, 4, 2, 64, 45, 4), (1, 400, 0, 8, 2, 128, 200, 0)]
+
+
+def _ratios(got, exact):
+    return {n: float((got[n].double().cpu() - e).norm() / (e.to(torch.bfloat16).double() - e).norm()) for n, e in exact.items()}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n_ctx,nb,Hq,Hk,D,W,S", ACCURATE + ROUNDED)
+def test_window_attention_aggregate_errors(cuda, B, n_ctx, nb, Hq, Hk, D, W, S):
+    few = (B, n_ctx, nb, Hq, Hk, D, W, S) in ACCURATE
+    T = n_ctx + nb
+    q, do = _rand(B, T, Hq, D, seed=1), _rand(B, T, Hq, D, seed=2)
+    k, v = _rand(B, T, Hk, D, seed=3), _rand(B, T, Hk, D, seed=4)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = drafter.window_attention(*x, n_ctx, window=W, sinks=S)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, x, do))))
+    tok = _tokens(T, n_ctx, n_ctx)
+    vis = _visible(tok, tok, n_ctx, W or 10 ** 9, S)
+    each = [_oracle(q[b].detach(), k[b].detach(), v[b].detach(), vis, do[b]) for b in range(B)]
+    exact = {n: torch.stack([e[n][0] for e in each]) for n in got}
+    for n, r in _ratios(got, exact).items():
+        assert r <= (1.05 if few and n != "dv" else 1.6), (n, r)
+
+
+@pytest.mark.parametrize("T,W", [(3, None), (64, None), (300, 2), (300, 16), (300, 60)])
+def test_the_aggregate_errors_notice_a_missing_second_product(T, W):
+    """The same roundings made in fp64 on the CPU: with all the second parts
+    the ratios are 1.00, without any one of them (or with it the wrong way round)
+    some ratio is above 1.05."""
+    D, B = 64, 8
+    g = torch.Generator().manual_seed(T)
+    q, k, v, do = (torch.randn(B, T, D, generator=g).to(torch.bfloat16).double() for _ in range(4))
+    p, j = torch.arange(T)[:, None], torch.arange(T)[None]
+    vis = (j <= p) & (p - j < (W or T))
+
+    def two(t, part):  # t as bf16 and, times ``part``, the bf16 rest
+        high = t.to(torch.bfloat16).double()
+        return high + part * (t - high).to(torch.bfloat16).double()
+
+    def run(pp, ds_part, o_part, rounded=True):
+        s = (q @ k.mT / 8).masked_fill(~vis, -math.inf)
+        P = torch.softmax(s, -1)
+        o = (two(P, pp) if rounded else P) @ v
+        delta = (do * (two(o, o_part) if rounded else o)).sum(-1, keepdim=True)
+        dS = P * (do @ v.mT - delta) / 8
+        dS = two(dS, ds_part) if rounded else dS
+        out = dict(o=o, dq=dS @ k, dk=dS.mT @ q)
+        return {n: t.to(torch.bfloat16) for n, t in out.items()} if rounded else out
+
+    exact = run(1, 1, 1, rounded=False)
+    assert max(_ratios(run(1, 1, 1), exact).values()) <= 1.01
+    for wrong in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (-1, 1, 1), (1, -1, 1), (1, 1, -1)):
+        assert max(_ratios(run(*wrong), exact).values()) > 1.05, wrong

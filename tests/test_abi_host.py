@@ -171,3 +171,24 @@ def test_kept_buffers_are_never_inference_tensors(monkeypatch):
     assert not words.is_inference() and not counters.is_inference()
     words[3:4].zero_()
     ws.reset_counters()
+
+
+def test_the_library_builds_without_torch():
+    """The Makefile's plans, nothing is run: the torch binding only where the
+    Python at hand has torch, never for `lib`."""
+    import shutil
+    import subprocess
+    import sys
+
+    if shutil.which("make") is None:
+        pytest.skip("no make")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(_lib.LIB_PATH)), "csrc")
+
+    def plan(*args):
+        r = subprocess.run(["make", "-n", "-B", "-C", csrc, *args], capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr
+        return r.stdout
+
+    for args, binding in ((("PYTHON=false",), False), (("lib", f"PYTHON={sys.executable}"), False), ((f"PYTHON={sys.executable}",), True)):
+        out = plan(*args)
+        assert "libspecdec.so" in out and ("drafter_bind.cpp" in out) == binding, args

@@ -33,11 +33,12 @@
 //
 // Measured: rotation of [2, 8191, 16, 128] fp32, interleaved, 46 us (5.9 TB/s);
 // norm and rotation of [1, 32768, 32 + 8, 128] bf16, 111 us (6.0 TB/s) forward,
-// 191 us (5.3 TB/s) backward, bound by issue slots and the wait for shared memory
-// and shuffles as much as by HBM. 16-byte loads of tables and weights in planes
-// without bank conflicts took 8% off. A ring of rows filled with asynchronous
-// copies was a quarter slower: it spends more instructions. One token of 32
-// sequences takes 3.5 us, the time of a launch and one chain of loads.
+// 191 us (5.3 TB/s) backward, fp32 219 us (6.1 TB/s) and 353 us (5.7 TB/s), bound
+// by issue slots and the wait for shared memory and shuffles as much as by HBM.
+// 16-byte loads of tables and weights in planes without bank conflicts took 8%
+// off. A ring of rows filled with asynchronous copies was a quarter slower: it
+// spends more instructions. One token of 32 sequences takes 3.5 us, the time of a
+// launch and one chain of loads.
 #include <algorithm>
 
 #include "specdec_common.cuh"
@@ -50,7 +51,7 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kMaxHead = 512;
-constexpr int kTableFloats = 512;  // a warp's table: cos, sin and -sin of at most 256 pairs
+constexpr int kTableFloats = 512;  // a warp's table: cos and sin of at most 256 pairs
 
 // V consecutive elements of a row, as loaded: one element, or a 16-byte vector.
 template <class T, int V>

@@ -12,8 +12,10 @@
 //
 // Rows. In a training batch [B, T, ...] sequence b's context is rows
 // 0 .. c_b-1 (c_b = ctx_lens[b], or n_ctx), rows c_b .. n_ctx-1 are padding and
-// rows n_ctx .. T-1 the block. Padding is never read (its rows enter the
-// products as zeros) and its outputs and gradients are zero. In a cache the
+// rows n_ctx .. T-1 the block. Padding may hold anything; its outputs and
+// gradients are zero. As streamed rows (which every row of a tile multiplies) it
+// enters as zeros and is not read; as rows of a CTA's own tile it may be loaded,
+// and what comes of it stays in its own result rows, which are overwritten. In a cache the
 // block follows the context directly and the queries are the last Tq tokens;
 // rows behind the last token and rows that no query sees may hold anything.
 //
@@ -27,7 +29,8 @@
 //
 // Softmax: one pass, p = 2^(s - m_ref) with the row's reference maximum raised
 // only when a tile exceeds it by more than 2^8 (then O is rescaled in tensor
-// memory), fp32 sums, P rounded to bf16 for the second product (the operand
+// memory: a published refinement of the online softmax of Milakov and
+// Gimelshein, 2018, arXiv:1805.02867), fp32 sums, P rounded to bf16 for the second product (the operand
 // type; its relative error, half a step, equals that of the rounded output).
 #include <algorithm>
 #include <atomic>
@@ -201,16 +204,14 @@ __device__ __forceinline__ void flush_rows(uint32_t tile, int rows, int lt, bool
 //   softmax   S(i) from tensor memory, P(i) in bf16 back over S(i)'s columns (the
 //             A operand of the next product is read from tensor memory), O
 //             rescaled there when the reference maximum rises
-// Two buffers of scores took [2, 4096, 16 heads, 128] W 1024 from 108 to 87 us
-// (83 with masks as bit words and the later boxes requested after the CTA has
-// met), [1, 8208, 32 / 8, 128] W 2048 to 235 us (1.03 PFLOP/s of the visible
-// pairs), one token of 16 sequences over 24576 cached rows from 249 to 220-228 us
-// (7 TB/s of them), the drafter's [32, 528, 4, 64] W 128 from 30 to 25 us. What
-// bounds it with heads of 128 is the operands' way from shared memory (S reads Q
-// and K, 192 bytes a cycle of 128); with short walks a CTA's set-up and end
-// (a third of 17 thousand cycles). Slower at every size were two query tiles per
-// CTA (268 us for the second), two softmax warpgroups in turn (89 for the first),
-// a part of the exponentials as polynomials (1 to 6% behind).
+// Measured: [1, 8208, 32 / 8, 128] W 2048 229 us (1.05 PFLOP/s of the visible
+// pairs; 267 under the power cap at 1.59 GHz), [2, 4096, 16 heads, 128] W 1024 81 us
+// (0.75; 3.5 waves of tiles), the drafter's [32, 528, 4, 64] W 128 21.5 us, one token
+// of 16 sequences over 24576 cached rows 220-228 us in a row (7 TB/s). With heads of 128
+// the tensor pipe is busy 53% of the time, the exponentials' unit as much, issue
+// slots 47%: the operands' way from shared memory (S reads Q and K, 192 bytes a
+// cycle of 128) would allow about 80, the rest is one waiting for the other. With
+// short walks it is a CTA's set-up and end (a third of 17 thousand cycles).
 // Every wait is bounded and watches a shared flag that the first expired wait
 // raises; all warps then leave for the common end.
 // How the parts of a row's keys come together: one part; unnormalised fp32 rows
@@ -747,8 +748,8 @@ __global__ void __launch_bounds__(128) window_join_kernel(const __grid_constant_
 // columns of scores, then the accumulators. A product of 128 x 64 reads more
 // operand bytes from shared memory than it has cycles for (192 of 128 bytes a
 // cycle), so the dq role, whose accumulator leaves room, keeps X in tensor
-// memory: [1, 8208, 32 / 8 heads, 128] W 2048 took 793 us with X in shared memory
-// in both roles, 751 so.
+// memory (6% of [1, 8208, 32 / 8 heads, 128] W 2048, which takes 730 to 750 us: 0.8
+// PFLOP/s of five products, tensor pipe 59%, issue slots 34%).
 //
 // The first key tile holds the sinks: every later context query sees them, far
 // more than see any other tile. Tiles with sinks are split over their queries
@@ -1526,7 +1527,8 @@ int64_t walk_steps(const WindowArgs& A) {
 // 1024) 135 / 158, [4, 4096, 8] W 2048 (34, 1024) 280 / 298; [1, 3000, 32 / 8]
 // W 512 (40, 192) 101 / 99, [1, 32768, 4 / 1] W 1024 (72, 256) 204 / 210,
 // [1, 8192, 16 / 2] W 512 (80, 128) 157 / 133, [1, 6000, 8] (94, 376) 204 / 185,
-// [1, 6000, 8 / 4] (188, 188) 255 / 176, [1, 16384, 8] (256, 1024) 1137 / 1144.
+// [1, 6000, 8 / 4] (188, 188) 255 / 176, [1, 16384, 8] (256, 1024) 1137 / 1144. (At two
+// of these the other one would be 3% faster.)
 bool bwd_one_buffer(const WindowArgs& A, int sms) {
   const int64_t tiles = (int64_t)(A.Tq + kTM - 1) / kTM * A.B * A.Hk;
   return walk_steps(A) < 32 || tiles > 3 * (int64_t)sms;

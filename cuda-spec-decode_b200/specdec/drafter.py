@@ -261,7 +261,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, n_ctx: i
     a block query sees every block token, the last ``window`` context tokens and
     the sinks. ctx_lens int32 [B] (None: all n_ctx): sequence b has only
     ctx_lens[b] context tokens, in rows 0 .. ctx_lens[b]-1; the rows behind
-    them up to n_ctx are padding, never read, with zero outputs and gradients.
+    them up to n_ctx are padding: they may hold anything, their outputs and
+    gradients are zero.
     Differentiable in q, k, v; scale None = D^-0.5. Products take bf16 operands
     and sum in fp32; where no query can see more than 64 keys (min(T, window +
     sinks + block)) the probabilities of the forward and the scores' gradients

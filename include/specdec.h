@@ -405,8 +405,9 @@ int specdec_qk_norm_rotary_backward(const void* q, const int64_t* q_strides, con
  * rows, and rows n_ctx .. T-1. A context query sees the keys up to itself
  * that are among the last `window` (itself included) or the first `sinks`
  * tokens; a block query sees every block token, the last `window` context
- * tokens and the sinks. Rows c .. n_ctx-1 are padding: never read (they may
- * hold anything), their outputs and gradients are zero.
+ * tokens and the sinks. Rows c .. n_ctx-1 are padding: they may hold anything
+ * (a kernel may load them and discards what comes of it), their outputs and
+ * gradients are zero.
  *   q, o          [batch, T, q_heads, head_dim], k, v [batch, T, k_heads,
  *                 head_dim] bf16 patterns; head h of q reads head
  *                 h / (q_heads / k_heads) of k and v; head_dim 64 or 128;

@@ -146,8 +146,9 @@ class DFlashAttention(nn.Module):
 
     def _apply(self, fn, *args, **kwargs):  # .to(), .cuda(), ...
         super()._apply(fn, *args, **kwargs)
-        if self.rotary is not None:
-            self._frequencies(self.q_proj.weight.device)
+        first = next(self.parameters(), None)
+        if self.rotary is not None and first is not None:
+            self._frequencies(first.device)
         return self
 
     def _project(self, x: torch.Tensor, positions: torch.Tensor):

@@ -249,6 +249,12 @@ class DFlashAttention(nn.Module):
         return self.out_proj(y.reshape(b, s, self.d_model))
 
 
+def _lens(ctx_lens: torch.Tensor | None) -> dict:
+    """ctx_lens as a keyword, where given: a subclass or a replaced layer without
+    it still takes whole contexts."""
+    return {} if ctx_lens is None else {"ctx_lens": ctx_lens}
+
+
 class DFlashTransformerLayer(nn.Module):
     """Pre-norm block: x + attn(norm(x)), then x + mlp(norm(x)) (reference
     model.py:56-73). ``attention``: DFlashAttention's options."""
@@ -263,7 +269,7 @@ class DFlashTransformerLayer(nn.Module):
 
     def forward(self, x: torch.Tensor, attn_mask: torch.Tensor | None = None,
                 n_ctx: int | None = None, ctx_lens: torch.Tensor | None = None) -> torch.Tensor:
-        x = x + self.attn(self.norm1(x), attn_mask=attn_mask, n_ctx=n_ctx, ctx_lens=ctx_lens)
+        x = x + self.attn(self.norm1(x), attn_mask=attn_mask, n_ctx=n_ctx, **_lens(ctx_lens))
         return x + self.mlp(self.norm2(x))
 
     def forward_cached(self, x: torch.Tensor, *cached) -> torch.Tensor:
@@ -366,14 +372,14 @@ class DFlashSpeculator(nn.Module):
         h = self._embed(target_features)
         # the _build_dflash_mask rule, applied by structure (no [T, T] mask tensor)
         for layer in self.layers:
-            h = layer(h, n_ctx=s_ctx, ctx_lens=ctx_lens)
+            h = layer(h, n_ctx=s_ctx, **_lens(ctx_lens))
         return self._block_logits(h)
 
     def compute_loss(self, target_features: torch.Tensor, ground_truth_block_tokens: torch.Tensor,
                      loss_fn=None, ctx_lens: torch.Tensor | None = None) -> torch.Tensor:
         """Training loss over the block slots. ``loss_fn(logits, targets) -> scalar``
         swaps the objective (dpace_loss, dflash_objective(...)); None = plain CE."""
-        logits = self.forward(target_features, ctx_lens)
+        logits = self.forward(target_features, **_lens(ctx_lens))
         if loss_fn is not None:
             return loss_fn(logits, ground_truth_block_tokens)
         return F.cross_entropy(logits.reshape(-1, self.target_vocab_size),
@@ -398,7 +404,7 @@ class DFlashSpeculator(nn.Module):
         Without room for them ValueError; in a replayed graph, where the host does
         not look, the sequence keeps what it has and its logits are NaN."""
         if cache is None:
-            logits = self.forward(target_features, ctx_lens)
+            logits = self.forward(target_features, **_lens(ctx_lens))
             return logits.argmax(dim=-1), logits
         b, n_new, _ = target_features.shape
         if b != cache.lens.shape[0]:

@@ -271,6 +271,35 @@ def test_a_draft_after_replays_is_checked_against_the_real_lengths(monkeypatch):
         m.draft(x[:, 8:9], cache=cache)
 
 
+def test_subclasses_without_ctx_lens_take_whole_contexts():
+    """forward(target_features) and layers called with n_ctx alone, as they were
+    before contexts had lengths of their own."""
+    class Layer(nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x, attn_mask=None, n_ctx=None):
+            return self.inner(x, attn_mask=attn_mask, n_ctx=n_ctx)
+
+    class Attention(DFlashAttention):
+        def forward(self, x, attn_mask=None, n_ctx=None):
+            return super().forward(x, attn_mask, n_ctx)
+
+    class Speculator(DFlashSpeculator):
+        def forward(self, target_features):
+            return super().forward(target_features)
+
+    a, b = _model(None), _model(None)
+    b.__class__ = Speculator
+    for layer in b.layers:
+        layer.attn.__class__ = Attention
+    b.layers = nn.ModuleList(Layer(layer) for layer in b.layers)
+    x, tokens = torch.randn(2, 9, 48), torch.randint(0, 50, (2, 4))
+    assert torch.equal(a.compute_loss(x, tokens), b.compute_loss(x, tokens))
+    assert torch.equal(a.draft(x)[1], b.draft(x)[1])
+
+
 # ---- on the GPU ------------------------------------------------------------------
 
 GPU_OPTIONS = [

@@ -350,6 +350,12 @@ class DFlashSpeculator(nn.Module):
         mask.masked_fill_(~visible, float("-inf"))
         return mask.view(1, 1, T, T)
 
+    @staticmethod
+    def _check_lens(ctx_lens: torch.Tensor, target_features: torch.Tensor) -> None:
+        if ctx_lens.shape != target_features.shape[:1] or ctx_lens.dtype.is_floating_point or ctx_lens.dtype == torch.bool:
+            raise AssertionError(f"ctx_lens must be int [batch], got {ctx_lens.dtype} {list(ctx_lens.shape)} for a batch of "
+                                 f"{target_features.shape[0]}")
+
     def _embed(self, target_features: torch.Tensor) -> torch.Tensor:
         return torch.cat([self.proj_in(target_features),
                           self.slot_queries.expand(target_features.shape[0], -1, -1).to(target_features.dtype)], dim=1)
@@ -367,6 +373,7 @@ class DFlashSpeculator(nn.Module):
         with them too)."""
         s_ctx = target_features.shape[1]
         if ctx_lens is not None:
+            self._check_lens(ctx_lens, target_features)
             live = torch.arange(s_ctx, device=target_features.device) < ctx_lens.to(target_features.device)[:, None]
             target_features = torch.where(live[:, :, None], target_features, 0)
         h = self._embed(target_features)
@@ -406,6 +413,8 @@ class DFlashSpeculator(nn.Module):
         if cache is None:
             logits = self.forward(target_features, **_lens(ctx_lens))
             return logits.argmax(dim=-1), logits
+        if ctx_lens is not None:
+            self._check_lens(ctx_lens, target_features)
         b, n_new, _ = target_features.shape
         if b != cache.lens.shape[0]:
             raise ValueError(f"the cache is for {cache.lens.shape[0]} sequences, got {b}")

@@ -300,6 +300,19 @@ def test_subclasses_without_ctx_lens_take_whole_contexts():
     assert torch.equal(a.draft(x)[1], b.draft(x)[1])
 
 
+def test_ctx_lens_of_another_batch_are_refused():
+    """They would be broadcast, one sequence to several."""
+    m = _model(dict(rotary={}))
+    x, tokens = torch.randn(1, 6, 48), torch.randint(0, 50, (1, 4))
+    for bad in (torch.tensor([3, 4, 5]), torch.tensor(3), torch.tensor([[3]]), torch.tensor([3.0]), torch.tensor([True])):
+        for call in (lambda: m(x, bad), lambda: m.compute_loss(x, tokens, ctx_lens=bad), lambda: m.draft(x, bad),
+                     lambda: m.draft(x, bad, cache=m.new_cache(1, 20, dtype=torch.float32))):
+            with pytest.raises(AssertionError):
+                call()
+    with pytest.raises(AssertionError):
+        m(x.expand(3, -1, -1), torch.tensor([3]))
+
+
 # ---- on the GPU ------------------------------------------------------------------
 
 GPU_OPTIONS = [
